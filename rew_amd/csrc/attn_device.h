@@ -1,0 +1,229 @@
+// Device helpers shared by the attention kernels: MFMA operand types, the hardware
+// exp2 and max, packing to 16 bits, and the DMA from memory into LDS.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace rew {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// 2^x with the hardware v_exp_f32 (1 ulp) and no denormal-range fix-up:
+// every argument here is <= 0 (a score minus its running max), and results
+// below 2^-126 are probabilities far under one bf16 ulp of the row sum.
+// (The library exp2f wraps the instruction in a range test and two
+// rescales; on the Llama shape the flash kernel ran 9 % faster without.)
+__device__ __forceinline__ float fa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max(a, b, c) in one v_max3_f32.  fmaxf would first quiet signalling NaNs
+// with a v_max_f32 x, x per operand (MFMA results are not known to be
+// canonical); a quiet NaN operand is ignored either way.  The compiler does
+// not see that this reads a register: the wait states between a MFMA and the
+// first use of its result must come from a builtin (fa_max2) before it.
+__device__ __forceinline__ float fa_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// max(a, b) as one v_med3_f32, which the compiler knows: the first read of
+// MFMA results, later ones by fa_max3 then being chained to it.
+__device__ __forceinline__ float fa_max2(float a, float b) {
+  return __builtin_amdgcn_fmed3f(a, b, INFINITY);
+}
+
+// Two fp32 values rounded to bf16 (RNE; v_cvt_pk_bf16_f32), packed.
+__device__ __forceinline__ uint32_t cvt_bf16x2(float a, float b) {
+  const bf16x2_t v = __builtin_convertvector((f32x2_t){a, b}, bf16x2_t);
+  uint32_t u;
+  __builtin_memcpy(&u, &v, 4);
+  return u;
+}
+
+__device__ __forceinline__ void dma16(const void* src, uint16_t* lds) {
+  __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0);
+}
+
+// Buffer descriptor over `bytes` bytes at `base`; a read past them returns
+// zeros and touches no memory.  Both are wave-uniform and readfirstlane says
+// so, which keeps the descriptor in SGPRs.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fa_rsrc(const void* base,
+                                                          uint32_t bytes = 0x7fffffff) {
+  const uint64_t a = (uint64_t)(uintptr_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  void* p = (void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+  return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, (int)__builtin_amdgcn_readfirstlane(bytes),
+                                           0x00020000);
+}
+// 16 bytes per lane from base + voff + soff into LDS (buffer_load ... lds):
+// the per-lane offset is fixed, the tile advance is the scalar `soff`.
+__device__ __forceinline__ void dma16_buf(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
+                                          uint16_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, voff, soff, 0, 0);
+}
+
+__device__ __forceinline__ void dma16_lds(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
+                                          lds_void* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, voff, soff, 0, 0);
+}
+
+// Workgroup barrier without the memory fence of __syncthreads (which would
+// also wait for every DMA in flight); callers wait for what they need first.
+// No instruction is scheduled across it: the ping-pong phases it separates
+// must keep their own MFMA or VALU work.
+__device__ __forceinline__ void block_barrier_fa() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// ---- operand types of the packed and paged kernels --------------------------------
+//
+// The 16-bit type of Q, K, V and of the probabilities that feed the second
+// product.  kShift: the probabilities are stored as 2^kShift p, and kLazy2:
+// the running max of the softmax moves only when a row's max grew by more
+// than 2^kLazy2.  bfloat16 has float32's range, so it needs no shift; float16
+// is normal from 2^-14 to 2^16: 2^11 p stays below 2^15 and keeps 11 bits
+// down to p = 2^-25, where an unshifted probability would have lost them at
+// 2^-14.
+struct MmaBf16 {
+  typedef bf16x8_t frag;
+  static constexpr float kShift = 0.0f, kLazy2 = 11.5f, kGradShift = 0.0f;
+  static constexpr bool kScaled = false;  // dS is stored scaled (k_packed_grad.hip)
+  static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return cvt_bf16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u << 16); }
+  static __device__ __forceinline__ float hi(uint32_t u) {
+    return __uint_as_float(u & 0xffff0000u);
+  }
+};
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+struct MmaF16 {
+  typedef f16x8_t frag;
+  static constexpr float kShift = 11.0f, kLazy2 = 4.0f, kGradShift = 15.0f;
+  static constexpr bool kScaled = true;
+  static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const f16x2_t v = __builtin_convertvector((f32x2_t){a, b}, f16x2_t);
+    uint32_t u;
+    __builtin_memcpy(&u, &v, 4);
+    return u;
+  }
+  static __device__ __forceinline__ float lo(uint32_t u) {
+    f16x2_t v;
+    __builtin_memcpy(&v, &u, 4);
+    return (float)v[0];
+  }
+  static __device__ __forceinline__ float hi(uint32_t u) {
+    f16x2_t v;
+    __builtin_memcpy(&v, &u, 4);
+    return (float)v[1];
+  }
+};
+
+// max over lanes l and l ^ 32
+__device__ __forceinline__ float fa_max_halves(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fa_max3(__uint_as_float(s[0]), __uint_as_float(s[1]), -INFINITY);
+}
+__device__ __forceinline__ float fa_sum_halves(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// ---- packed sequences ---------------------------------------------------------------
+//
+// Sequence s owns rows [starts[s], starts[s + 1]) of T.  The rows before the
+// first and behind the last sequence belong to none: they count as sequences
+// -1 and n_seq, without keys.  starts is device data that the host does not
+// see, so every value is clamped into [0, T] and a decreasing one makes an
+// empty sequence: no row outside the tensors is ever touched.
+struct SeqTile {
+  int seq;     // -1 .. n_seq; -2: there is no such tile
+  int first;   // its first row
+  int n;       // its rows
+  int tile;    // the tile's index in the sequence
+  __device__ __forceinline__ bool real(int n_seq) const { return seq >= 0 && seq < n_seq; }
+};
+__device__ __forceinline__ int seq_bound(const int32_t* starts, int n_seq, int T, int s) {
+  if (s < 0) return 0;
+  if (s > n_seq) return T;
+  return min(max(starts[s], 0), T);
+}
+// Tile `idx` of the sequences' tiles of `per` units, a row holding `units`
+// (query heads of a KV head; 1 for keys), in sequence order.  One wave (every
+// wave of a workgroup does the same): 64 sequences a step, their tile counts
+// summed over the lanes.
+__device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, int T, int units,
+                                             int per, int idx) {
+  const int lane = threadIdx.x & 63;
+  SeqTile r;
+  r.seq = -2;
+  r.first = r.n = r.tile = 0;
+  for (int base = -1; base <= n_seq; base += 64) {
+    const int s = base + lane;
+    const int b0 = seq_bound(starts, n_seq, T, s);
+    const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
+    const int tiles = (int)(((int64_t)n * units + per - 1) / per);
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const int total = __builtin_amdgcn_readlane(sum, 63);
+    if (idx < total) {
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
+      r.seq = base + at;
+      r.first = __builtin_amdgcn_readlane(b0, at);
+      r.n = __builtin_amdgcn_readlane(n, at);
+      r.tile = idx - __builtin_amdgcn_readlane(sum - tiles, at);
+      return r;
+    }
+    idx -= total;
+  }
+  return r;
+}
+// A bound on find_tile's tiles, known on the host.
+inline int64_t max_seq_tiles(int64_t T, int n_seq, int64_t units, int64_t per) {
+  return T * units / per + n_seq + 2;
+}
+
+// Rows of D 16-bit values, `stride` elements apart, read a tile of `step_rows`
+// at a time through a descriptor that ends with the last row: what lies
+// behind it reads as zeros and touches no memory.
+struct RowTiles {
+  const uint16_t* p;
+  int64_t step, left;  // elements per tile; bytes from p to the end of the last row
+  __device__ __forceinline__ RowTiles(const uint16_t* base, int64_t row, int64_t rows,
+                                      int64_t stride, int D, int step_rows)
+      : p(base + row * stride), step(step_rows * stride),
+        left(rows > row ? ((rows - 1 - row) * stride + D) * 2 : 0) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t next() {
+    const __amdgpu_buffer_rsrc_t r =
+        fa_rsrc(p, (uint32_t)(left < 0 ? 0 : left < 0x7fffffff ? left : 0x7fffffff));
+    p += step;
+    left -= step * 2;
+    return r;
+  }
+};
+
+}  // namespace rew

@@ -45,18 +45,11 @@
 #include <cstdlib>
 #include <string>
 
+#include "attn_device.h"
 #include "kernels.h"
 #include "vm_device.h"
 
 namespace rew {
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s;
-typedef __attribute__((address_space(3))) void lds_void;
 
 namespace fa {
 constexpr int BQ = 128;  // queries per workgroup
@@ -98,46 +91,6 @@ __device__ __forceinline__ bool fa_all_visible(int cmp, int q0, int q1, int k0, 
   }
 }
 
-// 2^x with the hardware v_exp_f32 (1 ulp) and no denormal-range fix-up:
-// every argument here is <= 0 (a score minus its running max), and results
-// below 2^-126 are probabilities far under one bf16 ulp of the row sum.
-// (The library exp2f wraps the instruction in a range test and two
-// rescales; on the Llama shape the flash kernel ran 9 % faster without.)
-__device__ __forceinline__ float fa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// max(a, b, c) in one v_max3_f32.  fmaxf would first quiet signalling NaNs
-// with a v_max_f32 x, x per operand (MFMA results are not known to be
-// canonical); a quiet NaN operand is ignored either way.
-__device__ __forceinline__ float fa_max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-
-// Two fp32 values rounded to bf16 (RNE; v_cvt_pk_bf16_f32), packed.
-__device__ __forceinline__ uint32_t cvt_bf16x2(float a, float b) {
-  const bf16x2_t v = __builtin_convertvector((f32x2_t){a, b}, bf16x2_t);
-  uint32_t u;
-  __builtin_memcpy(&u, &v, 4);
-  return u;
-}
-
-__device__ __forceinline__ void dma16(const void* src, uint16_t* lds) {
-  __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0);
-}
-
-// Buffer descriptor over `bytes` bytes at `base`; a read past them returns
-// zeros and touches no memory.  Both are wave-uniform and readfirstlane says
-// so, which keeps the descriptor in SGPRs.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t fa_rsrc(const void* base,
-                                                          uint32_t bytes = 0x7fffffff) {
-  const uint64_t a = (uint64_t)(uintptr_t)base;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
-  void* p = (void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
-  return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, (int)__builtin_amdgcn_readfirstlane(bytes),
-                                           0x00020000);
-}
 // Walks key rows of D bf16 values, `stride` (>= 0) apart, a tile at a time
 // from row k0 of `rows` to the next one `step` rows on (additions on the
 // scalar ALU only: a multiplication per tile cost a decode step up to 10 %).
@@ -161,18 +114,6 @@ struct FaRows {
     return r;
   }
 };
-// 16 bytes per lane from base + voff + soff into LDS (buffer_load ... lds):
-// the per-lane offset is fixed, the tile advance is the scalar `soff`.
-__device__ __forceinline__ void dma16_buf(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
-                                          uint16_t* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, voff, soff, 0, 0);
-}
-
-__device__ __forceinline__ void dma16_lds(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
-                                          lds_void* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, voff, soff, 0, 0);
-}
-
 // Tile kinds of the softmax step, each straight-line code:
 //   0 plain     every key in range and visible, scale > 0: t is formed
 //               inside the exp's FMA and the max comes from the raw
@@ -380,18 +321,6 @@ __device__ __forceinline__ void fa_softmax_any(int kind, const FlashArgs& a, int
   else
     fa_softmax_tile<DT, FA_GENERAL>(a, k0, qi, g, sl2, sacc, mr, pk, m_run, l_run, alpha);
   fa_rescale<DT>(o, alpha);
-}
-
-// Workgroup barrier without the memory fence of __syncthreads (which would
-// also wait for every DMA in flight); callers wait for what they need first.
-// No instruction is scheduled across it: the ping-pong phases it separates
-// must keep their own MFMA or VALU work.
-__device__ __forceinline__ void block_barrier_fa() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
 }
 
 // BUF: every byte offset into K and V is below 2^31, so the tiles move by

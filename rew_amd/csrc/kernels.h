@@ -546,6 +546,82 @@ void init_silu_table(hipStream_t stream);
 // Profile name of the kernel launch_flash runs for `a`.
 const char* flash_variant(const FlashArgs& a);
 
+// ---- attention over packed sequences and paged caches -----------------------------
+// (k_prompt.hip; k_packed_grad.hip its gradient)
+// q, out [T, H, D]; sequence s owns rows [starts[s], starts[s + 1]) (n of
+// them).  Packed: k, v [T, Hkv, D], and a row sees the keys of its own
+// sequence, those up to its own row when causal.  Paged (table set): k, v
+// [pages, Hkv, 2^log_page, D]; request s has lens[s] keys, key j being row
+// j % 2^log_page of page table[s, j / 2^log_page]; its i-th row is at
+// position lens[s] - n + i and sees the keys up to it (all, if not causal).
+// A key whose page is not in [0, pages) or lies past the table's width is not
+// seen.  With s_j = scale q . k_j over the keys seen (head h reads KV head
+// h / (H / Hkv)):
+//   lse = log sum_j exp(s_j)   (f32 [T, H]; -inf without keys)
+//   out = sum_j exp(s_j - lse) v_j   (0 without keys)
+// A row of no sequence has no keys.
+struct PackedArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;  // null: not stored
+  const int32_t *starts, *table, *lens;
+  int64_t T, pages;
+  int n_seq, H, Hkv, D, width, log_page, f16, causal;
+  float scale;
+};
+// 16-bit operands, D of 32, 64 or 128, Hkv divides H.
+void launch_packed_attn(const PackedArgs& a, hipStream_t stream);
+const char* packed_attn_variant(const PackedArgs& a);
+
+// The gradients of packed attention for the gradient `dout` of out: with
+// p_j = exp(s_j - lse), delta = dout . out and ds_j = p_j (dout . v_j - delta)
+//   dq = scale sum_j ds_j k_j;  dk_j = scale sum ds_j q, dv_j = sum p_j dout,
+// the last two over the rows that see j and the H / Hkv heads that read it.
+// Rows of no sequence get zeros.  work: packed_grad_ws_bytes.
+struct PackedGradArgs {
+  const void *q, *k, *v, *out, *dout;
+  const float* lse;
+  const int32_t* starts;
+  void *dq, *dk, *dv, *work;
+  int64_t T;
+  int n_seq, H, Hkv, D, f16, causal;
+  int delta_blocks;  // set by the launch
+  float scale;
+};
+size_t packed_grad_ws_bytes(int64_t T, int H);
+void launch_packed_grad(const PackedGradArgs& a, hipStream_t stream);
+
+// ---- pages of a key / value cache (k_pages.hip) -------------------------------------
+// The tables of a step that adds fresh[r] tokens to request r, which has
+// cached[r] of them (negative counts are 0): with have = ceil(cached / page),
+// want = ceil((cached + fresh) / page) and take[r] = want - have,
+//   table'[r, j] = table[r, j] for j < have, pool[sum_{i<r} take[i] + j - have]
+//     for have <= j < want (-1 past the pool's end), -1 behind;
+//   position[t] = cached[r] + i, slot[t] = table'[r, p / page] page + p % page
+//     (-1 without a page) for the i-th new token t of request r, requests one
+//     after another; 0 and -1 for t >= sum fresh;
+//   starts = the exclusive sums of fresh (clamped to tokens), total last;
+//   lens = cached + fresh (at most 2^31 - 1);  taken = sum of take.
+struct PageTablesArgs {
+  const int32_t *cached, *fresh, *table, *pool;
+  int32_t *out_table, *slots, *positions, *starts, *lens, *taken;
+  int64_t n, width, pool_n, tokens;
+  int log_page;
+};
+void launch_page_tables(const PageTablesArgs& a, hipStream_t stream);
+
+// Row slots[t] (page slots[t] >> log_page, row slots[t] % 2^log_page) of every
+// KV head of the pages becomes row t of k and v [T, Hkv, D]; a slot outside
+// the pages is skipped.
+struct PageWriteArgs {
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  const int32_t* slots;
+  int64_t T, pages;
+  int Hkv, row_bytes, log_page;  // row_bytes: D values, a multiple of 16
+};
+void launch_page_write(const PageWriteArgs& a, hipStream_t stream);
+
 // ---- row composites (k_rows.hip) ----------------------------------------------
 // rmsNorm over rows of n contiguous elements (x row stride x_rs elements):
 // y[r, j] = gamma[j] * (x[r, j] / sqrt(sum_j x^2 / divisor + eps)).

@@ -387,6 +387,9 @@ struct Lower {
   void emit_index_map(Node* n);
   void emit_window(Node* n);
   void emit_cholesky(Node* n);
+  void emit_packed_attn(Node* n);
+  void emit_packed_grad(Node* n);
+  void emit_page_tables(Node* n);
   void emit_trisolve(Node* n);
   void emit_complex(Node* n);
   void emit_fft1(Node* n);
@@ -1109,6 +1112,9 @@ void Lower::emit_anchor(Node* n) {
     case K_SCATTER: emit_index_map(n); break;
     case K_WINDOW: emit_window(n); break;
     case K_CHOLESKY: emit_cholesky(n); break;
+    case K_PACKED_ATTN: emit_packed_attn(n); break;
+    case K_PACKED_GRAD: emit_packed_grad(n); break;
+    case K_PAGE_TABLES: emit_page_tables(n); break;
     case K_TRISOLVE: emit_trisolve(n); break;
     case K_COMPLEX: emit_complex(n); break;
     case K_FFT1: emit_fft1(n); break;
@@ -3458,6 +3464,98 @@ void Lower::emit_cholesky(Node* n) {
   Launch L{a};
   if (c->profiling)
     L.name = "cholesky{" + std::to_string(a.batch) + "x" + std::to_string(a.n) + "}";
+  run_launch(c, std::move(L));
+}
+
+static std::string heads_label(int64_t T, int H, int Hkv, int D) {
+  return "{" + std::to_string(T) + "x" + std::to_string(H) + "/" + std::to_string(Hkv) + "x" +
+         std::to_string(D) + "}";
+}
+
+// packedAttention: q, k, v, starts; pagedAttention (sub 1): q, the pages, the
+// block table, starts, lens.
+void Lower::emit_packed_attn(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  PackedArgs a;
+  std::memset(&a, 0, sizeof a);
+  Tensor *q = n->in[0], *k = n->in[1];
+  a.q = q->data();
+  a.k = k->data();
+  a.v = n->in[2]->data();
+  a.out = n->out[0]->data();
+  a.T = q->shape.d[0];
+  a.H = (int)q->shape.d[1];
+  a.Hkv = (int)k->shape.d[1];
+  a.D = (int)q->shape.d[2];
+  a.f16 = q->dt == kF16;
+  a.causal = (int)n->i0;
+  std::memcpy(&a.scale, &n->i1, sizeof a.scale);
+  if (n->sub) {
+    Tensor* table = n->in[3];
+    a.table = (const int32_t*)table->data();
+    a.starts = (const int32_t*)n->in[4]->data();
+    a.lens = (const int32_t*)n->in[5]->data();
+    a.pages = k->shape.d[0];
+    a.n_seq = (int)table->shape.d[0];
+    a.width = (int)table->shape.d[1];
+    while ((1ll << a.log_page) < k->shape.d[2]) a.log_page++;
+  } else {
+    a.lse = (float*)n->out[1]->data();
+    a.starts = (const int32_t*)n->in[3]->data();
+    a.n_seq = (int)n->in[3]->shape.d[0] - 1;
+  }
+  Launch L{a};
+  if (c->profiling) L.name = packed_attn_variant(a) + heads_label(a.T, a.H, a.Hkv, a.D);
+  run_launch(c, std::move(L));
+}
+
+void Lower::emit_packed_grad(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  PackedGradArgs a;
+  std::memset(&a, 0, sizeof a);
+  Tensor *q = n->in[0], *k = n->in[1];
+  a.q = q->data();
+  a.k = k->data();
+  a.v = n->in[2]->data();
+  a.starts = (const int32_t*)n->in[3]->data();
+  a.n_seq = (int)n->in[3]->shape.d[0] - 1;
+  a.out = n->in[4]->data();
+  a.lse = (const float*)n->in[5]->data();
+  a.dout = n->in[6]->data();
+  a.dq = n->out[0]->data();
+  a.dk = n->out[1]->data();
+  a.dv = n->out[2]->data();
+  a.work = (char*)a.dq + tensor_tail_offset(n->out[0]);
+  a.T = q->shape.d[0];
+  a.H = (int)q->shape.d[1];
+  a.Hkv = (int)k->shape.d[1];
+  a.D = (int)q->shape.d[2];
+  a.f16 = q->dt == kF16;
+  a.causal = (int)n->i0;
+  std::memcpy(&a.scale, &n->i1, sizeof a.scale);
+  Launch L{a};
+  if (c->profiling) L.name = "packed_attn_grad" + heads_label(a.T, a.H, a.Hkv, a.D);
+  run_launch(c, std::move(L));
+}
+
+void Lower::emit_page_tables(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  PageTablesArgs a;
+  std::memset(&a, 0, sizeof a);
+  const int32_t** in[4] = {&a.cached, &a.fresh, &a.table, &a.pool};
+  int32_t** out[6] = {&a.out_table, &a.slots, &a.positions, &a.starts, &a.lens, &a.taken};
+  for (int i = 0; i < 4; ++i) *in[i] = (const int32_t*)n->in[i]->data();
+  for (int i = 0; i < 6; ++i) *out[i] = (int32_t*)n->out[i]->data();
+  a.n = n->in[2]->shape.d[0];
+  a.width = n->in[2]->shape.d[1];
+  a.pool_n = n->in[3]->shape.d[0];
+  a.tokens = n->i1;
+  a.log_page = (int)n->i0;
+  Launch L{a};
+  if (c->profiling) L.name = "page_tables{" + std::to_string(a.n) + "}";
   run_launch(c, std::move(L));
 }
 

@@ -5,6 +5,7 @@
 // shape/dtype at record time, and every error names the op.
 #include <algorithm>
 #include <cctype>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <unordered_map>
@@ -113,6 +114,10 @@ static const std::unordered_map<std::string, OpSpec>& op_table() {
       {"batchNormInference", {K_BATCHNORM, kBnInference}},
       {"batchNormTraining", {K_BATCHNORM, kBnTraining}},
       {"batchNormGrad", {K_BATCHNORM, kBnGrad}},
+      // sequences of unequal lengths and their cache (no counterpart in the
+      // reference; pagedCacheWrite, which updates its pages, is not recorded)
+      {"packedAttention", {K_PACKED_ATTN, 0}}, {"pagedAttention", {K_PACKED_ATTN, 1}},
+      {"packedAttentionGrad", {K_PACKED_GRAD, 0}}, {"pagedBlockTables", {K_PAGE_TABLES, 0}},
   };
   return t;
 }
@@ -258,6 +263,159 @@ static void require_vm_dtype(int dt, const std::string& op) {
 }
 
 static const int64_t kMaxElems = (int64_t)1 << 31;
+
+// ---- packed sequences and paged caches ----------------------------------------------
+
+static void check_i32(const Tensor* t, int rank, const char* what, const std::string& op) {
+  if (t->dt != kI32 || t->shape.rank != rank)
+    invalid("eager '" + op + "': " + what + " must be an int32 tensor of rank " +
+            std::to_string(rank) + ", got " + dt_enum_name(t->dt) + t->shape.str());
+}
+
+// The log2 of a page size (a power of two up to 65536).
+static int page_log2(int64_t page, const std::string& op) {
+  int l = 0;
+  while (l < 16 && (1ll << l) < page) ++l;
+  if (page < 1 || (1ll << l) != page)
+    invalid("eager '" + op + "': page size " + std::to_string(page) +
+            " must be a power of two from 1 to 65536");
+  return l;
+}
+
+static void check_pages(const Tensor* kp, const Tensor* vp, const std::string& op) {
+  if (kp->shape.rank != 4 || kp->shape != vp->shape || kp->dt != vp->dt)
+    invalid("eager '" + op + "': kPages and vPages must be [pages, kvHeads, pageSize, headDim] "
+            "of one dtype, got " + kp->shape.str() + " and " + vp->shape.str());
+  page_log2(kp->shape.d[2], op);
+  if (kp->shape.d[0] * kp->shape.d[2] >= (1ll << 31))
+    invalid("eager '" + op + "': the pages hold 2^31 tokens or more");
+}
+
+static bool flag_attr(const Attrs& attrs, const char* key, const std::string& op) {
+  const std::string v = strip(find_attr(attrs, key, op));
+  if (v != "true" && v != "false") invalid("eager '" + op + "': " + key + " must be true or false");
+  return v == "true";
+}
+
+// The float32 attr "scale": positive, or 0 for 1 / sqrt(headDim).
+static float scale_attr(const Attrs& attrs, int64_t D, const std::string& op) {
+  const std::string v = strip(find_attr(attrs, "scale", op));
+  char* end = nullptr;
+  const float x = std::strtof(v.c_str(), &end);
+  if (v.empty() || *end || !(x >= 0.0f) || !(x < INFINITY))
+    invalid("eager '" + op + "': scale must be a finite number >= 0, got '" + v + "'");
+  return x == 0.0f ? 1.0f / std::sqrt((float)D) : x;
+}
+
+// q [T, H, D] with k and v (or pages) of Hkv heads: what the kernels take.
+static void check_heads(const Tensor* q, int dt, int64_t hkv, int64_t d, const std::string& op) {
+  if (q->shape.rank != 3) invalid("eager '" + op + "': q must be [tokens, heads, headDim], got " +
+                                  q->shape.str());
+  if (q->dt != dt)
+    invalid("eager '" + op + "': dtype mismatch (" + dt_enum_name(q->dt) + " vs " +
+            dt_enum_name(dt) + ")");
+  if (q->shape.d[2] != d)
+    invalid("eager '" + op + "': head dims of q and k differ (" + std::to_string(q->shape.d[2]) +
+            " and " + std::to_string(d) + ")");
+  if (hkv < 1 || q->shape.d[1] < 1 || q->shape.d[1] % hkv)
+    invalid("eager '" + op + "': " + std::to_string(q->shape.d[1]) +
+            " query heads do not divide among " + std::to_string(hkv) + " KV heads");
+  if (dt != kBF16 && dt != kF16)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': only bfloat16 / float16, got " +
+                                         dt_enum_name(dt));
+  if (d != 32 && d != 64 && d != 128)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': head dim " + std::to_string(d) +
+                                         " (32, 64 and 128 are supported)");
+  if (q->shape.d[1] * d > (1 << 20))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': more than 2^20 values per token");
+}
+
+using OutSpecs = std::vector<std::pair<int, Shape>>;
+
+// packedAttention(q, k, v, starts): attrs causal, scale; out, lse.
+static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*>& ins,
+                                const Attrs& attrs, Node* n, OutSpecs& outs) {
+  Tensor *q = ins[0], *k = ins[1], *v = ins[2];
+  if (k->shape.rank != 3 || k->shape != v->shape || k->dt != v->dt)
+    invalid("eager '" + op + "': k and v must be [tokens, kvHeads, headDim] of one dtype, got " +
+            k->shape.str() + " and " + v->shape.str());
+  check_heads(q, k->dt, k->shape.d[1], k->shape.d[2], op);
+  if (q->shape.d[0] != k->shape.d[0])
+    invalid("eager '" + op + "': q has " + std::to_string(q->shape.d[0]) + " tokens, k has " +
+            std::to_string(k->shape.d[0]));
+  check_i32(ins[3], 1, "starts", op);
+  if (ins[3]->shape.d[0] < 1) invalid("eager '" + op + "': starts must hold at least one value");
+  n->i0 = flag_attr(attrs, "causal", op);
+  const float scale = scale_attr(attrs, q->shape.d[2], op);
+  std::memcpy(&n->i1, &scale, sizeof scale);
+  if (n->kind == K_PACKED_ATTN) {
+    outs.push_back({q->dt, q->shape});
+    outs.push_back({kF32, Shape(std::vector<int64_t>{q->shape.d[0], q->shape.d[1]})});
+    return;
+  }
+  // packedAttentionGrad(q, k, v, starts, out, lse, gradOut): the gradients of q, k, v
+  Tensor *o = ins[4], *lse = ins[5], *go = ins[6];
+  if (o->dt != q->dt || o->shape != q->shape)
+    invalid("eager '" + op + "': out must have q's dtype and shape");
+  if (go->dt != q->dt || go->shape != q->shape)
+    invalid("eager '" + op + "': gradOut must have q's dtype and shape");
+  if (lse->dt != kF32 || lse->shape.rank != 2 || lse->shape.d[0] != q->shape.d[0] ||
+      lse->shape.d[1] != q->shape.d[1])
+    invalid("eager '" + op + "': lse must be float32 [tokens, heads]");
+  n->tail = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1]);
+  outs.push_back({q->dt, q->shape});
+  outs.push_back({k->dt, k->shape});
+  outs.push_back({v->dt, v->shape});
+}
+
+// pagedAttention(q, kPages, vPages, blockTable, starts, lens): attrs causal,
+// scale; out.
+static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>& ins,
+                               const Attrs& attrs, Node* n, OutSpecs& outs) {
+  Tensor *q = ins[0], *kp = ins[1], *vp = ins[2], *table = ins[3];
+  check_pages(kp, vp, op);
+  check_heads(q, kp->dt, kp->shape.d[1], kp->shape.d[3], op);
+  check_i32(table, 2, "blockTable", op);
+  check_i32(ins[4], 1, "starts", op);
+  check_i32(ins[5], 1, "lens", op);
+  const int64_t R = table->shape.d[0];
+  if (ins[4]->shape.d[0] != R + 1 || ins[5]->shape.d[0] != R)
+    invalid("eager '" + op + "': blockTable has " + std::to_string(R) + " requests, starts " +
+            ins[4]->shape.str() + " and lens " + ins[5]->shape.str() + " need one more and as many");
+  if (table->shape.d[1] * kp->shape.d[2] > (1ll << 30))
+    invalid("eager '" + op + "': the block table reaches past 2^30 tokens per request");
+  n->i0 = flag_attr(attrs, "causal", op);
+  const float scale = scale_attr(attrs, q->shape.d[2], op);
+  std::memcpy(&n->i1, &scale, sizeof scale);
+  outs.push_back({q->dt, q->shape});
+}
+
+// pagedBlockTables(cachedLens, newLens, blockTable, freePages): attrs
+// page_size, tokens; blockTable, slots, positions, starts, lens, taken.
+static void prepare_page_tables(const std::string& op, const std::vector<Tensor*>& ins,
+                                const Attrs& attrs, Node* n, OutSpecs& outs) {
+  check_i32(ins[0], 1, "cachedLens", op);
+  check_i32(ins[1], 1, "newLens", op);
+  check_i32(ins[2], 2, "blockTable", op);
+  check_i32(ins[3], 1, "freePages", op);
+  const int64_t R = ins[2]->shape.d[0];
+  if (ins[0]->shape.d[0] != R || ins[1]->shape.d[0] != R)
+    invalid("eager '" + op + "': cachedLens " + ins[0]->shape.str() + ", newLens " +
+            ins[1]->shape.str() + " and blockTable " + ins[2]->shape.str() +
+            " need one row per request");
+  if (R >= (1 << 20)) fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': 2^20 requests or more");
+  n->i0 = page_log2(parse_int(find_attr(attrs, "page_size", op), op), op);
+  n->i1 = parse_int(find_attr(attrs, "tokens", op), op);
+  if (n->i1 < 0 || n->i1 >= kMaxElems) invalid("eager '" + op + "': tokens out of range");
+  auto vec = [](int64_t k) { return Shape(std::vector<int64_t>{k}); };
+  outs.push_back({kI32, ins[2]->shape});
+  outs.push_back({kI32, vec(n->i1)});
+  outs.push_back({kI32, vec(n->i1)});
+  outs.push_back({kI32, vec(R + 1)});
+  outs.push_back({kI32, vec(R)});
+  outs.push_back({kI32, vec(1)});
+}
+
 
 // ---- record ------------------------------------------------------------------------
 
@@ -919,6 +1077,19 @@ Node* prepare_node(Ctx* c, const std::string& op, const std::vector<Tensor*>& in
         }
         break;
       }
+      case K_PACKED_ATTN:
+        nin(spec.sub ? 6 : 4);
+        if (spec.sub) prepare_paged_attn(op, ins, attrs, n, outs);
+        else prepare_packed_attn(op, ins, attrs, n, outs);
+        break;
+      case K_PACKED_GRAD:
+        nin(7);
+        prepare_packed_attn(op, ins, attrs, n, outs);
+        break;
+      case K_PAGE_TABLES:
+        nin(4);
+        prepare_page_tables(op, ins, attrs, n, outs);
+        break;
       case K_CHOLESKY: {
         // stablehlo.cholesky (src/rew/ops/linalg.nim:177-202)
         nin(1);
@@ -1145,6 +1316,7 @@ std::vector<Tensor*> commit_node(Ctx* c, Node* n, const std::vector<Tensor*>& in
     t->prod = n;
     t->prod_out = (int)i;
     t->ext = 1;
+    if (i == 0) t->tail = n->tail;
     n->out.push_back(t);
     result.push_back(t);
   }
@@ -1491,9 +1663,65 @@ static std::vector<Tensor*> record_fft(Ctx* c, const std::vector<Tensor*>& ins,
   return {y};
 }
 
+// pagedCacheWrite(kPages, vPages, k, v, slots): rows of k and v [T, kvHeads,
+// headDim] into the pages, in place, without outputs.  Tensors are otherwise
+// immutable, so the pages must be tensors of rew_mi355x_alloc; what is
+// pending is launched first (it reads them as they were), and what is
+// recorded later reads them as written.
+static std::vector<Tensor*> run_page_write(Ctx* c, const std::vector<Tensor*>& ins) {
+  const std::string op = "pagedCacheWrite";
+  if (ins.size() != 5)
+    invalid("eager '" + op + "': expected 5 operand(s), got " + std::to_string(ins.size()));
+  Tensor *kp = ins[0], *vp = ins[1], *k = ins[2], *v = ins[3], *slots = ins[4];
+  check_pages(kp, vp, op);
+  if (!kp->writable || !vp->writable)
+    invalid("eager '" + op + "': kPages and vPages must come from rew_mi355x_alloc (other "
+            "tensors are immutable)");
+  if (kp->st == vp->st) invalid("eager '" + op + "': kPages and vPages are one tensor");
+  if (k->shape.rank != 3 || k->shape != v->shape || k->dt != v->dt)
+    invalid("eager '" + op + "': k and v must be [tokens, kvHeads, headDim] of one dtype, got " +
+            k->shape.str() + " and " + v->shape.str());
+  if (k->dt != kp->dt || k->shape.d[1] != kp->shape.d[1] || k->shape.d[2] != kp->shape.d[3])
+    invalid("eager '" + op + "': rows " + std::string(dt_enum_name(k->dt)) + k->shape.str() +
+            " do not fit pages " + dt_enum_name(kp->dt) + kp->shape.str());
+  check_i32(slots, 1, "slots", op);
+  if (slots->shape.d[0] != k->shape.d[0])
+    invalid("eager '" + op + "': " + std::to_string(k->shape.d[0]) + " tokens, " +
+            std::to_string(slots->shape.d[0]) + " slots");
+  if (k->dt != kBF16 && k->dt != kF16)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': only bfloat16 / float16, got " +
+                                         dt_enum_name(k->dt));
+  const int64_t row = k->shape.d[2] * dt_size(k->dt);
+  if (row % 16 || k->shape.d[1] * row > (1 << 21))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': rows must be a multiple of 16 bytes, at "
+                                     "most 2^21 of them per token");
+  flush(c);
+  for (Tensor* t : ins)
+    if (!t->st) invalid("eager '" + op + "': an operand has no data (an earlier flush failed)");
+  PageWriteArgs a;
+  std::memset(&a, 0, sizeof a);
+  a.k = k->data();
+  a.v = v->data();
+  a.k_pages = kp->data();
+  a.v_pages = vp->data();
+  a.slots = (const int32_t*)slots->data();
+  a.T = k->shape.d[0];
+  a.pages = kp->shape.d[0];
+  a.Hkv = (int)kp->shape.d[1];
+  a.row_bytes = (int)row;
+  a.log_page = page_log2(kp->shape.d[2], op);
+  if (a.T * a.Hkv == 0) return {};
+  if (c->profiling) prof_begin(c, "page_write{" + std::to_string(a.T) + "}");
+  launch_page_write(a, c->stream);
+  prof_end(c);
+  c->stats.kernels_launched++;
+  return {};
+}
+
 std::vector<Tensor*> record_op(Ctx* c, const std::string& op,
                                const std::vector<Tensor*>& ins,
                                const Attrs& attrs) {
+  if (op == "pagedCacheWrite") return run_page_write(c, ins);
   if (op == "einsum" || op == "unaryEinsum") return record_einsum(c, op, ins, attrs);
   if (op == "fft") return record_fft(c, ins, attrs);
   if (op == "dynamicPad" || op == "realDynamicSlice" || op == "dynamicBroadcastInDim")

@@ -159,6 +159,23 @@ struct PtrVisit {
     field(f, a.probs);
     field(f, a.ids);
   }
+  void operator()(PackedArgs& a) {
+    for (const void** p : {&a.q, &a.k, &a.v}) field(f, *p);
+    field(f, a.out);
+    field(f, a.lse);
+    for (const int32_t** p : {&a.starts, &a.table, &a.lens}) field(f, *p);
+  }
+  void operator()(PackedGradArgs& a) {
+    for (const void** p : {&a.q, &a.k, &a.v, &a.out, &a.dout}) field(f, *p);
+    field(f, a.lse);
+    field(f, a.starts);
+    for (void** p : {&a.dq, &a.dk, &a.dv, &a.work}) field(f, *p);
+  }
+  void operator()(PageTablesArgs& a) {
+    for (const int32_t** p : {&a.cached, &a.fresh, &a.table, &a.pool}) field(f, *p);
+    for (int32_t** p : {&a.out_table, &a.slots, &a.positions, &a.starts, &a.lens, &a.taken})
+      field(f, *p);
+  }
   void operator()(RouterArgs& a) {
     field(f, a.x);
     field(f, a.w);
@@ -216,6 +233,12 @@ struct Exec {
   void operator()(BatchNormArgs& a) { launch_batchnorm(a, c->stream); }
   void operator()(HeadArgs& a) { launch_class_head(a, c->stream); }
   void operator()(RouterArgs& a) { launch_moe_router(a, c->stream); }
+  void operator()(PackedArgs& a) { launch_packed_attn(a, c->stream); }
+  void operator()(PackedGradArgs& a) {  // (three kernels)
+    launch_packed_grad(a, c->stream);
+    c->stats.kernels_launched += 2;
+  }
+  void operator()(PageTablesArgs& a) { launch_page_tables(a, c->stream); }
   void operator()(FillL& l) {
     if (l.bytes == 0) return;
     if (l.src)

@@ -59,7 +59,8 @@ struct FillL {
 using LaunchArgs = std::variant<EwL, ReduceL, GemmL, FlashArgs, RowNormArgs, SoftmaxArgs,
                                 RopeArgs, GatherArgs, ArgmaxArgs, TopkArgs, SortArgs,
                                 IndexMapL, MoeL, FillL, WindowArgs, CholeskyArgs, TriSolveArgs, ComplexArgs, Fft1Args,
-                                BatchNormArgs, HeadArgs, RouterArgs>;
+                                BatchNormArgs, HeadArgs, RouterArgs, PackedArgs,
+                                PackedGradArgs, PageTablesArgs>;
 
 struct Launch {
   LaunchArgs args;

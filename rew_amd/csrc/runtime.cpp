@@ -114,6 +114,7 @@ void tensor_alloc(Tensor* t) {
   Storage* s = new Storage();
   s->ctx = t->ctx;
   size_t bytes = (size_t)t->nbytes();
+  if (t->tail) bytes = tensor_tail_offset(t) + t->tail;
   s->ptr = t->ctx->alloc.get(bytes, &s->bytes);
   s->refs = 1;
   t->st = s;
@@ -438,6 +439,7 @@ int rew_mi355x_alloc(rew_mi355x_ctx* ctx, int dtype, const int64_t* shape, int r
       throw;
     }
     t->ext = 1;
+    t->writable = true;
     *out = reinterpret_cast<rew_mi355x_buf*>(t);
   });
 }

@@ -41,6 +41,10 @@ struct Tensor {
   Storage* st = nullptr;    // dense row-major data once materialized
   Node* prod = nullptr;     // pending producer, nullptr once materialized
   int prod_out = 0;         // which output of `prod`
+  size_t tail = 0;          // bytes of working memory behind the data, for the launch that
+                            // writes it: they live as long as the tensor, so launches captured
+                            // into different graphs never share them
+  bool writable = false;    // made by rew_mi355x_alloc: an op may update it in place
   bool has_host = false;    // small constant whose bytes are known on host
   uint8_t host[16] = {0};
   // planner scratch (valid during one flush)
@@ -66,6 +70,9 @@ enum Kind : int {
   K_TRISOLVE,
   K_COMPLEX,
   K_FFT1,
+  K_PACKED_ATTN,  // packedAttention, pagedAttention (sub 1)
+  K_PACKED_GRAD,  // packedAttentionGrad
+  K_PAGE_TABLES,  // pagedBlockTables
   K_BATCHNORM, // batchNormInference / Training / Grad (sub: kBn*)
   // composite kernels created by the planner (never recorded directly)
   K_COUNT
@@ -82,6 +89,7 @@ struct Node {
   int64_t i0 = 0, i1 = 0, i2 = 0;
   int dt_attr = -1;
   int cmp = 0;
+  size_t tail = 0;          // output 0's Tensor::tail
   int n_in_keep = -1;       // >= 0: only the first n_in_keep operands are read
                             // (the rest only fix static shapes)
   // planner scratch
@@ -168,6 +176,10 @@ struct Ctx {
 // ---- runtime services (runtime.cpp) -----------------------------------------
 Tensor* new_tensor(Ctx* c, int dt, const Shape& s);
 void tensor_alloc(Tensor* t);                 // give t fresh storage
+// where t's working memory starts in its storage (256-byte aligned)
+inline size_t tensor_tail_offset(const Tensor* t) {
+  return ((size_t)t->nbytes() + 255) & ~(size_t)255;
+}
 void storage_release(Storage* s);             // drop one reference
 void const_cache_clear(Ctx* c);               // release every cached constant
 void tensor_alias(Tensor* t, Tensor* src);    // share src's storage

@@ -457,6 +457,7 @@ def dispatchEager(op: str, operands: Sequence[Tensor] = (),
     return be(op, operands, list(attrs))
 
 
+_MAX_OUTS = 8  # outputs of one op (pagedBlockTables has 6)
 _META = 2 + 8  # per output: dtype, rank, 8 dims (rew_mi355x_execute_ex)
 _DTYPE_OF = {int(d): d for d in DType}
 _enc_cache: dict = {}
@@ -478,9 +479,9 @@ class _Scratch(threading.local):
         self.ops = (C.c_void_p * 16)()
         self.keys = (C.c_char_p * 16)()
         self.vals = (C.c_char_p * 16)()
-        self.outs = (C.c_void_p * 4)()
+        self.outs = (C.c_void_p * _MAX_OUTS)()
         self.nout = C.c_int()
-        self.meta = (C.c_int64 * (4 * _META))()
+        self.meta = (C.c_int64 * (_MAX_OUTS * _META))()
 
 
 _scratch = _Scratch()
@@ -513,8 +514,8 @@ def executeMi355xOp(op: str, operands: Sequence[Tensor],
     for i, (k, v) in enumerate(attrs):
         keys[i] = _enc(k)
         vals[i] = _enc(v)
-    rc = lib.rew_mi355x_execute_ex(context(d), _enc(op), ops, n, keys, vals, na, sc.outs, 4,
-                                   C.byref(sc.nout), sc.meta)
+    rc = lib.rew_mi355x_execute_ex(context(d), _enc(op), ops, n, keys, vals, na, sc.outs,
+                                   _MAX_OUTS, C.byref(sc.nout), sc.meta)
     _check(rc)
     res = []
     meta = sc.meta

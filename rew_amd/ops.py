@@ -757,3 +757,191 @@ def imag(a: Tensor) -> Tensor:
 def fft(a: Tensor, fftType: str, fftLength: Sequence[int]) -> Tensor:
     """src/rew/ops/linalg.nim:328-348 (fftType FFT, IFFT, RFFT or IRFFT)."""
     return _one("fft", [a], [("fft_type", fftType), ("fft_length", _join_ints(fftLength))])
+
+
+# ---- sequences of unequal lengths and their paged cache ---------------------------------
+# Backend extensions without a counterpart in the reference, eager only.  Rows of
+# all sequences lie one after another (no padding): sequence s owns rows
+# [starts[s], starts[s + 1]).  Lengths and tables are device tensors that no call
+# reads back; values out of range never reach memory outside the tensors.
+
+def _packed_call(op: str, operands, attrs, nouts: int) -> list:
+    if _jit.currentMode() == "trace":
+        raise TensorError(f"{op}: eager only (it has no StableHLO form)")
+    for t in operands[1:]:
+        if t.device != operands[0].device:
+            raise TensorError(f"{op}: device mismatch")
+    outs = dispatchEager(op, operands, attrs)
+    assert len(outs) == nouts, f"{op}: eager backend returned wrong arity"
+    return outs
+
+
+def _check_i32(op: str, t: Tensor, name: str, shape) -> None:
+    """`shape`: the extents, None where any will do."""
+    if t.dtype != DType.INT32 or len(t.shape) != len(shape) or any(
+            w is not None and w != d for w, d in zip(shape, t.shape)):
+        want = ["*" if w is None else w for w in shape]
+        raise TensorError(f"{op}: {name} must be int32 {want}, got {t.dtype.rew_name} "
+                          f"{list(t.shape)}")
+
+
+def _check_heads(op: str, q: Tensor, dtype: DType, kvHeads: int, headDim: int) -> None:
+    if len(q.shape) != 3:
+        raise TensorError(f"{op}: q must be [tokens, heads, headDim], got {list(q.shape)}")
+    if q.dtype != dtype:
+        raise TensorError(f"{op}: dtype mismatch ({q.dtype.enum_name} vs {dtype.enum_name})")
+    if q.shape[2] != headDim:
+        raise TensorError(f"{op}: head dims of q and k differ ({q.shape[2]} and {headDim})")
+    if kvHeads < 1 or q.shape[1] < 1 or q.shape[1] % kvHeads:
+        raise TensorError(f"{op}: {q.shape[1]} query heads do not divide among {kvHeads} "
+                          "KV heads")
+
+
+def _check_packed(op: str, q: Tensor, k: Tensor, v: Tensor, starts: Tensor) -> None:
+    if len(k.shape) != 3 or k.shape != v.shape or k.dtype != v.dtype:
+        raise TensorError(f"{op}: k and v must be [tokens, kvHeads, headDim] of one dtype, got "
+                          f"{list(k.shape)} and {list(v.shape)}")
+    _check_heads(op, q, k.dtype, k.shape[1], k.shape[2])
+    if q.shape[0] != k.shape[0]:
+        raise TensorError(f"{op}: q has {q.shape[0]} tokens, k has {k.shape[0]}")
+    _check_i32(op, starts, "starts", (None,))
+    if starts.shape[0] < 1:
+        raise TensorError(f"{op}: starts must hold at least one value")
+
+
+def _check_pages(op: str, kPages: Tensor, vPages: Tensor) -> int:
+    if len(kPages.shape) != 4 or kPages.shape != vPages.shape or kPages.dtype != vPages.dtype:
+        raise TensorError(f"{op}: kPages and vPages must be [pages, kvHeads, pageSize, headDim] "
+                          f"of one dtype, got {list(kPages.shape)} and {list(vPages.shape)}")
+    return _check_page_size(op, kPages.shape[2])
+
+
+def _check_page_size(op: str, page: int) -> int:
+    if page < 1 or page > 65536 or page & (page - 1):
+        raise TensorError(f"{op}: page size {page} must be a power of two from 1 to 65536")
+    return page
+
+
+def _attn_attrs(op: str, causal: bool, scale: float) -> list:
+    if not 0.0 <= scale < float("inf"):
+        raise TensorError(f"{op}: scale must be a finite number >= 0, got {scale}")
+    return [("causal", "true" if causal else "false"),
+            ("scale", repr(float(np.float32(scale))))]
+
+
+def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: bool = True,
+                    scale: float = 0.0, withLse: bool = False):
+    """softmax(scale q k^T) v within each of the packed sequences.
+
+    ``q`` [tokens, heads, headDim]; ``k``, ``v`` [tokens, kvHeads, headDim] (head h reads
+    KV head h / (heads / kvHeads)); bfloat16 or float16; headDim 32, 64 or 128; ``starts``
+    int32 [sequences + 1].  ``causal``: a row sees the rows of its sequence up to itself
+    (unlike ``nn.makeCausalMask``, whose orientation is the reference's); otherwise all of
+    them.  ``scale`` 0: 1 / sqrt(headDim).  The softmax is float32; the probabilities are
+    rounded to the operands' dtype before the second product, the result once.  A row of no
+    sequence (before ``starts[0]``, behind ``starts[-1]``) gives zeros.
+
+    ``withLse``: (out, lse), lse float32 [tokens, heads] the log of the row's sum of
+    exponentials (-inf for a row of no sequence), which ``packedAttentionGrad`` takes."""
+    _check_packed("packedAttention", q, k, v, starts)
+    out, lse = _packed_call("packedAttention", [q, k, v, starts],
+                            _attn_attrs("packedAttention", causal, scale), 2)
+    return (out, lse) if withLse else out
+
+
+def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Tensor,
+                        lse: Tensor, gradOut: Tensor, causal: bool = True, scale: float = 0.0):
+    """(gradQ, gradK, gradV) of ``packedAttention(q, k, v, starts, causal, scale)`` for the
+    gradient ``gradOut`` of its result, given its ``out`` and ``lse``.  gradK and gradV are
+    summed over the query heads of each KV head; sums are float32 in a fixed order."""
+    op = "packedAttentionGrad"
+    _check_packed(op, q, k, v, starts)
+    for t, name in ((out, "out"), (gradOut, "gradOut")):
+        if t.dtype != q.dtype or t.shape != q.shape:
+            raise TensorError(f"{op}: {name} must have q's dtype and shape")
+    if lse.dtype != DType.FLOAT32 or lse.shape != q.shape[:2]:
+        raise TensorError(f"{op}: lse must be float32 [tokens, heads]")
+    return tuple(_packed_call(op, [q, k, v, starts, out, lse, gradOut],
+                              _attn_attrs(op, causal, scale), 3))
+
+
+def pagedBlockTables(cachedLens: Tensor, newLens: Tensor, blockTable: Tensor,
+                     freePages: Tensor, pageSize: int, tokens: int):
+    """The tables of a serving step that adds ``newLens[r]`` tokens to request r, which has
+    ``cachedLens[r]`` tokens in the pages ``blockTable[r]`` (all int32; blockTable
+    [requests, blocks]).  Requests that need more pages take them from the front of
+    ``freePages``, in request order.  ``tokens``: the sum of newLens, or more.
+
+    Returns int32 (blockTable, slots, positions, starts, lens, taken):
+
+    * blockTable [requests, blocks]: the pages each request had, then the new ones; -1 behind
+      them, and where freePages ran out;
+    * slots [tokens]: the cache row page * pageSize + offset of each new token (requests one
+      after another), -1 for a token without a page and behind the last token;
+    * positions [tokens]: its position in its request (0 behind the last token);
+    * starts [requests + 1]: the first new token of each request, then their number;
+    * lens [requests]: cachedLens + newLens;
+    * taken [1]: the pages needed (more than freePages holds: they ran out).
+
+    Negative lengths count as 0."""
+    op = "pagedBlockTables"
+    _check_page_size(op, pageSize)
+    _check_i32(op, blockTable, "blockTable", (None, None))
+    r = blockTable.shape[0]
+    _check_i32(op, cachedLens, "cachedLens", (r,))
+    _check_i32(op, newLens, "newLens", (r,))
+    _check_i32(op, freePages, "freePages", (None,))
+    if tokens < 0:
+        raise TensorError(f"{op}: tokens must be non-negative, got {tokens}")
+    return tuple(_packed_call(op, [cachedLens, newLens, blockTable, freePages],
+                              [("page_size", str(pageSize)), ("tokens", str(tokens))], 6))
+
+
+def pagedCacheWrite(kPages: Tensor, vPages: Tensor, k: Tensor, v: Tensor,
+                    slots: Tensor) -> None:
+    """Writes rows t of ``k`` and ``v`` [tokens, kvHeads, headDim] into row ``slots[t]`` of the
+    pages [pages, kvHeads, pageSize, headDim], in place: page slots[t] / pageSize, row
+    slots[t] % pageSize of every KV head.  A negative slot, or one past the pages, writes
+    nothing.  Slots must be distinct: of two tokens in one slot either may stay, in parts.
+
+    The one op that changes its operands: the pages must come from ``eager.empty``.  What was
+    recorded before reads the old rows, what is recorded later the new ones."""
+    op = "pagedCacheWrite"
+    _check_pages(op, kPages, vPages)
+    if len(k.shape) != 3 or k.shape != v.shape or k.dtype != v.dtype:
+        raise TensorError(f"{op}: k and v must be [tokens, kvHeads, headDim] of one dtype, got "
+                          f"{list(k.shape)} and {list(v.shape)}")
+    if k.dtype != kPages.dtype or k.shape[1] != kPages.shape[1] or k.shape[2] != kPages.shape[3]:
+        raise TensorError(f"{op}: rows {k.dtype.rew_name} {list(k.shape)} do not fit pages "
+                          f"{kPages.dtype.rew_name} {list(kPages.shape)}")
+    _check_i32(op, slots, "slots", (k.shape[0],))
+    _packed_call(op, [kPages, vPages, k, v, slots], [], 0)
+
+
+def pagedAttention(q: Tensor, kPages: Tensor, vPages: Tensor, blockTable: Tensor,
+                   starts: Tensor, lens: Tensor, causal: bool = True, scale: float = 0.0,
+                   maxNew: int = 0) -> Tensor:
+    """Attention of each request's new tokens over its cached keys and values.
+
+    ``q`` [tokens, heads, headDim]: request r's n = starts[r + 1] - starts[r] rows from
+    starts[r], at positions lens[r] - n and on.  Its ``lens[r]`` keys (the new tokens' own
+    among them, written before by ``pagedCacheWrite``) lie in the pages ``blockTable[r]``:
+    key j in row j % pageSize of page blockTable[r, j / pageSize].  ``causal``: a row sees
+    the keys up to its own position; otherwise all ``lens[r]``.  A key without a valid page
+    is not seen, and a row that sees none, or belongs to no request, gives zeros.  One token
+    per request is a decode step, a whole prompt over an empty cache a prefill, and requests
+    of both kinds may be mixed.  dtypes, head dims, scale and rounding as in
+    ``packedAttention``.
+
+    ``maxNew``: at least the largest n, if the caller knows it (0: not); it chooses the
+    kernels, never the result."""
+    op = "pagedAttention"
+    _check_pages(op, kPages, vPages)
+    _check_heads(op, q, kPages.dtype, kPages.shape[1], kPages.shape[3])
+    _check_i32(op, blockTable, "blockTable", (None, None))
+    _check_i32(op, starts, "starts", (blockTable.shape[0] + 1,))
+    _check_i32(op, lens, "lens", (blockTable.shape[0],))
+    if maxNew < 0:
+        raise TensorError(f"{op}: maxNew must be non-negative, got {maxNew}")
+    attrs = _attn_attrs(op, causal, scale) + [("max_new", str(maxNew))]
+    return _packed_call(op, [q, kPages, vPages, blockTable, starts, lens], attrs, 1)[0]
