@@ -202,6 +202,73 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, i
   }
   return r;
 }
+// Lane-wise sum over the wave, the same in every lane.
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+// The rank-th of the sequences' tiles in the order of falling level: a
+// sequence's tiles have the levels lift + 1 .. lift + tiles (its own per
+// lane; level by level, in sequence order), tile = level - lift - 1.  A level
+// stands for the tile's work, so the heaviest tiles of all sequences start
+// first.  At most 64 sequences (kLevelSeqs real ones), one per lane.
+constexpr int kLevelSeqs = 62;
+__device__ __forceinline__ SeqTile level_tile(int s, int first, int n, int tiles, int lift,
+                                              int rank) {
+  SeqTile r;
+  r.seq = -2;
+  r.first = r.n = r.tile = 0;
+  if (rank >= wave_sum(tiles)) return r;
+  auto above = [&](int level) { return min(max(lift + tiles - level + 1, 0), tiles); };
+  int top = lift + tiles;  // the levels of all lanes end here
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = max(top, __shfl_xor(top, d));
+  // the highest level that, with those above it, has more than `rank` tiles
+  int lo = 1, hi = __builtin_amdgcn_readfirstlane(top) + 1;
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (wave_sum(above(mid)) > rank) lo = mid;
+    else hi = mid;
+  }
+  rank -= wave_sum(above(lo + 1));
+  const uint64_t have = __builtin_amdgcn_ballot_w64(lift < lo && lo <= lift + tiles);
+  const int lane = threadIdx.x & 63;
+  const uint64_t before = have & ((1ull << lane) - 1);
+  const int at = __builtin_ctzll(
+      __builtin_amdgcn_ballot_w64(((have >> lane) & 1) && __builtin_popcountll(before) == rank));
+  r.seq = __builtin_amdgcn_readlane(s, at);
+  r.first = __builtin_amdgcn_readlane(first, at);
+  r.n = __builtin_amdgcn_readlane(n, at);
+  r.tile = lo - __builtin_amdgcn_readlane(lift, at) - 1;
+  return r;
+}
+// level_tile over tiles of `per` units (find_tile's), the work growing with
+// the tile's index.
+__device__ __forceinline__ SeqTile rising_tile(const int32_t* starts, int n_seq, int T, int units,
+                                               int per, int rank) {
+  const int s = (int)(threadIdx.x & 63) - 1;
+  const int b0 = seq_bound(starts, n_seq, T, s);
+  const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
+  return level_tile(s, b0, n, (int)(((int64_t)n * units + per - 1) / per), 0, rank);
+}
+
+// r / g and r % g for 0 <= r < 2^31: one multiplication by floor((2^32 - 1) / g)
+// falls short of the quotient by at most one.
+struct DivBy {
+  uint32_t g, m;
+  __device__ __forceinline__ explicit DivBy(int d) : g(d), m(0xffffffffu / (uint32_t)d) {}
+  __device__ __forceinline__ int div(int r, int& rem) const {
+    uint32_t q = __umulhi((uint32_t)r, m);
+    uint32_t x = (uint32_t)r - q * g;
+    const bool up = x >= g;
+    q += up;
+    x -= up ? g : 0;
+    rem = (int)x;
+    return (int)q;
+  }
+};
+
 // A bound on find_tile's tiles, known on the host.
 inline int64_t max_seq_tiles(int64_t T, int n_seq, int64_t units, int64_t per) {
   return T * units / per + n_seq + 2;

@@ -16,6 +16,7 @@
 // and dS go from the accumulators straight into the next product, as in the
 // forward kernel, and the LDS operand of that product is read transposed.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_device.h"
 #include "kernels.h"
@@ -41,7 +42,8 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 }
 
 // ---- delta --------------------------------------------------------------------------
-// D / 8 lanes per row of T H rows.  float16 has no room for dS at any scale:
+// Per row (D / 8 lanes each of T H rows) what the scores and dP are added to:
+// kGradShift - log2(e) lse, and -delta.  float16 has no room for dS at any scale:
 // it is stored as F dS, F the power of two that takes the bound
 // |dS| <= 2 D max|dout| max|V| to 2^15, so this kernel also leaves the maxima
 // of its workgroups (a maximum does not depend on their order).
@@ -50,7 +52,7 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   constexpr int L = D / 8;
   const int64_t rows = a.T * a.H, step = gridDim.x * (256ll / L);
   const int ch = threadIdx.x % L;
-  float* delta = (float*)a.work;
+  float *neg_lse = (float*)a.work, *neg_delta = neg_lse + rows;
   float most = 0.0f, most_v = 0.0f;
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
@@ -65,7 +67,10 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
     }
 #pragma unroll
     for (int d = L / 2; d > 0; d >>= 1) s += __shfl_xor(s, d);
-    if (ch == 0) delta[i] = s;
+    if (ch == 0) {
+      neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
+      neg_delta[i] = -s;
+    }
   }
   if constexpr (M::kScaled) {
     const int64_t n = a.T * a.Hkv * L;
@@ -87,19 +92,19 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
     __syncthreads();
     if (threadIdx.x < 2) {
       const float* q = part + 4 * threadIdx.x;
-      delta[rows + blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+      neg_delta[rows + blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
     }
   }
 }
 // F, from the maxima of the delta kernel's workgroups (a power of two; 1 for
-// bfloat16).  Every thread of a workgroup of 256 calls it.
-template <class M, int D>
+// bfloat16).  Every thread of a workgroup of N calls it.
+template <class M, int D, int N>
 __device__ __forceinline__ float grad_factor(const PackedGradArgs& a) {
   if constexpr (!M::kScaled) return 1.0f;
-  __shared__ float part[8];
-  const float* m = (const float*)a.work + a.T * a.H;
+  __shared__ float part[2 * N / 64];
+  const float* m = (const float*)a.work + 2 * a.T * a.H;
   float d = 0.0f, v = 0.0f;
-  for (int i = threadIdx.x; i < a.delta_blocks; i += 256) {
+  for (int i = threadIdx.x; i < a.delta_blocks; i += N) {
     d = fmaxf(d, m[2 * i]);
     v = fmaxf(v, m[2 * i + 1]);
   }
@@ -110,11 +115,14 @@ __device__ __forceinline__ float grad_factor(const PackedGradArgs& a) {
   }
   if ((threadIdx.x & 63) == 0) {
     part[threadIdx.x >> 6] = d;
-    part[4 + (threadIdx.x >> 6)] = v;
+    part[N / 64 + (threadIdx.x >> 6)] = v;
   }
   __syncthreads();
-  d = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  v = fmaxf(fmaxf(part[4], part[5]), fmaxf(part[6], part[7]));
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) {
+    d = fmaxf(d, part[w]);
+    v = fmaxf(v, part[N / 64 + w]);
+  }
   const float bound = 2.0f * D * d * v;
   if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
   int e;
@@ -122,183 +130,358 @@ __device__ __forceinline__ float grad_factor(const PackedGradArgs& a) {
   return ldexpf(1.0f, min(max(15 - e, -60), 60));
 }
 
-// Fragment offsets in an LDS tile of D columns: `rows` for the operand whose
-// rows lie along the lanes (row c, chunk 2t + g), `cols` for the transposed
-// read (ds_read_b64_tr_b16) of 8 rows' columns dt 32 + 16 (G & 1) ..; the
-// second half of it, 8 rows on, is at (cols ^ 16) + 8 D.
+// Where a lane reads its fragments in an LDS tile of D columns, in bytes.
+// `rows`, for the operand whose rows lie along the lanes: row c, chunk g; chunk
+// 2t + g is at rows ^ 32 t.  `cols`, for the transposed read
+// (ds_read_b64_tr_b16) of 8 rows' columns 16 (G & 1) ..: columns 32 dt on are
+// at cols ^ 64 dt, the next 8 rows at (cols ^ 32) + 16 D.  A tile starts at a
+// multiple of 256 bytes, so its address can be added first and one XOR per
+// fragment remains; kept as registers, the offsets would be 16 for each array.
 template <int D>
 struct GradFrags {
-  int rows[D / 16], cols[D / 32];
+  uint32_t rows, cols;
   __device__ __forceinline__ GradFrags() {
     constexpr int CPR = D / 8;
     const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
     const int g16 = lane >> 4, s16 = lane & 15;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t)
-      rows[t] = c * D + (((2 * t + g) ^ grad_swizzle<CPR>(c)) * 8);
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) {
-      const int r = 4 * (g16 >> 1) + (s16 >> 2), col = dt * 32 + 16 * (g16 & 1) + 4 * (s16 & 3);
-      cols[dt] = r * D + (((col >> 3) ^ grad_swizzle<CPR>(r)) * 8) + (col & 7);
-    }
+    rows = (c * D + ((g ^ grad_swizzle<CPR>(c)) * 8)) * 2;
+    const int r = 4 * (g16 >> 1) + (s16 >> 2), col = 16 * (g16 & 1) + 4 * (s16 & 3);
+    cols = (r * D + (((col >> 3) ^ grad_swizzle<CPR>(r)) * 8) + (col & 7)) * 2;
   }
 };
-template <class M, int D>
-__device__ __forceinline__ typename M::frag grad_cols(const uint16_t* tile, int off) {
+typedef __attribute__((address_space(3))) const char lds_char;
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(lds_char*)p;
+}
+// Makes x a value that the compiler cannot compute ahead (the XORs of a
+// loop-invariant address would be hoisted, into registers that are not there).
+__device__ __forceinline__ void opaque(uint32_t& x) { asm volatile("" : "+v"(x)); }
+// Reads at an offset: in an array (while a DMA into another array is in
+// flight, which the compiler then need not wait for) or at a whole address.
+struct InTile {
+  lds_char* p;
+  __device__ __forceinline__ lds_char* operator()(uint32_t off) const { return p + off; }
+};
+struct Whole {
+  __device__ __forceinline__ lds_char* operator()(uint32_t at) const {
+    return (lds_char*)(uintptr_t)at;
+  }
+};
+template <class F, class At>
+__device__ __forceinline__ F grad_read(At at, uint32_t off) {
+  return *(__attribute__((address_space(3))) const F*)at(off);
+}
+template <class M, int D, class At>
+__device__ __forceinline__ typename M::frag grad_cols(At at, uint32_t off, uint32_t up, int plus) {
   union {
     v4s h[2];
     typename M::frag v;
   } f;
-  f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + off));
-  f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(tile + ((off ^ 16) + 8 * D)));
+  f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at(off) + plus));
+  f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at(up) + (plus + 16 * D)));
   return f.v;
 }
-// acc[dt] += (columns of 16 rows of `tile`)^T x the packed values of those rows
-template <class M, int D>
-__device__ __forceinline__ void grad_accumulate(f32x16_t (&acc)[D / 32], const uint16_t* tile,
-                                                const GradFrags<D>& fr, const uint32_t (&pk)[8]) {
+// acc[dt] += (columns of 32 rows of a tile)^T x the packed values of those
+// rows, for N tiles (addresses cols[i], values pk[i]) in turn; the fragments
+// are read four products ahead.
+template <class M, int D, int N, class At>
+__device__ __forceinline__ void grad_accumulate(f32x16_t (*const (&acc)[N])[D / 32],
+                                                At at, const uint32_t (&cols)[N],
+                                                const uint32_t (*const (&pk)[N])[8]) {
+  typedef typename M::frag frag;
+  constexpr int PER = 2 * (D / 32), ALL = N * PER, AHEAD = ALL < 4 ? ALL : 4;
+  frag p[N][2], f[AHEAD];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    union {
-      uint32_t w[4];
-      typename M::frag v;
-    } p;
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p.w[i] = pk[u * 4 + i];
+    for (int u = 0; u < 2; ++u) {
+      union {
+        uint32_t w[4];
+        frag v;
+      } x;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-      acc[dt] = M::mma(grad_cols<M, D>(tile + u * 16 * D, fr.cols[dt]), p.v, acc[dt]);
+      for (int i = 0; i < 4; ++i) x.w[i] = (*pk[n])[u * 4 + i];
+      p[n][u] = x.v;
+    }
+  auto read = [&](int i) {  // product i: tile i / PER, columns 32 dt, rows 16 u
+    const int n = i / PER, dt = i % PER / 2, u = i & 1;
+    f[i % AHEAD] =
+        grad_cols<M, D>(at, cols[n] ^ (64 * dt), cols[n] ^ (64 * dt + 32), u * 32 * D);
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) read(i);
+#pragma unroll
+  for (int i = 0; i < ALL; ++i) {
+    const int n = i / PER, dt = i % PER / 2, u = i & 1;
+    (*acc[n])[dt] = M::mma(f[i % AHEAD], p[n][u], (*acc[n])[dt]);
+    if (i + AHEAD < ALL) read(i + AHEAD);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < ALL; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i + AHEAD < ALL) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
 }
 
 // ---- dK, dV -----------------------------------------------------------------------------
+//
+// Eight waves over 128 keys in two groups of four; wave w of a group owns keys
+// 32 w .. + 31, and the groups take turns at the blocks of 32 rows.  Halving
+// the rows of each wave halves the longest workgroup, which is what a causal
+// batch waits for (the first keys of a long sequence are seen by all its
+// rows); the halves meet in LDS at the end.  dK and dV take half of the
+// registers, so K and V are read from LDS like the rows.
+//
+// Waves w of both groups share a SIMD and alternate between a phase of products
+// (dV and dK of their last block, S and dP of the next) and one of
+// exponentials, a barrier apart, so that each phase runs beside the other
+// group's other one; left to themselves both waves of a SIMD did the same at
+// the same time (39 % of the matrix core's cycles in use).  A group requests
+// its next block by DMA when a phase of exponentials begins, into the buffer
+// that its products have just finished with, and waits for it at that
+// phase's end.
 template <class M, int D>
-__global__ void __launch_bounds__(256, 1) grad_kv_kernel(PackedGradArgs a) {
+__global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
   using namespace pg;
   typedef typename M::frag frag;
-  constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, TILE = BT * D, RPD = 64 / CPR;
-  constexpr int NDMA = TILE / 512 / 4;
-  __shared__ __attribute__((aligned(1024))) uint16_t Qs[TILE], Ds[TILE];
-  __shared__ __attribute__((aligned(16))) float lse_s[BT], delta_s[BT];
-  __shared__ __attribute__((aligned(16))) int seen_s[BT];
+  constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, RPD = 64 / CPR;
+  constexpr int BLK = 32 * D;               // elements of 32 rows of Q (or dout)
+  constexpr int NDMA = 2 * BLK / 512 / 4;   // DMA instructions per wave and block
+  __shared__ __attribute__((aligned(1024))) uint16_t S[4 * 2 * BLK];  // [group][slot] Q, dout
+  __shared__ __attribute__((aligned(1024))) uint16_t Ks[BR * D];
+  // V, then the meeting of the row halves (32 KiB)
+  __shared__ __attribute__((aligned(1024))) uint16_t Vs[BR * D < 16384 ? 16384 : BR * D];
+  __shared__ __attribute__((aligned(256))) float R[4 * 64];  // [group][slot] -lse, -delta
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 31, g = lane >> 5;
-  const int G = a.H / a.Hkv, hk = blockIdx.x % a.Hkv;
-  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, 1, BR, blockIdx.x / a.Hkv);
+  const int c = lane & 31, g = lane >> 5, kw = wave & 3, grp = wave >> 2;
+  const int G = a.H / a.Hkv, hk = blockIdx.x % a.Hkv, rank = blockIdx.x / a.Hkv;
+  SeqTile st = a.n_seq <= kLevelSeqs ? rising_tile(a.starts, a.n_seq, (int)a.T, 1, BR, rank)
+                                     : find_tile(a.starts, a.n_seq, (int)a.T, 1, BR, rank);
   if (st.seq == -2) return;
+  // causal work falls with the key: the order of rising work runs backwards
+  if (a.n_seq <= kLevelSeqs) st.tile = (st.n - 1) / BR - st.tile;
   const int rows = st.real(a.n_seq) ? st.n * G : 0;
-  const int k0 = st.tile * BR, key = k0 + wave * 32 + c;  // this lane's key
+  const int k0 = st.tile * BR, wk = k0 + kw * 32, key = wk + c;  // this lane's key
   const int64_t kstride = (int64_t)a.Hkv * D;
-  frag kf[NT], vf[NT];
-  {
-    const int64_t at = (st.first + min(key, st.n - 1)) * kstride + hk * D;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      kf[t] = *(const frag*)((const uint16_t*)a.k + at + t * 16 + g * 8);
-      vf[t] = *(const frag*)((const uint16_t*)a.v + at + t * 16 + g * 8);
-    }
-  }
+  const DivBy by_g(G);
   const GradFrags<D> fr;
   const int row_in = lane / CPR, pc = lane % CPR;
+#pragma unroll
+  for (int i = 0; i < BR * D / 512 / 8; ++i) {
+    const int blk = wave + i * 8, lr = blk * RPD + row_in;
+    const int64_t at = (st.first + min(k0 + lr, st.n - 1)) * kstride + hk * D;
+    const int ch = (pc ^ grad_swizzle<CPR>(lr)) * 8;
+    dma16((const uint16_t*)a.k + at + ch, Ks + blk * 512);
+    dma16((const uint16_t*)a.v + at + ch, Vs + blk * 512);
+  }
   f32x16_t dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[dt][e] = dv[dt][e] = 0.0f;
   const float sl2 = a.scale * kLog2e;
-  const float* delta = (const float*)a.work;
-  const float F = grad_factor<M, D>(a), fs = F * exp2f(-M::kGradShift);
+  const float F = grad_factor<M, D, 512>(a), fs = F * exp2f(-M::kGradShift);
+  const int64_t base = (int64_t)st.first * a.H + hk * G;  // row (tok, hg): base + tok H + hg
+  const float* stats = (const float*)a.work;
   // causal: rows of tokens before the workgroup's first key do not see it
-  const int first_row = a.causal ? k0 * G / BT * BT : 0;
-  for (int r0 = first_row; r0 < rows; r0 += BT) {
-    __syncthreads();
+  const int r0 = a.causal ? k0 * G / 64 * 64 : 0;
+  const int n = (rows - r0 + 63) / 64;  // blocks of each group (the last may be empty)
+  auto row_of = [&](int m) { return r0 + (2 * m + grp) * 32; };
+  auto slot = [&](int m) { return grp * 2 + (m & 1); };
+
+  auto request = [&](int m) {
+    const int w0 = row_of(m);
+    uint16_t* s = S + slot(m) * 2 * BLK;
 #pragma unroll
-    for (int q = 0; q < NDMA; ++q) {
-      const int blk = wave * NDMA + q, lr = blk * RPD + row_in;
-      const int r = min(r0 + lr, rows - 1), t = r / G, hg = r - t * G;
-      const int64_t at = ((int64_t)(st.first + t) * a.H + hk * G + hg) * D +
-                         (pc ^ grad_swizzle<CPR>(lr)) * 8;
-      dma16((const uint16_t*)a.q + at, Qs + blk * 512);
-      dma16((const uint16_t*)a.dout + at, Ds + blk * 512);
+    for (int i = 0; i < NDMA; ++i) {
+      const int x = kw + i * 4, blk = x % (BLK / 512), lr = blk * RPD + row_in;
+      const bool q = x < BLK / 512;
+      int hg;
+      const int tok = by_g.div(min(w0 + lr, rows - 1), hg);
+      const int64_t at = (base + (int64_t)tok * a.H + hg) * D + (pc ^ grad_swizzle<CPR>(lr)) * 8;
+      dma16((const uint16_t*)(q ? a.q : a.dout) + at, s + x * 512);
     }
-    if (threadIdx.x < BT) {
-      const int r = r0 + threadIdx.x, rr = min(r, rows - 1), t = rr / G;
-      const int64_t at = (int64_t)(st.first + t) * a.H + hk * G + rr - t * G;
-      lse_s[threadIdx.x] = a.lse[at] * kLog2e - M::kGradShift;
-      delta_s[threadIdx.x] = delta[at];
-      // keys below it are seen by this row; a row past the last one sees none
-      seen_s[threadIdx.x] = r >= rows ? 0 : a.causal ? t + 1 : st.n;
+    if (kw == 0) {  // lanes 0..31: -lse, 32..63: -delta
+      int hg;
+      const int tok = by_g.div(min(w0 + c, rows - 1), hg);
+      const float* src = stats + (g ? a.T * a.H : 0) + base + (int64_t)tok * a.H + hg;
+      __builtin_amdgcn_global_load_lds(src, (lds_void*)(R + slot(m) * 64), 4, 0, 0);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const bool all = r0 + BT <= rows && (!a.causal || r0 / G >= k0 + BR - 1);
+  };
+  // whether any row of block m sees any of this wave's keys (row r sees key j
+  // from r = j G on, if causal)
+  auto live = [&](int m) {
+    const int w0 = row_of(m);
+    return w0 < rows && (!a.causal || w0 + 31 >= wk * G);
+  };
+  f32x16_t x, dp;
+  float4 l4[4];
+  uint32_t pp[8], pd[8];
+  auto scores = [&](int m) {
+    if (!live(m)) return;
+    const uint16_t* Qt = S + slot(m) * 2 * BLK;
+    const float* rt = R + slot(m) * 64 + g * 4;
 #pragma unroll
-    for (int h = 0; h < BT / 32; ++h) {
-      const uint16_t *Qt = Qs + h * 32 * D, *Dt = Ds + h * 32 * D;
-      f32x16_t s, dp;
+    for (int e4 = 0; e4 < 4; ++e4) {
+      l4[e4] = *(const float4*)(rt + e4 * 8);
+      const float4 d4 = *(const float4*)(rt + 32 + e4 * 8);
+      const float d[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        s = M::mma(*(const frag*)(Qt + fr.rows[t]), kf[t], s);
-        dp = M::mma(*(const frag*)(Dt + fr.rows[t]), vf[t], dp);
+      for (int i = 0; i < 4; ++i) {
+        x[e4 * 4 + i] = 0.0f;
+        dp[e4 * 4 + i] = d[i];
       }
-      uint32_t pp[8], pd[8];
+    }
+    // Q, dout, K and V fragments are read two k-steps ahead (three: six registers
+    // too many, and a spill's reload costs half of the phase)
+    constexpr int AHEAD = 2;
+    uint32_t qa = lds_at(Qt) + fr.rows, ka = lds_at(Ks) + kw * BLK * 2 + fr.rows,
+             va = lds_at(Vs) + kw * BLK * 2 + fr.rows;
+    opaque(ka);
+    opaque(va);
+    frag f[AHEAD][4];
+    auto read = [&](int t) {
+      f[t % AHEAD][0] = grad_read<frag>(Whole(), qa ^ (32 * t));
+      f[t % AHEAD][1] = grad_read<frag>(Whole(), ka ^ (32 * t));
+      f[t % AHEAD][2] = grad_read<frag>(Whole(), (qa ^ (32 * t)) + BLK * 2);
+      f[t % AHEAD][3] = grad_read<frag>(Whole(), va ^ (32 * t));
+    };
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) read(t);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      x = M::mma(f[t % AHEAD][0], f[t % AHEAD][1], x);
+      dp = M::mma(f[t % AHEAD][2], f[t % AHEAD][3], dp);
+      if (t + AHEAD < NT) read(t + AHEAD);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 8 + 4 * AHEAD, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      if (t + AHEAD < NT) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    }
+  };
+  auto values = [&](int m) {
+    if (!live(m)) return;
+    const int w0 = row_of(m);
+    // rows of the block that see this lane's key: span of them from lo
+    const int lo = a.causal ? key * G - w0 - g * 4 : -64;
+    const uint32_t span = (uint32_t)max(rows - w0 - g * 4 - lo, 0);
+    auto go = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
-        const int lr = h * 32 + e4 * 8 + g * 4;
-        const float4 l4 = *(const float4*)(lse_s + lr), d4 = *(const float4*)(delta_s + lr);
-        const int4 t4 = *(const int4*)(seen_s + lr);
-        const float l[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
-        const int seen[4] = {t4.x, t4.y, t4.z, t4.w};
+        const float l[4] = {l4[e4].x, l4[e4].y, l4[e4].z, l4[e4].w};
         float p[4], ds[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = e4 * 4 + i;
-          const bool see = all || key < seen[i];
-          const float x = fa_exp2(fmaf(s[e], sl2, -l[i]));
-          float y = x * (dp[e] - dl[i]);
-          if constexpr (M::kScaled) y *= fs;
-          p[i] = see ? x : 0.0f;
-          ds[i] = see ? y : 0.0f;
+          if constexpr (masked) {  // (selects of the inputs: no branches)
+            const bool see = (uint32_t)(e4 * 8 + i - lo) < span;
+            x[e] = see ? x[e] : -INFINITY;
+            dp[e] = see ? dp[e] : 0.0f;
+          }
+          p[i] = fa_exp2(fmaf(x[e], sl2, l[i]));
+          ds[i] = p[i] * dp[e];
+          if constexpr (M::kScaled) ds[i] *= fs;
         }
         pp[e4 * 2] = M::pack(p[0], p[1]);
         pp[e4 * 2 + 1] = M::pack(p[2], p[3]);
         pd[e4 * 2] = M::pack(ds[0], ds[1]);
         pd[e4 * 2 + 1] = M::pack(ds[2], ds[3]);
       }
-      grad_accumulate<M, D>(dv, Dt, fr, pp);
-      grad_accumulate<M, D>(dk, Qt, fr, pd);
+    };
+    if (w0 + 32 <= rows && (!a.causal || w0 >= (wk + 31) * G)) go(std::false_type());
+    else go(std::true_type());
+  };
+  auto accumulate = [&](int m) {
+    if (!live(m)) return;
+    const uint32_t at = lds_at(S + slot(m) * 2 * BLK) + fr.cols;
+    grad_accumulate<M, D, 2>({&dv, &dk}, Whole(), {at + BLK * 2, at}, {&pp, &pd});
+  };
+  auto vm_wait = []() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+
+  // half-step   0     1     2           3           ...  2n - 1    2n
+  // group 0     S 0   exp 0 dKV 0, S 1  exp 1            exp n-1   dKV n-1
+  // group 1     -     S 0   exp 0       dKV 0, S 1       ..        exp n-1, dKV n-1
+  if (n > 0) {
+    request(0);
+    vm_wait();
+    block_barrier_fa();
+    if (grp == 1) block_barrier_fa();
+    __builtin_amdgcn_s_setprio(1);
+    scores(0);
+    block_barrier_fa();
+    for (int m = 1; m < n; ++m) {
+      __builtin_amdgcn_s_setprio(0);
+      request(m);
+      values(m - 1);
+      vm_wait();
+      block_barrier_fa();
+      __builtin_amdgcn_s_setprio(1);
+      accumulate(m - 1);
+      scores(m);
+      block_barrier_fa();
     }
+    __builtin_amdgcn_s_setprio(0);
+    values(n - 1);
+    if (grp == 0) block_barrier_fa();
+    accumulate(n - 1);
   }
-  if (key >= st.n) return;
-  const int64_t at = (st.first + key) * kstride + hk * D;
-  uint16_t *DK = (uint16_t*)a.dk + at, *DV = (uint16_t*)a.dv + at;
-  const float sv = exp2f(-M::kGradShift), sk = a.scale / F;
+  // the two row halves meet: wave w keeps dK and takes the other's, wave w + 4
+  // likewise dV
+  typedef float f32x4_t __attribute__((ext_vector_type(4)));
+  f32x4_t* X = (f32x4_t*)Vs;  // [8 waves][4][64 lanes]
+  vm_wait();  // (V's own DMA, where there were no rows)
+  auto meet = [&](f32x16_t(&mine)[DT], f32x16_t(&other)[DT], void* to, float m) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt) {
+      __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = dt * 32 + r * 8 + g * 4;
-      *(uint2*)(DK + d) = make_uint2(M::pack(dk[dt][r * 4] * sk, dk[dt][r * 4 + 1] * sk),
-                                     M::pack(dk[dt][r * 4 + 2] * sk, dk[dt][r * 4 + 3] * sk));
-      *(uint2*)(DV + d) = make_uint2(M::pack(dv[dt][r * 4] * sv, dv[dt][r * 4 + 1] * sv),
-                                     M::pack(dv[dt][r * 4 + 2] * sv, dv[dt][r * 4 + 3] * sv));
+      for (int i = 0; i < 4; ++i)
+        X[(wave * 4 + i) * 64 + lane] = (f32x4_t){other[dt][i * 4], other[dt][i * 4 + 1],
+                                                  other[dt][i * 4 + 2], other[dt][i * 4 + 3]};
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_t v = X[((wave ^ 4) * 4 + i) * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[dt][i * 4 + j] += v[j];
+      }
     }
+    if (key >= st.n) return;
+    uint16_t* out = (uint16_t*)to + (st.first + key) * kstride + hk * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *(uint2*)(out + dt * 32 + r * 8 + g * 4) =
+            make_uint2(M::pack(mine[dt][r * 4] * m, mine[dt][r * 4 + 1] * m),
+                       M::pack(mine[dt][r * 4 + 2] * m, mine[dt][r * 4 + 3] * m));
+  };
+  // (both branches pass the same barriers)
+  if (grp == 0) meet(dk, dv, a.dk, a.scale / F);
+  else meet(dv, dk, a.dv, exp2f(-M::kGradShift));
 }
 
 // ---- dQ -----------------------------------------------------------------------------------
+//
+// Four waves of 32 rows, as in the forward kernel: Q and dout of a row in
+// registers, K and V tiles of 64 keys by DMA, one ahead, lse and delta of the
+// row one value per lane.
 template <class M, int D>
 __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   using namespace pg;
   typedef typename M::frag frag;
   constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, TILE = BT * D, RPD = 64 / CPR;
   constexpr int NDMA = TILE / 512 / 4;
-  __shared__ __attribute__((aligned(1024))) uint16_t Ks[TILE], Vs[TILE];
+  __shared__ __attribute__((aligned(1024))) uint16_t K0[TILE], K1[TILE], V0[TILE], V1[TILE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, g = lane >> 5;
-  const int G = a.H / a.Hkv, hk = blockIdx.x % a.Hkv;
-  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv);
+  const int G = a.H / a.Hkv, hk = blockIdx.x % a.Hkv, rank = blockIdx.x / a.Hkv;
+  const SeqTile st = a.n_seq <= kLevelSeqs
+                         ? rising_tile(a.starts, a.n_seq, (int)a.T, G, BR, rank)
+                         : find_tile(a.starts, a.n_seq, (int)a.T, G, BR, rank);
   if (st.seq == -2) return;
   const int rows = st.n * G, keys = st.real(a.n_seq) ? st.n : 0;
   const int r0 = st.tile * BR + wave * 32, row = r0 + c;
@@ -314,8 +497,8 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     df[t] = *(const frag*)((const uint16_t*)a.dout + at * D + t * 16 + g * 8);
   }
   const float sl2 = a.scale * kLog2e;
-  const float F = grad_factor<M, D>(a), fs = F * exp2f(-M::kGradShift);
-  const float l = a.lse[at] * kLog2e - M::kGradShift, dl = ((const float*)a.work)[at];
+  const float F = grad_factor<M, D, 256>(a), fs = F * exp2f(-M::kGradShift);
+  const float l = ((const float*)a.work)[at], dl = ((const float*)a.work)[a.T * a.H + at];
   const GradFrags<D> fr;
   const int row_in = lane / CPR, pc = lane % CPR;
   const int64_t kstride = (int64_t)a.Hkv * D, kbase = (st.first * (int64_t)a.Hkv + hk) * D;
@@ -327,48 +510,84 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     const int lr = (wave * NDMA + q) * RPD + row_in;
     src[q] = (uint32_t)((lr * kstride + (pc ^ grad_swizzle<CPR>(lr)) * 8) * 2);
   }
+  auto dma_tile = [&](uint16_t* ks, uint16_t* vs) {
+    const __amdgpu_buffer_rsrc_t rk = kr.next(), rv = vr.next();
+#pragma unroll
+    for (int q = 0; q < NDMA; ++q) {
+      const int blk = wave * NDMA + q;
+      dma16_buf(rk, src[q], 0, ks + blk * 512);
+      dma16_buf(rv, src[q], 0, vs + blk * 512);
+    }
+  };
   f32x16_t dq[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[dt][e] = 0.0f;
-  for (int kt = 0; kt < nkt; ++kt) {
-    __syncthreads();
-    const __amdgpu_buffer_rsrc_t rk = kr.next(), rv = vr.next();
+  auto tile = [&](const uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n, int kt) {
+    if (kt + 1 < nkt) dma_tile(ks_n, vs_n);
 #pragma unroll
-    for (int q = 0; q < NDMA; ++q) {
-      const int blk = wave * NDMA + q;
-      dma16_buf(rk, src[q], 0, Ks + blk * 512);
-      dma16_buf(rv, src[q], 0, Vs + blk * 512);
+    for (int h = 0; h < BT / 32; ++h) {
+      const InTile Kt{(lds_char*)(ks + h * 32 * D)}, Vt{(lds_char*)(vs + h * 32 * D)};
+      uint32_t rows_at = fr.rows, cols_at = fr.cols;
+      opaque(rows_at);
+      opaque(cols_at);
+      f32x16_t s, dp;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = 0.0f;
+        dp[e] = dl;
+      }
+      constexpr int AHEAD = NT < 3 ? NT : 3;
+      frag f[AHEAD][2];
+      auto read = [&](int t) {
+        f[t % AHEAD][0] = grad_read<frag>(Kt, rows_at ^ (32 * t));
+        f[t % AHEAD][1] = grad_read<frag>(Vt, rows_at ^ (32 * t));
+      };
+#pragma unroll
+      for (int t = 0; t < AHEAD; ++t) read(t);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        s = M::mma(f[t % AHEAD][0], qf[t], s);
+        dp = M::mma(f[t % AHEAD][1], df[t], dp);
+        if (t + AHEAD < NT) read(t + AHEAD);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        if (t + AHEAD < NT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      uint32_t pd[8];
+      auto values = [&](auto masked) __attribute__((always_inline)) {
+        const int seen = my_limit - kt * BT - h * 32 - g * 4;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const int off = (e >> 2) * 8 + (e & 3);
+          float y[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            y[i] = fa_exp2(fmaf(s[e + i], sl2, l)) * dp[e + i];
+            if constexpr (M::kScaled) y[i] *= fs;
+            if constexpr (masked) y[i] = off + i < seen ? y[i] : 0.0f;
+          }
+          pd[e >> 1] = M::pack(y[0], y[1]);
+        }
+      };
+      if (kt * BT + BT <= least) values(std::false_type());
+      else values(std::true_type());
+      grad_accumulate<M, D, 1>({&dq}, Kt, {cols_at}, {&pd});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const bool all = kt * BT + BT <= least;
-#pragma unroll
-    for (int h = 0; h < BT / 32; ++h) {
-      const uint16_t *Kt = Ks + h * 32 * D, *Vt = Vs + h * 32 * D;
-      const int seen = my_limit - kt * BT - h * 32 - g * 4;
-      f32x16_t s, dp;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        s = M::mma(*(const frag*)(Kt + fr.rows[t]), qf[t], s);
-        dp = M::mma(*(const frag*)(Vt + fr.rows[t]), df[t], dp);
-      }
-      uint32_t pd[8];
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const int off = (e >> 2) * 8 + (e & 3);
-        float y0 = fa_exp2(fmaf(s[e], sl2, -l)) * (dp[e] - dl);
-        float y1 = fa_exp2(fmaf(s[e + 1], sl2, -l)) * (dp[e + 1] - dl);
-        if constexpr (M::kScaled) {
-          y0 *= fs;
-          y1 *= fs;
-        }
-        pd[e >> 1] = M::pack(all || off < seen ? y0 : 0.0f, all || off + 1 < seen ? y1 : 0.0f);
-      }
-      grad_accumulate<M, D>(dq, Kt, fr, pd);
+  };
+  if (nkt > 0) {
+    dma_tile(K0, V0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int kt = 0; kt < nkt; kt += 2) {
+      tile(K0, V0, K1, V1, kt);
+      if (kt + 1 < nkt) tile(K1, V1, K0, V0, kt + 1);
     }
   }
   if (row >= rows) return;
@@ -383,9 +602,9 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
                      M::pack(dq[dt][r * 4 + 2] * sq, dq[dt][r * 4 + 3] * sq));
 }
 
-// delta, then two maxima for each workgroup of the delta kernel
+// two values per row, then two maxima for each workgroup of the first kernel
 size_t packed_grad_ws_bytes(int64_t T, int H) {
-  return (size_t)(T * H + 2 * pg::kDeltaBlocks) * 4;
+  return (size_t)(2 * T * H + 2 * pg::kDeltaBlocks) * 4;
 }
 
 template <class M, int D>
@@ -397,7 +616,7 @@ static void launch_grad(PackedGradArgs a, hipStream_t stream) {
     fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention gradient: too many tiles");
   hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)a.delta_blocks), dim3(256), 0,
                      stream, a);
-  hipLaunchKernelGGL((grad_kv_kernel<M, D>), dim3((unsigned)kv), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((grad_kv_kernel<M, D>), dim3((unsigned)kv), dim3(512), 0, stream, a);
   hipLaunchKernelGGL((grad_q_kernel<M, D>), dim3((unsigned)q), dim3(256), 0, stream, a);
 }
 template <class M>
