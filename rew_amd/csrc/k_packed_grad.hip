@@ -1,7 +1,9 @@
 // The gradients of packed attention (PackedGradArgs in kernels.h), without
 // anything of size rows x keys in memory.
 //
-// Three launches.  The first writes delta = dout . out per row.  The second
+// Three launches.  The first writes delta = dout . out per row, from out and
+// what its rounding left (out alone would put out's rounding into every dS,
+// next to dS's own).  The second
 // gives each workgroup 128 keys of one KV head and walks the rows that see
 // them, dK and dV staying in registers; the third gives each workgroup 128
 // rows and walks their keys, dQ staying in registers.  Both recompute
@@ -56,17 +58,27 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   float most = 0.0f, most_v = 0.0f;
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-    float s = 0.0f;
+    const uint2 z = ((const uint2*)a.rest)[i * L + ch];
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[2] = {z.x, z.y};
+    float s = 0.0f, rest = 0.0f, row = 0.0f;  // dout . out, dout . rest, max |out|
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float y0 = M::lo(ys[k]), y1 = M::hi(ys[k]);
-      s = fmaf(M::lo(xs[k]), y0, s);
-      s = fmaf(M::hi(xs[k]), y1, s);
+      const float y0 = M::lo(ys[k]), y1 = M::hi(ys[k]), x0 = M::lo(xs[k]), x1 = M::hi(xs[k]);
+      s = fmaf(x0, y0, s);
+      s = fmaf(x1, y1, s);
+      const int sh = (k & 1) * 16;
+      rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
+      rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
+      row = fmaxf(row, fmaxf(fabsf(x0), fabsf(x1)));
       if constexpr (M::kScaled) most = fmaxf(most, fmaxf(fabsf(y0), fabsf(y1)));
     }
 #pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    for (int d = L / 2; d > 0; d >>= 1) {
+      s += __shfl_xor(s, d);
+      rest += __shfl_xor(rest, d);
+      row = fmaxf(row, __shfl_xor(row, d));
+    }
+    s = fmaf(rest, row * M::kRestStep, s);
     if (ch == 0) {
       neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
       neg_delta[i] = -s;

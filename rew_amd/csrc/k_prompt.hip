@@ -280,13 +280,40 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   const int64_t at = (int64_t)(st.first + tok) * a.H + hk * G + hg;
   if (a.lse && g == 0) a.lse[at] = (m_run - M::kShift + __log2f(l)) * kLn2;
   uint16_t* O = (uint16_t*)a.out + at * D;
+  float most = 0.0f;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      *(uint2*)(O + dt * 32 + r * 8 + g * 4) =
-          make_uint2(M::pack(o[dt][r * 4] * inv, o[dt][r * 4 + 1] * inv),
-                     M::pack(o[dt][r * 4 + 2] * inv, o[dt][r * 4 + 3] * inv));
+    for (int r = 0; r < 4; ++r) {
+      float* x = (float*)&o[dt] + r * 4;
+      const uint2 w = make_uint2(M::pack(x[0] * inv, x[1] * inv), M::pack(x[2] * inv, x[3] * inv));
+      *(uint2*)(O + dt * 32 + r * 8 + g * 4) = w;
+      if (a.rest) {  // (uniform)
+        const float y[4] = {M::lo(w.x), M::hi(w.x), M::lo(w.y), M::hi(w.y)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          most = fmaxf(most, fabsf(y[i]));
+          x[i] = fmaf(x[i], inv, -y[i]);
+        }
+      }
+    }
+  if (!a.rest) return;
+  // (lanes of a row, l and l ^ 32, are both here)
+  most = fa_max_halves(most);
+  const float per_step = most > 0.0f ? 1.0f / (most * M::kRestStep) : 0.0f;
+  int8_t* rest = a.rest + at * D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float q = rintf(fminf(fmaxf(o[dt][r * 4 + i] * per_step, -127.0f), 127.0f));
+        w |= ((uint32_t)(int)q & 255u) << (8 * i);
+      }
+      *(uint32_t*)(rest + dt * 32 + r * 8 + g * 4) = w;
+    }
 }
 
 template <class M, int D>

@@ -559,11 +559,14 @@ const char* flash_variant(const FlashArgs& a);
 // h / (H / Hkv)):
 //   lse = log sum_j exp(s_j)   (f32 [T, H]; -inf without keys)
 //   out = sum_j exp(s_j - lse) v_j   (0 without keys)
-// A row of no sequence has no keys.
+// A row of no sequence has no keys.  Of a row, out + rest rest_step, with
+// rest_step = h m / 127, m the row's largest |out| and h half a step of the
+// dtype relative to a value, has out's value 100 times as exactly as out.
 struct PackedArgs {
   const void *q, *k, *v;
   void* out;
-  float* lse;  // null: not stored
+  float* lse;      // with rest, or both null
+  int8_t* rest;    // [T, H, D]: what rounding took from out, in steps of rest_step
   const int32_t *starts, *table, *lens;
   int64_t T, pages;
   int n_seq, H, Hkv, D, width, log_page, f16, causal;
@@ -574,13 +577,14 @@ void launch_packed_attn(const PackedArgs& a, hipStream_t stream);
 const char* packed_attn_variant(const PackedArgs& a);
 
 // The gradients of packed attention for the gradient `dout` of out: with
-// p_j = exp(s_j - lse), delta = dout . out and ds_j = p_j (dout . v_j - delta)
+// p_j = exp(s_j - lse), delta = dout . (out + rest rest_step) and ds_j = p_j (dout . v_j - delta)
 //   dq = scale sum_j ds_j k_j;  dk_j = scale sum ds_j q, dv_j = sum p_j dout,
 // the last two over the rows that see j and the H / Hkv heads that read it.
 // Rows of no sequence get zeros.  work: packed_grad_ws_bytes.
 struct PackedGradArgs {
   const void *q, *k, *v, *out, *dout;
   const float* lse;
+  const int8_t* rest;
   const int32_t* starts;
   void *dq, *dk, *dv, *work;
   int64_t T;

@@ -3501,7 +3501,10 @@ void Lower::emit_packed_attn(Node* n) {
     a.width = (int)table->shape.d[1];
     while ((1ll << a.log_page) < k->shape.d[2]) a.log_page++;
   } else {
-    a.lse = (float*)n->out[1]->data();
+    if (n->out.size() > 1) {
+      a.lse = (float*)n->out[1]->data();
+      a.rest = (int8_t*)n->out[2]->data();
+    }
     a.starts = (const int32_t*)n->in[3]->data();
     a.n_seq = (int)n->in[3]->shape.d[0] - 1;
   }
@@ -3523,7 +3526,8 @@ void Lower::emit_packed_grad(Node* n) {
   a.n_seq = (int)n->in[3]->shape.d[0] - 1;
   a.out = n->in[4]->data();
   a.lse = (const float*)n->in[5]->data();
-  a.dout = n->in[6]->data();
+  a.rest = (const int8_t*)n->in[6]->data();
+  a.dout = n->in[7]->data();
   a.dq = n->out[0]->data();
   a.dk = n->out[1]->data();
   a.dv = n->out[2]->data();

@@ -332,7 +332,8 @@ static void check_heads(const Tensor* q, int dt, int64_t hkv, int64_t d, const s
 
 using OutSpecs = std::vector<std::pair<int, Shape>>;
 
-// packedAttention(q, k, v, starts): attrs causal, scale; out, lse.
+// packedAttention(q, k, v, starts): attrs causal, scale, stats; out and, with
+// stats, lse and rest.
 static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*>& ins,
                                 const Attrs& attrs, Node* n, OutSpecs& outs) {
   Tensor *q = ins[0], *k = ins[1], *v = ins[2];
@@ -350,11 +351,14 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
   std::memcpy(&n->i1, &scale, sizeof scale);
   if (n->kind == K_PACKED_ATTN) {
     outs.push_back({q->dt, q->shape});
-    outs.push_back({kF32, Shape(std::vector<int64_t>{q->shape.d[0], q->shape.d[1]})});
+    if (flag_attr(attrs, "stats", op)) {
+      outs.push_back({kF32, Shape(std::vector<int64_t>{q->shape.d[0], q->shape.d[1]})});
+      outs.push_back({kI8, q->shape});
+    }
     return;
   }
-  // packedAttentionGrad(q, k, v, starts, out, lse, gradOut): the gradients of q, k, v
-  Tensor *o = ins[4], *lse = ins[5], *go = ins[6];
+  // packedAttentionGrad(q, k, v, starts, out, lse, rest, gradOut): the gradients of q, k, v
+  Tensor *o = ins[4], *lse = ins[5], *rest = ins[6], *go = ins[7];
   if (o->dt != q->dt || o->shape != q->shape)
     invalid("eager '" + op + "': out must have q's dtype and shape");
   if (go->dt != q->dt || go->shape != q->shape)
@@ -362,6 +366,8 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
   if (lse->dt != kF32 || lse->shape.rank != 2 || lse->shape.d[0] != q->shape.d[0] ||
       lse->shape.d[1] != q->shape.d[1])
     invalid("eager '" + op + "': lse must be float32 [tokens, heads]");
+  if (rest->dt != kI8 || rest->shape != q->shape)
+    invalid("eager '" + op + "': rest must be int8 of q's shape");
   n->tail = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1]);
   outs.push_back({q->dt, q->shape});
   outs.push_back({k->dt, k->shape});
@@ -1083,7 +1089,7 @@ Node* prepare_node(Ctx* c, const std::string& op, const std::vector<Tensor*>& in
         else prepare_packed_attn(op, ins, attrs, n, outs);
         break;
       case K_PACKED_GRAD:
-        nin(7);
+        nin(8);
         prepare_packed_attn(op, ins, attrs, n, outs);
         break;
       case K_PAGE_TABLES:

@@ -163,11 +163,13 @@ struct PtrVisit {
     for (const void** p : {&a.q, &a.k, &a.v}) field(f, *p);
     field(f, a.out);
     field(f, a.lse);
+    field(f, a.rest);
     for (const int32_t** p : {&a.starts, &a.table, &a.lens}) field(f, *p);
   }
   void operator()(PackedGradArgs& a) {
     for (const void** p : {&a.q, &a.k, &a.v, &a.out, &a.dout}) field(f, *p);
     field(f, a.lse);
+    field(f, a.rest);
     field(f, a.starts);
     for (void** p : {&a.dq, &a.dk, &a.dv, &a.work}) field(f, *p);
   }

@@ -12,7 +12,7 @@ format, so the native backend sees exactly what rew would send it:
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 
@@ -829,6 +829,14 @@ def _attn_attrs(op: str, causal: bool, scale: float) -> list:
             ("scale", repr(float(np.float32(scale))))]
 
 
+class PackedStats(NamedTuple):
+    """What ``packedAttention`` leaves for its gradient, beside its result."""
+    lse: Tensor   # float32 [tokens, heads]: log of the row's sum of exponentials, -inf for
+                  # a row of no sequence
+    rest: Tensor  # int8 [tokens, heads, headDim]: what rounding took from the result, in
+                  # 1/127 of half a step (bfloat16 2^-8, float16 2^-11) of the row's largest
+
+
 def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: bool = True,
                     scale: float = 0.0, withLse: bool = False):
     """softmax(scale q k^T) v within each of the packed sequences.
@@ -841,27 +849,31 @@ def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: boo
     rounded to the operands' dtype before the second product, the result once.  A row of no
     sequence (before ``starts[0]``, behind ``starts[-1]``) gives zeros.
 
-    ``withLse``: (out, lse), lse float32 [tokens, heads] the log of the row's sum of
-    exponentials (-inf for a row of no sequence), which ``packedAttentionGrad`` takes."""
+    ``withLse``: (out, stats), the ``PackedStats`` that ``packedAttentionGrad`` takes."""
     _check_packed("packedAttention", q, k, v, starts)
-    out, lse = _packed_call("packedAttention", [q, k, v, starts],
-                            _attn_attrs("packedAttention", causal, scale), 2)
-    return (out, lse) if withLse else out
+    attrs = _attn_attrs("packedAttention", causal, scale)
+    attrs.append(("stats", "true" if withLse else "false"))
+    res = _packed_call("packedAttention", [q, k, v, starts], attrs, 3 if withLse else 1)
+    return (res[0], PackedStats(res[1], res[2])) if withLse else res[0]
 
 
 def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Tensor,
-                        lse: Tensor, gradOut: Tensor, causal: bool = True, scale: float = 0.0):
+                        stats: PackedStats, gradOut: Tensor, causal: bool = True,
+                        scale: float = 0.0):
     """(gradQ, gradK, gradV) of ``packedAttention(q, k, v, starts, causal, scale)`` for the
-    gradient ``gradOut`` of its result, given its ``out`` and ``lse``.  gradK and gradV are
+    gradient ``gradOut`` of its result, given its ``out`` and ``stats``.  gradK and gradV are
     summed over the query heads of each KV head; sums are float32 in a fixed order."""
     op = "packedAttentionGrad"
     _check_packed(op, q, k, v, starts)
     for t, name in ((out, "out"), (gradOut, "gradOut")):
         if t.dtype != q.dtype or t.shape != q.shape:
             raise TensorError(f"{op}: {name} must have q's dtype and shape")
+    lse, rest = stats
     if lse.dtype != DType.FLOAT32 or lse.shape != q.shape[:2]:
         raise TensorError(f"{op}: lse must be float32 [tokens, heads]")
-    return tuple(_packed_call(op, [q, k, v, starts, out, lse, gradOut],
+    if rest.dtype != DType.INT8 or rest.shape != q.shape:
+        raise TensorError(f"{op}: rest must be int8 of q's shape")
+    return tuple(_packed_call(op, [q, k, v, starts, out, lse, rest, gradOut],
                               _attn_attrs(op, causal, scale), 3))
 
 

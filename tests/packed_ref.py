@@ -78,10 +78,12 @@ def packed_grad(q, k, v, starts, do, causal, scale, dtype):
         dp = np.matmul(dh, vh.transpose(0, 2, 1))
         delta = (dh * oh).sum(2, keepdims=True)
         ds = p * (dp - delta)
-        # dS: one rounding, the rounding of out inside delta, float32 sums
+        # dS: one rounding, half a step of the rest that delta adds to out (of the row's
+        # largest value), float32 sums
         mag_dp = np.matmul(np.abs(dh), np.abs(vh).transpose(0, 2, 1))
         mag_delta = (np.abs(dh) * np.abs(oh)).sum(2, keepdims=True)
-        e_ds = h * np.abs(ds) + p * (h * mag_delta + F32 * (mag_dp + mag_delta))
+        e_rest = h / 254 * np.abs(dh).sum(2, keepdims=True) * np.abs(oh).max(2, keepdims=True)
+        e_ds = h * np.abs(ds) + p * (1.1 * e_rest + F32 * (mag_dp + mag_delta))
         e_p = (h + F32) * p
 
         def group(x):  # [H, n, D] -> [n, Hkv, D], summed over each group

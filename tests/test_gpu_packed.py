@@ -52,9 +52,17 @@ def test_packed_attention(gpu, lens, H, Hkv, D, dtype, causal):
     r = np.random.default_rng(sum(lens) + H + D)
     starts = np.concatenate([[0], np.cumsum(lens)])
     (q, qh), (k, kh), (v, vh) = make(r, starts[-1], H, Hkv, D, dtype)
-    out, lse = O.packedAttention(q, k, v, ints(starts), causal=causal, withLse=True)
+    out, (lse, rest) = O.packedAttention(q, k, v, ints(starts), causal=causal, withLse=True)
     want, wl, mag = R.packed(qh, kh, vh, starts, causal, D ** -0.5)
     check(out, want, R.out_bound(want, mag, dtype))
+    np.testing.assert_array_equal(
+        E.toHost(out), E.toHost(O.packedAttention(q, k, v, ints(starts), causal=causal)))
+    # out with its rest: half a step of the rest in place of the output's rounding
+    got = E.toHostF32(out).astype(np.float64)
+    step = np.abs(got).max(2, keepdims=True) * R.HALF[dtype] / 127
+    # (a float16 below 2^-14 is rounded by more than 2^-11 of itself: 2^-25)
+    got += E.toHost(rest) * step
+    assert (np.abs(got - want) <= (R.HALF[dtype] + R.F32) * mag + step + 2.0 ** -25).all()
     # no rounding to the dtype in it: the scores' and the sum's float32
     check(lse, wl, R.F32 + 1e-6 * np.abs(wl))
 
@@ -64,12 +72,12 @@ def test_packed_rows_of_no_sequence_are_zero(gpu):
     starts = np.array([7, 40, 40, 171])
     (q, qh), (k, kh), (v, vh) = make(r, 300, 4, 2, 64, "bfloat16")
     (g, gh) = tensor(r.standard_normal((300, 4, 64)), "bfloat16")
-    out, lse = O.packedAttention(q, k, v, ints(starts), withLse=True)
+    out, stats = O.packedAttention(q, k, v, ints(starts), withLse=True)
     want, wl, mag = R.packed(qh, kh, vh, starts, True, 0.125)
     check(out, want, R.out_bound(want, mag, "bfloat16"))
-    np.testing.assert_array_equal(np.isneginf(E.toHost(lse)), np.isneginf(wl))
+    np.testing.assert_array_equal(np.isneginf(E.toHost(stats.lse)), np.isneginf(wl))
     res, bnd = R.packed_grad(qh, kh, vh, starts, gh, True, 0.125, "bfloat16")
-    for t, w, b in zip(O.packedAttentionGrad(q, k, v, ints(starts), out, lse, g), res, bnd):
+    for t, w, b in zip(O.packedAttentionGrad(q, k, v, ints(starts), out, stats, g), res, bnd):
         check(t, w, b)
         assert not E.toHostF32(t)[:7].any() and not E.toHostF32(t)[171:].any()
 
@@ -77,18 +85,18 @@ def test_packed_rows_of_no_sequence_are_zero(gpu):
 @pytest.mark.parametrize("starts", [[0], [0, 0], [5, 5]])
 def test_packed_without_tokens_in_sequences(gpu, starts):
     (q, _), (k, _), (v, _) = make(np.random.default_rng(1), 9, 2, 1, 32, "float16")
-    out, lse = O.packedAttention(q, k, v, ints(starts), withLse=True)
-    assert not E.toHostF32(out).any() and np.isneginf(E.toHost(lse)).all()
-    for t in O.packedAttentionGrad(q, k, v, ints(starts), out, lse, q):
+    out, stats = O.packedAttention(q, k, v, ints(starts), withLse=True)
+    assert not E.toHostF32(out).any() and np.isneginf(E.toHost(stats.lse)).all()
+    for t in O.packedAttentionGrad(q, k, v, ints(starts), out, stats, q):
         assert not E.toHostF32(t).any()
 
 
 def test_packed_no_tokens(gpu):
     q = E.empty(DType.BFLOAT16, (0, 4, 64))
     k = E.empty(DType.BFLOAT16, (0, 2, 64))
-    out, lse = O.packedAttention(q, k, k, ints([0]), withLse=True)
-    assert out.shape == (0, 4, 64) and E.toHost(lse).shape == (0, 4)
-    dq, dk, dv = O.packedAttentionGrad(q, k, k, ints([0]), out, lse, q)
+    out, stats = O.packedAttention(q, k, k, ints([0]), withLse=True)
+    assert out.shape == (0, 4, 64) and E.toHost(stats.lse).shape == (0, 4)
+    dq, dk, dv = O.packedAttentionGrad(q, k, k, ints([0]), out, stats, q)
     assert E.toHost(dq).size == E.toHost(dk).size == E.toHost(dv).size == 0
 
 
@@ -96,11 +104,11 @@ def test_packed_starts_out_of_order_stay_inside(gpu):
     """Wrong starts give some result, and the sequences before the fault the right one."""
     r = np.random.default_rng(8)
     (q, qh), (k, kh), (v, vh) = make(r, 100, 2, 2, 64, "bfloat16")
-    out, lse = O.packedAttention(q, k, v, ints([0, 60, 20, 5000, -3]), withLse=True)
+    out, stats = O.packedAttention(q, k, v, ints([0, 60, 20, 5000, -3]), withLse=True)
     want, _, mag = R.packed(qh, kh, vh, np.array([0, 60]), True, 0.125)
     got = E.toHostF32(out)[:20]
     assert (np.abs(got - want[:20]) <= R.out_bound(want, mag, "bfloat16")[:20]).all()
-    O.packedAttentionGrad(q, k, v, ints([0, 60, 20, 5000, -3]), out, lse, q)
+    O.packedAttentionGrad(q, k, v, ints([0, 60, 20, 5000, -3]), out, stats, q)
     E.sync()
 
 
@@ -130,8 +138,8 @@ def test_packed_attention_grad(gpu, lens, H, Hkv, D, dtype, causal):
     (q, qh), (k, kh), (v, vh) = make(r, starts[-1], H, Hkv, D, dtype)
     (g, gh) = tensor(r.standard_normal((starts[-1], H, D)), dtype)
     s = ints(starts)
-    out, lse = O.packedAttention(q, k, v, s, causal=causal, withLse=True)
-    got = O.packedAttentionGrad(q, k, v, s, out, lse, g, causal=causal)
+    out, stats = O.packedAttention(q, k, v, s, causal=causal, withLse=True)
+    got = O.packedAttentionGrad(q, k, v, s, out, stats, g, causal=causal)
     res, bnd = R.packed_grad(qh, kh, vh, starts, gh, causal, D ** -0.5, dtype)
     for t, w, b in zip(got, res, bnd):
         check(t, w, b)
@@ -144,9 +152,9 @@ def test_packed_grad_float16_of_any_size(gpu, size):
     starts = np.array([0, 150, 260])
     (q, qh), (k, kh), (v, vh) = make(r, 260, 4, 2, 64, "float16")
     (g, gh) = tensor(r.standard_normal((260, 4, 64)) * size, "float16")
-    out, lse = O.packedAttention(q, k, v, ints(starts), withLse=True)
+    out, stats = O.packedAttention(q, k, v, ints(starts), withLse=True)
     res, bnd = R.packed_grad(qh, kh, vh, starts, gh, True, 0.125, "float16")
-    for t, w, b in zip(O.packedAttentionGrad(q, k, v, ints(starts), out, lse, g), res, bnd):
+    for t, w, b in zip(O.packedAttentionGrad(q, k, v, ints(starts), out, stats, g), res, bnd):
         # a result below 2^-14 is rounded to a multiple of 2^-24
         check(t, w, b + 2.0 ** -25)
 
@@ -177,8 +185,8 @@ def test_packed_call_is_repeatable(gpu):
     (q, _), (k, _), (v, _) = make(r, 999, 8, 2, 128, "bfloat16")
     first = None
     for _ in range(3):
-        out, lse = O.packedAttention(q, k, v, starts, withLse=True)
-        got = [E.toHost(t) for t in (out, lse, *O.packedAttentionGrad(q, k, v, starts, out, lse, q))]
+        out, stats = O.packedAttention(q, k, v, starts, withLse=True)
+        got = [E.toHost(t) for t in (out, *stats, *O.packedAttentionGrad(q, k, v, starts, out, stats, q))]
         for a, b in zip(got, first or got):
             np.testing.assert_array_equal(a, b)
         first = first or got

@@ -46,12 +46,15 @@ def test_packed_refusals(match, args, kw):
 
 
 def test_packed_grad_refusals():
-    lse = t(F32, 10, 8)
-    refuse("out must", O.packedAttentionGrad, Q, K, K, S, K, lse, Q)
-    refuse("gradOut must", O.packedAttentionGrad, Q, K, K, S, Q, lse, t(F32, 10, 8, 64))
-    refuse("lse must", O.packedAttentionGrad, Q, K, K, S, Q, t(F32, 8, 10), Q)
-    refuse("lse must", O.packedAttentionGrad, Q, K, K, S, Q, t(BF, 10, 8), Q)
-    refuse("head dims", O.packedAttentionGrad, t(BF, 10, 8, 32), K, K, S, Q, lse, Q)
+    lse, rest = t(F32, 10, 8), t(DType.INT8, 10, 8, 64)
+    st = O.PackedStats(lse, rest)
+    refuse("out must", O.packedAttentionGrad, Q, K, K, S, K, st, Q)
+    refuse("gradOut must", O.packedAttentionGrad, Q, K, K, S, Q, st, t(F32, 10, 8, 64))
+    refuse("lse must", O.packedAttentionGrad, Q, K, K, S, Q, (t(F32, 8, 10), rest), Q)
+    refuse("lse must", O.packedAttentionGrad, Q, K, K, S, Q, (t(BF, 10, 8), rest), Q)
+    refuse("rest must", O.packedAttentionGrad, Q, K, K, S, Q, (lse, Q), Q)
+    refuse("rest must", O.packedAttentionGrad, Q, K, K, S, Q, (lse, t(DType.INT8, 10, 512)), Q)
+    refuse("head dims", O.packedAttentionGrad, t(BF, 10, 8, 32), K, K, S, Q, st, Q)
 
 
 P = t(BF, 30, 2, 16, 64)
