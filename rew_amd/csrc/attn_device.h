@@ -151,6 +151,26 @@ __device__ __forceinline__ float fa_sum_halves(float x) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// A value that is the same in every lane, as the compiler does not know.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Sums over the wave with the data-parallel moves of the vector ALU (a shuffle
+// through LDS per step takes ten times as long): rows of 16 lanes by shifts,
+// then lanes 15, 31 and 47 onto the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_moved(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive
+  x = add_moved<0x111, 0xf>(x);
+  x = add_moved<0x112, 0xf>(x);
+  x = add_moved<0x114, 0xf>(x);
+  x = add_moved<0x118, 0xf>(x);
+  x = add_moved<0x142, 0xa>(x);
+  return add_moved<0x143, 0xc>(x);
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  return __builtin_amdgcn_readlane(wave_scan(x), 63);
+}
 // ---- packed sequences ---------------------------------------------------------------
 //
 // Sequence s owns rows [starts[s], starts[s + 1]) of T.  The rows before the
@@ -174,8 +194,9 @@ __device__ __forceinline__ int seq_bound(const int32_t* starts, int n_seq, int T
 // (query heads of a KV head; 1 for keys), in sequence order.  One wave (every
 // wave of a workgroup does the same): 64 sequences a step, their tile counts
 // summed over the lanes.
+// Sequences of at most `skip` units have no tiles.
 __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, int T, int units,
-                                             int per, int idx) {
+                                             int per, int idx, int skip = 0) {
   const int lane = threadIdx.x & 63;
   SeqTile r;
   r.seq = -2;
@@ -184,13 +205,9 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, i
     const int s = base + lane;
     const int b0 = seq_bound(starts, n_seq, T, s);
     const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
-    const int tiles = (int)(((int64_t)n * units + per - 1) / per);
-    int sum = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
+    int tiles = (int)(((int64_t)n * units + per - 1) / per);
+    if (n * units <= skip) tiles = 0;
+    const int sum = wave_scan(tiles);
     const int total = __builtin_amdgcn_readlane(sum, 63);
     if (idx < total) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
@@ -203,12 +220,6 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, i
     idx -= total;
   }
   return r;
-}
-// Lane-wise sum over the wave, the same in every lane.
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-  return __builtin_amdgcn_readfirstlane(x);
 }
 // The rank-th of the sequences' tiles in the order of falling level: a
 // sequence's tiles have the levels lift + 1 .. lift + tiles (its own per
@@ -294,5 +305,96 @@ struct RowTiles {
     return r;
   }
 };
+
+// ---- keys of packed and paged attention ----------------------------------------------
+
+namespace pa {
+constexpr int BK = 64;  // keys per tile
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+}  // namespace pa
+
+// Zeros that stand for the rows of keys that are not there.
+static __device__ __attribute__((aligned(256))) uint16_t g_zero_row[128];
+
+// A request's block table, 64 entries at a time, one per lane; pages outside
+// the cache (or the table) are -1.
+struct PageWindow {
+  const int32_t* row;
+  int width, log_page, base, id;
+  uint32_t pages;
+  uint64_t bad;  // lanes without a page
+  __device__ __forceinline__ PageWindow(const int32_t* r, int w, int lp, int64_t p)
+      : row(r), width(w), log_page(lp), base(-64), id(-1), pages((uint32_t)min(p, (int64_t)0x7fffffff)),
+        bad(~0ull) {}
+  // makes the window hold the pages of the 64 keys from k0 (a multiple of 64)
+  __device__ __forceinline__ void reach(int k0) {
+    const int b = (k0 >> log_page) & ~63;
+    if (b == base) return;
+    base = b;
+    const int i = b + (int)(threadIdx.x & 63);
+    const int v = i < width ? row[i] : -1;
+    id = (uint32_t)v < pages ? v : -1;
+    bad = __builtin_amdgcn_ballot_w64(id < 0);
+  }
+  // the page of key j (of a tile that the window holds)
+  __device__ __forceinline__ int page(int j) const {
+    return __builtin_amdgcn_ds_bpermute(((j >> log_page) - base) * 4, id);
+  }
+  __device__ __forceinline__ bool missing(int j) const {
+    return (bad >> ((j >> log_page) - base)) & 1;
+  }
+  // whether any of the 64 keys from k0, up to key `end` - 1, has no page
+  __device__ __forceinline__ bool any_missing(int k0, int end) const {
+    const int first = (k0 >> log_page) - base;
+    const int n = ((min(end - k0, 64) - 1) >> log_page) + 1;
+    return end > k0 && ((bad >> first) & (n == 64 ? ~0ull : (1ull << n) - 1)) != 0;
+  }
+};
+
+// One softmax step over a tile of S^T (64 keys x 32 rows): lane (c, g) holds
+// row c's scores of keys kb 32 + (e / 4) 8 + g 4 + e % 4 in s[kb][e].  `seen`:
+// keys of the tile below it are visible.  PLAIN: all are.  The running max
+// (of t = log2(e) scale s) moves, rescaling O and the sum, only when some
+// row's max grew by more than 2^kLazy2; until then the probabilities stay
+// below 2^(kLazy2 + kShift).
+template <class M, bool PLAIN, class Missing>
+__device__ __forceinline__ float soft_step(f32x16_t (&s)[2], int seen, int g, float sl2,
+                                           uint32_t (&pk)[2][8], float& m_run, float& l_run,
+                                           Missing missing) {
+  float m0, m1;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      if constexpr (!PLAIN) {
+        const int off = kb * 32 + (e >> 2) * 8 + (e & 3) + g * 4;
+        s[kb][e] = off < seen && !missing(off) ? s[kb][e] : -INFINITY;
+        s[kb][e + 1] = off + 1 < seen && !missing(off + 1) ? s[kb][e + 1] : -INFINITY;
+      }
+      float& m = kb == 0 ? m0 : m1;
+      m = e == 0 ? fa_max2(s[kb][0], s[kb][1]) : fa_max3(m, s[kb][e], s[kb][e + 1]);
+    }
+  const float mt = fa_max_halves(fa_max3(m0, m1, -INFINITY)) * sl2;
+  const float m_new = fmaxf(m_run, mt);
+  const bool grow = !(m_new - m_run <= M::kLazy2);  // (also while m_run is -inf)
+  const bool rescale = __builtin_amdgcn_ballot_w64(grow) != 0;
+  const float m_use = (rescale ? (m_new == -INFINITY ? 0.0f : m_new) : m_run);
+  const float alpha = rescale ? fa_exp2(m_run - m_use) : 1.0f;
+  m_run = rescale ? m_new : m_run;
+  const float base = M::kShift - m_use;
+  float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float p0 = fa_exp2(fmaf(s[kb][e], sl2, base));
+      const float p1 = fa_exp2(fmaf(s[kb][e + 1], sl2, base));
+      pk[kb][e >> 1] = M::pack(p0, p1);
+      ps[e & 2] += p0;
+      ps[(e & 2) + 1] += p1;
+    }
+  l_run = l_run * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+  return alpha;
+}
 
 }  // namespace rew

@@ -21,92 +21,7 @@ namespace rew {
 
 namespace pa {
 constexpr int BR = 128;  // rows per workgroup
-constexpr int BK = 64;   // keys per tile
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 }  // namespace pa
-
-// Zeros that stand for the rows of keys that are not there.
-__device__ __attribute__((aligned(256))) uint16_t g_zero_row[128];
-
-// A request's block table, 64 entries at a time, one per lane; pages outside
-// the cache (or the table) are -1.
-struct PageWindow {
-  const int32_t* row;
-  int width, log_page, base, id;
-  uint32_t pages;
-  uint64_t bad;  // lanes without a page
-  __device__ __forceinline__ PageWindow(const int32_t* r, int w, int lp, int64_t p)
-      : row(r), width(w), log_page(lp), base(-64), id(-1), pages((uint32_t)min(p, (int64_t)0x7fffffff)),
-        bad(~0ull) {}
-  // makes the window hold the pages of the 64 keys from k0 (a multiple of 64)
-  __device__ __forceinline__ void reach(int k0) {
-    const int b = (k0 >> log_page) & ~63;
-    if (b == base) return;
-    base = b;
-    const int i = b + (int)(threadIdx.x & 63);
-    const int v = i < width ? row[i] : -1;
-    id = (uint32_t)v < pages ? v : -1;
-    bad = __builtin_amdgcn_ballot_w64(id < 0);
-  }
-  // the page of key j (of a tile that the window holds)
-  __device__ __forceinline__ int page(int j) const {
-    return __builtin_amdgcn_ds_bpermute(((j >> log_page) - base) * 4, id);
-  }
-  __device__ __forceinline__ bool missing(int j) const {
-    return (bad >> ((j >> log_page) - base)) & 1;
-  }
-  // whether any of the 64 keys from k0 has no page
-  __device__ __forceinline__ bool any_missing(int k0) const {
-    const int first = (k0 >> log_page) - base, n = log_page >= 6 ? 1 : 64 >> log_page;
-    return ((bad >> first) & (n == 64 ? ~0ull : (1ull << n) - 1)) != 0;
-  }
-};
-
-// One softmax step over a tile of S^T (64 keys x 32 rows): lane (c, g) holds
-// row c's scores of keys kb 32 + (e / 4) 8 + g 4 + e % 4 in s[kb][e].  `seen`:
-// keys of the tile below it are visible.  PLAIN: all are.  The running max
-// (of t = log2(e) scale s) moves, rescaling O and the sum, only when some
-// row's max grew by more than 2^kLazy2; until then the probabilities stay
-// below 2^(kLazy2 + kShift).
-template <class M, bool PLAIN, class Missing>
-__device__ __forceinline__ float soft_step(f32x16_t (&s)[2], int seen, int g, float sl2,
-                                           uint32_t (&pk)[2][8], float& m_run, float& l_run,
-                                           Missing missing) {
-  float m0, m1;
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      if constexpr (!PLAIN) {
-        const int off = kb * 32 + (e >> 2) * 8 + (e & 3) + g * 4;
-        s[kb][e] = off < seen && !missing(off) ? s[kb][e] : -INFINITY;
-        s[kb][e + 1] = off + 1 < seen && !missing(off + 1) ? s[kb][e + 1] : -INFINITY;
-      }
-      float& m = kb == 0 ? m0 : m1;
-      m = e == 0 ? fa_max2(s[kb][0], s[kb][1]) : fa_max3(m, s[kb][e], s[kb][e + 1]);
-    }
-  const float mt = fa_max_halves(fa_max3(m0, m1, -INFINITY)) * sl2;
-  const float m_new = fmaxf(m_run, mt);
-  const bool grow = !(m_new - m_run <= M::kLazy2);  // (also while m_run is -inf)
-  const bool rescale = __builtin_amdgcn_ballot_w64(grow) != 0;
-  const float m_use = (rescale ? (m_new == -INFINITY ? 0.0f : m_new) : m_run);
-  const float alpha = rescale ? fa_exp2(m_run - m_use) : 1.0f;
-  m_run = rescale ? m_new : m_run;
-  const float base = M::kShift - m_use;
-  float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float p0 = fa_exp2(fmaf(s[kb][e], sl2, base));
-      const float p1 = fa_exp2(fmaf(s[kb][e + 1], sl2, base));
-      pk[kb][e >> 1] = M::pack(p0, p1);
-      ps[e & 2] += p0;
-      ps[(e & 2) + 1] += p1;
-    }
-  l_run = l_run * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-  return alpha;
-}
 
 template <class M, int D, bool PAGED>
 __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
@@ -120,7 +35,8 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   const int c = lane & 31, g = lane >> 5;
   const int G = a.H / a.Hkv;
   const int hk = blockIdx.x % a.Hkv;
-  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv);
+  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv,
+                               PAGED ? kDecodeRows : 0);
   if (st.seq == -2) return;
   const bool real = st.real(a.n_seq);
   const int rows = st.n * G;
@@ -211,7 +127,7 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   // missing: whether a key of this tile has no page, and the window that knows
   auto k_tile = [&](const uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n,
                     int kt) {
-    const bool holes = PAGED && win.any_missing(kt * BK);
+    const bool holes = PAGED && win.any_missing(kt * BK, cap);
     const PageWindow w = win;
     if (kt + 1 < nkt) dma_tile(ks_n, vs_n, kt + 1);
     f32x16_t s[2];
@@ -334,13 +250,26 @@ const char* packed_attn_variant(const PackedArgs& a) {
   return a.table ? "paged_attn" : "packed_attn";
 }
 
-void launch_packed_attn(const PackedArgs& a, hipStream_t stream) {
-  if (a.T == 0) return;
-  const int64_t tiles = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pa::BR) * a.Hkv;
+// Paged: requests of few rows go to the decode kernels; so do all where the
+// caller expects no other (they are right for any number of rows).
+int launch_packed_attn(const PackedArgs& a, hipStream_t stream) {
+  if (a.T == 0) return 0;
+  const int64_t G = a.H / a.Hkv;
+  if (a.table) {
+    const int64_t most = a.max_new > 0 ? std::min(a.max_new, a.T) : a.T;
+    const bool all = most * G <= kDecodeRows;
+    launch_paged_decode(a, all, stream);
+    if (all) {
+      REW_HIP(hipGetLastError());
+      return 2;
+    }
+  }
+  const int64_t tiles = max_seq_tiles(a.T, a.n_seq, G, pa::BR) * a.Hkv;
   if (tiles >= (1ll << 31)) fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention: too many tiles");
   if (a.f16) launch_prompt_t<MmaF16>(a, (unsigned)tiles, stream);
   else launch_prompt_t<MmaBf16>(a, (unsigned)tiles, stream);
   REW_HIP(hipGetLastError());
+  return a.table ? 3 : 1;
 }
 
 }  // namespace rew

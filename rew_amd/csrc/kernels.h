@@ -571,9 +571,19 @@ struct PackedArgs {
   int64_t T, pages;
   int n_seq, H, Hkv, D, width, log_page, f16, causal;
   float scale;
+  // paged: partial results (paged_ws_bytes), and the most new tokens of a
+  // request that the caller expects (0: any number)
+  float* work;
+  int64_t max_new;
 };
-// 16-bit operands, D of 32, 64 or 128, Hkv divides H.
-void launch_packed_attn(const PackedArgs& a, hipStream_t stream);
+size_t paged_ws_bytes(int D);
+// 16-bit operands, D of 32, 64 or 128, Hkv divides H.  Returns the kernels
+// launched.
+int launch_packed_attn(const PackedArgs& a, hipStream_t stream);
+// The requests whose rows (tokens x H / Hkv) fill at most one block of 32, or
+// all (k_decode.hip).
+void launch_paged_decode(const PackedArgs& a, bool all, hipStream_t stream);
+constexpr int kDecodeRows = 32;
 const char* packed_attn_variant(const PackedArgs& a);
 
 // The gradients of packed attention for the gradient `dout` of out: with

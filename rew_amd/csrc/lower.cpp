@@ -3497,6 +3497,8 @@ void Lower::emit_packed_attn(Node* n) {
     a.starts = (const int32_t*)n->in[4]->data();
     a.lens = (const int32_t*)n->in[5]->data();
     a.pages = k->shape.d[0];
+    a.work = (float*)((char*)a.out + tensor_tail_offset(n->out[0]));
+    a.max_new = n->i2;
     a.n_seq = (int)table->shape.d[0];
     a.width = (int)table->shape.d[1];
     while ((1ll << a.log_page) < k->shape.d[2]) a.log_page++;

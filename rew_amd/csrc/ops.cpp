@@ -375,7 +375,7 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
 }
 
 // pagedAttention(q, kPages, vPages, blockTable, starts, lens): attrs causal,
-// scale; out.
+// scale, max_new; out.
 static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>& ins,
                                const Attrs& attrs, Node* n, OutSpecs& outs) {
   Tensor *q = ins[0], *kp = ins[1], *vp = ins[2], *table = ins[3];
@@ -393,6 +393,9 @@ static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>
   n->i0 = flag_attr(attrs, "causal", op);
   const float scale = scale_attr(attrs, q->shape.d[2], op);
   std::memcpy(&n->i1, &scale, sizeof scale);
+  n->i2 = parse_int(find_attr(attrs, "max_new", op), op);
+  if (n->i2 < 0) invalid("eager '" + op + "': max_new must be non-negative");
+  n->tail = paged_ws_bytes((int)q->shape.d[2]);
   outs.push_back({q->dt, q->shape});
 }
 

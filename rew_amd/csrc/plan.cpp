@@ -165,6 +165,7 @@ struct PtrVisit {
     field(f, a.lse);
     field(f, a.rest);
     for (const int32_t** p : {&a.starts, &a.table, &a.lens}) field(f, *p);
+    field(f, a.work);
   }
   void operator()(PackedGradArgs& a) {
     for (const void** p : {&a.q, &a.k, &a.v, &a.out, &a.dout}) field(f, *p);
@@ -235,7 +236,9 @@ struct Exec {
   void operator()(BatchNormArgs& a) { launch_batchnorm(a, c->stream); }
   void operator()(HeadArgs& a) { launch_class_head(a, c->stream); }
   void operator()(RouterArgs& a) { launch_moe_router(a, c->stream); }
-  void operator()(PackedArgs& a) { launch_packed_attn(a, c->stream); }
+  void operator()(PackedArgs& a) {
+    c->stats.kernels_launched += launch_packed_attn(a, c->stream) - 1;
+  }
   void operator()(PackedGradArgs& a) {  // (three kernels)
     launch_packed_grad(a, c->stream);
     c->stats.kernels_launched += 2;
