@@ -194,9 +194,8 @@ __device__ __forceinline__ int seq_bound(const int32_t* starts, int n_seq, int T
 // (query heads of a KV head; 1 for keys), in sequence order.  One wave (every
 // wave of a workgroup does the same): 64 sequences a step, their tile counts
 // summed over the lanes.
-// Sequences of at most `skip` units have no tiles.
 __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, int T, int units,
-                                             int per, int idx, int skip = 0) {
+                                             int per, int idx) {
   const int lane = threadIdx.x & 63;
   SeqTile r;
   r.seq = -2;
@@ -205,8 +204,7 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, i
     const int s = base + lane;
     const int b0 = seq_bound(starts, n_seq, T, s);
     const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
-    int tiles = (int)(((int64_t)n * units + per - 1) / per);
-    if (n * units <= skip) tiles = 0;
+    const int tiles = (int)(((int64_t)n * units + per - 1) / per);
     const int sum = wave_scan(tiles);
     const int total = __builtin_amdgcn_readlane(sum, 63);
     if (idx < total) {
@@ -326,7 +324,7 @@ struct PageWindow {
   __device__ __forceinline__ PageWindow(const int32_t* r, int w, int lp, int64_t p)
       : row(r), width(w), log_page(lp), base(-64), id(-1), pages((uint32_t)min(p, (int64_t)0x7fffffff)),
         bad(~0ull) {}
-  // makes the window hold the pages of the 64 keys from k0 (a multiple of 64)
+  // makes the window hold the pages of the 64 keys from k0 (or 32, a multiple of it)
   __device__ __forceinline__ void reach(int k0) {
     const int b = (k0 >> log_page) & ~63;
     if (b == base) return;
@@ -343,38 +341,55 @@ struct PageWindow {
   __device__ __forceinline__ bool missing(int j) const {
     return (bad >> ((j >> log_page) - base)) & 1;
   }
-  // whether any of the 64 keys from k0, up to key `end` - 1, has no page
-  __device__ __forceinline__ bool any_missing(int k0, int end) const {
+  // whether any of the `keys` keys from k0, up to key `end` - 1, has no page
+  __device__ __forceinline__ bool any_missing(int k0, int keys, int end) const {
     const int first = (k0 >> log_page) - base;
-    const int n = ((min(end - k0, 64) - 1) >> log_page) + 1;
+    const int n = ((min(end - k0, keys) - 1) >> log_page) + 1;
     return end > k0 && ((bad >> first) & (n == 64 ? ~0ull : (1ull << n) - 1)) != 0;
   }
 };
 
-// One softmax step over a tile of S^T (64 keys x 32 rows): lane (c, g) holds
-// row c's scores of keys kb 32 + (e / 4) 8 + g 4 + e % 4 in s[kb][e].  `seen`:
-// keys of the tile below it are visible.  PLAIN: all are.  The running max
-// (of t = log2(e) scale s) moves, rescaling O and the sum, only when some
-// row's max grew by more than 2^kLazy2; until then the probabilities stay
-// below 2^(kLazy2 + kShift).
-template <class M, bool PLAIN, class Missing>
-__device__ __forceinline__ float soft_step(f32x16_t (&s)[2], int seen, int g, float sl2,
-                                           uint32_t (&pk)[2][8], float& m_run, float& l_run,
-                                           Missing missing) {
-  float m0, m1;
+// The keys of a tile that a lane's row sees, one word per 32 keys: bit p for key
+// p + g 4, below `seen` of the tile and with its bit in `none` clear.
+template <int NB>
+struct Seen {
+  uint32_t bits[NB];
+  __device__ __forceinline__ Seen(int seen, uint64_t none, int g) {
 #pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < NB; ++kb) {
+      const int n = seen - kb * 32 - g * 4;
+      const uint32_t below = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+      bits[kb] = below & ~(uint32_t)(none >> (kb * 32 + g * 4));
+    }
+  }
+};
+
+// One softmax step over a tile of S^T (32 NB keys x 32 rows): lane (c, g) holds
+// row c's scores of keys kb 32 + (e / 4) 8 + g 4 + e % 4 in s[kb][e], of which
+// `vis` are visible (all, if PLAIN).  The running max (of t = log2(e) scale s)
+// moves, rescaling O and the sum, only when some row's max grew by more than
+// 2^kLazy2; until then the probabilities stay below 2^(kLazy2 + kShift).
+template <class M, bool PLAIN, int NB>
+__device__ __forceinline__ float soft_step(f32x16_t (&s)[NB], const Seen<NB>& vis, float sl2,
+                                           uint32_t (&pk)[NB][8], float& m_run, float& l_run) {
+  float mx[NB];
+#pragma unroll
+  for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      if constexpr (!PLAIN) {
-        const int off = kb * 32 + (e >> 2) * 8 + (e & 3) + g * 4;
-        s[kb][e] = off < seen && !missing(off) ? s[kb][e] : -INFINITY;
-        s[kb][e + 1] = off + 1 < seen && !missing(off + 1) ? s[kb][e + 1] : -INFINITY;
+      if constexpr (!PLAIN) {  // (two instructions per score, a bit's field and a bitwise select)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)vis.bits[kb],
+                                                             ((e >> 2) * 8 + (e & 3)) + i, 1);
+          s[kb][e + i] =
+              __uint_as_float((__float_as_uint(s[kb][e + i]) & m) | (0xff800000u & ~m));
+        }
       }
-      float& m = kb == 0 ? m0 : m1;
+      float& m = mx[kb];
       m = e == 0 ? fa_max2(s[kb][0], s[kb][1]) : fa_max3(m, s[kb][e], s[kb][e + 1]);
     }
-  const float mt = fa_max_halves(fa_max3(m0, m1, -INFINITY)) * sl2;
+  const float mt = fa_max_halves(NB == 1 ? mx[0] : fa_max3(mx[0], mx[NB - 1], -INFINITY)) * sl2;
   const float m_new = fmaxf(m_run, mt);
   const bool grow = !(m_new - m_run <= M::kLazy2);  // (also while m_run is -inf)
   const bool rescale = __builtin_amdgcn_ballot_w64(grow) != 0;
@@ -384,7 +399,7 @@ __device__ __forceinline__ float soft_step(f32x16_t (&s)[2], int seen, int g, fl
   const float base = M::kShift - m_use;
   float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
+  for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const float p0 = fa_exp2(fmaf(s[kb][e], sl2, base));

@@ -1,62 +1,67 @@
-// Attention over packed sequences and paged caches (PackedArgs in kernels.h).
+// Attention of many rows over packed sequences and paged caches (PackedArgs in
+// kernels.h).
 //
 // The H / Hkv query heads of a KV head read the same keys, so the rows of a
-// tile are (token, head of the group) pairs in token order: 128 of them per
+// block are (token, head of the group) pairs in token order: 128 of them per
 // workgroup share each K and V tile, whatever the group's size, and a causal
-// tile ends with the last of its few tokens.  Four waves of 32 rows; key
+// block ends with the last of its few tokens.  Four waves of 32 rows; key
 // tiles of 64 keys move by DMA into two LDS stages.  S^T = K Q^T leaves the
 // scores of one row in a lane and its neighbour lane ^ 32, so the softmax's
 // running max and sum need one exchange; O^T = V^T P^T takes the
-// probabilities from the accumulators, with V read transposed from LDS.
+// probabilities from the accumulators, with V read transposed from LDS.  Two
+// workgroups fit a CU, and one's products run beside the other's exponentials.
 //
 // Rounding: scores, max, sum and O in float32; the probabilities are rounded
 // to the operands' 16 bits for the second product (not in the sum, which the
 // gradients need), the output once.
 #include <algorithm>
 
-#include "attn_device.h"
-#include "kernels.h"
+#include "attn_line.h"
 
 namespace rew {
 
 namespace pa {
-constexpr int BR = 128;  // rows per workgroup
+constexpr int BR = 128;           // rows per block
+constexpr int kChunkSlots = 512;  // workgroups that run at once: two on each of 256 CUs
+constexpr int kPieceTiles = 16;   // key tiles that are worth a piece of a block
 }  // namespace pa
 
+// Tokens of a sequence or request whose rows one block holds, as a lane sees
+// them.
+struct BlockRows {
+  int row, tok, hg;  // this lane's row of the sequence; its token, its head of the group
+  __device__ __forceinline__ BlockRows(int block, int rows, int G) {
+    const int wave = threadIdx.x >> 6, c = threadIdx.x & 31;
+    row = block * pa::BR + wave * 32 + c;
+    const int r = min(row, rows - 1);
+    tok = r / G;
+    hg = r - tok * G;
+  }
+};
+
+// O (unnormalised), running max and this lane's part of the running sum of a
+// block's rows over key tiles [kt0, kt1) of a sequence that starts at token
+// `first` (or, PAGED, of the request with block table `table`): `cap` keys,
+// this lane's row sees those below my_limit, every row of the wave those below
+// `least`.  Four waves; ends with a barrier behind the last read of LDS.
 template <class M, int D, bool PAGED>
-__global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
+__device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRows& br, int first,
+                                             const int32_t* table, int hk, int cap, int my_limit,
+                                             int least, int kt0, int kt1, f32x16_t (&o)[D / 32],
+                                             float& m_run, float& l_run) {
   using namespace pa;
   typedef typename M::frag frag;
   constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, TILE = BK * D;
-  constexpr int RPD = 64 / CPR;        // key rows per DMA instruction
+  constexpr int RPD = 64 / CPR;         // key rows per DMA instruction
   constexpr int NDMA = TILE / 512 / 4;  // instructions per wave and K (or V) tile
   __shared__ __attribute__((aligned(1024))) uint16_t Ks0[TILE], Ks1[TILE], Vs0[TILE], Vs1[TILE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, g = lane >> 5;
-  const int G = a.H / a.Hkv;
-  const int hk = blockIdx.x % a.Hkv;
-  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv,
-                               PAGED ? kDecodeRows : 0);
-  if (st.seq == -2) return;
-  const bool real = st.real(a.n_seq);
-  const int rows = st.n * G;
-  const int len = !real ? 0 : PAGED ? max(a.lens[st.seq], 0) : st.n;
-  const int cap = !real ? 0 : PAGED ? (int)min((int64_t)len, (int64_t)a.width << a.log_page) : len;
-  // keys that row r sees: [0, limit(r)), growing with r
-  auto limit = [&](int r) -> int {
-    const int t = min(r, rows - 1) / G;
-    return min(max(a.causal ? len - st.n + t + 1 : len, 0), cap);
-  };
-  const int r0 = st.tile * BR + wave * 32;
-  const int row = r0 + c;
-  const int tok = min(row, rows - 1) / G, hg = min(row, rows - 1) - tok * G;
-  const int my_limit = limit(row), least = limit(r0);
-  const int nkt = (limit(st.tile * BR + BR - 1) + BK - 1) / BK;
-
+  const int G = a.H / a.Hkv, tok = br.tok, hg = br.hg;
   frag qf[NT];
   {
     const uint16_t* qp = (const uint16_t*)a.q +
-                         ((int64_t)(st.first + tok) * a.H + hk * G + hg) * D;
+                         ((int64_t)(first + tok) * a.H + hk * G + hg) * D;
 #pragma unroll
     for (int t = 0; t < NT; ++t) qf[t] = *(const frag*)(qp + t * 16 + g * 8);
   }
@@ -65,28 +70,28 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   // pc ^ (4 (r & 3)) of V: both reads then spread over the LDS banks
   const int row_in = lane / CPR, pc = lane % CPR;
   const int64_t kstride = (int64_t)a.Hkv * D;
-  const uint16_t* K = (const uint16_t*)a.k + (PAGED ? 0 : (st.first * (int64_t)a.Hkv + hk) * D);
-  const uint16_t* V = (const uint16_t*)a.v + (PAGED ? 0 : (st.first * (int64_t)a.Hkv + hk) * D);
-  RowTiles kr(K, 0, cap, kstride, D, BK), vr(V, 0, cap, kstride, D, BK);
+  const uint16_t* K = (const uint16_t*)a.k + (PAGED ? 0 : (first * (int64_t)a.Hkv + hk) * D);
+  const uint16_t* V = (const uint16_t*)a.v + (PAGED ? 0 : (first * (int64_t)a.Hkv + hk) * D);
+  RowTiles kr(K, kt0 * BK, cap, kstride, D, BK), vr(V, kt0 * BK, cap, kstride, D, BK);
   uint32_t k_src[NDMA], v_src[NDMA];
-  int key_row[NDMA];
 #pragma unroll
   for (int q = 0; q < NDMA; ++q) {
     const int r = (wave * NDMA + q) * RPD + row_in;
-    key_row[q] = r;
     const int ck = (pc ^ (r % CPR)) * 8, cv = (pc ^ ((4 * (r & 3)) % CPR)) * 8;
     k_src[q] = PAGED ? (uint32_t)ck : (uint32_t)((r * kstride + ck) * 2);
     v_src[q] = PAGED ? (uint32_t)cv : (uint32_t)((r * kstride + cv) * 2);
   }
-  PageWindow win(PAGED && real ? a.table + (int64_t)st.seq * a.width : nullptr,
-                 PAGED && real ? a.width : 0, a.log_page, a.pages);
+  PageWindow win(table, table ? a.width : 0, a.log_page, a.pages);
+  uint64_t none_next = 0;  // of the tile last requested: bit i for a key i without a page
   auto dma_tile = [&](uint16_t* ks, uint16_t* vs, int kt) {  // (kt: one after another)
     if constexpr (PAGED) {
-      if (kt >= nkt) return;
       win.reach(kt * BK);
+      none_next = win.any_missing(kt * BK, BK, cap)
+                      ? __builtin_amdgcn_ballot_w64(win.missing(kt * BK + lane))
+                      : 0;
 #pragma unroll
       for (int q = 0; q < NDMA; ++q) {
-        const int j = kt * BK + key_row[q];
+        const int j = kt * BK + (wave * NDMA + q) * RPD + row_in;
         const int pg = win.page(j);
         const bool there = pg >= 0 && j < cap;
         const int64_t at = ((((int64_t)(there ? pg : 0) * a.Hkv + hk) << a.log_page) +
@@ -116,20 +121,18 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
     v_off[dt] = r * D + (((col >> 3) ^ ((4 * (r & 3)) % CPR)) * 8) + (col & 7);
   }
 
-  f32x16_t o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-  float m_run = -INFINITY, l_run = 0.0f;
+  m_run = -INFINITY;
+  l_run = 0.0f;
   const float sl2 = a.scale * kLog2e;
 
-  // missing: whether a key of this tile has no page, and the window that knows
   auto k_tile = [&](const uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n,
                     int kt) {
-    const bool holes = PAGED && win.any_missing(kt * BK, cap);
-    const PageWindow w = win;
-    if (kt + 1 < nkt) dma_tile(ks_n, vs_n, kt + 1);
+    const uint64_t none = none_next;
+    if (kt + 1 < kt1) dma_tile(ks_n, vs_n, kt + 1);
     f32x16_t s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -143,14 +146,10 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
     uint32_t pk[2][8];
     float alpha;
     const int k0 = kt * BK;
-    if (k0 + BK <= least && !holes)
-      alpha = soft_step<M, true>(s, 0, g, sl2, pk, m_run, l_run, [](int) { return false; });
-    else if (!holes)
-      alpha = soft_step<M, false>(s, my_limit - k0, g, sl2, pk, m_run, l_run,
-                                  [](int) { return false; });
-    else
-      alpha = soft_step<M, false>(s, my_limit - k0, g, sl2, pk, m_run, l_run,
-                                  [&](int off) { return w.missing(k0 + off); });
+    const Seen<2> vis(my_limit - k0, none, g);
+    alpha = k0 + BK <= least && none == 0
+                ? soft_step<M, true, 2>(s, vis, sl2, pk, m_run, l_run)
+                : soft_step<M, false, 2>(s, vis, sl2, pk, m_run, l_run);
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -180,21 +179,43 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
-  if (nkt > 0) {
-    dma_tile(Ks0, Vs0, 0);
+  if (kt0 < kt1) {
+    dma_tile(Ks0, Vs0, kt0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int kt = 0; kt < nkt; kt += 2) {
+    for (int kt = kt0; kt < kt1; kt += 2) {
       k_tile(Ks0, Vs0, Ks1, Vs1, kt);
-      if (kt + 1 < nkt) k_tile(Ks1, Vs1, Ks0, Vs0, kt + 1);
+      if (kt + 1 < kt1) k_tile(Ks1, Vs1, Ks0, Vs0, kt + 1);
     }
   }
+}
 
+template <class M, int D>
+__global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
+  using namespace pa;
+  constexpr int DT = D / 32;
+  const int G = a.H / a.Hkv, g = (threadIdx.x & 63) >> 5;
+  const int hk = blockIdx.x % a.Hkv;
+  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv);
+  if (st.seq == -2) return;
+  const int rows = st.n * G, len = st.real(a.n_seq) ? st.n : 0;
+  // keys that row r sees: [0, limit(r)), growing with r
+  auto limit = [&](int r) { return a.causal ? min(min(r, rows - 1) / G + 1, len) : len; };
+  const BlockRows br(st.tile, rows, G);
+  f32x16_t o[DT];
+  float m_run, l_run;
+  attend_block<M, D, false>(a, br, st.first, nullptr, hk, len, limit(br.row),
+                            limit(st.tile * BR + (threadIdx.x >> 6) * 32), 0,
+                            (limit(st.tile * BR + BR - 1) + BK - 1) / BK, o, m_run, l_run);
   const float l = fa_sum_halves(l_run);
+  if (br.row >= rows) return;
+  const int64_t at = (int64_t)(st.first + br.tok) * a.H + hk * G + br.hg;
+  if (!a.rest) {
+    store_whole<M, D>((uint16_t*)a.out + at * D, o, l, g);
+    return;
+  }
+  if (g == 0) a.lse[at] = (m_run - M::kShift + __log2f(l)) * kLn2;
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (NaN stays NaN)
-  if (row >= rows) return;
-  const int64_t at = (int64_t)(st.first + tok) * a.H + hk * G + hg;
-  if (a.lse && g == 0) a.lse[at] = (m_run - M::kShift + __log2f(l)) * kLn2;
   uint16_t* O = (uint16_t*)a.out + at * D;
   float most = 0.0f;
 #pragma unroll
@@ -204,16 +225,13 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
       float* x = (float*)&o[dt] + r * 4;
       const uint2 w = make_uint2(M::pack(x[0] * inv, x[1] * inv), M::pack(x[2] * inv, x[3] * inv));
       *(uint2*)(O + dt * 32 + r * 8 + g * 4) = w;
-      if (a.rest) {  // (uniform)
-        const float y[4] = {M::lo(w.x), M::hi(w.x), M::lo(w.y), M::hi(w.y)};
+      const float y[4] = {M::lo(w.x), M::hi(w.x), M::lo(w.y), M::hi(w.y)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          most = fmaxf(most, fabsf(y[i]));
-          x[i] = fmaf(x[i], inv, -y[i]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        most = fmaxf(most, fabsf(y[i]));
+        x[i] = fmaf(x[i], inv, -y[i]);
       }
     }
-  if (!a.rest) return;
   // (lanes of a row, l and l ^ 32, are both here)
   most = fa_max_halves(most);
   const float per_step = most > 0.0f ? 1.0f / (most * M::kRestStep) : 0.0f;
@@ -232,44 +250,183 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
     }
 }
 
+// ---- chunks over a paged cache -----------------------------------------------------
+//
+// A chunk of a few hundred tokens over a long cache is few blocks of many key
+// tiles, so a request's blocks may each be split over P workgroups, which leave
+// partial results for a second launch to join.  A piece costs about six tiles'
+// time (its 64 KiB are written and read), so P is the number of times that the
+// request's middle block holds C tiles, rounded, C being a CU's share of all
+// tiles or at least kPieceTiles: no block is split where the blocks fill the
+// CUs by themselves (2048 tokens over 30001 keys: 1140 us; cut into 512 equal
+// runs, 1300 us and 140 us of joining).  Single tokens of other requests in
+// the same step are blocks of few rows here.
+struct ChunkPlan {
+  const PackedArgs& a;
+  int G, C;
+  // what this lane's request has: row blocks, workgroups per block and KV head
+  struct Share {
+    Request r;
+    int blocks, P;
+  };
+  static __device__ __forceinline__ int tiles_of(const PackedArgs& a, int G, const Request& r,
+                                                 int qt) {
+    return (r.limit(a, G, qt * pa::BR + pa::BR - 1) + pa::BK - 1) / pa::BK;
+  }
+  __device__ __forceinline__ Share share(int s) const {
+    Share x;
+    x.r = request_at(a, G, s);
+    x.blocks = (x.r.rows + pa::BR - 1) / pa::BR;
+    x.P = x.blocks ? max((tiles_of(a, G, x.r, x.blocks / 2) + C / 2) / C, 1) : 0;
+    return x;
+  }
+  __device__ __forceinline__ explicit ChunkPlan(const PackedArgs& a_)
+      : a(a_), G(a_.H / a_.Hkv), C(0x7fffffff / 2) {
+    int n = 0;
+    for (int base = -1; base <= a.n_seq; base += 64) {
+      const Share x = share(base + (int)(threadIdx.x & 63));
+      n += wave_sum(x.blocks ? x.blocks * tiles_of(a, G, x.r, x.blocks / 2) * a.Hkv : 0);
+    }
+    C = max((n + pa::kChunkSlots - 1) / pa::kChunkSlots, pa::kPieceTiles);
+  }
+};
+// Workgroup `idx` of the plan's (or, SPLIT, of the split blocks' joins, one per
+// block and KV head).
+template <bool SPLIT>
+struct ChunkPlace {
+  bool found;
+  int s, hk, qt, part, P, slot;  // slot: of this block's first partial result, if P > 1
+  Request r;
+  __device__ __forceinline__ ChunkPlace(const ChunkPlan& plan, int idx) : found(false) {
+    int slots = 0;
+    const int Hkv = plan.a.Hkv;
+    for (int base = -1; base <= plan.a.n_seq; base += 64) {
+      const ChunkPlan::Share x = plan.share(base + (int)(threadIdx.x & 63));
+      const int pieces = x.P > 1 ? x.blocks * x.P * Hkv : 0;
+      const int mine = !SPLIT ? x.blocks * x.P * Hkv : x.P > 1 ? x.blocks * Hkv : 0;
+      const int sum = wave_scan(mine), psum = wave_scan(pieces);
+      const int total = __builtin_amdgcn_readlane(sum, 63);
+      if (idx >= total) {
+        idx -= total;
+        slots += __builtin_amdgcn_readlane(psum, 63);
+        continue;
+      }
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
+      found = true;
+      s = base + at;
+      r = request_at(plan.a, plan.G, s);
+      P = __builtin_amdgcn_readlane(x.P, at);
+      const int blocks = __builtin_amdgcn_readlane(x.blocks, at);
+      int u = idx - __builtin_amdgcn_readlane(sum - mine, at);
+      // KV heads first: with eight of them a head's workgroups share an XCD (those
+      // whose indices agree mod 8 do) and its L2; the blocks of most keys first
+      hk = u % Hkv;
+      u /= Hkv;
+      part = SPLIT ? 0 : u % P;
+      qt = blocks - 1 - (SPLIT ? u : u / P);
+      slot = slots + __builtin_amdgcn_readlane(psum - pieces, at) + (qt * Hkv + hk) * P;
+      return;
+    }
+  }
+};
+
 template <class M, int D>
-static void launch_prompt(const PackedArgs& a, unsigned grid, hipStream_t stream) {
-  if (a.table)
-    hipLaunchKernelGGL((prompt_attn_kernel<M, D, true>), dim3(grid), dim3(256), 0, stream, a);
+__global__ void __launch_bounds__(256, 2) chunk_attn_kernel(PackedArgs a) {
+  using namespace pa;
+  constexpr int DT = D / 32;
+  const int G = a.H / a.Hkv, g = (threadIdx.x & 63) >> 5;
+  const ChunkPlace<false> at(ChunkPlan(a), blockIdx.x);
+  if (!at.found) return;
+  const Request& r = at.r;
+  const int tiles = ChunkPlan::tiles_of(a, G, r, at.qt);
+  const bool real = at.s >= 0 && at.s < a.n_seq;
+  const BlockRows br(at.qt, r.rows, G);
+  f32x16_t o[DT];
+  float m_run, l_run;
+  attend_block<M, D, true>(a, br, r.first, real ? a.table + (int64_t)at.s * a.width : nullptr,
+                           at.hk, r.cap, r.limit(a, G, br.row),
+                           uniform(r.limit(a, G, at.qt * BR + (threadIdx.x >> 6) * 32)),
+                           (int)((int64_t)tiles * at.part / at.P),
+                           (int)((int64_t)tiles * (at.part + 1) / at.P), o, m_run, l_run);
+  const float l = fa_sum_halves(l_run);
+  if (br.row >= r.rows) return;
+  if (at.P == 1)
+    store_whole<M, D>(
+        (uint16_t*)a.out + ((int64_t)(r.first + br.tok) * a.H + at.hk * G + br.hg) * D, o, l, g);
   else
-    hipLaunchKernelGGL((prompt_attn_kernel<M, D, false>), dim3(grid), dim3(256), 0, stream, a);
+    store_part<D>(a.work + (int64_t)(at.slot + at.part) * part_floats(BR, D), BR,
+                  br.row - at.qt * BR, o, m_run, l, g);
+}
+
+template <class M, int D>
+__global__ void __launch_bounds__(256) chunk_join_kernel(PackedArgs a) {
+  using namespace pa;
+  const ChunkPlace<true> at(ChunkPlan(a), blockIdx.x);
+  if (!at.found) return;
+  const int G = a.H / a.Hkv;
+  join_rows<M, D, BR>(
+      min(at.r.rows - at.qt * BR, BR), at.P,
+      [&](int k) { return a.work + (int64_t)(at.slot + k) * part_floats(BR, D); },
+      [&](int i) {
+        const int row = at.qt * BR + i, tok = row / G, hg = row - tok * G;
+        return (uint16_t*)a.out + ((int64_t)(at.r.first + tok) * a.H + at.hk * G + hg) * D;
+      });
+}
+
+// ---- launches ---------------------------------------------------------------------------
+
+// Whether the caller expects a request whose rows fill more than one block of the
+// decode kernels; both they and the chunk kernels are right for any rows.
+static bool expects_chunks(const PackedArgs& a) {
+  const int64_t most = a.max_new > 0 ? std::min(a.max_new, a.T) : a.T;
+  return most * (a.H / a.Hkv) > kDecodeRows;
+}
+// Split blocks have P >= 2 and P <= 4/3 of their tiles / C, all tiles together at
+// most kChunkSlots C.
+constexpr int kChunkPieces = pa::kChunkSlots * 4 / 3;
+size_t paged_ws_bytes(const PackedArgs& a) {
+  // (the finest cut, the decode kernels' blocks and tiles)
+  const int64_t keys = ((int64_t)a.width << a.log_page) / 32 + 1;
+  if (max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, kDecodeRows) * keys >= (1ll << 31) / a.Hkv)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "paged attention: 2^31 key tiles or more");
+  return (expects_chunks(a) ? (size_t)kChunkPieces * part_floats(pa::BR, a.D)
+                            : decode_ws_floats(a)) * 4;
+}
+
+template <class M, int D>
+static int launch_prompt(const PackedArgs& a, hipStream_t stream) {
+  if (a.table && !expects_chunks(a)) {
+    launch_paged_decode(a, stream);
+    return 2;
+  }
+  const int64_t tiles = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pa::BR) * a.Hkv;
+  if (tiles >= (1ll << 30)) fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention: too many tiles");
+  if (!a.table) {
+    hipLaunchKernelGGL((prompt_attn_kernel<M, D>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
+    return 1;
+  }
+  hipLaunchKernelGGL((chunk_attn_kernel<M, D>), dim3((unsigned)tiles + kChunkPieces), dim3(256), 0,
+                     stream, a);
+  // 32 rows of a block per workgroup
+  hipLaunchKernelGGL((chunk_join_kernel<M, D>), dim3(kChunkPieces / 2, 4), dim3(256), 0, stream, a);
+  return 2;
 }
 template <class M>
-static void launch_prompt_t(const PackedArgs& a, unsigned grid, hipStream_t stream) {
-  if (a.D == 32) launch_prompt<M, 32>(a, grid, stream);
-  else if (a.D == 64) launch_prompt<M, 64>(a, grid, stream);
-  else launch_prompt<M, 128>(a, grid, stream);
+static int launch_prompt_t(const PackedArgs& a, hipStream_t stream) {
+  if (a.D == 32) return launch_prompt<M, 32>(a, stream);
+  if (a.D == 64) return launch_prompt<M, 64>(a, stream);
+  return launch_prompt<M, 128>(a, stream);
 }
 
 const char* packed_attn_variant(const PackedArgs& a) {
-  return a.table ? "paged_attn" : "packed_attn";
+  return !a.table ? "packed_attn" : expects_chunks(a) ? "paged_attn_chunks" : "paged_attn_decode";
 }
 
-// Paged: requests of few rows go to the decode kernels; so do all where the
-// caller expects no other (they are right for any number of rows).
 int launch_packed_attn(const PackedArgs& a, hipStream_t stream) {
   if (a.T == 0) return 0;
-  const int64_t G = a.H / a.Hkv;
-  if (a.table) {
-    const int64_t most = a.max_new > 0 ? std::min(a.max_new, a.T) : a.T;
-    const bool all = most * G <= kDecodeRows;
-    launch_paged_decode(a, all, stream);
-    if (all) {
-      REW_HIP(hipGetLastError());
-      return 2;
-    }
-  }
-  const int64_t tiles = max_seq_tiles(a.T, a.n_seq, G, pa::BR) * a.Hkv;
-  if (tiles >= (1ll << 31)) fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention: too many tiles");
-  if (a.f16) launch_prompt_t<MmaF16>(a, (unsigned)tiles, stream);
-  else launch_prompt_t<MmaBf16>(a, (unsigned)tiles, stream);
+  const int n = a.f16 ? launch_prompt_t<MmaF16>(a, stream) : launch_prompt_t<MmaBf16>(a, stream);
   REW_HIP(hipGetLastError());
-  return a.table ? 3 : 1;
+  return n;
 }
 
 }  // namespace rew

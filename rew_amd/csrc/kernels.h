@@ -576,13 +576,14 @@ struct PackedArgs {
   float* work;
   int64_t max_new;
 };
-size_t paged_ws_bytes(int D);
+// Bytes of work; throws where the launch would have 2^31 key tiles.
+size_t paged_ws_bytes(const PackedArgs& a);
 // 16-bit operands, D of 32, 64 or 128, Hkv divides H.  Returns the kernels
 // launched.
 int launch_packed_attn(const PackedArgs& a, hipStream_t stream);
-// The requests whose rows (tokens x H / Hkv) fill at most one block of 32, or
-// all (k_decode.hip).
-void launch_paged_decode(const PackedArgs& a, bool all, hipStream_t stream);
+// The form for requests of few rows, tokens x H / Hkv (k_decode.hip).
+void launch_paged_decode(const PackedArgs& a, hipStream_t stream);
+size_t decode_ws_floats(const PackedArgs& a);
 constexpr int kDecodeRows = 32;
 const char* packed_attn_variant(const PackedArgs& a);
 

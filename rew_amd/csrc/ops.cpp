@@ -395,7 +395,17 @@ static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>
   std::memcpy(&n->i1, &scale, sizeof scale);
   n->i2 = parse_int(find_attr(attrs, "max_new", op), op);
   if (n->i2 < 0) invalid("eager '" + op + "': max_new must be non-negative");
-  n->tail = paged_ws_bytes((int)q->shape.d[2]);
+  PackedArgs a;
+  std::memset(&a, 0, sizeof a);
+  a.T = q->shape.d[0];
+  a.H = (int)q->shape.d[1];
+  a.D = (int)q->shape.d[2];
+  a.Hkv = (int)kp->shape.d[1];
+  a.n_seq = (int)R;
+  a.width = (int)table->shape.d[1];
+  a.log_page = page_log2(kp->shape.d[2], op);
+  a.max_new = n->i2;
+  n->tail = paged_ws_bytes(a);
   outs.push_back({q->dt, q->shape});
 }
 
