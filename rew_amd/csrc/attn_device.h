@@ -27,17 +27,17 @@ __device__ __forceinline__ float fa_exp2(float x) { return __builtin_amdgcn_exp2
 // with a v_max_f32 x, x per operand (MFMA results are not known to be
 // canonical); a quiet NaN operand is ignored either way.  The compiler does
 // not see that this reads a register: the wait states between a MFMA and the
-// first use of its result must come from a builtin (fa_max2) before it.
+// first use of its result must come from other code before it.
 __device__ __forceinline__ float fa_max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 
-// max(a, b) as one v_med3_f32, which the compiler knows: the first read of
-// MFMA results, later ones by fa_max3 then being chained to it.
-__device__ __forceinline__ float fa_max2(float a, float b) {
-  return __builtin_amdgcn_fmed3f(a, b, INFINITY);
+// max(a, b, c) in one v_maximum3_f32, which the compiler knows and schedules; NaN
+// if one is.
+__device__ __forceinline__ float fa_maximum3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(a, __builtin_elementwise_maximum(b, c));
 }
 
 // Two fp32 values rounded to bf16 (RNE; v_cvt_pk_bf16_f32), packed.
@@ -143,7 +143,7 @@ struct MmaF16 {
 __device__ __forceinline__ float fa_max_halves(float x) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
                                                   false);
-  return fa_max3(__uint_as_float(s[0]), __uint_as_float(s[1]), -INFINITY);
+  return __builtin_elementwise_maximum(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float fa_sum_halves(float x) {
   const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
@@ -369,9 +369,12 @@ struct Seen {
 // `vis` are visible (all, if PLAIN).  The running max (of t = log2(e) scale s)
 // moves, rescaling O and the sum, only when some row's max grew by more than
 // 2^kLazy2; until then the probabilities stay below 2^(kLazy2 + kShift).
+//
+// First half: the scores masked, the max moved; the factor for O and the sum
+// (1 in every lane of the wave, mostly).
 template <class M, bool PLAIN, int NB>
-__device__ __forceinline__ float soft_step(f32x16_t (&s)[NB], const Seen<NB>& vis, float sl2,
-                                           uint32_t (&pk)[NB][8], float& m_run, float& l_run) {
+__device__ __forceinline__ float soft_max(f32x16_t (&s)[NB], const Seen<NB>& vis, float sl2,
+                                          float& m_run) {
   float mx[NB];
 #pragma unroll
   for (int kb = 0; kb < NB; ++kb)
@@ -387,16 +390,24 @@ __device__ __forceinline__ float soft_step(f32x16_t (&s)[NB], const Seen<NB>& vi
         }
       }
       float& m = mx[kb];
-      m = e == 0 ? fa_max2(s[kb][0], s[kb][1]) : fa_max3(m, s[kb][e], s[kb][e + 1]);
+      m = e == 0 ? __builtin_elementwise_maximum(s[kb][0], s[kb][1])
+                 : fa_maximum3(m, s[kb][e], s[kb][e + 1]);
     }
-  const float mt = fa_max_halves(NB == 1 ? mx[0] : fa_max3(mx[0], mx[NB - 1], -INFINITY)) * sl2;
-  const float m_new = fmaxf(m_run, mt);
+  const float mt =
+      fa_max_halves(NB == 1 ? mx[0] : __builtin_elementwise_maximum(mx[0], mx[NB - 1])) * sl2;
+  const float m_new = __builtin_elementwise_maximum(m_run, mt);
   const bool grow = !(m_new - m_run <= M::kLazy2);  // (also while m_run is -inf)
   const bool rescale = __builtin_amdgcn_ballot_w64(grow) != 0;
-  const float m_use = (rescale ? (m_new == -INFINITY ? 0.0f : m_new) : m_run);
+  const float m_use = m_new == -INFINITY ? 0.0f : m_new;
   const float alpha = rescale ? fa_exp2(m_run - m_use) : 1.0f;
   m_run = rescale ? m_new : m_run;
-  const float base = M::kShift - m_use;
+  return alpha;
+}
+// Second half: the probabilities, packed for the second product, and their sum.
+template <class M, int NB>
+__device__ __forceinline__ void soft_exp(const f32x16_t (&s)[NB], float sl2, float m_run,
+                                         uint32_t (&pk)[NB][8], float& l_run) {
+  const float base = M::kShift - (m_run == -INFINITY ? 0.0f : m_run);
   float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int kb = 0; kb < NB; ++kb)
@@ -408,8 +419,17 @@ __device__ __forceinline__ float soft_step(f32x16_t (&s)[NB], const Seen<NB>& vi
       ps[e & 2] += p0;
       ps[(e & 2) + 1] += p1;
     }
-  l_run = l_run * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-  return alpha;
+  l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+}
+// O and the sum take the factor of soft_max.
+template <int DT>
+__device__ __forceinline__ void soft_rescale(f32x16_t (&o)[DT], float& l_run, float alpha) {
+  if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) == 0) return;
+  l_run *= alpha;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
 }
 
 }  // namespace rew

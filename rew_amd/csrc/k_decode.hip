@@ -136,15 +136,10 @@ __global__ void __launch_bounds__(64, D == 128 ? 1 : 2) decode_kernel(PackedArgs
       const int k0 = kt * BK;
       const uint32_t none = holes[stage];
       const Seen<1> vis(my_limit - k0, none, g);
-      alpha = k0 + BK <= least && none == 0
-                  ? soft_step<M, true, 1>(s, vis, sl2, pk, m_run, l_run)
-                  : soft_step<M, false, 1>(s, vis, sl2, pk, m_run, l_run);
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-      }
+      alpha = k0 + BK <= least && none == 0 ? soft_max<M, true, 1>(s, vis, sl2, m_run)
+                                            : soft_max<M, false, 1>(s, vis, sl2, m_run);
+      soft_rescale<DT>(o, l_run, alpha);
+      soft_exp<M, 1>(s, sl2, m_run, pk, l_run);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         union {

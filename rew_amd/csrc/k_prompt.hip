@@ -138,24 +138,35 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+    // the K fragments of k-step t + AHEAD are read while step t multiplies
+    constexpr int AHEAD = NT < 3 ? NT : 3;
+    frag kf[AHEAD][2];
+    auto ld_k = [&](int t) {
+      kf[t % AHEAD][0] = *(const frag*)(ks + k_off[t]);
+      kf[t % AHEAD][1] = *(const frag*)(ks + k_off[t] + 32 * D);
+    };
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) ld_k(t);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      s[0] = M::mma(*(const frag*)(ks + k_off[t]), qf[t], s[0]);
-      s[1] = M::mma(*(const frag*)(ks + k_off[t] + 32 * D), qf[t], s[1]);
+      s[0] = M::mma(kf[t % AHEAD][0], qf[t], s[0]);
+      s[1] = M::mma(kf[t % AHEAD][1], qf[t], s[1]);
+      if (t + AHEAD < NT) ld_k(t + AHEAD);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      if (t + AHEAD < NT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
     uint32_t pk[2][8];
     float alpha;
     const int k0 = kt * BK;
     const Seen<2> vis(my_limit - k0, none, g);
-    alpha = k0 + BK <= least && none == 0
-                ? soft_step<M, true, 2>(s, vis, sl2, pk, m_run, l_run)
-                : soft_step<M, false, 2>(s, vis, sl2, pk, m_run, l_run);
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-    }
+    alpha = k0 + BK <= least && none == 0 ? soft_max<M, true, 2>(s, vis, sl2, m_run)
+                                          : soft_max<M, false, 2>(s, vis, sl2, m_run);
+    soft_rescale<DT>(o, l_run, alpha);
+    soft_exp<M, 2>(s, sl2, m_run, pk, l_run);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       union {
@@ -205,7 +216,7 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   f32x16_t o[DT];
   float m_run, l_run;
   attend_block<M, D, false>(a, br, st.first, nullptr, hk, len, limit(br.row),
-                            limit(st.tile * BR + (threadIdx.x >> 6) * 32), 0,
+                            uniform(limit(st.tile * BR + (threadIdx.x >> 6) * 32)), 0,
                             (limit(st.tile * BR + BR - 1) + BK - 1) / BK, o, m_run, l_run);
   const float l = fa_sum_halves(l_run);
   if (br.row >= rows) return;
