@@ -207,7 +207,13 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   constexpr int DT = D / 32;
   const int G = a.H / a.Hkv, g = (threadIdx.x & 63) >> 5;
   const int hk = blockIdx.x % a.Hkv;
-  const SeqTile st = find_tile(a.starts, a.n_seq, (int)a.T, G, BR, blockIdx.x / a.Hkv);
+  // Under causality a block's work grows with its place in its sequence: the
+  // heaviest start first (8 ragged prompts, 8 times the blocks that run at once:
+  // 219 us in sequence order, 200 us so; the search costs 0.3 us).
+  const int rank = blockIdx.x / a.Hkv;
+  const SeqTile st = a.causal && a.n_seq <= kLevelSeqs
+                         ? rising_tile(a.starts, a.n_seq, (int)a.T, G, BR, rank)
+                         : find_tile(a.starts, a.n_seq, (int)a.T, G, BR, rank);
   if (st.seq == -2) return;
   const int rows = st.n * G, len = st.real(a.n_seq) ? st.n : 0;
   // keys that row r sees: [0, limit(r)), growing with r
