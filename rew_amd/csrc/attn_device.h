@@ -102,6 +102,7 @@ struct MmaBf16 {
   static constexpr float kShift = 0.0f, kLazy2 = 11.5f, kGradShift = 0.0f;
   static constexpr bool kScaled = false;  // dS is stored scaled (k_packed_grad.hip)
   static constexpr float kRestStep = 0x1p-8f / 127.0f;  // of PackedArgs::rest, by the row's max
+  static constexpr uint32_t kInf = 0x7f80;
   static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -118,6 +119,7 @@ struct MmaF16 {
   static constexpr float kShift = 11.0f, kLazy2 = 4.0f, kGradShift = 15.0f;
   static constexpr bool kScaled = true;
   static constexpr float kRestStep = 0x1p-11f / 127.0f;
+  static constexpr uint32_t kInf = 0x7c00;
   static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -420,6 +422,71 @@ __device__ __forceinline__ void soft_exp(const f32x16_t (&s)[NB], float sl2, flo
       ps[(e & 2) + 1] += p1;
     }
   l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+}
+// A value that a row does not see must not reach its output, and 0 times an
+// infinity or NaN would.  Where some row of a block does not see all keys of a
+// tile (the last tiles of causal blocks), the tile of V is looked through
+// first; the infinities and NaN found are added to the rows that see them
+// by themselves, and are zeros in the product.
+//
+// Whether an LDS tile of KEYS rows of D holds an infinity or NaN.
+template <class M, int KEYS, int D, class P>
+__device__ __forceinline__ bool any_special(P tile) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u16x2 most = {0, 0};
+#pragma unroll
+  for (int i = 0; i < KEYS * D / 512; ++i) {
+    const u32x4 w =
+        *(__attribute__((address_space(3))) const u32x4*)(tile + i * 512 + (threadIdx.x & 63) * 8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = w[j] & 0x7fff7fffu;
+      u16x2 y;
+      __builtin_memcpy(&y, &x, 4);
+      most = __builtin_elementwise_max(most, y);
+    }
+  }
+  return __builtin_amdgcn_ballot_w64(most[0] >= M::kInf || most[1] >= M::kInf) != 0;
+}
+// The infinities and NaN of two values, zeros for others.
+template <class M>
+__device__ __forceinline__ uint32_t special(uint32_t w) {
+  const uint32_t lo = (w & 0x7fffu) >= M::kInf ? 0xffffu : 0u;
+  const uint32_t hi = (w & 0x7fff0000u) >= M::kInf << 16 ? 0xffff0000u : 0u;
+  return w & (lo | hi);
+}
+// o += the infinities and NaN of the first `seen` of KEYS keys of a V tile
+// (o[dt][r 4 + i]: column dt 32 + r 8 + g 4 + i; key j's chunk x of 8 columns at
+// x ^ 4 (j & 3)).
+template <class M, int KEYS, int D, class P>
+__device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int seen, int g) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll 1
+      for (int j = 0; j < KEYS; ++j) {
+        const int ch = (dt * 4 + r) ^ ((4 * (j & 3)) % (D / 8));
+        const u32x2 w =
+            *(__attribute__((address_space(3))) const u32x2*)(tile + j * D + ch * 8 + g * 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x = j < seen ? special<M>(w[i]) : 0u;
+          o[dt][r * 4 + i * 2] += M::lo(x);
+          o[dt][r * 4 + i * 2 + 1] += M::hi(x);
+        }
+      }
+}
+// The tile's infinities and NaN become zeros; thread t of N has its part.
+template <class M, int KEYS, int D, int N, class P>
+__device__ __forceinline__ void clear_special(P tile, int t) {
+#pragma unroll 1
+  for (int i = t; i < KEYS * D / 2; i += N) {
+    auto* p = (__attribute__((address_space(3))) uint32_t*)tile + i;
+    *p ^= special<M>(*p);
+  }
 }
 // O and the sum take the factor of soft_max.
 template <int DT>

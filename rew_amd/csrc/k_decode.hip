@@ -140,6 +140,11 @@ __global__ void __launch_bounds__(64, D == 128 ? 1 : 2) decode_kernel(PackedArgs
                                             : soft_max<M, false, 1>(s, vis, sl2, m_run);
       soft_rescale<DT>(o, l_run, alpha);
       soft_exp<M, 1>(s, sl2, m_run, pk, l_run);
+      if (least < min(k0 + BK, r.cap) && any_special<M, BK, D>(st + TILE)) {
+        add_special<M, BK, D>(o, st + TILE, my_limit - k0, g);
+        clear_special<M, BK, D, 64>(st + TILE, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         union {

@@ -48,12 +48,17 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 // kGradShift - log2(e) lse, and -delta.  float16 has no room for dS at any scale:
 // it is stored as F dS, F the power of two that takes the bound
 // |dS| <= 2 D max|dout| max|V| to 2^15, so this kernel also leaves the maxima
-// of its workgroups (a maximum does not depend on their order).
+// of its workgroups (a maximum does not depend on their order): over the
+// sequences' rows, and over finite values, so that neither what lies outside
+// the sequences nor one sequence's infinity takes the others' bits.
 template <class M, int D>
 __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   constexpr int L = D / 8;
   const int64_t rows = a.T * a.H, step = gridDim.x * (256ll / L);
   const int ch = threadIdx.x % L;
+  const int64_t tok0 = seq_bound(a.starts, a.n_seq, (int)a.T, 0);
+  const int64_t tok1 = seq_bound(a.starts, a.n_seq, (int)a.T, a.n_seq);
+  auto finite = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; };
   float *neg_lse = (float*)a.work, *neg_delta = neg_lse + rows;
   float most = 0.0f, most_v = 0.0f;
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
@@ -70,7 +75,9 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
       rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
       rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
       row = fmaxf(row, fmaxf(fabsf(x0), fabsf(x1)));
-      if constexpr (M::kScaled) most = fmaxf(most, fmaxf(fabsf(y0), fabsf(y1)));
+      if constexpr (M::kScaled) {
+        if (i >= tok0 * a.H && i < tok1 * a.H) most = fmaxf(most, fmaxf(finite(y0), finite(y1)));
+      }
     }
 #pragma unroll
     for (int d = L / 2; d > 0; d >>= 1) {
@@ -85,11 +92,11 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
     }
   }
   if constexpr (M::kScaled) {
-    const int64_t n = a.T * a.Hkv * L;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t n = tok1 * a.Hkv * L;
+    for (int64_t i = tok0 * a.Hkv * L + blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
       const uint4 x = ((const uint4*)a.v)[i];
       for (uint32_t w : {x.x, x.y, x.z, x.w})
-        most_v = fmaxf(most_v, fmaxf(fabsf(M::lo(w)), fabsf(M::hi(w))));
+        most_v = fmaxf(most_v, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
     }
     __shared__ float part[8];
 #pragma unroll

@@ -43,14 +43,17 @@ struct BlockRows {
 // block's rows over key tiles [kt0, kt1) of a sequence that starts at token
 // `first` (or, PAGED, of the request with block table `table`): `cap` keys,
 // this lane's row sees those below my_limit, every row of the wave those below
-// `least`.  Four waves; ends with a barrier behind the last read of LDS.
+// `least`, every row of the block those below block_least.  Four waves; ends
+// with a barrier behind the last read of LDS.
 template <class M, int D, bool PAGED>
 __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRows& br, int first,
                                              const int32_t* table, int hk, int cap, int my_limit,
-                                             int least, int kt0, int kt1, f32x16_t (&o)[D / 32],
+                                             int least, int block_least, int kt0, int kt1,
+                                             f32x16_t (&o)[D / 32],
                                              float& m_run, float& l_run) {
   using namespace pa;
   typedef typename M::frag frag;
+  typedef __attribute__((address_space(3))) uint16_t lds_u16;
   constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, TILE = BK * D;
   constexpr int RPD = 64 / CPR;         // key rows per DMA instruction
   constexpr int NDMA = TILE / 512 / 4;  // instructions per wave and K (or V) tile
@@ -129,7 +132,7 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
   l_run = 0.0f;
   const float sl2 = a.scale * kLog2e;
 
-  auto k_tile = [&](const uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n,
+  auto k_tile = [&](const uint16_t* ks, uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n,
                     int kt) {
     const uint64_t none = none_next;
     if (kt + 1 < kt1) dma_tile(ks_n, vs_n, kt + 1);
@@ -167,6 +170,13 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
                                           : soft_max<M, false, 2>(s, vis, sl2, m_run);
     soft_rescale<DT>(o, l_run, alpha);
     soft_exp<M, 2>(s, sl2, m_run, pk, l_run);
+    // (the same answer in all waves)
+    if (block_least < min(k0 + BK, cap) && any_special<M, BK, D>((lds_u16*)vs)) {
+      add_special<M, BK, D>(o, (lds_u16*)vs, my_limit - k0, g);
+      __syncthreads();
+      clear_special<M, BK, D, 256>((lds_u16*)vs, threadIdx.x);
+      __syncthreads();
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       union {
@@ -222,8 +232,9 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   f32x16_t o[DT];
   float m_run, l_run;
   attend_block<M, D, false>(a, br, st.first, nullptr, hk, len, limit(br.row),
-                            uniform(limit(st.tile * BR + (threadIdx.x >> 6) * 32)), 0,
-                            (limit(st.tile * BR + BR - 1) + BK - 1) / BK, o, m_run, l_run);
+                            uniform(limit(st.tile * BR + (threadIdx.x >> 6) * 32)),
+                            limit(st.tile * BR), 0, (limit(st.tile * BR + BR - 1) + BK - 1) / BK, o,
+                            m_run, l_run);
   const float l = fa_sum_halves(l_run);
   if (br.row >= rows) return;
   const int64_t at = (int64_t)(st.first + br.tok) * a.H + hk * G + br.hg;
@@ -363,6 +374,7 @@ __global__ void __launch_bounds__(256, 2) chunk_attn_kernel(PackedArgs a) {
   attend_block<M, D, true>(a, br, r.first, real ? a.table + (int64_t)at.s * a.width : nullptr,
                            at.hk, r.cap, r.limit(a, G, br.row),
                            uniform(r.limit(a, G, at.qt * BR + (threadIdx.x >> 6) * 32)),
+                           r.limit(a, G, at.qt * BR),
                            (int)((int64_t)tiles * at.part / at.P),
                            (int)((int64_t)tiles * (at.part + 1) / at.P), o, m_run, l_run);
   const float l = fa_sum_halves(l_run);
