@@ -528,7 +528,7 @@ void launch_rmsnorm_rows(const RowNormArgs& a, hipStream_t stream) {
     const int ch = (int)((chunks + 63) / 64);
     // whole rows of 2, 4 or 8 chunks per lane: the pipelined kernel, at most
     // 2048 waves (two workgroups per CU)
-    if (chunks == 64 * ch && ch <= 8 && ((uintptr_t)a.gamma & 15) == 0) {
+    if (chunks == 64 * ch && (ch == 2 || ch == 4 || ch == 8) && ((uintptr_t)a.gamma & 15) == 0) {
       const dim3 grid_pipe((unsigned)(blocks < 512 ? blocks : 512));
 #define REW_RMS(XB, YB, CH) hipLaunchKernelGGL((rmsnorm_pipe_kernel<XB, YB, CH>), grid_pipe, block, 0, stream, a)
 #define REW_RMS_CH(XB, YB) \
