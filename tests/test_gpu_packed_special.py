@@ -53,15 +53,16 @@ def test_packed_later_keys(gpu, dtype, H, Hkv, D, which, value):
                                               clean[row][np.isfinite(seen)])
 
 
-@pytest.mark.parametrize("news,lens", [([3, 1, 6], [130, 40, 6]), ([150, 1, 70], [500, 300, 70])],
-                         ids=["few", "chunks"])
+@pytest.mark.parametrize("news,lens,width", [
+    ([3, 1, 6], [130, 40, 6], None), ([3, 1, 6], [130, 40, 6], 300),
+    ([150, 1, 70], [500, 300, 70], None)], ids=["few", "few_wide", "chunks"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("value", SPECIAL)
-def test_paged_later_keys(gpu, news, lens, dtype, D, value):
+def test_paged_later_keys(gpu, news, lens, width, dtype, D, value):
     """The last new token of each request holds it in V: only its own row sees it."""
     r = np.random.default_rng(D + len(news))
-    c = paged_case(r, news, lens, 8, 2, D, 16, dtype)
+    c = paged_case(r, news, lens, 8, 2, D, 16, dtype, width=width)
     clean = E.toHostF32(paged_call(c))
     for n, row in zip(lens, c["table"]):
         c["vh"][row[(n - 1) // 16], :, (n - 1) % 16, 3::7] = value

@@ -150,6 +150,18 @@ def test_paged_attention(gpu, step, H, Hkv, D, page, dtype):
     check(paged_call(c, maxNew=max(news)), want, R.out_bound(want, mag, dtype))
 
 
+@pytest.mark.parametrize("step", ["first", "decode", "many", "verify"])
+@pytest.mark.parametrize("H,Hkv,D,page", [(4, 4, 32, 1), (8, 2, 64, 16), (6, 2, 128, 128)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_wide_tables(gpu, step, H, Hkv, D, page, dtype):
+    """A table with room for many more keys chooses other kernels."""
+    news, lens = STEPS[step]
+    r = np.random.default_rng(sum(lens) + D + page)
+    c = paged_case(r, news, lens, H, Hkv, D, page, dtype, width=5000 // page)
+    want, mag = paged_want(c, True, D ** -0.5)
+    check(paged_call(c), want, R.out_bound(want, mag, dtype))
+
+
 @pytest.mark.parametrize("step", ["decode", "mixed"])
 def test_paged_attention_all_keys_and_scale(gpu, step):
     news, lens = STEPS[step]
