@@ -17,7 +17,7 @@ from typing import Sequence
 import numpy as np
 
 from . import ops as O
-from .eager import DType, Tensor, TensorError
+from .eager import DType, Tensor, TensorError, empty
 
 
 def _f32(x: Tensor) -> Tensor:
@@ -232,6 +232,20 @@ class RotaryPositionEncoding:
         # mixed precision: the tables are fp32, so the rotation runs in fp32
         return _to(applyRotate(_f32(x), cosB, sinB), x.dtype)
 
+    def forwardAt(self, x: Tensor, positions: Tensor) -> Tensor:
+        """x [tokens, heads, headDim], row t rotated by the position ``positions[t]`` (an
+        integer tensor; the tables' last row for one of maxSeqLen or more).  A backend
+        extension for packed and paged rows."""
+        if len(x.shape) != 3 or tuple(positions.shape) != (x.shape[0],):
+            raise TensorError("RotaryPositionEncoding.forwardAt: x must be [tokens, heads, "
+                              f"headDim] and positions [tokens], got {list(x.shape)} and "
+                              f"{list(positions.shape)}")
+        if x.shape[2] != self.headDim:
+            raise TensorError("RotaryPositionEncoding.forwardAt: headDim mismatch")
+        cosB, sinB = (O.broadcastTo(O.torchIndexSelect(t, positions, 0, 0), x.shape, [0, 2])
+                      for t in (self.cosCached, self.sinCached))
+        return _to(applyRotate(_f32(x), cosB, sinB), x.dtype)
+
 
 # ---- attention (src/rew/nn/attention.nim:18-81) ------------------------------------------
 
@@ -269,6 +283,29 @@ def scaledDotProductAttention(q: Tensor, k: Tensor, v: Tensor, causal: bool = Fa
     attn = softmax(scores, len(scores.shape) - 1)
     attn = _to(attn, v.dtype)
     return O.dotGeneral(attn, v, batchDims, batchDims, [rank - 1], [rank - 2])
+
+
+@dataclass
+class PagedKVCache:
+    """The keys and values of one layer's requests: pages of ``pageSize`` tokens, of which a
+    request's block table names those it has.  One ``ops.pagedBlockTables`` per serving step
+    serves all layers.  A backend extension."""
+    kPages: Tensor  # [pages, numKVHeads, pageSize, headDim]
+    vPages: Tensor
+
+    @staticmethod
+    def init(pages: int, numKVHeads: int, pageSize: int, headDim: int,
+             dtype: DType = DType.BFLOAT16, device=None) -> "PagedKVCache":
+        """The memory is not cleared: a request reads the rows that its steps wrote."""
+        shape = (pages, numKVHeads, pageSize, headDim)
+        return PagedKVCache(empty(dtype, shape, device), empty(dtype, shape, device))
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor, step: O.PagedStep, causal: bool = True,
+               scale: float = 0.0, maxNew: int = 0) -> Tensor:
+        """Writes the step's new keys and values, then attends over all."""
+        O.pagedCacheWrite(self.kPages, self.vPages, k, v, step.slots)
+        return O.pagedAttention(q, self.kPages, self.vPages, step.blockTable, step.starts,
+                                step.lens, causal, scale, maxNew)
 
 
 @dataclass
@@ -314,6 +351,38 @@ class GroupedQueryAttention:
         outFlat = self.outProj.forward(attnFlat2d)
         return O.reshape(outFlat, [batch, seqLen, outFlat.shape[1]])
 
+    def _rows(self, x: Tensor, positions: Tensor | None):
+        """Rotated q [tokens, heads, headDim], rotated k and v [tokens, KV heads, headDim]."""
+        if len(x.shape) != 2:
+            raise TensorError("GroupedQueryAttention: packed rows must be [tokens, embed], got "
+                              f"{list(x.shape)}")
+        if self.rope is not None and positions is None:
+            raise TensorError("GroupedQueryAttention: rotary encoding needs positions")
+        n = x.shape[0]
+        q = O.reshape(self.qProj.forward(x), [n, self.numHeads, self.headDim])
+        k = O.reshape(self.kProj.forward(x), [n, self.numKVHeads, self.headDim])
+        v = O.reshape(self.vProj.forward(x), [n, self.numKVHeads, self.headDim])
+        if self.rope is not None:
+            q, k = self.rope.forwardAt(q, positions), self.rope.forwardAt(k, positions)
+        return q, k, v
+
+    def _project(self, attn: Tensor) -> Tensor:
+        return self.outProj.forward(O.reshape(attn, [attn.shape[0],
+                                                     self.numHeads * self.headDim]))
+
+    def forwardPacked(self, x: Tensor, starts: Tensor, positions: Tensor | None = None,
+                      causal: bool = True) -> Tensor:
+        """Self-attention over packed sequences, x [tokens, embed] (``ops.packedAttention``)."""
+        q, k, v = self._rows(x, positions)
+        return self._project(O.packedAttention(q, k, v, starts, causal))
+
+    def forwardPaged(self, x: Tensor, cache: PagedKVCache, step: O.PagedStep,
+                     causal: bool = True, maxNew: int = 0) -> Tensor:
+        """A serving step's new tokens x [tokens, embed] over their requests' cache, which
+        takes their keys and values (``ops.pagedAttention``)."""
+        q, k, v = self._rows(x, step.positions)
+        return self._project(cache.attend(q, k, v, step, causal, maxNew=maxNew))
+
 
 # ---- models (src/rew/models/llama.nim:106-117, deepseek.nim:74-145) -----------------------
 
@@ -331,6 +400,24 @@ class LlamaDecoderLayer:
         normed2 = _to(self.postAttentionLayernorm.forward(_f32(res)), x.dtype)
         mlp = self.mlp.forward(normed2)
         return O.add(res, mlp)
+
+    def _around(self, x: Tensor, attention) -> Tensor:
+        res = O.add(x, attention(_to(self.inputLayernorm.forward(_f32(x)), x.dtype)))
+        normed = _to(self.postAttentionLayernorm.forward(_f32(res)), x.dtype)
+        mlp = self.mlp.forward(O.reshape(normed, [1, *normed.shape]))
+        return O.add(res, O.reshape(mlp, list(res.shape)))
+
+    def forwardPacked(self, x: Tensor, starts: Tensor, positions: Tensor | None = None,
+                      causal: bool = True) -> Tensor:
+        """The layer over packed sequences, x [tokens, embed]."""
+        return self._around(x, lambda n: self.selfAttn.forwardPacked(n, starts, positions,
+                                                                     causal))
+
+    def forwardPaged(self, x: Tensor, cache: PagedKVCache, step: O.PagedStep,
+                     causal: bool = True, maxNew: int = 0) -> Tensor:
+        """The layer over a serving step's new tokens, x [tokens, embed]."""
+        return self._around(x, lambda n: self.selfAttn.forwardPaged(n, cache, step, causal,
+                                                                    maxNew))
 
 
 @dataclass

@@ -768,8 +768,9 @@ def fft(a: Tensor, fftType: str, fftLength: Sequence[int]) -> Tensor:
 def _packed_call(op: str, operands, attrs, nouts: int) -> list:
     if _jit.currentMode() == "trace":
         raise TensorError(f"{op}: eager only (it has no StableHLO form)")
-    for t in operands[1:]:
-        if t.device != operands[0].device:
+    d = operands[0].device
+    for t in operands:
+        if t.device is not d and t.device != d:
             raise TensorError(f"{op}: device mismatch")
     outs = dispatchEager(op, operands, attrs)
     assert len(outs) == nouts, f"{op}: eager backend returned wrong arity"
@@ -778,8 +779,9 @@ def _packed_call(op: str, operands, attrs, nouts: int) -> list:
 
 def _check_i32(op: str, t: Tensor, name: str, shape) -> None:
     """`shape`: the extents, None where any will do."""
-    if t.dtype != DType.INT32 or len(t.shape) != len(shape) or any(
-            w is not None and w != d for w, d in zip(shape, t.shape)):
+    if t.dtype != DType.INT32 or t.shape != shape and (
+            len(t.shape) != len(shape) or
+            any(w is not None and w != d for w, d in zip(shape, t.shape))):
         want = ["*" if w is None else w for w in shape]
         raise TensorError(f"{op}: {name} must be int32 {want}, got {t.dtype.rew_name} "
                           f"{list(t.shape)}")
@@ -826,7 +828,7 @@ def _attn_attrs(op: str, causal: bool, scale: float) -> list:
     if not 0.0 <= scale < float("inf"):
         raise TensorError(f"{op}: scale must be a finite number >= 0, got {scale}")
     return [("causal", "true" if causal else "false"),
-            ("scale", repr(float(np.float32(scale))))]
+            ("scale", repr(float(np.float32(scale))) if scale else "0.0")]
 
 
 class PackedStats(NamedTuple):
@@ -877,14 +879,24 @@ def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Te
                               _attn_attrs(op, causal, scale), 3))
 
 
+class PagedStep(NamedTuple):
+    """The tables of one serving step (``pagedBlockTables``), all int32."""
+    blockTable: Tensor  # [requests, blocks]
+    slots: Tensor       # [tokens]
+    positions: Tensor   # [tokens]
+    starts: Tensor      # [requests + 1]
+    lens: Tensor        # [requests]
+    taken: Tensor       # [1]
+
+
 def pagedBlockTables(cachedLens: Tensor, newLens: Tensor, blockTable: Tensor,
-                     freePages: Tensor, pageSize: int, tokens: int):
+                     freePages: Tensor, pageSize: int, tokens: int) -> PagedStep:
     """The tables of a serving step that adds ``newLens[r]`` tokens to request r, which has
     ``cachedLens[r]`` tokens in the pages ``blockTable[r]`` (all int32; blockTable
     [requests, blocks]).  Requests that need more pages take them from the front of
     ``freePages``, in request order.  ``tokens``: the sum of newLens, or more.
 
-    Returns int32 (blockTable, slots, positions, starts, lens, taken):
+    Returns (blockTable, slots, positions, starts, lens, taken), all int32:
 
     * blockTable [requests, blocks]: the pages each request had, then the new ones; -1 behind
       them, and where freePages ran out;
@@ -905,8 +917,8 @@ def pagedBlockTables(cachedLens: Tensor, newLens: Tensor, blockTable: Tensor,
     _check_i32(op, freePages, "freePages", (None,))
     if tokens < 0:
         raise TensorError(f"{op}: tokens must be non-negative, got {tokens}")
-    return tuple(_packed_call(op, [cachedLens, newLens, blockTable, freePages],
-                              [("page_size", str(pageSize)), ("tokens", str(tokens))], 6))
+    return PagedStep(*_packed_call(op, [cachedLens, newLens, blockTable, freePages],
+                                   [("page_size", str(pageSize)), ("tokens", str(tokens))], 6))
 
 
 def pagedCacheWrite(kPages: Tensor, vPages: Tensor, k: Tensor, v: Tensor,
