@@ -10,6 +10,7 @@ namespace rew {
 
 namespace {
 constexpr int kThreads = 256;
+constexpr int kResident = 256 * 8;  // workgroups of the tables kernel on 256 CUs
 
 __device__ __forceinline__ int64_t blocks_of(int64_t n, int log_page) {
   return (n + (1ll << log_page) - 1) >> log_page;
@@ -80,9 +81,11 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(PageTablesArgs a)
 }
 
 void launch_page_tables(const PageTablesArgs& a, hipStream_t stream) {
-  // shares per request: about one table row or token run per thread
+  // shares per request: about one table row or token run per thread, as long as
+  // all workgroups run at once (each has the same sums to do first)
   const int64_t per = std::max(a.width, a.tokens / std::max<int64_t>(a.n, 1));
-  const unsigned y = (unsigned)std::min<int64_t>(16, std::max<int64_t>(1, per / kThreads));
+  const int64_t most = std::min<int64_t>(16, kResident / (a.n + 1));
+  const unsigned y = (unsigned)std::max<int64_t>(1, std::min(most, per / kThreads));
   hipLaunchKernelGGL(page_tables_kernel, dim3((unsigned)(a.n + 1), y), dim3(kThreads), 0, stream,
                      a);
   REW_HIP(hipGetLastError());

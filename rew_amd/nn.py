@@ -232,19 +232,21 @@ class RotaryPositionEncoding:
         # mixed precision: the tables are fp32, so the rotation runs in fp32
         return _to(applyRotate(_f32(x), cosB, sinB), x.dtype)
 
-    def forwardAt(self, x: Tensor, positions: Tensor) -> Tensor:
-        """x [tokens, heads, headDim], row t rotated by the position ``positions[t]`` (an
-        integer tensor; the tables' last row for one of maxSeqLen or more).  A backend
-        extension for packed and paged rows."""
-        if len(x.shape) != 3 or tuple(positions.shape) != (x.shape[0],):
-            raise TensorError("RotaryPositionEncoding.forwardAt: x must be [tokens, heads, "
-                              f"headDim] and positions [tokens], got {list(x.shape)} and "
-                              f"{list(positions.shape)}")
-        if x.shape[2] != self.headDim:
-            raise TensorError("RotaryPositionEncoding.forwardAt: headDim mismatch")
-        cosB, sinB = (O.broadcastTo(O.torchIndexSelect(t, positions, 0, 0), x.shape, [0, 2])
-                      for t in (self.cosCached, self.sinCached))
-        return _to(applyRotate(_f32(x), cosB, sinB), x.dtype)
+    def forwardAt(self, xs: Sequence[Tensor], positions: Tensor) -> list:
+        """Each x of ``xs`` [tokens, heads, headDim] with row t rotated by the position
+        ``positions[t]`` (an integer tensor; the tables' last row for one of maxSeqLen or
+        more).  A backend extension for packed and paged rows."""
+        for x in xs:
+            if len(x.shape) != 3 or tuple(positions.shape) != (x.shape[0],):
+                raise TensorError("RotaryPositionEncoding.forwardAt: x must be [tokens, heads, "
+                                  f"headDim] and positions [tokens], got {list(x.shape)} and "
+                                  f"{list(positions.shape)}")
+            if x.shape[2] != self.headDim:
+                raise TensorError("RotaryPositionEncoding.forwardAt: headDim mismatch")
+        cos, sin = (O.torchIndexSelect(t, positions, 0, 0)
+                    for t in (self.cosCached, self.sinCached))
+        return [_to(applyRotate(_f32(x), O.broadcastTo(cos, x.shape, [0, 2]),
+                                O.broadcastTo(sin, x.shape, [0, 2])), x.dtype) for x in xs]
 
 
 # ---- attention (src/rew/nn/attention.nim:18-81) ------------------------------------------
@@ -363,7 +365,7 @@ class GroupedQueryAttention:
         k = O.reshape(self.kProj.forward(x), [n, self.numKVHeads, self.headDim])
         v = O.reshape(self.vProj.forward(x), [n, self.numKVHeads, self.headDim])
         if self.rope is not None:
-            q, k = self.rope.forwardAt(q, positions), self.rope.forwardAt(k, positions)
+            q, k = self.rope.forwardAt([q, k], positions)
         return q, k, v
 
     def _project(self, attn: Tensor) -> Tensor:

@@ -93,10 +93,11 @@ def test_rope_at_positions(gpu):
     rope = nn.RotaryPositionEncoding.init(64, 96, 10000.0)
     x = np.random.default_rng(0).standard_normal((50, 3, 64)).astype(np.float32)
     want = host(rope.forward(dev(x.transpose(1, 0, 2)), 7)).transpose(1, 0, 2)
-    got = host(rope.forwardAt(dev(x), ints(np.arange(7, 57))))
+    got, twice = map(host, rope.forwardAt([dev(x), dev(2 * x[:, :1])], ints(np.arange(7, 57))))
+    np.testing.assert_array_equal(twice, 2 * got[:, :1])
     np.testing.assert_allclose(got, want, rtol=0, atol=4 * 2.0 ** -23 * np.abs(x).max())
-    last = host(rope.forwardAt(dev(x), ints(np.full(50, 95))))
-    np.testing.assert_array_equal(host(rope.forwardAt(dev(x), ints(np.full(50, 1000)))), last)
+    last, far = (host(rope.forwardAt([dev(x)], ints(np.full(50, p)))[0]) for p in (95, 1000))
+    np.testing.assert_array_equal(far, last)
 
 
 def _replays(capture, other, times=4):
