@@ -1696,7 +1696,7 @@ static std::vector<Tensor*> run_page_write(Ctx* c, const std::vector<Tensor*>& i
   if (!kp->writable || !vp->writable)
     invalid("eager '" + op + "': kPages and vPages must come from rew_mi355x_alloc (other "
             "tensors are immutable)");
-  if (kp->st == vp->st) invalid("eager '" + op + "': kPages and vPages are one tensor");
+  if (kp == vp) invalid("eager '" + op + "': kPages and vPages are one tensor");
   if (k->shape.rank != 3 || k->shape != v->shape || k->dt != v->dt)
     invalid("eager '" + op + "': k and v must be [tokens, kvHeads, headDim] of one dtype, got " +
             k->shape.str() + " and " + v->shape.str());
@@ -1717,6 +1717,9 @@ static std::vector<Tensor*> run_page_write(Ctx* c, const std::vector<Tensor*>& i
   flush(c);
   for (Tensor* t : ins)
     if (!t->st) invalid("eager '" + op + "': an operand has no data (an earlier flush failed)");
+  // a reshape of the pages that is alive would change with them
+  if (kp->st->refs != 1 || vp->st->refs != 1)
+    invalid("eager '" + op + "': kPages or vPages shares its memory with another tensor");
   PageWriteArgs a;
   std::memset(&a, 0, sizeof a);
   a.k = k->data();

@@ -928,8 +928,9 @@ def pagedCacheWrite(kPages: Tensor, vPages: Tensor, k: Tensor, v: Tensor,
     slots[t] % pageSize of every KV head.  A negative slot, or one past the pages, writes
     nothing.  Slots must be distinct: of two tokens in one slot either may stay, in parts.
 
-    The one op that changes its operands: the pages must come from ``eager.empty``.  What was
-    recorded before reads the old rows, what is recorded later the new ones."""
+    The one op that changes its operands: the pages must come from ``eager.empty``, and no
+    tensor that shares their memory (a reshape of them) may be alive.  What was recorded before
+    reads the old rows, what is recorded later the new ones."""
     op = "pagedCacheWrite"
     _check_pages(op, kPages, vPages)
     if len(k.shape) != 3 or k.shape != v.shape or k.dtype != v.dtype:

@@ -163,3 +163,15 @@ def test_library_refusals(gpu):
            [("page_size", "4"), ("tokens", "-2")])
     refuse("eager", "pagedBlockTables", [ints([1]), i2, tab, i2],
            [("page_size", "4"), ("tokens", "2")])
+
+
+def test_write_beside_a_view(gpu):
+    """Pages that another tensor shares are not changed under it."""
+    pages = [E.empty(DType.BFLOAT16, (2, 1, 4, 32)) for _ in range(2)]
+    row, slot = E.empty(DType.BFLOAT16, (1, 1, 32)), ints([5])
+    for p in pages:
+        view = O.reshape(p, [8, 1, 32])
+        with pytest.raises(EagerError, match="shares its memory"):
+            O.pagedCacheWrite(*pages, row, row, slot)
+        del view
+    O.pagedCacheWrite(*pages, row, row, slot)
