@@ -106,7 +106,8 @@ int rew_mi355x_from_host(rew_mi355x_ctx* ctx, int dtype, const int64_t* shape,
 int rew_mi355x_to_host(rew_mi355x_buf* buf, void* host, int64_t nbytes);
 
 /* A new tensor of `dtype`/`shape` whose contents are undefined until a
- * caller writes them on the device (through rew_mi355x_buf_device_ptr).
+ * caller writes them on the device (through rew_mi355x_buf_device_ptr, or,
+ * pages of a key/value cache, by the op pagedCacheWrite).
  * Replaces: the uninitialised-buffer slot of the PJRT C API that rew's
  * binding carries (fnClientCreateUninitializedBuffer,
  * src/rew/pjrt/capi.nim:109); the shim's alloc(ctx, bytes, &h). */
@@ -137,10 +138,14 @@ int rew_mi355x_retain(rew_mi355x_buf* buf);
 void rew_mi355x_release(rew_mi355x_buf* buf);
 
 /* Execute one eager op.  `op` is the op name rew's {.rewOp.} procs pass to
- * dispatchEager; `attr_keys`/`attr_vals` are the same stringly-typed attrs
+ * dispatchEager (and those of the backend's own ops, such as packedAttention);
+ * `attr_keys`/`attr_vals` are the same stringly-typed attrs
  * in the same wire format ("[1,2]", "@[1, 2]", "float32", "dtInt32",
  * "cpu:0", ...).  On success writes up to `max_outs` new handles (each with
  * one owner reference) and their count.  Errors carry the op name.
+ * One op changes its operands: pagedCacheWrite flushes what is pending, then
+ * writes rows into two tensors made by rew_mi355x_alloc whose memory nothing
+ * else shares, in the order of the context's stream, and has no outputs.
  * Replaces: executeEagerOp, the EagerBackend installed by
  * installEagerBackend (src/rew/eager.nim:1717-1772, src/rew/dispatch.nim:47-50, 75-85). */
 int rew_mi355x_execute(rew_mi355x_ctx* ctx, const char* op,

@@ -8,7 +8,7 @@
 // chain of dependent steps (about 2 us), so it takes four workers on a CU, one
 // per SIMD, to ask for the memory's rate (D = 128: 64 KiB in flight per CU).
 // 64 requests of 400 to 16000 keys, 32 / 8 heads x 128: 198 us, 5.5 TB/s of keys
-// and values; two workers with tiles of 64 keys 225 us, with four stages of 32
+// and values, and 8 us of joining; two workers with tiles of 64 keys 225 us, with four stages of 32
 // keys 246 us.  The partial results lie behind the output in its own block:
 // two captured launches never share them.
 #include <algorithm>

@@ -11,7 +11,8 @@
 // x D where 5 would do, for sums whose order never changes (a single pass
 // would add dQ across workgroups with atomics).  The rows of the H / Hkv heads
 // of a KV head are walked together, so the sum over the group is part of the
-// accumulation.
+// accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16: 31,
+// 500 (0.71 PFLOP/s) and 295 us (0.90 PFLOP/s).
 //
 // In each product one operand stays in registers and the other is read from
 // LDS; S and dP come out with the operand in registers along the lanes, so P

@@ -849,7 +849,8 @@ def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: boo
     (unlike ``nn.makeCausalMask``, whose orientation is the reference's); otherwise all of
     them.  ``scale`` 0: 1 / sqrt(headDim).  The softmax is float32; the probabilities are
     rounded to the operands' dtype before the second product, the result once.  A row of no
-    sequence (before ``starts[0]``, behind ``starts[-1]``) gives zeros.
+    sequence (before ``starts[0]``, behind ``starts[-1]``) gives zeros.  What a row does not
+    see does not reach its result, infinities and NaN included.
 
     ``withLse``: (out, stats), the ``PackedStats`` that ``packedAttentionGrad`` takes."""
     _check_packed("packedAttention", q, k, v, starts)
@@ -864,7 +865,8 @@ def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Te
                         scale: float = 0.0):
     """(gradQ, gradK, gradV) of ``packedAttention(q, k, v, starts, causal, scale)`` for the
     gradient ``gradOut`` of its result, given its ``out`` and ``stats``.  gradK and gradV are
-    summed over the query heads of each KV head; sums are float32 in a fixed order."""
+    summed over the query heads of each KV head; sums are float32 in a fixed order.  An infinity
+    or NaN in a sequence may reach all of its gradients, but no other sequence's."""
     op = "packedAttentionGrad"
     _check_packed(op, q, k, v, starts)
     for t, name in ((out, "out"), (gradOut, "gradOut")):
@@ -959,7 +961,7 @@ def pagedAttention(q: Tensor, kPages: Tensor, vPages: Tensor, blockTable: Tensor
     ``packedAttention``.
 
     ``maxNew``: at least the largest n, if the caller knows it (0: not); it chooses the
-    kernels, never the result."""
+    kernels, and with them the order of sums, never what is computed."""
     op = "pagedAttention"
     _check_pages(op, kPages, vPages)
     _check_heads(op, q, kPages.dtype, kPages.shape[1], kPages.shape[3])
