@@ -385,31 +385,31 @@ size_t decode_ws_floats(const PackedArgs& a) {
 }
 
 template <class M, int D>
-static void launch_decode(const PackedArgs& a, hipStream_t stream) {
+static int launch_decode(const PackedArgs& a, hipStream_t stream) {
   if (const int64_t n = short_groups(a)) {
     hipLaunchKernelGGL((decode_block_kernel<M, D>), dim3((unsigned)n), dim3(64 * pd::kWaves), 0,
                        stream, a);
-    return;
+    return 1;
   }
   const unsigned W = (unsigned)decode_workers(a);
   hipLaunchKernelGGL((decode_kernel<M, D>), dim3(W), dim3(64), 0, stream, a);
-  if (W == 1) return;
+  if (W == 1) return 1;
   // the rows that a block is expected to hold, 1024 / D of them per workgroup
   const int64_t most = (a.max_new > 0 ? std::min(a.max_new, a.T) : a.T) * (a.H / a.Hkv);
   const unsigned y = (unsigned)((std::min<int64_t>(pd::kRows, most) * D + 1023) / 1024);
   hipLaunchKernelGGL((decode_join_kernel<M, D>), dim3(W - 1, y), dim3(256), 0, stream, a,
                      (int)W);
+  return 2;
 }
 template <class M>
-static void launch_decode_t(const PackedArgs& a, hipStream_t stream) {
-  if (a.D == 32) launch_decode<M, 32>(a, stream);
-  else if (a.D == 64) launch_decode<M, 64>(a, stream);
-  else launch_decode<M, 128>(a, stream);
+static int launch_decode_t(const PackedArgs& a, hipStream_t stream) {
+  if (a.D == 32) return launch_decode<M, 32>(a, stream);
+  if (a.D == 64) return launch_decode<M, 64>(a, stream);
+  return launch_decode<M, 128>(a, stream);
 }
 
-void launch_paged_decode(const PackedArgs& a, hipStream_t stream) {
-  if (a.f16) launch_decode_t<MmaF16>(a, stream);
-  else launch_decode_t<MmaBf16>(a, stream);
+int launch_paged_decode(const PackedArgs& a, hipStream_t stream) {
+  return a.f16 ? launch_decode_t<MmaF16>(a, stream) : launch_decode_t<MmaBf16>(a, stream);
 }
 
 }  // namespace rew

@@ -433,10 +433,7 @@ size_t paged_ws_bytes(const PackedArgs& a) {
 
 template <class M, int D>
 static int launch_prompt(const PackedArgs& a, hipStream_t stream) {
-  if (a.table && !expects_chunks(a)) {
-    launch_paged_decode(a, stream);
-    return 2;
-  }
+  if (a.table && !expects_chunks(a)) return launch_paged_decode(a, stream);
   const int64_t tiles = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pa::BR) * a.Hkv;
   if (tiles >= (1ll << 30)) fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention: too many tiles");
   if (!a.table) {

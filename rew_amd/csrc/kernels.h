@@ -581,8 +581,8 @@ size_t paged_ws_bytes(const PackedArgs& a);
 // 16-bit operands, D of 32, 64 or 128, Hkv divides H.  Returns the kernels
 // launched.
 int launch_packed_attn(const PackedArgs& a, hipStream_t stream);
-// The form for requests of few rows, tokens x H / Hkv (k_decode.hip).
-void launch_paged_decode(const PackedArgs& a, hipStream_t stream);
+// The form for requests of few rows, tokens x H / Hkv (k_decode.hip); likewise.
+int launch_paged_decode(const PackedArgs& a, hipStream_t stream);
 size_t decode_ws_floats(const PackedArgs& a);
 constexpr int kDecodeRows = 32;
 const char* packed_attn_variant(const PackedArgs& a);

@@ -175,3 +175,58 @@ def test_write_beside_a_view(gpu):
             O.pagedCacheWrite(*pages, row, row, slot)
         del view
     O.pagedCacheWrite(*pages, row, row, slot)
+
+
+def test_operands_that_are_views(gpu):
+    """Transposed, sliced, broadcast and computed operands, not yet materialized."""
+    r = np.random.default_rng(12)
+    T, H, D = 77, 4, 64
+    x, xh = tensor(r.standard_normal((H, T, D)), "bfloat16")
+    y, yh = tensor(r.standard_normal((T + 9, 2, 2 * D)), "bfloat16")
+    z, zh = tensor(r.standard_normal((T, D)), "bfloat16")
+    qh, kh = xh.transpose(1, 0, 2), yh[4:4 + T, :, D:]
+    vh = np.repeat(zh[:, None], 2, axis=1)
+    starts = [0, 20, 77]
+
+    def operands():
+        return (O.transpose(x, [1, 0, 2]),
+                O.slice_(y, [4, 0, D], [4 + T, 2, 2 * D], [1, 1, 1]),
+                O.broadcastTo(z, [T, 2, D], [0, 2]))
+
+    out, stats = O.packedAttention(*operands(), ints(starts), withLse=True)
+    want, _, mag = R.packed(qh, kh, vh, starts, True, D ** -0.5)
+    check(out, want, R.out_bound(want, mag, "bfloat16"))
+    one = O.broadcastTo(E.fromHost(np.float32(1.0).reshape(1), DType.BFLOAT16), [T, H, D], [0])
+    got = O.packedAttentionGrad(*operands(), ints(starts), out, stats, one)
+    for g, w, b in zip(got, *R.packed_grad(qh, kh, vh, starts, np.ones((T, H, D)), True,
+                                           D ** -0.5, "bfloat16")):
+        check(g, w, b)
+    page = 4
+    kp, vp = (E.empty(DType.BFLOAT16, (20, 2, page, D)) for _ in range(2))
+    _, k, v = operands()
+    O.pagedCacheWrite(kp, vp, k, v, O.iota(DType.INT32, [T], 0))
+    table = O.reshape(O.iota(DType.INT32, [20], 0), [1, 20])
+    check(O.pagedAttention(operands()[0], kp, vp, table, ints([0, T]), ints([T])),
+          *[f(*R.packed(qh, kh, vh, [0, T], True, D ** -0.5)[::2]) for f in
+            (lambda w, m: w, lambda w, m: R.out_bound(w, m, "bfloat16"))])
+
+
+@pytest.mark.parametrize("news", [[3, 0], [50, 2]])
+def test_nothing_to_attend(gpu, news):
+    """No requests, tables of no width, a cache of no pages, a free list of none."""
+    r = np.random.default_rng(1)
+    T = sum(news)
+    q, _ = tensor(r.standard_normal((T, 4, 64)), "bfloat16")
+    starts, lens = ints(np.concatenate([[0], np.cumsum(news)])), ints([60, 2])
+    kp, vp = (E.empty(DType.BFLOAT16, (3, 2, 16, 64)) for _ in range(2))
+    no_pages = [E.empty(DType.BFLOAT16, (0, 2, 16, 64)) for _ in range(2)]
+    for args in ((kp, vp, E.empty(DType.INT32, (0, 4)), ints([0]), E.empty(DType.INT32, (0,))),
+                 (kp, vp, E.empty(DType.INT32, (2, 0)), starts, lens),
+                 (*no_pages, ints([[0, 1, 2, 3], [2, 1, 0, 0]]), starts, lens)):
+        assert not E.toHostF32(O.pagedAttention(q, *args)).any()
+    k, _ = tensor(r.standard_normal((T, 2, 64)), "bfloat16")
+    O.pagedCacheWrite(*no_pages, k, k, O.iota(DType.INT32, [T], 0))
+    for table, pool in ((np.zeros((2, 0)), [4, 5]), (np.zeros((2, 4)), [])):
+        got = O.pagedBlockTables(ints([0, 0]), ints(news), ints(table), ints(pool), 16, T)
+        for g, w in zip(got, R.block_tables([0, 0], news, table.astype(np.int64), pool, 16, T)):
+            np.testing.assert_array_equal(E.toHost(g), w)
