@@ -340,6 +340,10 @@ struct PageWindow {
   __device__ __forceinline__ int page(int j) const {
     return __builtin_amdgcn_ds_bpermute(((j >> log_page) - base) * 4, id);
   }
+  // .. of a key j that is the same in all lanes
+  __device__ __forceinline__ int page_uniform(int j) const {
+    return __builtin_amdgcn_readlane(id, (j >> log_page) - base);
+  }
   __device__ __forceinline__ bool missing(int j) const {
     return (bad >> ((j >> log_page) - base)) & 1;
   }

@@ -93,6 +93,29 @@ struct DecodeRows {
                                               int hk, int kt, lds_u16* ks, lds_u16* vs) const {
     const int lane = threadIdx.x & 63, row_in = lane / CPR, pc = lane % CPR;
     win.reach(kt * pd::BK);
+    const uint32_t none =
+        win.any_missing(kt * pd::BK, pd::BK, cap)
+            ? (uint32_t)__builtin_amdgcn_ballot_w64(win.missing(kt * pd::BK + (lane & 31)))
+            : 0;
+    // whole tiles of whole pages: an instruction's rows lie in one page, whose
+    // address the scalar unit computes
+    if ((1 << a.log_page) >= RPD && none == 0 && kt * pd::BK + pd::BK <= cap) {
+#pragma unroll
+      for (int q = 0; q < NDMA; ++q) {
+        const int lr = q * RPD + row_in, j = kt * pd::BK + q * RPD;
+        const int64_t x = ((((int64_t)win.page_uniform(j) * a.Hkv + hk) << a.log_page) +
+                           (j & ((1 << a.log_page) - 1))) * D;
+        const uint32_t k = row_in * D + (pc ^ (lr % CPR)) * 8;
+        const uint32_t v = row_in * D + (pc ^ ((4 * (lr & 3)) % CPR)) * 8;
+        if constexpr (KEYS)
+          __builtin_amdgcn_global_load_lds((const uint16_t*)a.k + x + k,
+                                           (lds_void*)(ks + q * 512), 16, 0, 0);
+        if constexpr (VALUES)
+          __builtin_amdgcn_global_load_lds((const uint16_t*)a.v + x + v,
+                                           (lds_void*)(vs + q * 512), 16, 0, 0);
+      }
+      return none;
+    }
 #pragma unroll
     for (int q = 0; q < NDMA; ++q) {
       const int lr = q * RPD + row_in, j = kt * pd::BK + lr;
@@ -109,9 +132,7 @@ struct DecodeRows {
         __builtin_amdgcn_global_load_lds(there ? v : g_zero_row, (lds_void*)(vs + q * 512), 16, 0,
                                          0);
     }
-    return win.any_missing(kt * pd::BK, pd::BK, cap)
-               ? (uint32_t)__builtin_amdgcn_ballot_w64(win.missing(kt * pd::BK + (lane & 31)))
-               : 0;
+    return none;
   }
   __device__ __forceinline__ f32x16_t scores(lds_u16* ks) const {
     f32x16_t s;

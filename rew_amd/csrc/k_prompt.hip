@@ -88,8 +88,8 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
   for (int q = 0; q < NDMA; ++q) {
     const int r = (wave * NDMA + q) * RPD + row_in;
     const int ck = (pc ^ (r % CPR)) * 8, cv = (pc ^ ((4 * (r & 3)) % CPR)) * 8;
-    k_src[q] = PAGED ? (uint32_t)ck : (uint32_t)((r * kstride + ck) * 2);
-    v_src[q] = PAGED ? (uint32_t)cv : (uint32_t)((r * kstride + cv) * 2);
+    k_src[q] = PAGED ? (uint32_t)(row_in * D + ck) : (uint32_t)((r * kstride + ck) * 2);
+    v_src[q] = PAGED ? (uint32_t)(row_in * D + cv) : (uint32_t)((r * kstride + cv) * 2);
   }
   PageWindow win(table, table ? a.width : 0, a.log_page, a.pages);
   uint64_t none_next = 0;  // of the tile last requested: bit i for a key i without a page
@@ -99,13 +99,26 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
       none_next = win.any_missing(kt * BK, BK, cap)
                       ? __builtin_amdgcn_ballot_w64(win.missing(kt * BK + lane))
                       : 0;
+      // whole tiles of whole pages: an instruction's rows lie in one page, whose
+      // address the scalar unit computes beside the vector unit's work
+      if ((1 << a.log_page) >= RPD && none_next == 0 && kt * BK + BK <= cap) {
+#pragma unroll
+        for (int q = 0; q < NDMA; ++q) {
+          const int blk = wave * NDMA + q, j = kt * BK + blk * RPD;
+          const int64_t at = ((((int64_t)win.page_uniform(j) * a.Hkv + hk) << a.log_page) +
+                              (j & ((1 << a.log_page) - 1))) * D;
+          dma16(K + at + k_src[q], ks + blk * 512);
+          dma16(V + at + v_src[q], vs + blk * 512);
+        }
+        return;
+      }
 #pragma unroll
       for (int q = 0; q < NDMA; ++q) {
         const int j = kt * BK + (wave * NDMA + q) * RPD + row_in;
         const int pg = win.page(j);
         const bool there = pg >= 0 && j < cap;
         const int64_t at = ((((int64_t)(there ? pg : 0) * a.Hkv + hk) << a.log_page) +
-                            (j & ((1 << a.log_page) - 1))) * D;
+                            (j & ((1 << a.log_page) - 1)) - row_in) * D;
         const int blk = wave * NDMA + q;
         dma16(there ? K + at + k_src[q] : g_zero_row, ks + blk * 512);
         dma16(there ? V + at + v_src[q] : g_zero_row, vs + blk * 512);
@@ -326,6 +339,31 @@ struct ChunkPlan {
     }
     C = max((n + pa::kChunkSlots - 1) / pa::kChunkSlots, pa::kPieceTiles);
   }
+  // The 64 requests from `base`, one per lane, those of the longest pieces first,
+  // so that these start first.
+  struct Sorted {
+    int s, blocks, P;
+    __device__ __forceinline__ Sorted(const ChunkPlan& plan, int base) {
+      const int lane = threadIdx.x & 63;
+      const Share x = plan.share(base + lane);
+      const int piece =
+          x.blocks ? tiles_of(plan.a, plan.G, x.r, x.blocks / 2) / x.P : -1;
+      const int n = uniform(min(plan.a.n_seq + 1 - base, 64));
+      int rank = lane;
+      if (n > 1) {
+        rank = 0;
+        for (int j = 0; j < n; ++j) {
+          const int other = __builtin_amdgcn_readlane(piece, j);
+          rank += other > piece || (other == piece && j < lane);
+        }
+        if (lane >= n) rank = lane;
+      }
+      const int from = __builtin_amdgcn_ds_permute(rank * 4, lane) * 4;
+      s = base + from / 4;
+      blocks = __builtin_amdgcn_ds_bpermute(from, x.blocks);
+      P = __builtin_amdgcn_ds_bpermute(from, x.P);
+    }
+  };
 };
 // Workgroup `idx` of the plan's (or, SPLIT, of the split blocks' joins, one per
 // block and KV head).
@@ -338,7 +376,7 @@ struct ChunkPlace {
     int slots = 0;
     const int Hkv = plan.a.Hkv;
     for (int base = -1; base <= plan.a.n_seq; base += 64) {
-      const ChunkPlan::Share x = plan.share(base + (int)(threadIdx.x & 63));
+      const ChunkPlan::Sorted x(plan, base);
       const int pieces = x.P > 1 ? x.blocks * x.P * Hkv : 0;
       const int mine = !SPLIT ? x.blocks * x.P * Hkv : x.P > 1 ? x.blocks * Hkv : 0;
       const int sum = wave_scan(mine), psum = wave_scan(pieces);
@@ -350,7 +388,7 @@ struct ChunkPlace {
       }
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
       found = true;
-      s = base + at;
+      s = __builtin_amdgcn_readlane(x.s, at);
       r = request_at(plan.a, plan.G, s);
       P = __builtin_amdgcn_readlane(x.P, at);
       const int blocks = __builtin_amdgcn_readlane(x.blocks, at);
