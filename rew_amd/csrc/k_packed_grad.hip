@@ -12,7 +12,7 @@
 // would add dQ across workgroups with atomics).  The rows of the H / Hkv heads
 // of a KV head are walked together, so the sum over the group is part of the
 // accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16: 31,
-// 500 (0.71 PFLOP/s) and 295 us (0.90 PFLOP/s).
+// 450-510 (0.70-0.79 PFLOP/s) and 270-295 us (0.90-0.99 PFLOP/s) as the clock falls.
 //
 // In each product one operand stays in registers and the other is read from
 // LDS; S and dP come out with the operand in registers along the lanes, so P
@@ -344,7 +344,6 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
     const float* rt = R + slot(m) * 64 + g * 4;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      l4[e4] = *(const float4*)(rt + e4 * 8);
       const float4 d4 = *(const float4*)(rt + 32 + e4 * 8);
       const float d[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
@@ -353,9 +352,9 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
         dp[e4 * 4 + i] = d[i];
       }
     }
-    // Q, dout, K and V fragments are read two k-steps ahead (three: six registers
-    // too many, and a spill's reload costs half of the phase)
-    constexpr int AHEAD = 2;
+    // Q, dout, K and V fragments are read three k-steps ahead (two: 2 % more cycles;
+    // four: spills, whose reloads wait for every DMA)
+    constexpr int AHEAD = NT < 3 ? NT : 3;
     uint32_t qa = lds_at(Qt) + fr.rows, ka = lds_at(Ks) + kw * BLK * 2 + fr.rows,
              va = lds_at(Vs) + kw * BLK * 2 + fr.rows;
     opaque(ka);
@@ -375,12 +374,18 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
       dp = M::mma(f[t % AHEAD][2], f[t % AHEAD][3], dp);
       if (t + AHEAD < NT) read(t + AHEAD);
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, 8 + 4 * AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4 + 4 * AHEAD, 0);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
       if (t + AHEAD < NT) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
     }
+  };
+  // (before the next request: the compiler makes a read of R wait for a DMA into it)
+  auto read_lse = [&](int m) {
+    const float* rt = R + slot(m) * 64 + g * 4;
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) l4[e4] = *(const float4*)(rt + e4 * 8);
   };
   auto values = [&](int m) {
     if (!live(m)) return;
@@ -434,6 +439,7 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
     block_barrier_fa();
     for (int m = 1; m < n; ++m) {
       __builtin_amdgcn_s_setprio(0);
+      read_lse(m - 1);
       request(m);
       values(m - 1);
       vm_wait();
@@ -444,6 +450,7 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
       block_barrier_fa();
     }
     __builtin_amdgcn_s_setprio(0);
+    read_lse(n - 1);
     values(n - 1);
     if (grp == 0) block_barrier_fa();
     accumulate(n - 1);

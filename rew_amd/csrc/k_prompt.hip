@@ -306,11 +306,11 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
 // time (its 64 KiB are written and read), so P is the number of times that the
 // request's middle block holds C tiles, rounded, C being a CU's share of all
 // tiles or at least kPieceTiles: no block is split where the blocks fill the
-// CUs by themselves (2048 tokens over 30001 keys: 1.19 ms, 0.87 PFLOP/s; cut
+// CUs by themselves (2048 tokens over 30001 keys: 1.11 ms, 0.94 PFLOP/s; cut
 // into 512 equal runs, 1.30 ms and 140 us of joining).  Single tokens of other
 // requests in the same step are blocks of few rows here: 13 requests of 1 to
-// 539 new tokens over up to 4400 keys take 52 us and 6 us of joining, with
-// pieces of 8 or 12 tiles the same, of 24 more.
+// 539 new tokens over up to 4400 keys take 47 us and 8 us of joining, with
+// pieces of 8 or 12 tiles the same, of 20 more.
 struct ChunkPlan {
   const PackedArgs& a;
   int G, C;
