@@ -1691,6 +1691,8 @@ static std::vector<Tensor*> run_page_write(Ctx* c, const std::vector<Tensor*>& i
   const std::string op = "pagedCacheWrite";
   if (ins.size() != 5)
     invalid("eager '" + op + "': expected 5 operand(s), got " + std::to_string(ins.size()));
+  for (Tensor* t : ins)
+    if (t->ctx != c) invalid("eager '" + op + "': cross-device operands forbidden");
   Tensor *kp = ins[0], *vp = ins[1], *k = ins[2], *v = ins[3], *slots = ins[4];
   check_pages(kp, vp, op);
   if (!kp->writable || !vp->writable)

@@ -517,7 +517,7 @@ static int execute_impl(rew_mi355x_ctx* ctx, const char* op,
     std::lock_guard<std::recursive_mutex> g(c->mu);
     REW_HIP(hipSetDevice(c->ordinal));
     std::vector<Tensor*> res = record_op(c, op, ins, attrs);
-    if ((int)res.size() > max_outs || !outs) {
+    if ((int)res.size() > max_outs || (!outs && !res.empty())) {
       for (Tensor* t : res) {
         t->ext--;
         maybe_destroy(t);

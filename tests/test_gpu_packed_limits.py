@@ -1,11 +1,14 @@
 """GPU checks of the packed and paged operators at the edges of their use: splits, hints, long
 caches, replayed plans, single launches and the refusals of the library itself."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 import packed_ref as R
+from rew_amd import _lib
 from rew_amd import eager as E
 from rew_amd import ops as O
 from rew_amd.eager import DType, EagerError
@@ -230,3 +233,29 @@ def test_nothing_to_attend(gpu, news):
         got = O.pagedBlockTables(ints([0, 0]), ints(news), ints(table), ints(pool), 16, T)
         for g, w in zip(got, R.block_tables([0, 0], news, table.astype(np.int64), pool, 16, T)):
             np.testing.assert_array_equal(E.toHost(g), w)
+
+
+def test_write_through_the_c_interface(gpu):
+    """No room for outputs is needed, and tensors of another context are refused."""
+    lib = _lib.load()
+    kp, vp = (E.empty(DType.BFLOAT16, (2, 1, 4, 32)) for _ in range(2))
+    row, want = tensor(np.random.default_rng(0).standard_normal((1, 1, 32)), "bfloat16")
+    slot, n = ints([6]), C.c_int(9)
+
+    def call(ctx, operands):
+        ops = (C.c_void_p * 5)(*operands)
+        return lib.rew_mi355x_execute(ctx, b"pagedCacheWrite", ops, 5, None, None, 0, None, 0,
+                                      C.byref(n))
+
+    mine = [t.handle for t in (kp, vp, row, row, slot)]
+    assert call(E.context(), mine) == 0 and n.value == 0
+    for p in (kp, vp):
+        np.testing.assert_array_equal(E.toHostF32(p)[1, 0, 2], want[0, 0])
+    other, shape, far = C.c_void_p(), (C.c_int64 * 4)(2, 1, 4, 32), C.c_void_p()
+    assert lib.rew_mi355x_init(0, C.byref(other)) == 0
+    if other.value == C.cast(E.context(), C.c_void_p).value:
+        return  # (contexts of a device are shared)
+    assert lib.rew_mi355x_alloc(other, int(DType.BFLOAT16), shape, 4, C.byref(far)) == 0
+    assert call(E.context(), [far.value, *mine[1:]]) != 0
+    assert b"cross-device" in lib.rew_mi355x_last_error()
+    lib.rew_mi355x_release(far)
