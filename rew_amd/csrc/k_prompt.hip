@@ -288,13 +288,14 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      uint32_t w = 0;
+      // 1.5 2^23 + x holds x, rounded, in its low bits (|x| <= 127 by the step)
+      uint32_t b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float q = rintf(fminf(fmaxf(o[dt][r * 4 + i] * per_step, -127.0f), 127.0f));
-        w |= ((uint32_t)(int)q & 255u) << (8 * i);
-      }
-      *(uint32_t*)(rest + dt * 32 + r * 8 + g * 4) = w;
+      for (int i = 0; i < 4; ++i)
+        b[i] = __float_as_uint(fmaf(o[dt][r * 4 + i], per_step, 0x1.8p23f));
+      *(uint32_t*)(rest + dt * 32 + r * 8 + g * 4) =
+          __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400) |
+          __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
     }
 }
 
