@@ -1,18 +1,19 @@
 // The gradients of packed attention (PackedGradArgs in kernels.h), without
 // anything of size rows x keys in memory.
 //
-// Three launches.  The first writes delta = dout . out per row, from out and
-// what its rounding left (out alone would put out's rounding into every dS,
-// next to dS's own).  The second
-// gives each workgroup 128 keys of one KV head and walks the rows that see
-// them, dK and dV staying in registers; the third gives each workgroup 128
-// rows and walks their keys, dQ staying in registers.  Both recompute
+// delta = dout . out per row is taken from out and what its rounding left (out
+// alone would put out's rounding into every dS, next to dS's own): by a first
+// launch for float16, by the dQ kernel for bfloat16 (939 -> 922 us for the case
+// below, forward pass included).  The dQ kernel gives each workgroup 128 rows and walks their keys, dQ
+// staying in registers; the last launch gives each workgroup 128 keys of one KV
+// head and walks the rows that see them, dK and dV staying in registers.  Both recompute
 // P = exp(S - lse), so the scores are formed twice: 7 products of rows x keys
 // x D where 5 would do, for sums whose order never changes (a single pass
 // would add dQ across workgroups with atomics).  The rows of the H / Hkv heads
 // of a KV head are walked together, so the sum over the group is part of the
-// accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16: 31,
-// 450-510 (0.70-0.79 PFLOP/s) and 270-295 us (0.90-0.99 PFLOP/s) as the clock falls.
+// accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16:
+// 290-340 (267 GFLOP, 0.79-0.92 PFLOP/s) and 440-520 us (357 GFLOP, 0.69-0.81 PFLOP/s)
+// as the clock falls.
 //
 // In each product one operand stays in registers and the other is read from
 // LDS; S and dP come out with the operand in registers along the lanes, so P
@@ -52,6 +53,25 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 // of its workgroups (a maximum does not depend on their order): over the
 // sequences' rows, and over finite values, so that neither what lies outside
 // the sequences nor one sequence's infinity takes the others' bits.
+// (bfloat16 needs no maxima: its dQ kernel forms these values from its own rows.)
+//
+// Adds to s, rest and most what eight values x of a row of out, y of dout and z of
+// what rounding took from out give: dout . out, dout . rest, max |out|.
+template <class M>
+__device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s, float& rest,
+                                            float& most) {
+  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[2] = {z.x, z.y};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float y0 = M::lo(ys[k]), y1 = M::hi(ys[k]), x0 = M::lo(xs[k]), x1 = M::hi(xs[k]);
+    s = fmaf(x0, y0, s);
+    s = fmaf(x1, y1, s);
+    const int sh = (k & 1) * 16;
+    rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
+    rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
+    most = fmaxf(most, fmaxf(fabsf(x0), fabsf(x1)));
+  }
+}
 template <class M, int D>
 __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   constexpr int L = D / 8;
@@ -64,22 +84,11 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   float most = 0.0f, most_v = 0.0f;
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
-    const uint2 z = ((const uint2*)a.rest)[i * L + ch];
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[2] = {z.x, z.y};
-    float s = 0.0f, rest = 0.0f, row = 0.0f;  // dout . out, dout . rest, max |out|
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float y0 = M::lo(ys[k]), y1 = M::hi(ys[k]), x0 = M::lo(xs[k]), x1 = M::hi(xs[k]);
-      s = fmaf(x0, y0, s);
-      s = fmaf(x1, y1, s);
-      const int sh = (k & 1) * 16;
-      rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
-      rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
-      row = fmaxf(row, fmaxf(fabsf(x0), fabsf(x1)));
-      if constexpr (M::kScaled) {
-        if (i >= tok0 * a.H && i < tok1 * a.H) most = fmaxf(most, fmaxf(finite(y0), finite(y1)));
-      }
-    }
+    float s = 0.0f, rest = 0.0f, row = 0.0f;
+    delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row);
+    if (i >= tok0 * a.H && i < tok1 * a.H)
+      for (uint32_t w : {y.x, y.y, y.z, y.w})
+        most = fmaxf(most, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
 #pragma unroll
     for (int d = L / 2; d > 0; d >>= 1) {
       s += __shfl_xor(s, d);
@@ -92,28 +101,27 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
       neg_delta[i] = -s;
     }
   }
-  if constexpr (M::kScaled) {
-    const int64_t n = tok1 * a.Hkv * L;
-    for (int64_t i = tok0 * a.Hkv * L + blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-      const uint4 x = ((const uint4*)a.v)[i];
-      for (uint32_t w : {x.x, x.y, x.z, x.w})
-        most_v = fmaxf(most_v, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
-    }
-    __shared__ float part[8];
+  const int64_t n = tok1 * a.Hkv * L;
+  for (int64_t i = tok0 * a.Hkv * L + blockIdx.x * 256ll + threadIdx.x; i < n;
+       i += gridDim.x * 256ll) {
+    const uint4 x = ((const uint4*)a.v)[i];
+    for (uint32_t w : {x.x, x.y, x.z, x.w})
+      most_v = fmaxf(most_v, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
+  }
+  __shared__ float part[8];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      most = fmaxf(most, __shfl_xor(most, d));
-      most_v = fmaxf(most_v, __shfl_xor(most_v, d));
-    }
-    if ((threadIdx.x & 63) == 0) {
-      part[threadIdx.x >> 6] = most;
-      part[4 + (threadIdx.x >> 6)] = most_v;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-      const float* q = part + 4 * threadIdx.x;
-      neg_delta[rows + blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
-    }
+  for (int d = 32; d > 0; d >>= 1) {
+    most = fmaxf(most, __shfl_xor(most, d));
+    most_v = fmaxf(most_v, __shfl_xor(most_v, d));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = most;
+    part[4 + (threadIdx.x >> 6)] = most_v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const float* q = part + 4 * threadIdx.x;
+    neg_delta[rows + blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
   }
 }
 // F, from the maxima of the delta kernel's workgroups (a power of two; 1 for
@@ -525,7 +533,28 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   }
   const float sl2 = a.scale * kLog2e;
   const float F = grad_factor<M, D, 256>(a), fs = F * exp2f(-M::kGradShift);
-  const float l = ((const float*)a.work)[at], dl = ((const float*)a.work)[a.T * a.H + at];
+  float l, dl;
+  if constexpr (M::kScaled) {
+    l = ((const float*)a.work)[at];
+    dl = ((const float*)a.work)[a.T * a.H + at];
+  } else {
+    float s = 0.0f, rest = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int64_t i = at * D + t * 16 + g * 8;
+      uint4 y;
+      __builtin_memcpy(&y, &df[t], 16);
+      delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
+                     s, rest, most);
+    }
+    s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
+    l = M::kGradShift - a.lse[at] * kLog2e;
+    dl = -s;
+    if (g == 0 && row < rows) {  // (for the dK, dV kernel)
+      ((float*)a.work)[at] = l;
+      ((float*)a.work)[a.T * a.H + at] = dl;
+    }
+  }
   const GradFrags<D> fr;
   const int row_in = lane / CPR, pc = lane % CPR;
   const int64_t kstride = (int64_t)a.Hkv * D, kbase = (st.first * (int64_t)a.Hkv + hk) * D;
@@ -641,10 +670,11 @@ static void launch_grad(PackedGradArgs a, hipStream_t stream) {
   const int64_t q = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pg::BR) * a.Hkv;
   if (kv >= (1ll << 31) || q >= (1ll << 31))
     fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention gradient: too many tiles");
-  hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)a.delta_blocks), dim3(256), 0,
-                     stream, a);
-  hipLaunchKernelGGL((grad_kv_kernel<M, D>), dim3((unsigned)kv), dim3(512), 0, stream, a);
+  if constexpr (M::kScaled)
+    hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)a.delta_blocks), dim3(256), 0,
+                       stream, a);
   hipLaunchKernelGGL((grad_q_kernel<M, D>), dim3((unsigned)q), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((grad_kv_kernel<M, D>), dim3((unsigned)kv), dim3(512), 0, stream, a);
 }
 template <class M>
 static void launch_grad_t(const PackedGradArgs& a, hipStream_t stream) {
@@ -653,11 +683,12 @@ static void launch_grad_t(const PackedGradArgs& a, hipStream_t stream) {
   else launch_grad<M, 128>(a, stream);
 }
 
-void launch_packed_grad(const PackedGradArgs& a, hipStream_t stream) {
-  if (a.T == 0) return;
+int launch_packed_grad(const PackedGradArgs& a, hipStream_t stream) {
+  if (a.T == 0) return 0;
   if (a.f16) launch_grad_t<MmaF16>(a, stream);
   else launch_grad_t<MmaBf16>(a, stream);
   REW_HIP(hipGetLastError());
+  return a.f16 ? 3 : 2;
 }
 
 }  // namespace rew

@@ -604,7 +604,7 @@ struct PackedGradArgs {
   float scale;
 };
 size_t packed_grad_ws_bytes(int64_t T, int H);
-void launch_packed_grad(const PackedGradArgs& a, hipStream_t stream);
+int launch_packed_grad(const PackedGradArgs& a, hipStream_t stream);
 
 // ---- pages of a key / value cache (k_pages.hip) -------------------------------------
 // The tables of a step that adds fresh[r] tokens to request r, which has

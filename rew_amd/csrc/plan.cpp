@@ -239,9 +239,8 @@ struct Exec {
   void operator()(PackedArgs& a) {
     c->stats.kernels_launched += launch_packed_attn(a, c->stream) - 1;
   }
-  void operator()(PackedGradArgs& a) {  // (three kernels)
-    launch_packed_grad(a, c->stream);
-    c->stats.kernels_launched += 2;
+  void operator()(PackedGradArgs& a) {
+    c->stats.kernels_launched += launch_packed_grad(a, c->stream) - 1;
   }
   void operator()(PageTablesArgs& a) { launch_page_tables(a, c->stream); }
   void operator()(FillL& l) {
