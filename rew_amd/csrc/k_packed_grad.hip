@@ -4,15 +4,15 @@
 // delta = dout . out per row is taken from out and what its rounding left (out
 // alone would put out's rounding into every dS, next to dS's own): by a first
 // launch for float16, by the dQ kernel for bfloat16 (939 -> 922 us for the case
-// below, forward pass included).  The dQ kernel gives each workgroup 128 rows and walks their keys, dQ
-// staying in registers; the last launch gives each workgroup 128 keys of one KV
-// head and walks the rows that see them, dK and dV staying in registers.  Both recompute
-// P = exp(S - lse), so the scores are formed twice: 7 products of rows x keys
-// x D where 5 would do, for sums whose order never changes (a single pass
-// would add dQ across workgroups with atomics).  The rows of the H / Hkv heads
-// of a KV head are walked together, so the sum over the group is part of the
-// accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16:
-// 290-340 (267 GFLOP, 0.79-0.92 PFLOP/s) and 440-520 us (357 GFLOP, 0.69-0.81 PFLOP/s)
+// below, forward pass included).  The dQ kernel gives each workgroup 128 rows and
+// walks their keys, dQ staying in registers; the last launch gives each
+// workgroup 128 keys of one KV head and walks the rows that see them, dK and dV
+// staying in registers.  Both recompute P = exp(S - lse), so the scores are
+// formed twice: 7 products of rows x keys x D where 5 would do, for sums whose
+// order never changes (a single pass would add dQ across workgroups with
+// atomics).  The rows of the H / Hkv heads of a KV head are walked together, so
+// the sum over the group is part of the accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16:
+// 290-340 (267 GFLOP, 0.79-0.92 PFLOP/s) and 425-520 us (357 GFLOP, 0.69-0.84 PFLOP/s)
 // as the clock falls.
 //
 // In each product one operand stays in registers and the other is read from
@@ -318,17 +318,44 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
   auto row_of = [&](int m) { return r0 + (2 * m + grp) * 32; };
   auto slot = [&](int m) { return grp * 2 + (m & 1); };
 
+  // groups that divide a block: its rows are whole tokens' heads, at the same
+  // offsets in each block, and only the scalar unit has addresses to compute
+  // (tokens behind the last read as zeros): 8 % fewer cycles than by rows
+  const bool whole = NDMA >= 2 && 32 % G == 0;
+  const int log_g = __builtin_ctz(G);
+  uint32_t row_at[NDMA < 2 ? 1 : NDMA / 2];
+#pragma unroll
+  for (int i = 0; i < NDMA / 2; ++i) {
+    const int lr = (kw + i * 4) * RPD + row_in;
+    row_at[i] = (uint32_t)(((lr / G * a.H + lr % G) * D + (pc ^ grad_swizzle<CPR>(lr)) * 8) * 2);
+  }
+
   auto request = [&](int m) {
     const int w0 = row_of(m);
     uint16_t* s = S + slot(m) * 2 * BLK;
+    if (whole) {
+      const int tok = w0 >> log_g;
+      const int64_t at = (base + (int64_t)tok * a.H) * D;
+      const int64_t left = w0 < rows ? ((int64_t)(st.n - 1 - tok) * a.H + G) * D * 2 : 0;
+      const uint32_t bytes = (uint32_t)min(left, (int64_t)0x7fffffff);
+      const __amdgpu_buffer_rsrc_t rq = fa_rsrc((const uint16_t*)a.q + at, bytes);
+      const __amdgpu_buffer_rsrc_t rd = fa_rsrc((const uint16_t*)a.dout + at, bytes);
 #pragma unroll
-    for (int i = 0; i < NDMA; ++i) {
-      const int x = kw + i * 4, blk = x % (BLK / 512), lr = blk * RPD + row_in;
-      const bool q = x < BLK / 512;
-      int hg;
-      const int tok = by_g.div(min(w0 + lr, rows - 1), hg);
-      const int64_t at = (base + (int64_t)tok * a.H + hg) * D + (pc ^ grad_swizzle<CPR>(lr)) * 8;
-      dma16((const uint16_t*)(q ? a.q : a.dout) + at, s + x * 512);
+      for (int i = 0; i < NDMA / 2; ++i) {
+        dma16_buf(rq, row_at[i], 0, s + (kw + i * 4) * 512);
+        dma16_buf(rd, row_at[i], 0, s + BLK + (kw + i * 4) * 512);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) {
+        const int x = kw + i * 4, blk = x % (BLK / 512), lr = blk * RPD + row_in;
+        const bool q = x < BLK / 512;
+        int hg;
+        const int tok = by_g.div(min(w0 + lr, rows - 1), hg);
+        const int64_t at =
+            (base + (int64_t)tok * a.H + hg) * D + (pc ^ grad_swizzle<CPR>(lr)) * 8;
+        dma16((const uint16_t*)(q ? a.q : a.dout) + at, s + x * 512);
+      }
     }
     if (kw == 0) {  // lanes 0..31: -lse, 32..63: -delta
       int hg;
