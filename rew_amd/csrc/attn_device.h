@@ -433,25 +433,34 @@ __device__ __forceinline__ void soft_exp(const f32x16_t (&s)[NB], float sl2, flo
 // first; the infinities and NaN found are added to the rows that see them
 // by themselves, and are zeros in the product.
 //
+// The largest magnitude (as bits) of the values seen, two by two.
+template <class M>
+struct Largest {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
+  __device__ __forceinline__ void add(uint32_t w) {
+    const uint32_t x = w & 0x7fff7fffu;
+    u16x2 y;
+    __builtin_memcpy(&y, &x, 4);
+    most = __builtin_elementwise_max(most, y);
+  }
+  __device__ __forceinline__ bool special() const {
+    return most[0] >= M::kInf || most[1] >= M::kInf;
+  }
+};
 // Whether an LDS tile of KEYS rows of D holds an infinity or NaN.
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 template <class M, int KEYS, int D, class P>
 __device__ __forceinline__ bool any_special(P tile) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  u16x2 most = {0, 0};
+  Largest<M> most;
 #pragma unroll
   for (int i = 0; i < KEYS * D / 512; ++i) {
-    const u32x4 w =
-        *(__attribute__((address_space(3))) const u32x4*)(tile + i * 512 + (threadIdx.x & 63) * 8);
+    const u32x4_t w = *(__attribute__((address_space(3))) const u32x4_t*)(
+        tile + i * 512 + (threadIdx.x & 63) * 8);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t x = w[j] & 0x7fff7fffu;
-      u16x2 y;
-      __builtin_memcpy(&y, &x, 4);
-      most = __builtin_elementwise_max(most, y);
-    }
+    for (int j = 0; j < 4; ++j) most.add(w[j]);
   }
-  return __builtin_amdgcn_ballot_w64(most[0] >= M::kInf || most[1] >= M::kInf) != 0;
+  return __builtin_amdgcn_ballot_w64(most.special()) != 0;
 }
 // The infinities and NaN of two values, zeros for others.
 template <class M>
@@ -460,11 +469,17 @@ __device__ __forceinline__ uint32_t special(uint32_t w) {
   const uint32_t hi = (w & 0x7fff0000u) >= M::kInf << 16 ? 0xffff0000u : 0u;
   return w & (lo | hi);
 }
-// o += the infinities and NaN of the first `seen` of KEYS keys of a V tile
-// (o[dt][r 4 + i]: column dt 32 + r 8 + g 4 + i; key j's chunk x of 8 columns at
-// x ^ 4 (j & 3)).
-template <class M, int KEYS, int D, class P>
-__device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int seen, int g) {
+// Key j's chunk x of 8 columns of a V tile lies at x ^ value_swizzle(j).
+template <int D>
+__device__ __forceinline__ int value_swizzle(int j) {
+  return (4 * (j & 3)) % (D / 8);
+}
+// o += the infinities and NaN of the first `seen` of KEYS rows of a tile
+// (o[dt][r 4 + i]: column dt 32 + r 8 + g 4 + i; row j's chunk x of 8 columns at
+// x ^ swizzle(j)).
+template <class M, int KEYS, int D, class P, class Swizzle>
+__device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int seen, int g,
+                                            Swizzle swizzle) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -472,7 +487,7 @@ __device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int s
     for (int r = 0; r < 4; ++r)
 #pragma unroll 1
       for (int j = 0; j < KEYS; ++j) {
-        const int ch = (dt * 4 + r) ^ ((4 * (j & 3)) % (D / 8));
+        const int ch = (dt * 4 + r) ^ swizzle(j);
         const u32x2 w =
             *(__attribute__((address_space(3))) const u32x2*)(tile + j * D + ch * 8 + g * 4);
 #pragma unroll

@@ -12,7 +12,7 @@
 // order never changes (a single pass would add dQ across workgroups with
 // atomics).  The rows of the H / Hkv heads of a KV head are walked together, so
 // the sum over the group is part of the accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16:
-// 290-340 (267 GFLOP, 0.79-0.92 PFLOP/s) and 425-520 us (357 GFLOP, 0.69-0.84 PFLOP/s)
+// 297-340 (267 GFLOP, 0.79-0.90 PFLOP/s) and 412-500 us (357 GFLOP, 0.71-0.87 PFLOP/s)
 // as the clock falls.
 //
 // In each product one operand stays in registers and the other is read from
@@ -56,10 +56,11 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 // (bfloat16 needs no maxima: its dQ kernel forms these values from its own rows.)
 //
 // Adds to s, rest and most what eight values x of a row of out, y of dout and z of
-// what rounding took from out give: dout . out, dout . rest, max |out|.
+// what rounding took from out give: dout . out, dout . rest, max |out|; and to
+// `largest` y.
 template <class M>
 __device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s, float& rest,
-                                            float& most) {
+                                            float& most, Largest<M>& largest) {
   const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[2] = {z.x, z.y};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -70,6 +71,7 @@ __device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s,
     rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
     rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
     most = fmaxf(most, fmaxf(fabsf(x0), fabsf(x1)));
+    largest.add(ys[k]);
   }
 }
 template <class M, int D>
@@ -85,7 +87,9 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
     float s = 0.0f, rest = 0.0f, row = 0.0f;
-    delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row);
+    Largest<M> largest;
+    delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row, largest);
+    float bad = largest.special() ? 1.0f : 0.0f;
     if (i >= tok0 * a.H && i < tok1 * a.H)
       for (uint32_t w : {y.x, y.y, y.z, y.w})
         most = fmaxf(most, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
@@ -94,10 +98,11 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
       s += __shfl_xor(s, d);
       rest += __shfl_xor(rest, d);
       row = fmaxf(row, __shfl_xor(row, d));
+      bad = fmaxf(bad, __shfl_xor(bad, d));
     }
     s = fmaf(rest, row * M::kRestStep, s);
     if (ch == 0) {
-      neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
+      neg_lse[i] = bad > 0.0f ? NAN : M::kGradShift - a.lse[i] * pg::kLog2e;
       neg_delta[i] = -s;
     }
   }
@@ -370,6 +375,31 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
     const int w0 = row_of(m);
     return w0 < rows && (!a.causal || w0 + 31 >= wk * G);
   };
+  // Where some row does not see all of the workgroup's keys, infinities and NaN
+  // of Q and dout become zeros before the products (0 times them would reach the
+  // keys that do not see the row): each wave's own part of the block, once it
+  // is there.  Keys that do see it take NaN from the row's lse (its scores were not
+  // finite, or see delta).
+  auto clean = [&](int m) {
+    if (!a.causal || row_of(m) >= (k0 + BR - 1) * G) return;
+    Largest<M> most;
+#pragma unroll
+    for (int i = 0; i < NDMA; ++i) {
+      const u32x4_t w = *(const u32x4_t*)(S + slot(m) * 2 * BLK + (kw + i * 4) * 512 + lane * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most.add(w[j]);
+    }
+    if (__builtin_amdgcn_ballot_w64(most.special()) == 0) return;
+#pragma unroll 1
+    for (int i = 0; i < NDMA; ++i) {
+      u32x4_t* p = (u32x4_t*)(S + slot(m) * 2 * BLK + (kw + i * 4) * 512 + lane * 8);
+      u32x4_t w = *p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] ^= special<M>(w[j]);
+      *p = w;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
   f32x16_t x, dp;
   float4 l4[4];
   uint32_t pp[8], pd[8];
@@ -436,12 +466,14 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = e4 * 4 + i;
-          if constexpr (masked) {  // (selects of the inputs: no branches)
+          if constexpr (masked) {  // (selects, no branches)
             const bool see = (uint32_t)(e4 * 8 + i - lo) < span;
-            x[e] = see ? x[e] : -INFINITY;
             dp[e] = see ? dp[e] : 0.0f;
+            p[i] = fa_exp2(fmaf(x[e], sl2, l[i]));
+            p[i] = see ? p[i] : 0.0f;
+          } else {
+            p[i] = fa_exp2(fmaf(x[e], sl2, l[i]));
           }
-          p[i] = fa_exp2(fmaf(x[e], sl2, l[i]));
           ds[i] = p[i] * dp[e];
           if constexpr (M::kScaled) ds[i] *= fs;
         }
@@ -467,6 +499,7 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
   if (n > 0) {
     request(0);
     vm_wait();
+    clean(0);
     block_barrier_fa();
     if (grp == 1) block_barrier_fa();
     __builtin_amdgcn_s_setprio(1);
@@ -478,6 +511,7 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
       request(m);
       values(m - 1);
       vm_wait();
+      clean(m);
       block_barrier_fa();
       __builtin_amdgcn_s_setprio(1);
       accumulate(m - 1);
@@ -566,16 +600,18 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     dl = ((const float*)a.work)[a.T * a.H + at];
   } else {
     float s = 0.0f, rest = 0.0f, most = 0.0f;
+    Largest<M> largest;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int64_t i = at * D + t * 16 + g * 8;
       uint4 y;
       __builtin_memcpy(&y, &df[t], 16);
       delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
-                     s, rest, most);
+                     s, rest, most, largest);
     }
+    const float bad = fa_max_halves(largest.special() ? 1.0f : 0.0f);
     s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
-    l = M::kGradShift - a.lse[at] * kLog2e;
+    l = bad > 0.0f ? NAN : M::kGradShift - a.lse[at] * kLog2e;
     dl = -s;
     if (g == 0 && row < rows) {  // (for the dK, dV kernel)
       ((float*)a.work)[at] = l;
@@ -607,7 +643,12 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[dt][e] = 0.0f;
-  auto tile = [&](const uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n, int kt) {
+  typedef __attribute__((address_space(3))) uint16_t lds_u16;
+  const int block_least = limit(st.tile * BR);
+  auto tile = [&](uint16_t* ks, const uint16_t* vs, uint16_t* ks_n, uint16_t* vs_n, int kt) {
+    // (as in the forward kernel's V: the same answer in all waves)
+    const bool special = block_least < min(kt * BT + BT, keys) &&
+                         any_special<M, BT, D>((lds_u16*)ks);
     if (kt + 1 < nkt) dma_tile(ks_n, vs_n);
 #pragma unroll
     for (int h = 0; h < BT / 32; ++h) {
@@ -659,6 +700,13 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
       };
       if (kt * BT + BT <= least) values(std::false_type());
       else values(std::true_type());
+      if (special) {
+        lds_u16* half = (lds_u16*)(ks + h * 32 * D);
+        add_special<M, 32, D>(dq, half, my_limit - kt * BT - h * 32, g, grad_swizzle<CPR>);
+        __syncthreads();
+        clear_special<M, 32, D, 256>(half, threadIdx.x);
+        __syncthreads();
+      }
       grad_accumulate<M, D, 1>({&dq}, Kt, {cols_at}, {&pd});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(PageTablesArgs a)
   for (int64_t i = first; i < f && tok + i < a.tokens; i += step) {
     const int64_t p = c + i, j = p >> a.log_page;
     const int32_t e = j < a.width ? entry(j) : -1;
-    a.slots[tok + i] = e < 0 ? -1 : (int32_t)(((int64_t)e << a.log_page) + (p & (page - 1)));
+    const int64_t slot = ((int64_t)e << a.log_page) + (p & (page - 1));
+    a.slots[tok + i] = e < 0 || slot > 0x7fffffff ? -1 : (int32_t)slot;
     a.positions[tok + i] = (int32_t)p;
   }
 }

@@ -865,8 +865,10 @@ def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Te
                         scale: float = 0.0):
     """(gradQ, gradK, gradV) of ``packedAttention(q, k, v, starts, causal, scale)`` for the
     gradient ``gradOut`` of its result, given its ``out`` and ``stats``.  gradK and gradV are
-    summed over the query heads of each KV head; sums are float32 in a fixed order.  An infinity
-    or NaN in a sequence may reach all of its gradients, but no other sequence's."""
+    summed over the query heads of each KV head; sums are float32 in a fixed order.  What a row
+    does not see takes no part, infinities and NaN included: under causality those of a token's
+    k and v do not reach gradQ of the rows before it, those of its q and gradOut not gradK and
+    gradV of the keys behind it."""
     op = "packedAttentionGrad"
     _check_packed(op, q, k, v, starts)
     for t, name in ((out, "out"), (gradOut, "gradOut")):

@@ -132,7 +132,7 @@ def block_tables(cached, new, table, free, page, tokens):
         for p in range(c, c + f):
             if t < tokens:
                 e = row[p // page] if p // page < table.shape[1] else -1
-                slots[t] = e * page + p % page if e >= 0 else -1
+                slots[t] = e * page + p % page if 0 <= e * page + p % page < 2 ** 31 else -1
                 positions[t] = p
             t += 1
         lens.append(c + f)

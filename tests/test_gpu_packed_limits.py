@@ -229,7 +229,8 @@ def test_nothing_to_attend(gpu, news):
         assert not E.toHostF32(O.pagedAttention(q, *args)).any()
     k, _ = tensor(r.standard_normal((T, 2, 64)), "bfloat16")
     O.pagedCacheWrite(*no_pages, k, k, O.iota(DType.INT32, [T], 0))
-    for table, pool in ((np.zeros((2, 0)), [4, 5]), (np.zeros((2, 4)), [])):
+    for table, pool in ((np.zeros((2, 0)), [4, 5]), (np.zeros((2, 4)), []),
+                        (np.zeros((2, 4)), [2 ** 27, -3, 2 ** 31 - 1, 2 ** 28, 1])):
         got = O.pagedBlockTables(ints([0, 0]), ints(news), ints(table), ints(pool), 16, T)
         for g, w in zip(got, R.block_tables([0, 0], news, table.astype(np.int64), pool, 16, T)):
             np.testing.assert_array_equal(E.toHost(g), w)

@@ -101,3 +101,34 @@ def test_grad_of_other_sequences(gpu, dtype, causal, value, which):
             assert np.isfinite(g[rows]).all()
             assert (np.abs(g[rows] - w[rows]) <= b[rows]).all()
         assert (g[301:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hkv,D", [(4, 4, 32), (8, 2, 64), (6, 2, 128), (4, 1, 128)])
+@pytest.mark.parametrize("value", SPECIAL)
+@pytest.mark.parametrize("which", range(4), ids=["q", "k", "v", "do"])
+@pytest.mark.parametrize("at", [0, 45, 131, 159])
+def test_causal_grad_of_one_token(gpu, dtype, H, Hkv, D, value, which, at):
+    """A token's infinities or NaN in k or v do not reach the gradient of q of rows before it,
+    those in q or gradOut only its own row's and not the keys behind it."""
+    a, n, T = 70, 160, 301
+    starts = [0, a, a + n, T]
+    r = np.random.default_rng(D + which)
+    x = [h for _, h in make(r, T, H, Hkv, D, dtype)] + [r.standard_normal((T, H, D))]
+    x[3] = tensor(x[3], dtype)[1]
+    want, bnd = R.packed_grad(*x[:3], starts, x[3], True, D ** -0.5, dtype)
+    x[which] = put(x[which], [a + at], value, dtype)[1]
+    q, k, v, do = (tensor(y, dtype)[0] for y in x)
+    out, stats = O.packedAttention(q, k, v, ints(starts), withLse=True)
+    got = [E.toHostF32(g).astype(np.float64)
+           for g in O.packedAttentionGrad(q, k, v, ints(starts), out, stats, do)]
+    own, rows = np.arange(a + at, a + at + 1), np.arange(T)
+    later = np.r_[a + at:a + n]
+    if which in (1, 2):  # k, v: rows that see it; every key has such a row behind it
+        clean = [np.setdiff1d(rows, later), np.r_[0:a, a + n:T], np.r_[0:a, a + n:T]]
+    else:
+        clean = [np.setdiff1d(rows, own)] + [np.r_[0:a, a + at + 1:T]] * 2
+    for g, w, b, c in zip(got, want, bnd, clean):
+        assert np.isfinite(g[c]).all()
+        assert (np.abs(g[c] - w[c]) <= b[c]).all()
+    assert not np.isfinite(got[0][own]).all() and not np.isfinite(got[1][a:a + at + 1]).all()
