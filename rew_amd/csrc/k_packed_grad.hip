@@ -595,29 +595,6 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   const float sl2 = a.scale * kLog2e;
   const float F = grad_factor<M, D, 256>(a), fs = F * exp2f(-M::kGradShift);
   float l, dl;
-  if constexpr (M::kScaled) {
-    l = ((const float*)a.work)[at];
-    dl = ((const float*)a.work)[a.T * a.H + at];
-  } else {
-    float s = 0.0f, rest = 0.0f, most = 0.0f;
-    Largest<M> largest;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int64_t i = at * D + t * 16 + g * 8;
-      uint4 y;
-      __builtin_memcpy(&y, &df[t], 16);
-      delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
-                     s, rest, most, largest);
-    }
-    const float bad = fa_max_halves(largest.special() ? 1.0f : 0.0f);
-    s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
-    l = bad > 0.0f ? NAN : M::kGradShift - a.lse[at] * kLog2e;
-    dl = -s;
-    if (g == 0 && row < rows) {  // (for the dK, dV kernel)
-      ((float*)a.work)[at] = l;
-      ((float*)a.work)[a.T * a.H + at] = dl;
-    }
-  }
   const GradFrags<D> fr;
   const int row_in = lane / CPR, pc = lane % CPR;
   const int64_t kstride = (int64_t)a.Hkv * D, kbase = (st.first * (int64_t)a.Hkv + hk) * D;
@@ -712,8 +689,31 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
+  if (nkt > 0) dma_tile(K0, V0);  // (on its way while delta is formed)
+  if constexpr (M::kScaled) {
+    l = ((const float*)a.work)[at];
+    dl = ((const float*)a.work)[a.T * a.H + at];
+  } else {
+    float s = 0.0f, rest = 0.0f, most = 0.0f;
+    Largest<M> largest;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int64_t i = at * D + t * 16 + g * 8;
+      uint4 y;
+      __builtin_memcpy(&y, &df[t], 16);
+      delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
+                     s, rest, most, largest);
+    }
+    const float bad = fa_max_halves(largest.special() ? 1.0f : 0.0f);
+    s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
+    l = bad > 0.0f ? NAN : M::kGradShift - a.lse[at] * kLog2e;
+    dl = -s;
+    if (g == 0 && row < rows) {  // (for the dK, dV kernel)
+      ((float*)a.work)[at] = l;
+      ((float*)a.work)[a.T * a.H + at] = dl;
+    }
+  }
   if (nkt > 0) {
-    dma_tile(K0, V0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     for (int kt = 0; kt < nkt; kt += 2) {
