@@ -173,13 +173,28 @@ __device__ __forceinline__ int wave_scan(int x) {  // inclusive
 __device__ __forceinline__ int wave_sum(int x) {
   return __builtin_amdgcn_readlane(wave_scan(x), 63);
 }
+// likewise the running max of values >= 0
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int max_moved(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_max_scan(int x) {
+  x = max_moved<0x111, 0xf>(x);
+  x = max_moved<0x112, 0xf>(x);
+  x = max_moved<0x114, 0xf>(x);
+  x = max_moved<0x118, 0xf>(x);
+  x = max_moved<0x142, 0xa>(x);
+  return max_moved<0x143, 0xc>(x);
+}
 // ---- packed sequences ---------------------------------------------------------------
 //
 // Sequence s owns rows [starts[s], starts[s + 1]) of T.  The rows before the
 // first and behind the last sequence belong to none: they count as sequences
 // -1 and n_seq, without keys.  starts is device data that the host does not
-// see, so every value is clamped into [0, T] and a decreasing one makes an
-// empty sequence: no row outside the tensors is ever touched.
+// see, so every value is clamped into [0, T], and one below an earlier value
+// counts as that: no row outside the tensors is touched, no row belongs to two
+// sequences, and the host's bounds on tiles, whose sums fit 31 bits, hold for any
+// starts.
 struct SeqTile {
   int seq;     // -1 .. n_seq; -2: there is no such tile
   int first;   // its first row
@@ -192,28 +207,39 @@ __device__ __forceinline__ int seq_bound(const int32_t* starts, int n_seq, int T
   if (s > n_seq) return T;
   return min(max(starts[s], 0), T);
 }
+// The rows of the 64 sequences from `base`, one per lane (none past n_seq).
+// floor: 0 for base -1, then what the step before left (the first row of
+// sequence base).
+struct SeqRows {
+  int s, first, n;
+  __device__ __forceinline__ SeqRows(const int32_t* starts, int n_seq, int T, int base, int& floor)
+      : s(base + (int)(threadIdx.x & 63)) {
+    first = max(wave_max_scan(seq_bound(starts, n_seq, T, s)), floor);
+    const int end = max(seq_bound(starts, n_seq, T, s + 1), first);
+    n = s > n_seq ? 0 : end - first;
+    floor = __builtin_amdgcn_readlane(end, 63);
+  }
+};
 // Tile `idx` of the sequences' tiles of `per` units, a row holding `units`
 // (query heads of a KV head; 1 for keys), in sequence order.  One wave (every
 // wave of a workgroup does the same): 64 sequences a step, their tile counts
 // summed over the lanes.
 __device__ __forceinline__ SeqTile find_tile(const int32_t* starts, int n_seq, int T, int units,
                                              int per, int idx) {
-  const int lane = threadIdx.x & 63;
   SeqTile r;
   r.seq = -2;
   r.first = r.n = r.tile = 0;
+  int floor = 0;
   for (int base = -1; base <= n_seq; base += 64) {
-    const int s = base + lane;
-    const int b0 = seq_bound(starts, n_seq, T, s);
-    const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
-    const int tiles = (int)(((int64_t)n * units + per - 1) / per);
+    const SeqRows x(starts, n_seq, T, base, floor);
+    const int tiles = (int)(((int64_t)x.n * units + per - 1) / per);
     const int sum = wave_scan(tiles);
     const int total = __builtin_amdgcn_readlane(sum, 63);
     if (idx < total) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
       r.seq = base + at;
-      r.first = __builtin_amdgcn_readlane(b0, at);
-      r.n = __builtin_amdgcn_readlane(n, at);
+      r.first = __builtin_amdgcn_readlane(x.first, at);
+      r.n = __builtin_amdgcn_readlane(x.n, at);
       r.tile = idx - __builtin_amdgcn_readlane(sum - tiles, at);
       return r;
     }
@@ -260,10 +286,9 @@ __device__ __forceinline__ SeqTile level_tile(int s, int first, int n, int tiles
 // the tile's index.
 __device__ __forceinline__ SeqTile rising_tile(const int32_t* starts, int n_seq, int T, int units,
                                                int per, int rank) {
-  const int s = (int)(threadIdx.x & 63) - 1;
-  const int b0 = seq_bound(starts, n_seq, T, s);
-  const int n = s > n_seq ? 0 : max(seq_bound(starts, n_seq, T, s + 1) - b0, 0);
-  return level_tile(s, b0, n, (int)(((int64_t)n * units + per - 1) / per), 0, rank);
+  int floor = 0;
+  const SeqRows x(starts, n_seq, T, -1, floor);
+  return level_tile(x.s, x.first, x.n, (int)(((int64_t)x.n * units + per - 1) / per), 0, rank);
 }
 
 // r / g and r % g for 0 <= r < 2^31: one multiplication by floor((2^32 - 1) / g)

@@ -23,15 +23,30 @@ struct Request {
     return min(max(a.causal ? len - n + t + 1 : len, 0), cap);
   }
 };
-// s: -1 .. n_seq (the rows of no request, as in SeqTile)
-__device__ __forceinline__ Request request_at(const PackedArgs& a, int G, int s) {
+// s: -1 .. n_seq (the rows of no request, as in SeqTile); its n rows from `first`
+__device__ __forceinline__ Request request_of(const PackedArgs& a, int G, int s, int first, int n) {
   Request r;
-  r.first = seq_bound(a.starts, a.n_seq, (int)a.T, s);
-  r.n = s > a.n_seq ? 0 : max(seq_bound(a.starts, a.n_seq, (int)a.T, s + 1) - r.first, 0);
-  r.rows = r.n * G;
+  r.first = first;
+  r.n = n;
+  r.rows = n * G;
   const bool real = s >= 0 && s < a.n_seq;
   r.len = real ? max(a.lens[s], 0) : 0;
   r.cap = real ? (int)min((int64_t)r.len, (int64_t)a.width << a.log_page) : 0;
+  return r;
+}
+// The 64 requests from `base`, one per lane (floor: SeqRows).
+__device__ __forceinline__ Request lane_request(const PackedArgs& a, int G, int base, int& floor) {
+  const SeqRows x(a.starts, a.n_seq, (int)a.T, base, floor);
+  return request_of(a, G, x.s, x.first, x.n);
+}
+// Lane `at`'s request, in every lane.
+__device__ __forceinline__ Request request_from(const Request& x, int at) {
+  Request r;
+  r.first = __builtin_amdgcn_readlane(x.first, at);
+  r.n = __builtin_amdgcn_readlane(x.n, at);
+  r.rows = __builtin_amdgcn_readlane(x.rows, at);
+  r.len = __builtin_amdgcn_readlane(x.len, at);
+  r.cap = __builtin_amdgcn_readlane(x.cap, at);
   return r;
 }
 
@@ -51,33 +66,36 @@ struct TileLine {
     for (int qt = 0; qt * ROWS < r.rows; ++qt) t += item_tiles(r, qt);
     return t;
   }
-  __device__ __forceinline__ int lane_tiles(int base) const {
-    const int s = base + (int)(threadIdx.x & 63);
-    return s > a.n_seq ? 0 : head_tiles(request_at(a, G, s)) * a.Hkv;
-  }
+};
+// 64 requests of the line, one per lane: their tiles and the running sum.
+struct LineStep {
+  Request r;
+  int x, sum;
+  template <class Line>
+  __device__ __forceinline__ LineStep(const Line& L, int base, int& floor)
+      : r(lane_request(L.a, L.G, base, floor)), x(L.head_tiles(r) * L.a.Hkv), sum(wave_scan(x)) {}
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, 63); }
 };
 // Where a tile of the line lies.
 template <class Line>
 struct TilePlace {
   int s, hk, qt, kt;
   Request r;
-  // (the line's total < 2^31 was checked on the host; x, sum: the first 64
-  // requests' tiles and their running sum, which the total needed already)
-  __device__ __forceinline__ void find(const Line& L, int t, int x, int sum) {
+  // (the line's total < 2^31 was checked on the host; step, floor: the first 64
+  // requests, which the total needed already)
+  __device__ __forceinline__ void find(const Line& L, int t, LineStep step, int floor) {
     int base = -1;
     for (;;) {
-      const int total = __builtin_amdgcn_readlane(sum, 63);
-      if (t < total || base + 64 > L.a.n_seq) break;
-      t -= total;
+      if (t < step.total() || base + 64 > L.a.n_seq) break;
+      t -= step.total();
       base += 64;
-      x = L.lane_tiles(base);
-      sum = wave_scan(x);
+      step = LineStep(L, base, floor);
     }
-    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > t));
-    t -= __builtin_amdgcn_readlane(sum - x, at);
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(step.sum > t));
+    t -= __builtin_amdgcn_readlane(step.sum - step.x, at);
     s = base + at;
-    r = request_at(L.a, L.G, s);
-    const int head = __builtin_amdgcn_readlane(x, at) / L.a.Hkv;
+    r = request_from(step.r, at);
+    const int head = __builtin_amdgcn_readlane(step.x, at) / L.a.Hkv;
     hk = t / head;
     t -= hk * head;
     for (qt = 0;; ++qt) {
@@ -99,21 +117,23 @@ struct TilePlace {
     hk = 0;
     do {
       ++s;
-      r = request_at(L.a, L.G, s);
+      const int first = r.first + r.n;
+      const int end = max(seq_bound(L.a.starts, L.a.n_seq, (int)L.a.T, s + 1), first);
+      r = request_of(L.a, L.G, s, first, end - first);
     } while (s <= L.a.n_seq && L.head_tiles(r) == 0);
   }
 };
 // The cut of the line into runs, as even as whole tiles allow and of at least
 // `least` tiles; run w is [start(w), start(w + 1)).
 struct Runs {
-  int x, sum;  // of the first 64 requests, for TilePlace::find
+  int floor = 0;  // behind the first 64 requests, `step`, for TilePlace::find
+  LineStep step;
   int total, count, each, more;
   template <class Line>
-  __device__ __forceinline__ Runs(const Line& L, int most, int least) {
-    x = L.lane_tiles(-1);
-    sum = wave_scan(x);
-    total = __builtin_amdgcn_readlane(sum, 63);
-    for (int base = 63; base <= L.a.n_seq; base += 64) total += wave_sum(L.lane_tiles(base));
+  __device__ __forceinline__ Runs(const Line& L, int most, int least) : step(L, -1, floor) {
+    total = step.total();
+    int at = floor;
+    for (int base = 63; base <= L.a.n_seq; base += 64) total += LineStep(L, base, at).total();
     count = min(most, max((total + least - 1) / least, 1));
     each = total / count;
     more = total - each * count;

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(64, D == 128 ? 1 : 2) decode_kernel(PackedArgs
   const int from = runs.start(w), to = runs.start(w + 1);
   if (from >= to) return;
   TilePlace<DecodeLine> at;
-  at.find(line, from, runs.x, runs.sum);
+  at.find(line, from, runs.step, runs.floor);
   const float sl2 = a.scale * pa::kLog2e;
   Rows x;
 
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(PackedArgs a, int work
   const int from = runs.start(w);
   if (from >= runs.total) return;
   TilePlace<DecodeLine> at;
-  at.find(line, from, runs.x, runs.sum);
+  at.find(line, from, runs.step, runs.floor);
   const int first = from - at.kt;  // the item's first tile
   if (at.kt == 0 || first < runs.start(w - 1)) return;
   const int end = first + line.item_tiles(at.r, at.qt);

@@ -80,7 +80,10 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   const int64_t rows = a.T * a.H, step = gridDim.x * (256ll / L);
   const int ch = threadIdx.x % L;
   const int64_t tok0 = seq_bound(a.starts, a.n_seq, (int)a.T, 0);
-  const int64_t tok1 = seq_bound(a.starts, a.n_seq, (int)a.T, a.n_seq);
+  int last = 0;  // (the largest start: SeqRows)
+  for (int s = threadIdx.x & 63; s <= a.n_seq; s += 64)
+    last = max(last, seq_bound(a.starts, a.n_seq, (int)a.T, s));
+  const int64_t tok1 = __builtin_amdgcn_readlane(wave_max_scan(last), 63);
   auto finite = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; };
   float *neg_lse = (float*)a.work, *neg_delta = neg_lse + rows;
   float most = 0.0f, most_v = 0.0f;

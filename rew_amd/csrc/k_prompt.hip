@@ -324,18 +324,18 @@ struct ChunkPlan {
                                                  int qt) {
     return (r.limit(a, G, qt * pa::BR + pa::BR - 1) + pa::BK - 1) / pa::BK;
   }
-  __device__ __forceinline__ Share share(int s) const {
+  __device__ __forceinline__ Share share(int base, int& floor) const {  // (floor: SeqRows)
     Share x;
-    x.r = request_at(a, G, s);
+    x.r = lane_request(a, G, base, floor);
     x.blocks = (x.r.rows + pa::BR - 1) / pa::BR;
     x.P = x.blocks ? max((tiles_of(a, G, x.r, x.blocks / 2) + C / 2) / C, 1) : 0;
     return x;
   }
   __device__ __forceinline__ explicit ChunkPlan(const PackedArgs& a_)
       : a(a_), G(a_.H / a_.Hkv), C(0x7fffffff / 2) {
-    int n = 0;
+    int n = 0, floor = 0;
     for (int base = -1; base <= a.n_seq; base += 64) {
-      const Share x = share(base + (int)(threadIdx.x & 63));
+      const Share x = share(base, floor);
       n += wave_sum(x.blocks ? x.blocks * tiles_of(a, G, x.r, x.blocks / 2) * a.Hkv : 0);
     }
     C = max((n + pa::kChunkSlots - 1) / pa::kChunkSlots, pa::kPieceTiles);
@@ -343,10 +343,11 @@ struct ChunkPlan {
   // The 64 requests from `base`, one per lane, those of the longest pieces first,
   // so that these start first.
   struct Sorted {
-    int s, blocks, P;
-    __device__ __forceinline__ Sorted(const ChunkPlan& plan, int base) {
+    Share x;          // of request base + lane
+    int s, blocks, P; // of the request that has this lane's place in the order
+    __device__ __forceinline__ Sorted(const ChunkPlan& plan, int base, int& floor)
+        : x(plan.share(base, floor)) {
       const int lane = threadIdx.x & 63;
-      const Share x = plan.share(base + lane);
       const int piece =
           x.blocks ? tiles_of(plan.a, plan.G, x.r, x.blocks / 2) / x.P : -1;
       const int n = uniform(min(plan.a.n_seq + 1 - base, 64));
@@ -374,10 +375,10 @@ struct ChunkPlace {
   int s, hk, qt, part, P, slot;  // slot: of this block's first partial result, if P > 1
   Request r;
   __device__ __forceinline__ ChunkPlace(const ChunkPlan& plan, int idx) : found(false) {
-    int slots = 0;
+    int slots = 0, floor = 0;
     const int Hkv = plan.a.Hkv;
     for (int base = -1; base <= plan.a.n_seq; base += 64) {
-      const ChunkPlan::Sorted x(plan, base);
+      const ChunkPlan::Sorted x(plan, base, floor);
       const int pieces = x.P > 1 ? x.blocks * x.P * Hkv : 0;
       const int mine = !SPLIT ? x.blocks * x.P * Hkv : x.P > 1 ? x.blocks * Hkv : 0;
       const int sum = wave_scan(mine), psum = wave_scan(pieces);
@@ -390,7 +391,7 @@ struct ChunkPlace {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > idx));
       found = true;
       s = __builtin_amdgcn_readlane(x.s, at);
-      r = request_at(plan.a, plan.G, s);
+      r = request_from(x.x.r, s - base);
       P = __builtin_amdgcn_readlane(x.P, at);
       const int blocks = __builtin_amdgcn_readlane(x.blocks, at);
       int u = idx - __builtin_amdgcn_readlane(sum - mine, at);

@@ -549,8 +549,9 @@ const char* flash_variant(const FlashArgs& a);
 // ---- attention over packed sequences and paged caches -----------------------------
 // (k_prompt.hip; k_packed_grad.hip its gradient)
 // q, out [T, H, D]; sequence s owns rows [starts[s], starts[s + 1]) (n of
-// them).  Packed: k, v [T, Hkv, D], and a row sees the keys of its own
-// sequence, those up to its own row when causal.  Paged (table set): k, v
+// them; starts in [0, T] and none below an earlier one, or clamped so).
+// Packed: k, v [T, Hkv, D], and a row sees the keys of its own sequence, those
+// up to its own row when causal.  Paged (table set): k, v
 // [pages, Hkv, 2^log_page, D]; request s has lens[s] keys, key j being row
 // j % 2^log_page of page table[s, j / 2^log_page]; its i-th row is at
 // position lens[s] - n + i and sees the keys up to it (all, if not causal).

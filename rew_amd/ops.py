@@ -763,7 +763,8 @@ def fft(a: Tensor, fftType: str, fftLength: Sequence[int]) -> Tensor:
 # Backend extensions without a counterpart in the reference, eager only.  Rows of
 # all sequences lie one after another (no padding): sequence s owns rows
 # [starts[s], starts[s + 1]).  Lengths and tables are device tensors that no call
-# reads back; values out of range never reach memory outside the tensors.
+# reads back; values out of range never reach memory outside the tensors: starts are
+# clamped into the rows, and one below an earlier one counts as that one.
 
 def _packed_call(op: str, operands, attrs, nouts: int) -> list:
     if _jit.currentMode() == "trace":
@@ -845,11 +846,12 @@ def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: boo
 
     ``q`` [tokens, heads, headDim]; ``k``, ``v`` [tokens, kvHeads, headDim] (head h reads
     KV head h / (heads / kvHeads)); bfloat16 or float16; headDim 32, 64 or 128; ``starts``
-    int32 [sequences + 1].  ``causal``: a row sees the rows of its sequence up to itself
-    (unlike ``nn.makeCausalMask``, whose orientation is the reference's); otherwise all of
-    them.  ``scale`` 0: 1 / sqrt(headDim).  The softmax is float32; the probabilities are
-    rounded to the operands' dtype before the second product, the result once.  A row of no
-    sequence (before ``starts[0]``, behind ``starts[-1]``) gives zeros.  What a row does not
+    int32 [sequences + 1] (one below an earlier one counts as that one).  ``causal``: a row
+    sees the rows of its sequence up to itself (unlike ``nn.makeCausalMask``, whose
+    orientation is the reference's); otherwise all of them.  ``scale`` 0: 1 / sqrt(headDim).
+    The softmax is float32; the probabilities are rounded to the operands' dtype before the
+    second product, the result once.  A row of no sequence (before ``starts[0]``, behind
+    ``starts[-1]``) gives zeros.  What a row does not
     see does not reach its result, infinities and NaN included.
 
     ``withLse``: (out, stats), the ``PackedStats`` that ``packedAttentionGrad`` takes."""
