@@ -476,12 +476,12 @@ struct Largest {
 // Whether an LDS tile of KEYS rows of D holds an infinity or NaN.
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 template <class M, int KEYS, int D, class P>
-__device__ __forceinline__ bool any_special(P tile) {
+__device__ __forceinline__ bool any_special(P tile, int lane = threadIdx.x & 63) {
   Largest<M> most;
 #pragma unroll
   for (int i = 0; i < KEYS * D / 512; ++i) {
     const u32x4_t w = *(__attribute__((address_space(3))) const u32x4_t*)(
-        tile + i * 512 + (threadIdx.x & 63) * 8);
+        tile + i * 512 + lane * 8);
 #pragma unroll
     for (int j = 0; j < 4; ++j) most.add(w[j]);
   }
@@ -499,11 +499,11 @@ template <int D>
 __device__ __forceinline__ int value_swizzle(int j) {
   return (4 * (j & 3)) % (D / 8);
 }
-// o += the infinities and NaN of the first `seen` of KEYS rows of a tile
+// o += the infinities and NaN of the rows [from, to) of a tile's KEYS rows
 // (o[dt][r 4 + i]: column dt 32 + r 8 + g 4 + i; row j's chunk x of 8 columns at
 // x ^ swizzle(j)).
 template <class M, int KEYS, int D, class P, class Swizzle>
-__device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int seen, int g,
+__device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int from, int to, int g,
                                             Swizzle swizzle) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -517,7 +517,7 @@ __device__ __forceinline__ void add_special(f32x16_t (&o)[D / 32], P tile, int s
             *(__attribute__((address_space(3))) const u32x2*)(tile + j * D + ch * 8 + g * 4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t x = j < seen ? special<M>(w[i]) : 0u;
+          const uint32_t x = j >= from && j < to ? special<M>(w[i]) : 0u;
           o[dt][r * 4 + i * 2] += M::lo(x);
           o[dt][r * 4 + i * 2 + 1] += M::hi(x);
         }

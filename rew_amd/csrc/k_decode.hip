@@ -159,7 +159,7 @@ struct DecodeRows {
                                              const uint32_t (&pk)[1][8]) {
     const int k0 = kt * pd::BK, lane = threadIdx.x & 63;
     if (least < min(k0 + pd::BK, cap) && any_special<M, pd::BK, D>(vs)) {
-      add_special<M, pd::BK, D>(o, vs, my_limit - k0, lane >> 5, value_swizzle<D>);
+      add_special<M, pd::BK, D>(o, vs, 0, my_limit - k0, lane >> 5, value_swizzle<D>);
       clear_special<M, pd::BK, D, 64>(vs, lane);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }

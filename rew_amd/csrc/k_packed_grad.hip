@@ -56,11 +56,10 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 // (bfloat16 needs no maxima: its dQ kernel forms these values from its own rows.)
 //
 // Adds to s, rest and most what eight values x of a row of out, y of dout and z of
-// what rounding took from out give: dout . out, dout . rest, max |out|; and to
-// `largest` y.
+// what rounding took from out give: dout . out, dout . rest, max |out|.
 template <class M>
 __device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s, float& rest,
-                                            float& most, Largest<M>& largest) {
+                                            float& most) {
   const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[2] = {z.x, z.y};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -71,7 +70,6 @@ __device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s,
     rest = fmaf((float)(int8_t)(zs[k >> 1] >> sh), y0, rest);
     rest = fmaf((float)(int8_t)(zs[k >> 1] >> (sh + 8)), y1, rest);
     most = fmaxf(most, fmaxf(fabsf(x0), fabsf(x1)));
-    largest.add(ys[k]);
   }
 }
 template <class M, int D>
@@ -90,9 +88,7 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
     float s = 0.0f, rest = 0.0f, row = 0.0f;
-    Largest<M> largest;
-    delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row, largest);
-    float bad = largest.special() ? 1.0f : 0.0f;
+    delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row);
     if (i >= tok0 * a.H && i < tok1 * a.H)
       for (uint32_t w : {y.x, y.y, y.z, y.w})
         most = fmaxf(most, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
@@ -101,11 +97,10 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
       s += __shfl_xor(s, d);
       rest += __shfl_xor(rest, d);
       row = fmaxf(row, __shfl_xor(row, d));
-      bad = fmaxf(bad, __shfl_xor(bad, d));
     }
     s = fmaf(rest, row * M::kRestStep, s);
     if (ch == 0) {
-      neg_lse[i] = bad > 0.0f ? NAN : M::kGradShift - a.lse[i] * pg::kLog2e;
+      neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
       neg_delta[i] = -s;
     }
   }
@@ -281,6 +276,7 @@ template <class M, int D>
 __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
   using namespace pg;
   typedef typename M::frag frag;
+  typedef __attribute__((address_space(3))) uint16_t lds_u16;
   constexpr int CPR = D / 8, NT = D / 16, DT = D / 32, RPD = 64 / CPR;
   constexpr int BLK = 32 * D;               // elements of 32 rows of Q (or dout)
   constexpr int NDMA = 2 * BLK / 512 / 4;   // DMA instructions per wave and block
@@ -378,24 +374,37 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
     const int w0 = row_of(m);
     return w0 < rows && (!a.causal || w0 + 31 >= wk * G);
   };
-  // Where some row does not see all of the workgroup's keys, infinities and NaN
-  // of Q and dout become zeros before the products (0 times them would reach the
-  // keys that do not see the row): each wave's own part of the block, once it
-  // is there.  Keys that do see it take NaN from the row's lse (its scores were not
-  // finite, or see delta).
+  f32x16_t x, dp;
+  float4 l4[4];
+  uint32_t pp[8], pd[8];
+  // An infinity or NaN of a row's Q makes its lse, one of its dout its delta such
+  // a value, and 0 times it would reach dK and dV of keys that do not see the row.
+  // So a block with such an lse or delta (`odd`, the same in all waves of the
+  // group) goes another way.  Beside its scores the infinities and NaN of dout are
+  // added to dV of the keys that see them, by column: P = 0 there only by underflow.
+  // (dK needs nothing: the row's dS is NaN.)
+  bool odd = false;
+  auto is_odd = [&](float stat) {  // (lane's of the block's 64 values)
+    odd = __builtin_amdgcn_ballot_w64(!(fabsf(stat) < INFINITY)) != 0;
+  };
+  auto add_odd = [&](int m) __attribute__((always_inline)) {
+    if (!odd || !live(m)) return;
+    uint32_t l = lane;
+    opaque(l);
+    lds_u16* Dt = (lds_u16*)(S + slot(m) * 2 * BLK + BLK);
+    if (!any_special<M, 32, D>(Dt, l)) return;
+    const int w0 = row_of(m);
+    add_special<M, 32, D>(dv, Dt, a.causal ? key * G - w0 : 0, rows - w0, (int)l >> 5,
+                          grad_swizzle<CPR>);
+  };
+  // Before its second products they are zeros, each wave's own part of the block.
   auto clean = [&](int m) {
-    if (!a.causal || row_of(m) >= (k0 + BR - 1) * G) return;
-    Largest<M> most;
-#pragma unroll
-    for (int i = 0; i < NDMA; ++i) {
-      const u32x4_t w = *(const u32x4_t*)(S + slot(m) * 2 * BLK + (kw + i * 4) * 512 + lane * 8);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) most.add(w[j]);
-    }
-    if (__builtin_amdgcn_ballot_w64(most.special()) == 0) return;
+    if (!odd) return;
+    uint32_t l = lane;
+    opaque(l);
 #pragma unroll 1
     for (int i = 0; i < NDMA; ++i) {
-      u32x4_t* p = (u32x4_t*)(S + slot(m) * 2 * BLK + (kw + i * 4) * 512 + lane * 8);
+      u32x4_t* p = (u32x4_t*)(S + slot(m) * 2 * BLK + (kw + i * 4) * 512 + l * 8);
       u32x4_t w = *p;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] ^= special<M>(w[j]);
@@ -403,9 +412,6 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
-  f32x16_t x, dp;
-  float4 l4[4];
-  uint32_t pp[8], pd[8];
   auto scores = [&](int m) {
     if (!live(m)) return;
     const uint16_t* Qt = S + slot(m) * 2 * BLK;
@@ -502,10 +508,11 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
   if (n > 0) {
     request(0);
     vm_wait();
-    clean(0);
     block_barrier_fa();
     if (grp == 1) block_barrier_fa();
     __builtin_amdgcn_s_setprio(1);
+    is_odd(R[slot(0) * 64 + lane]);
+    add_odd(0);
     scores(0);
     block_barrier_fa();
     for (int m = 1; m < n; ++m) {
@@ -514,18 +521,23 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
       request(m);
       values(m - 1);
       vm_wait();
-      clean(m);
+      clean(m - 1);
       block_barrier_fa();
       __builtin_amdgcn_s_setprio(1);
+      const float stat = R[slot(m) * 64 + lane];
       accumulate(m - 1);
+      is_odd(stat);
+      add_odd(m);
       scores(m);
       block_barrier_fa();
     }
     __builtin_amdgcn_s_setprio(0);
     read_lse(n - 1);
     values(n - 1);
-    if (grp == 0) block_barrier_fa();
+    clean(n - 1);
+    block_barrier_fa();
     accumulate(n - 1);
+    if (grp == 0) block_barrier_fa();
   }
   // the two row halves meet: wave w keeps dK and takes the other's, wave w + 4
   // likewise dV
@@ -682,7 +694,7 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
       else values(std::true_type());
       if (special) {
         lds_u16* half = (lds_u16*)(ks + h * 32 * D);
-        add_special<M, 32, D>(dq, half, my_limit - kt * BT - h * 32, g, grad_swizzle<CPR>);
+        add_special<M, 32, D>(dq, half, 0, my_limit - kt * BT - h * 32, g, grad_swizzle<CPR>);
         __syncthreads();
         clear_special<M, 32, D, 256>(half, threadIdx.x);
         __syncthreads();
@@ -698,18 +710,16 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     dl = ((const float*)a.work)[a.T * a.H + at];
   } else {
     float s = 0.0f, rest = 0.0f, most = 0.0f;
-    Largest<M> largest;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int64_t i = at * D + t * 16 + g * 8;
       uint4 y;
       __builtin_memcpy(&y, &df[t], 16);
       delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
-                     s, rest, most, largest);
+                     s, rest, most);
     }
-    const float bad = fa_max_halves(largest.special() ? 1.0f : 0.0f);
     s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
-    l = bad > 0.0f ? NAN : M::kGradShift - a.lse[at] * kLog2e;
+    l = M::kGradShift - a.lse[at] * kLog2e;
     dl = -s;
     if (g == 0 && row < rows) {  // (for the dK, dV kernel)
       ((float*)a.work)[at] = l;

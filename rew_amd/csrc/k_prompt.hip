@@ -192,7 +192,7 @@ __device__ __forceinline__ void attend_block(const PackedArgs& a, const BlockRow
     soft_exp<M, 2>(s, sl2, m_run, pk, l_run);
     // (the same answer in all waves)
     if (block_least < min(k0 + BK, cap) && any_special<M, BK, D>((lds_u16*)vs)) {
-      add_special<M, BK, D>(o, (lds_u16*)vs, my_limit - k0, g, value_swizzle<D>);
+      add_special<M, BK, D>(o, (lds_u16*)vs, 0, my_limit - k0, g, value_swizzle<D>);
       __syncthreads();
       clear_special<M, BK, D, 256>((lds_u16*)vs, threadIdx.x);
       __syncthreads();

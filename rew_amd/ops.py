@@ -870,7 +870,7 @@ def packedAttentionGrad(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, out: Te
     summed over the query heads of each KV head; sums are float32 in a fixed order.  What a row
     does not see takes no part, infinities and NaN included: under causality those of a token's
     k and v do not reach gradQ of the rows before it, those of its q and gradOut not gradK and
-    gradV of the keys behind it."""
+    gradV of the keys behind it.  Those of gradOut reach gradV in their own columns only."""
     op = "packedAttentionGrad"
     _check_packed(op, q, k, v, starts)
     for t, name in ((out, "out"), (gradOut, "gradOut")):
