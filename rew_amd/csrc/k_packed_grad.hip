@@ -48,13 +48,39 @@ __device__ __forceinline__ int grad_swizzle(int r) {
 // ---- delta --------------------------------------------------------------------------
 // Per row (D / 8 lanes each of T H rows) what the scores and dP are added to:
 // kGradShift - log2(e) lse, and -delta.  float16 has no room for dS at any scale:
-// it is stored as F dS, F the power of two that takes the bound
-// |dS| <= 2 D max|dout| max|V| to 2^15, so this kernel also leaves the maxima
-// of its workgroups (a maximum does not depend on their order): over the
-// sequences' rows, and over finite values, so that neither what lies outside
-// the sequences nor one sequence's infinity takes the others' bits.
-// (bfloat16 needs no maxima: its dQ kernel forms these values from its own rows.)
-//
+// it is stored as F dS, F a power of two that takes a bound on |dS| to 2^15.  Of the
+// rows and keys that share a sum nothing else may set it, or another document's (or
+// head's, or an unseen row's) large gradient would take this one's bits: dQ has
+// an F per row i, from
+//   |dS_ij| <= D max|dout_i| max|V seen by i| + |delta_i|,
+// dK one per key j, from
+//   |dS_ij| <= D max|dout of rows that see j| max|V_j| + max|delta of these rows|,
+// maxima over finite values.  So this kernel also leaves each row's max|dout| and
+// |delta|, and each key's max|V|, in the order in which a KV head's rows and keys are
+// read.  (bfloat16 needs none: its dQ kernel forms -lse and -delta from its own rows.)
+struct GradMaxima {
+  const float2* rows;  // [Hkv][T H / Hkv]: (max|dout|, |delta|)
+  const float* values; // [Hkv][T]: max|V|
+  __device__ __forceinline__ explicit GradMaxima(const PackedGradArgs& a)
+      : rows((const float2*)((const float*)a.work + 2 * a.T * a.H)),
+        values((const float*)a.work + 4 * a.T * a.H) {}
+};
+__device__ __forceinline__ float finite_abs(float x) {
+  return fabsf(x) < INFINITY ? fabsf(x) : 0.0f;
+}
+// F for a bound (1 without one)
+__device__ __forceinline__ float grad_factor(float bound) {
+  if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
+  int e;
+  (void)frexpf(bound, &e);  // bound < 2^e
+  return ldexpf(1.0f, min(max(15 - e, -60), 60));
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+
 // Adds to s, rest and most what eight values x of a row of out, y of dout and z of
 // what rounding took from out give: dout . out, dout . rest, max |out|.
 template <class M>
@@ -75,90 +101,106 @@ __device__ __forceinline__ void delta_terms(uint4 x, uint4 y, uint2 z, float& s,
 template <class M, int D>
 __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
   constexpr int L = D / 8;
-  const int64_t rows = a.T * a.H, step = gridDim.x * (256ll / L);
-  const int ch = threadIdx.x % L;
-  const int64_t tok0 = seq_bound(a.starts, a.n_seq, (int)a.T, 0);
-  int last = 0;  // (the largest start: SeqRows)
-  for (int s = threadIdx.x & 63; s <= a.n_seq; s += 64)
-    last = max(last, seq_bound(a.starts, a.n_seq, (int)a.T, s));
-  const int64_t tok1 = __builtin_amdgcn_readlane(wave_max_scan(last), 63);
-  auto finite = [](float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; };
+  const int64_t rows = a.T * a.H, keys = a.T * a.Hkv, step = gridDim.x * (256ll / L);
+  const int ch = threadIdx.x % L, G = a.H / a.Hkv;
+  const int64_t first = blockIdx.x * (256ll / L) + threadIdx.x / L;
   float *neg_lse = (float*)a.work, *neg_delta = neg_lse + rows;
-  float most = 0.0f, most_v = 0.0f;
-  for (int64_t i = blockIdx.x * (256ll / L) + threadIdx.x / L; i < rows; i += step) {
+  const GradMaxima maxima(a);
+  for (int64_t i = first; i < rows; i += step) {
     const uint4 x = ((const uint4*)a.out)[i * L + ch], y = ((const uint4*)a.dout)[i * L + ch];
-    float s = 0.0f, rest = 0.0f, row = 0.0f;
+    float s = 0.0f, rest = 0.0f, row = 0.0f, most = 0.0f;
     delta_terms<M>(x, y, ((const uint2*)a.rest)[i * L + ch], s, rest, row);
-    if (i >= tok0 * a.H && i < tok1 * a.H)
-      for (uint32_t w : {y.x, y.y, y.z, y.w})
-        most = fmaxf(most, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
+    for (uint32_t w : {y.x, y.y, y.z, y.w})
+      most = fmaxf(most, fmaxf(finite_abs(M::lo(w)), finite_abs(M::hi(w))));
 #pragma unroll
     for (int d = L / 2; d > 0; d >>= 1) {
       s += __shfl_xor(s, d);
       rest += __shfl_xor(rest, d);
       row = fmaxf(row, __shfl_xor(row, d));
+      most = fmaxf(most, __shfl_xor(most, d));
     }
     s = fmaf(rest, row * M::kRestStep, s);
     if (ch == 0) {
       neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
       neg_delta[i] = -s;
+      const int64_t t = i / a.H;
+      const int h = (int)(i - t * a.H), hk = h / G;
+      ((float2*)maxima.rows)[(hk * a.T + t) * G + h - hk * G] = make_float2(most, finite_abs(s));
     }
   }
-  const int64_t n = tok1 * a.Hkv * L;
-  for (int64_t i = tok0 * a.Hkv * L + blockIdx.x * 256ll + threadIdx.x; i < n;
-       i += gridDim.x * 256ll) {
-    const uint4 x = ((const uint4*)a.v)[i];
+  for (int64_t i = first; i < keys; i += step) {
+    const uint4 x = ((const uint4*)a.v)[i * L + ch];
+    float most = 0.0f;
     for (uint32_t w : {x.x, x.y, x.z, x.w})
-      most_v = fmaxf(most_v, fmaxf(finite(M::lo(w)), finite(M::hi(w))));
-  }
-  __shared__ float part[8];
+      most = fmaxf(most, fmaxf(finite_abs(M::lo(w)), finite_abs(M::hi(w))));
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    most = fmaxf(most, __shfl_xor(most, d));
-    most_v = fmaxf(most_v, __shfl_xor(most_v, d));
-  }
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6] = most;
-    part[4 + (threadIdx.x >> 6)] = most_v;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    const float* q = part + 4 * threadIdx.x;
-    neg_delta[rows + blockIdx.x * 2 + threadIdx.x] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+    for (int d = L / 2; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    const int64_t t = i / a.Hkv;
+    if (ch == 0) ((float*)maxima.values)[(i - t * a.Hkv) * a.T + t] = most;
   }
 }
-// F, from the maxima of the delta kernel's workgroups (a power of two; 1 for
-// bfloat16).  Every thread of a workgroup of N calls it.
-template <class M, int D, int N>
-__device__ __forceinline__ float grad_factor(const PackedGradArgs& a) {
-  if constexpr (!M::kScaled) return 1.0f;
-  __shared__ float part[2 * N / 64];
-  const float* m = (const float*)a.work + 2 * a.T * a.H;
-  float d = 0.0f, v = 0.0f;
-  for (int i = threadIdx.x; i < a.delta_blocks; i += N) {
-    d = fmaxf(d, m[2 * i]);
-    v = fmaxf(v, m[2 * i + 1]);
-  }
+// F of the lane's key in a dK, dV workgroup (keys k0 .. of KV head hk, 32 kw + c the
+// lane's).  Its eight waves call it.
+template <int D>
+__device__ __forceinline__ float key_factor(const PackedGradArgs& a, const SeqTile& st, int rows,
+                                            int hk, int k0, int kw) {
+  __shared__ float2 part[8 + 4];
+  const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5, G = a.H / a.Hkv;
+  const int key = k0 + kw * 32 + c;
+  const GradMaxima maxima(a);
+  const float2* of = maxima.rows + (hk * a.T + st.first) * G;  // of row r of the sequence
+  float2 x = make_float2(0.0f, 0.0f);
+  auto add = [](float2& m, float2 y) { m.x = fmaxf(m.x, y.x), m.y = fmaxf(m.y, y.y); };
+  // the rows that see all keys of the workgroup
+  const int from = a.causal ? (k0 + pg::BR) * G : 0;
+  for (int r = from + (int)threadIdx.x; r < rows; r += 512) add(x, of[r]);
+  part[threadIdx.x >> 6] = make_float2(wave_max(x.x), wave_max(x.y));
+  x = make_float2(0.0f, 0.0f);
+  if (a.causal) {  // those of the wave's own tokens, from each key's token on
+    const int last = min((key + 1) * G, rows);
+    for (int r = key * G + g; r < last; r += 2) add(x, of[r]);
+    x = make_float2(fa_max_halves(x.x), fa_max_halves(x.y));
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) {
-    d = fmaxf(d, __shfl_xor(d, x));
-    v = fmaxf(v, __shfl_xor(v, x));
-  }
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6] = d;
-    part[N / 64 + (threadIdx.x >> 6)] = v;
+    for (int d = 1; d < 32; d <<= 1) {
+      const float2 y = make_float2(__shfl_down(x.x, d, 32), __shfl_down(x.y, d, 32));
+      add(x, y);  // (the last d lanes have their own again)
+    }
+    if (lane == 0) part[8 + kw] = x;
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < N / 64; ++w) {
-    d = fmaxf(d, part[w]);
-    v = fmaxf(v, part[N / 64 + w]);
-  }
-  const float bound = 2.0f * D * d * v;
-  if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;
-  int e;
-  (void)frexpf(bound, &e);  // bound <= 2^e
-  return ldexpf(1.0f, min(max(15 - e, -60), 60));
+  for (int w = 0; w < 8; ++w) add(x, part[w]);
+  if (a.causal)
+    for (int w = kw + 1; w < 4; ++w) add(x, part[8 + w]);
+  const float v = key < st.n ? maxima.values[hk * a.T + st.first + key] : 0.0f;
+  return grad_factor(fmaf(D * x.x, v, x.y));
+}
+// F of the lane's row in a dQ workgroup: it sees the keys below my_limit (my_limit -
+// least < 32), every row of its wave those below `least`, of the workgroup those
+// below block_least.  Its four waves call it.
+template <int D>
+__device__ __forceinline__ float row_factor(const PackedGradArgs& a, const SeqTile& st, int hk,
+                                            int my_limit, int least, int block_least, float dout,
+                                            float delta) {
+  __shared__ float part[4];
+  const int lane = threadIdx.x & 63;
+  const float* of = GradMaxima(a).values + hk * a.T + st.first;
+  float v = 0.0f;
+  for (int j = threadIdx.x; j < block_least; j += 256) v = fmaxf(v, of[j]);
+  part[threadIdx.x >> 6] = wave_max(v);
+  __syncthreads();
+  v = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  float w = 0.0f;
+  for (int j = block_least + lane; j < least; j += 64) w = fmaxf(w, of[j]);
+  v = fmaxf(v, wave_max(w));
+  // the wave's own tokens' keys, up to each row's
+  const int j = least + (lane & 31);
+  float x = j < st.n && least < st.n ? of[j] : 0.0f;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) x = fmaxf(x, __shfl_up(x, d, 32));
+  const float own = __shfl(x, max(my_limit - least - 1, 0), 32);
+  if (my_limit > least) v = fmaxf(v, own);
+  return grad_factor(fmaf(D * dout, v, finite_abs(delta)));
 }
 
 // Where a lane reads its fragments in an LDS tile of D columns, in bytes.
@@ -313,7 +355,8 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[dt][e] = dv[dt][e] = 0.0f;
   const float sl2 = a.scale * kLog2e;
-  const float F = grad_factor<M, D, 512>(a), fs = F * exp2f(-M::kGradShift);
+  // (P has the factor 2^kGradShift already)
+  const float fs = M::kScaled ? key_factor<D>(a, st, rows, hk, k0, kw) * exp2f(-M::kGradShift) : 1.0f;
   const int64_t base = (int64_t)st.first * a.H + hk * G;  // row (tok, hg): base + tok H + hg
   const float* stats = (const float*)a.work;
   // causal: rows of tokens before the workgroup's first key do not see it
@@ -571,7 +614,7 @@ __global__ void __launch_bounds__(512, 1) grad_kv_kernel(PackedGradArgs a) {
                        M::pack(mine[dt][r * 4 + 2] * m, mine[dt][r * 4 + 3] * m));
   };
   // (both branches pass the same barriers)
-  if (grp == 0) meet(dk, dv, a.dk, a.scale / F);
+  if (grp == 0) meet(dk, dv, a.dk, a.scale * exp2f(-M::kGradShift) / fs);
   else meet(dv, dk, a.dv, exp2f(-M::kGradShift));
 }
 
@@ -608,8 +651,7 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
     df[t] = *(const frag*)((const uint16_t*)a.dout + at * D + t * 16 + g * 8);
   }
   const float sl2 = a.scale * kLog2e;
-  const float F = grad_factor<M, D, 256>(a), fs = F * exp2f(-M::kGradShift);
-  float l, dl;
+  float l, dl, fs = 1.0f;  // (fs: with P's factor 2^kGradShift, F)
   const GradFrags<D> fr;
   const int row_in = lane / CPR, pc = lane % CPR;
   const int64_t kstride = (int64_t)a.Hkv * D, kbase = (st.first * (int64_t)a.Hkv + hk) * D;
@@ -708,6 +750,16 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   if constexpr (M::kScaled) {
     l = ((const float*)a.work)[at];
     dl = ((const float*)a.work)[a.T * a.H + at];
+    float dout = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      uint4 y;
+      __builtin_memcpy(&y, &df[t], 16);
+      for (uint32_t w : {y.x, y.y, y.z, y.w})
+        dout = fmaxf(dout, fmaxf(finite_abs(M::lo(w)), finite_abs(M::hi(w))));
+    }
+    fs = row_factor<D>(a, st, hk, my_limit, uniform(least), block_least, fa_max_halves(dout), dl) *
+         exp2f(-M::kGradShift);
   } else {
     float s = 0.0f, rest = 0.0f, most = 0.0f;
 #pragma unroll
@@ -736,7 +788,7 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
   }
   if (row >= rows) return;
   uint16_t* DQ = (uint16_t*)a.dq + at * D;
-  const float sq = a.scale / F;
+  const float sq = a.scale * exp2f(-M::kGradShift) / fs;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -746,21 +798,21 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
                      M::pack(dq[dt][r * 4 + 2] * sq, dq[dt][r * 4 + 3] * sq));
 }
 
-// two values per row, then two maxima for each workgroup of the first kernel
-size_t packed_grad_ws_bytes(int64_t T, int H) {
-  return (size_t)(2 * T * H + 2 * pg::kDeltaBlocks) * 4;
+// two values per row, and for float16 two maxima per row and one per key
+size_t packed_grad_ws_bytes(int64_t T, int H, int Hkv, bool f16) {
+  return (size_t)(f16 ? 4 * T * H + T * Hkv : 2 * T * H) * 4;
 }
 
 template <class M, int D>
-static void launch_grad(PackedGradArgs a, hipStream_t stream) {
-  a.delta_blocks = (int)std::min(pg::kDeltaBlocks, (a.T * a.H * (D / 8) + 255) / 256);
+static void launch_grad(const PackedGradArgs& a, hipStream_t stream) {
   const int64_t kv = max_seq_tiles(a.T, a.n_seq, 1, pg::BR) * a.Hkv;
   const int64_t q = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pg::BR) * a.Hkv;
   if (kv >= (1ll << 31) || q >= (1ll << 31))
     fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention gradient: too many tiles");
-  if constexpr (M::kScaled)
-    hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)a.delta_blocks), dim3(256), 0,
-                       stream, a);
+  if constexpr (M::kScaled) {
+    const int64_t blocks = std::min(pg::kDeltaBlocks, (a.T * a.H * (D / 8) + 255) / 256);
+    hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  }
   hipLaunchKernelGGL((grad_q_kernel<M, D>), dim3((unsigned)q), dim3(256), 0, stream, a);
   hipLaunchKernelGGL((grad_kv_kernel<M, D>), dim3((unsigned)kv), dim3(512), 0, stream, a);
 }

@@ -601,10 +601,9 @@ struct PackedGradArgs {
   void *dq, *dk, *dv, *work;
   int64_t T;
   int n_seq, H, Hkv, D, f16, causal;
-  int delta_blocks;  // set by the launch
   float scale;
 };
-size_t packed_grad_ws_bytes(int64_t T, int H);
+size_t packed_grad_ws_bytes(int64_t T, int H, int Hkv, bool f16);
 int launch_packed_grad(const PackedGradArgs& a, hipStream_t stream);
 
 // ---- pages of a key / value cache (k_pages.hip) -------------------------------------

@@ -368,7 +368,8 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
     invalid("eager '" + op + "': lse must be float32 [tokens, heads]");
   if (rest->dt != kI8 || rest->shape != q->shape)
     invalid("eager '" + op + "': rest must be int8 of q's shape");
-  n->tail = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1]);
+  n->tail = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1], (int)k->shape.d[1],
+                                 q->dt == kF16);
   outs.push_back({q->dt, q->shape});
   outs.push_back({k->dt, k->shape});
   outs.push_back({v->dt, v->shape});
