@@ -3497,7 +3497,7 @@ void Lower::emit_packed_attn(Node* n) {
     a.starts = (const int32_t*)n->in[4]->data();
     a.lens = (const int32_t*)n->in[5]->data();
     a.pages = k->shape.d[0];
-    a.work = (float*)((char*)a.out + tensor_tail_offset(n->out[0]));
+    a.work = (float*)tensor_tail(n->out[0]);
     a.max_new = n->i2;
     a.n_seq = (int)table->shape.d[0];
     a.width = (int)table->shape.d[1];
@@ -3533,7 +3533,7 @@ void Lower::emit_packed_grad(Node* n) {
   a.dq = n->out[0]->data();
   a.dk = n->out[1]->data();
   a.dv = n->out[2]->data();
-  a.work = (char*)a.dq + tensor_tail_offset(n->out[0]);
+  a.work = tensor_tail(n->out[0]);
   a.T = q->shape.d[0];
   a.H = (int)q->shape.d[1];
   a.Hkv = (int)k->shape.d[1];

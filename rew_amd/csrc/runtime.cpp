@@ -121,6 +121,10 @@ void tensor_alloc(Tensor* t) {
   if (t->ctx->rec) plan_note_alloc(t);
 }
 
+void* tensor_tail(const Tensor* t) {
+  return t->tail ? (char*)t->data() + tensor_tail_offset(t) : nullptr;
+}
+
 void tensor_alias(Tensor* t, Tensor* src) {
   if (t->st) return;
   t->st = src->st;

@@ -180,6 +180,8 @@ void tensor_alloc(Tensor* t);                 // give t fresh storage
 inline size_t tensor_tail_offset(const Tensor* t) {
   return ((size_t)t->nbytes() + 255) & ~(size_t)255;
 }
+// .. as an address; null without any (a plan keeps no address outside its blocks)
+void* tensor_tail(const Tensor* t);
 void storage_release(Storage* s);             // drop one reference
 void const_cache_clear(Ctx* c);               // release every cached constant
 void tensor_alias(Tensor* t, Tensor* src);    // share src's storage
