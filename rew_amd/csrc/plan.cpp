@@ -416,6 +416,16 @@ std::string flush_signature(Ctx* c, const std::vector<Node*>& nodes,
     i32(n->cmp);
     i32((int64_t)n->in.size());
     i32((int64_t)n->out.size());
+    // Lowering may put the value of a scalar known on the host into a launch; the
+    // lengths and tables of the sequence ops are read on the device alone, and
+    // those of a few requests, another each step, must not make another plan.
+    const bool reads_host =
+        n->kind != K_PACKED_ATTN && n->kind != K_PACKED_GRAD && n->kind != K_PAGE_TABLES;
+    auto host_value = [&](const Tensor* t) {
+      const bool known = reads_host && t->has_host && t->numel() == 1;
+      i32(known ? 1 : 0);
+      if (known) put(t->host, sizeof t->host);
+    };
     for (Tensor* t : n->in) {
       auto w = where.find(t);
       if (w != where.end()) {
@@ -428,6 +438,7 @@ std::string flush_signature(Ctx* c, const std::vector<Node*>& nodes,
       if (l != leaf_of.end()) {
         i32(-2);
         i32(l->second);
+        host_value(t);
         continue;
       }
       // a leaf first used here: what lowering may read of it
@@ -451,8 +462,7 @@ std::string flush_signature(Ctx* c, const std::vector<Node*>& nodes,
       i32(slot);
       i32(t->st ? (int64_t)((uintptr_t)t->st->ptr & 255) : -1);
       i32(t->prod ? 1 : 0);
-      i32(t->has_host ? 1 : 0);
-      if (t->has_host) put(t->host, sizeof t->host);
+      host_value(t);
     }
     for (size_t o = 0; o < n->out.size(); ++o) {
       const Tensor* t = n->out[o];

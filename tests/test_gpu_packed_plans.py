@@ -84,3 +84,51 @@ def test_decode_step_of_a_layer(gpu, oracle):
         E.toHostF32(layer.forwardPaged(x, cache, step, maxNew=1))
         s = E.stats()
         assert i == 0 or s["flush_plan_hits"] == s["flushes"], (i, s)
+
+
+@pytest.mark.parametrize("R", [1, 2, 4])
+def test_other_lengths_of_few_requests(gpu, R):
+    """Lengths of up to 16 bytes are known on the host too, but read on the device: steps that
+    differ in them alone replay one plan."""
+    r = np.random.default_rng(R)
+    c = paged_case(r, [1] * R, [400] * R, 8, 2, 64, 16, "bfloat16", width=30)
+    (q, _), (k, _), (v, _) = make(r, 90, 4, 2, 64, "bfloat16")
+    results = []
+    for i in range(1, 6):
+        E.sync()
+        E.resetStats()
+        c["lens"] = list(r.integers(20, 400, R))
+        st = O.pagedBlockTables(ints([n + 500 + i for n in c["lens"]]), ints([i] * R),
+                                ints(c["table"]), ints([7 + i]), 16, 8)
+        cuts = np.sort(r.integers(0, 91, R + 1))
+        out, stats = O.packedAttention(q, k, v, ints(cuts), withLse=True)
+        tensors = [paged_call(c), out, *O.packedAttentionGrad(q, k, v, ints(cuts), out, stats, q),
+                   st.blockTable, st.slots, st.lens]
+        E.flush()
+        s = E.stats()
+        # (the first two may share the memory of equal lengths in another way)
+        assert i < 3 or s["flush_plan_hits"] == s["flushes"], (i, s)
+        results.append(([E.toHost(t) for t in tensors], c["lens"], cuts, i))
+    for got, lens, cuts, i in results:  # each lowered by itself
+        E.clearEagerCache()
+        c["lens"] = lens
+        out, stats = O.packedAttention(q, k, v, ints(cuts), withLse=True)
+        st = O.pagedBlockTables(ints([n + 500 + i for n in lens]), ints([i] * R),
+                                ints(c["table"]), ints([7 + i]), 16, 8)
+        for g, t in zip(got, [paged_call(c), out,
+                              *O.packedAttentionGrad(q, k, v, ints(cuts), out, stats, q),
+                              st.blockTable, st.slots, st.lens]):
+            np.testing.assert_array_equal(g, E.toHost(t))
+
+
+def test_scalars_are_told_apart(gpu):
+    """A scalar that a launch holds as a constant makes its own plan, also where a sequence op
+    reads the same tensor."""
+    (q, qh), (k, _), (v, _) = make(np.random.default_rng(0), 4, 2, 2, 32, "bfloat16")
+    for i in range(4):
+        n = ints([i])
+        out = O.packedAttention(q, k, v, n)  # (one start: no sequence)
+        x = O.add(O.broadcastTo(n, [6], [0]), O.iota(ints([0]).dtype, [6], 0))
+        E.flush()
+        np.testing.assert_array_equal(E.toHost(x), i + np.arange(6))
+        assert not E.toHostF32(out).any()
