@@ -5,6 +5,7 @@
 // shape/dtype at record time, and every error names the op.
 #include <algorithm>
 #include <cctype>
+#include <cerrno>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -301,9 +302,11 @@ static bool flag_attr(const Attrs& attrs, const char* key, const std::string& op
 static float scale_attr(const Attrs& attrs, int64_t D, const std::string& op) {
   const std::string v = strip(find_attr(attrs, "scale", op));
   char* end = nullptr;
+  errno = 0;
   const float x = std::strtof(v.c_str(), &end);
-  if (v.empty() || *end || !(x >= 0.0f) || !(x < INFINITY))
-    invalid("eager '" + op + "': scale must be a finite number >= 0, got '" + v + "'");
+  // (a value that underflows to 0 is no request for the default)
+  if (v.empty() || *end || !(x >= 0.0f) || !(x < INFINITY) || (x == 0.0f && errno == ERANGE))
+    invalid("eager '" + op + "': scale must be 0 or a positive float32, got '" + v + "'");
   return x == 0.0f ? 1.0f / std::sqrt((float)D) : x;
 }
 

@@ -826,10 +826,11 @@ def _check_page_size(op: str, page: int) -> int:
 
 
 def _attn_attrs(op: str, causal: bool, scale: float) -> list:
-    if not 0.0 <= scale < float("inf"):
-        raise TensorError(f"{op}: scale must be a finite number >= 0, got {scale}")
-    return [("causal", "true" if causal else "false"),
-            ("scale", repr(float(np.float32(scale))) if scale else "0.0")]
+    with np.errstate(over="ignore", under="ignore"):
+        value = float(np.float32(scale))
+    if not 0.0 <= value < float("inf") or (value == 0.0) != (scale == 0.0):
+        raise TensorError(f"{op}: scale must be 0 or a positive float32, got {scale}")
+    return [("causal", "true" if causal else "false"), ("scale", repr(value))]
 
 
 class PackedStats(NamedTuple):
