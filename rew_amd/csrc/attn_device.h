@@ -308,7 +308,7 @@ struct DivBy {
 };
 
 // A bound on find_tile's tiles, known on the host.
-inline int64_t max_seq_tiles(int64_t T, int n_seq, int64_t units, int64_t per) {
+inline int64_t max_seq_tiles(int64_t T, int64_t n_seq, int64_t units, int64_t per) {
   return T * units / per + n_seq + 2;
 }
 

@@ -807,8 +807,6 @@ template <class M, int D>
 static void launch_grad(const PackedGradArgs& a, hipStream_t stream) {
   const int64_t kv = max_seq_tiles(a.T, a.n_seq, 1, pg::BR) * a.Hkv;
   const int64_t q = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pg::BR) * a.Hkv;
-  if (kv >= (1ll << 31) || q >= (1ll << 31))
-    fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention gradient: too many tiles");
   if constexpr (M::kScaled) {
     const int64_t blocks = std::min(pg::kDeltaBlocks, (a.T * a.H * (D / 8) + 255) / 256);
     hipLaunchKernelGGL((grad_delta_kernel<M, D>), dim3((unsigned)blocks), dim3(256), 0, stream, a);

@@ -471,11 +471,16 @@ size_t paged_ws_bytes(const PackedArgs& a) {
                             : decode_ws_floats(a)) * 4;
 }
 
+int64_t packed_threads(int64_t T, int64_t n_seq, int H, int Hkv, bool grad) {
+  const int64_t rows = (max_seq_tiles(T, n_seq, H / Hkv, pa::BR) * Hkv + kChunkPieces) * 256;
+  // (dK, dV: workgroups of 512 threads, 128 keys each)
+  return grad ? std::max(rows, max_seq_tiles(T, n_seq, 1, 128) * Hkv * 512) : rows;
+}
+
 template <class M, int D>
 static int launch_prompt(const PackedArgs& a, hipStream_t stream) {
   if (a.table && !expects_chunks(a)) return launch_paged_decode(a, stream);
   const int64_t tiles = max_seq_tiles(a.T, a.n_seq, a.H / a.Hkv, pa::BR) * a.Hkv;
-  if (tiles >= (1ll << 30)) fail(REW_MI355X_ERR_UNSUPPORTED, "packed attention: too many tiles");
   if (!a.table) {
     hipLaunchKernelGGL((prompt_attn_kernel<M, D>), dim3((unsigned)tiles), dim3(256), 0, stream, a);
     return 1;

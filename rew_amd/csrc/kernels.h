@@ -579,6 +579,9 @@ struct PackedArgs {
 };
 // Bytes of work; throws where the launch would have 2^31 key tiles.
 size_t paged_ws_bytes(const PackedArgs& a);
+// Threads of the largest launch over n_seq sequences (of the gradients, if `grad`):
+// HIP takes fewer than 2^32.
+int64_t packed_threads(int64_t T, int64_t n_seq, int H, int Hkv, bool grad);
 // 16-bit operands, D of 32, 64 or 128, Hkv divides H.  Returns the kernels
 // launched.
 int launch_packed_attn(const PackedArgs& a, hipStream_t stream);

@@ -333,6 +333,18 @@ static void check_heads(const Tensor* q, int dt, int64_t hkv, int64_t d, const s
     fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': more than 2^20 values per token");
 }
 
+// What a launch over so many sequences (or requests) takes: each workgroup looks
+// through their bounds for its own rows.
+static void check_sequences(int64_t n_seq, int64_t T, int64_t H, int64_t hkv, bool grad,
+                            const std::string& op) {
+  if (n_seq >= (1 << 20))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': 2^20 sequences or more");
+  if (packed_threads(T, n_seq, (int)H, (int)hkv, grad) >= (1ll << 32))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': " + std::to_string(n_seq) +
+                                         " sequences of " + std::to_string(hkv) +
+                                         " KV heads need a launch of 2^32 threads or more");
+}
+
 using OutSpecs = std::vector<std::pair<int, Shape>>;
 
 // packedAttention(q, k, v, starts): attrs causal, scale, stats; out and, with
@@ -349,6 +361,8 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
             std::to_string(k->shape.d[0]));
   check_i32(ins[3], 1, "starts", op);
   if (ins[3]->shape.d[0] < 1) invalid("eager '" + op + "': starts must hold at least one value");
+  check_sequences(ins[3]->shape.d[0] - 1, q->shape.d[0], q->shape.d[1], k->shape.d[1],
+                  n->kind == K_PACKED_GRAD, op);
   n->i0 = flag_attr(attrs, "causal", op);
   const float scale = scale_attr(attrs, q->shape.d[2], op);
   std::memcpy(&n->i1, &scale, sizeof scale);
@@ -392,6 +406,7 @@ static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>
   if (ins[4]->shape.d[0] != R + 1 || ins[5]->shape.d[0] != R)
     invalid("eager '" + op + "': blockTable has " + std::to_string(R) + " requests, starts " +
             ins[4]->shape.str() + " and lens " + ins[5]->shape.str() + " need one more and as many");
+  check_sequences(R, q->shape.d[0], q->shape.d[1], kp->shape.d[1], false, op);
   if (table->shape.d[1] * kp->shape.d[2] > (1ll << 30))
     invalid("eager '" + op + "': the block table reaches past 2^30 tokens per request");
   n->i0 = flag_attr(attrs, "causal", op);

@@ -764,7 +764,8 @@ def fft(a: Tensor, fftType: str, fftLength: Sequence[int]) -> Tensor:
 # all sequences lie one after another (no padding): sequence s owns rows
 # [starts[s], starts[s + 1]).  Lengths and tables are device tensors that no call
 # reads back; values out of range never reach memory outside the tensors: starts are
-# clamped into the rows, and one below an earlier one counts as that one.
+# clamped into the rows, and one below an earlier one counts as that one.  Fewer than
+# 2^20 sequences, and at most about 2^23 / kvHeads of them.
 
 def _packed_call(op: str, operands, attrs, nouts: int) -> list:
     if _jit.currentMode() == "trace":
