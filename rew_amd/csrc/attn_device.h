@@ -101,7 +101,8 @@ struct MmaBf16 {
   typedef bf16x8_t frag;
   static constexpr float kShift = 0.0f, kLazy2 = 11.5f, kGradShift = 0.0f;
   static constexpr bool kScaled = false;  // dS is stored scaled (k_packed_grad.hip)
-  static constexpr float kRestStep = 0x1p-8f / 127.0f;  // of PackedArgs::rest, by the row's max
+  // PackedArgs::rest: a step, by the row's max, and the least max that counts
+  static constexpr float kRestStep = 0x1p-8f / 127.0f, kRestLeast = 0x1p-100f;
   static constexpr uint32_t kInf = 0x7f80;
   static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -118,7 +119,8 @@ struct MmaF16 {
   typedef f16x8_t frag;
   static constexpr float kShift = 11.0f, kLazy2 = 4.0f, kGradShift = 15.0f;
   static constexpr bool kScaled = true;
-  static constexpr float kRestStep = 0x1p-11f / 127.0f;
+  // (below 2^-14 a rounding takes up to 2^-25, whatever the value)
+  static constexpr float kRestStep = 0x1p-11f / 127.0f, kRestLeast = 0x1p-14f;
   static constexpr uint32_t kInf = 0x7c00;
   static __device__ __forceinline__ f32x16_t mma(frag a, frag b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

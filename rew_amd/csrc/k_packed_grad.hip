@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) grad_delta_kernel(PackedGradArgs a) {
       row = fmaxf(row, __shfl_xor(row, d));
       most = fmaxf(most, __shfl_xor(most, d));
     }
-    s = fmaf(rest, row * M::kRestStep, s);
+    s = fmaf(rest, fmaxf(row, M::kRestLeast) * M::kRestStep, s);
     if (ch == 0) {
       neg_lse[i] = M::kGradShift - a.lse[i] * pg::kLog2e;
       neg_delta[i] = -s;
@@ -770,7 +770,8 @@ __global__ void __launch_bounds__(256, 2) grad_q_kernel(PackedGradArgs a) {
       delta_terms<M>(*(const uint4*)((const uint16_t*)a.out + i), y, *(const uint2*)(a.rest + i),
                      s, rest, most);
     }
-    s = fa_sum_halves(fmaf(rest, fa_max_halves(most) * M::kRestStep, s));
+    most = fmaxf(fa_max_halves(most), M::kRestLeast);
+    s = fa_sum_halves(fmaf(rest, most * M::kRestStep, s));
     l = M::kGradShift - a.lse[at] * kLog2e;
     dl = -s;
     if (g == 0 && row < rows) {  // (for the dK, dV kernel)

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
     }
   // (lanes of a row, l and l ^ 32, are both here)
   most = fa_max_halves(most);
-  const float per_step = most > 0.0f ? 1.0f / (most * M::kRestStep) : 0.0f;
+  const float per_step = 1.0f / (fmaxf(most, M::kRestLeast) * M::kRestStep);
   int8_t* rest = a.rest + at * D;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)

@@ -561,8 +561,9 @@ const char* flash_variant(const FlashArgs& a);
 //   lse = log sum_j exp(s_j)   (f32 [T, H]; -inf without keys)
 //   out = sum_j exp(s_j - lse) v_j   (0 without keys)
 // A row of no sequence has no keys.  Of a row, out + rest rest_step, with
-// rest_step = h m / 127, m the row's largest |out| and h half a step of the
-// dtype relative to a value, has out's value 100 times as exactly as out.
+// rest_step = h m / 127, m the row's largest |out| (at least 2^-14 for float16,
+// 2^-100 for bfloat16) and h half a step of the dtype relative to a value, has
+// out's value 100 times as exactly as out.
 struct PackedArgs {
   const void *q, *k, *v;
   void* out;

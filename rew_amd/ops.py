@@ -840,6 +840,7 @@ class PackedStats(NamedTuple):
                   # a row of no sequence
     rest: Tensor  # int8 [tokens, heads, headDim]: what rounding took from the result, in
                   # 1/127 of half a step (bfloat16 2^-8, float16 2^-11) of the row's largest
+                  # (float16: of 2^-14 at least)
 
 
 def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: bool = True,
