@@ -374,14 +374,22 @@ class GroupedQueryAttention:
 
     def forwardPacked(self, x: Tensor, starts: Tensor, positions: Tensor | None = None,
                       causal: bool = True) -> Tensor:
-        """Self-attention over packed sequences, x [tokens, embed] (``ops.packedAttention``)."""
+        """Self-attention over packed sequences, x [tokens, embed] (``ops.packedAttention``).
+        ``positions`` are below the rotary encoding's maxSeqLen (device data: not checked)."""
         q, k, v = self._rows(x, positions)
         return self._project(O.packedAttention(q, k, v, starts, causal))
 
     def forwardPaged(self, x: Tensor, cache: PagedKVCache, step: O.PagedStep,
                      causal: bool = True, maxNew: int = 0) -> Tensor:
         """A serving step's new tokens x [tokens, embed] over their requests' cache, which
-        takes their keys and values (``ops.pagedAttention``)."""
+        takes their keys and values (``ops.pagedAttention``).  With rotary encoding the block
+        table holds maxSeqLen tokens at most: positions are device data, and a request of more
+        would go on with wrong rotations."""
+        room = step.blockTable.shape[1] * cache.kPages.shape[2]
+        if self.rope is not None and room > self.rope.maxSeqLen:
+            raise TensorError(f"GroupedQueryAttention.forwardPaged: a block table for {room} "
+                              "tokens per request exceeds the rotary encoding's maxSeqLen "
+                              f"{self.rope.maxSeqLen}")
         q, k, v = self._rows(x, step.positions)
         return self._project(cache.attend(q, k, v, step, causal, maxNew=maxNew))
 
