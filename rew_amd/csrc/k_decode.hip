@@ -7,10 +7,10 @@
 // two LDS stages of 32 keys of its own, no barrier anywhere.  A tile is a long
 // chain of dependent steps (about 2 us), so it takes four workers on a CU, one
 // per SIMD, to ask for the memory's rate (D = 128: 64 KiB in flight per CU).
-// 64 requests of 400 to 16000 keys, 32 / 8 heads x 128: 198 us, 5.5 TB/s of keys
-// and values, and 8 us of joining; two workers with tiles of 64 keys 225 us, with four stages of 32
-// keys 246 us.  The partial results lie behind the output in its own block:
-// two captured launches never share them.
+// 64 requests of 400 to 16000 keys, 32 / 8 heads x 128: 194 us, 5.7 TB/s of keys
+// and values, and 8 us of joining (two workers with tiles of 64 keys took 27 us
+// more, with four stages of 32 keys 48).  The partial results lie behind the output
+// in its own block: two captured launches never share them.
 #include <algorithm>
 #include <type_traits>
 

@@ -3,17 +3,17 @@
 //
 // delta = dout . out per row is taken from out and what its rounding left (out
 // alone would put out's rounding into every dS, next to dS's own): by a first
-// launch for float16, by the dQ kernel for bfloat16 (939 -> 922 us for the case
-// below, forward pass included).  The dQ kernel gives each workgroup 128 rows and
+// launch for float16, by the dQ kernel for bfloat16 (2 % of the case below,
+// forward pass included).  The dQ kernel gives each workgroup 128 rows and
 // walks their keys, dQ staying in registers; the last launch gives each
 // workgroup 128 keys of one KV head and walks the rows that see them, dK and dV
 // staying in registers.  Both recompute P = exp(S - lse), so the scores are
 // formed twice: 7 products of rows x keys x D where 5 would do, for sums whose
 // order never changes (a single pass would add dQ across workgroups with
 // atomics).  The rows of the H / Hkv heads of a KV head are walked together, so
-// the sum over the group is part of the accumulation.  6 documents of up to 4000 tokens, 32 / 8 heads x 128, bf16:
-// 297-340 (267 GFLOP, 0.79-0.90 PFLOP/s) and 412-500 us (357 GFLOP, 0.71-0.87 PFLOP/s)
-// as the clock falls.
+// the sum over the group is part of the accumulation.  6 documents of up to 4000
+// tokens, 32 / 8 heads x 128, bf16: 272 us (267 GFLOP, 0.98 PFLOP/s) and 401 us
+// (357 GFLOP, 0.89 PFLOP/s), passes back to back.
 //
 // In each product one operand stays in registers and the other is read from
 // LDS; S and dP come out with the operand in registers along the lanes, so P

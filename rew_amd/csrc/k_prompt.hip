@@ -9,14 +9,16 @@
 // scores of one row in a lane and its neighbour lane ^ 32, so the softmax's
 // running max and sum need one exchange; O^T = V^T P^T takes the
 // probabilities from the accumulators, with V read transposed from LDS.  Two
-// workgroups fit a CU, and one's products run beside the other's exponentials.
+// workgroups fit a CU, so that one's products can run beside the other's
+// exponentials; nothing but chance puts them there.
 //
 // 8 ragged prompts of up to 4001 tokens, 32 / 8 heads x 128, bf16 (173 GFLOP):
-// 203 us, 0.85 PFLOP/s, the matrix cores busy for 47 % of the cycles and the
-// vector ALUs for 50 %, at the 1.8 GHz that the card holds under this load (a
-// large product reaches 1.36 PFLOP/s).  Wave priorities changed nothing; the
-// scores of tile i + 1 formed beside the exponentials of tile i in one wave
-// need more registers than there are and were no faster.
+// 198 us, 0.87 PFLOP/s, at the 1.8 GHz that the card holds under this load (a
+// large product reaches 1.36 PFLOP/s).  The matrix cores are busy for 47 % of the
+// cycles and the vector ALUs for 50 %; 39 % of the former have one of the latter
+// beside them, and for a fifth of the time neither works.  Wave priorities
+// changed nothing; the scores of tile i + 1 formed beside the exponentials of tile i
+// in one wave need more registers than there are and were no faster.
 //
 // Rounding: scores, max, sum and O in float32; the probabilities are rounded
 // to the operands' 16 bits for the second product (not in the sum, which the
@@ -307,10 +309,10 @@ __global__ void __launch_bounds__(256, 2) prompt_attn_kernel(PackedArgs a) {
 // time (its 64 KiB are written and read), so P is the number of times that the
 // request's middle block holds C tiles, rounded, C being a CU's share of all
 // tiles or at least kPieceTiles: no block is split where the blocks fill the
-// CUs by themselves (2048 tokens over 30001 keys: 1.11 ms, 0.94 PFLOP/s; cut
+// CUs by themselves (2048 tokens over 30001 keys: 1.07 ms, 0.97 PFLOP/s; cut
 // into 512 equal runs, 1.30 ms and 140 us of joining).  Single tokens of other
 // requests in the same step are blocks of few rows here: 13 requests of 1 to
-// 539 new tokens over up to 4400 keys take 47 us and 8 us of joining, with
+// 539 new tokens over up to 4400 keys take 44 us and 8 us of joining, with
 // pieces of 8 or 12 tiles the same, of 20 more.
 struct ChunkPlan {
   const PackedArgs& a;

@@ -559,7 +559,7 @@ const char* flash_variant(const FlashArgs& a);
 // seen.  With s_j = scale q . k_j over the keys seen (head h reads KV head
 // h / (H / Hkv)):
 //   lse = log sum_j exp(s_j)   (f32 [T, H]; -inf without keys)
-//   out = sum_j exp(s_j - lse) v_j   (0 without keys)
+//   out = sum_j exp(s_j - lse) v_j   (0 without keys, and where all s_j are -inf)
 // A row of no sequence has no keys.  Of a row, out + rest rest_step, with
 // rest_step = h m / 127, m the row's largest |out| (at least 2^-14 for float16,
 // 2^-100 for bfloat16) and h half a step of the dtype relative to a value, has

@@ -854,8 +854,8 @@ def packedAttention(q: Tensor, k: Tensor, v: Tensor, starts: Tensor, causal: boo
     orientation is the reference's); otherwise all of them.  ``scale`` 0: 1 / sqrt(headDim).
     The softmax is float32; the probabilities are rounded to the operands' dtype before the
     second product, the result once.  A row of no sequence (before ``starts[0]``, behind
-    ``starts[-1]``) gives zeros.  What a row does not
-    see does not reach its result, infinities and NaN included.
+    ``starts[-1]``) gives zeros, and so does one whose every score is -infinity.  What a row
+    does not see does not reach its result, infinities and NaN included.
 
     ``withLse``: (out, stats), the ``PackedStats`` that ``packedAttentionGrad`` takes."""
     _check_packed("packedAttention", q, k, v, starts)
