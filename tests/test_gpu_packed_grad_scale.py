@@ -85,3 +85,39 @@ def test_row_of_its_own_size(gpu, causal):
     x[3] = tensor(x[3] * size[:, None, None], "float16")[1]
     want, bnd = R.packed_grad(*x[:3], starts, x[3], causal, 0.125, "float16")
     close(grads(x, starts, "float16", causal)[0], want[0], bnd[0], slice(None))
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(7, 7, 32), (40, 1, 64), (71, 1, 128), (15, 5, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_odd_groups(gpu, H, Hkv, D, causal):
+    """Groups that do not divide a block of rows, a large gradient in the document before."""
+    starts = [0, 30, 200]
+    x = case(H, 200, H, Hkv, D, "float16", 1e-3)
+    want, bnd = R.packed_grad(*x[:3], starts, x[3], causal, D ** -0.5, "float16")
+    x[3][[0, 29], :, 5] = tensor([6e4], "float16")[1]
+    for g, w, b in zip(grads(x, starts, "float16", causal), want, bnd):
+        close(g, w, b, slice(30, 200))
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [2, 31, 150, 400])
+def test_largest_values(gpu, D, causal, n):
+    """gradOut and V of one size and sign in all columns, near float16's largest: dS reaches the
+    bound that its factor comes from, D max|gradOut| max|V| + |delta|."""
+    r = np.random.default_rng(n + D)
+    q, k = (tensor(r.standard_normal((n, h, D)), "float16")[1] for h in (4, 2))
+    sign = lambda h: np.broadcast_to(r.choice([-1.0, 1.0], (n, h, 1)), (n, h, D))
+    v, do = sign(2) * 6e4, sign(4) * 6e4
+    x = [q, k, tensor(v, "float16")[1], tensor(do, "float16")[1]]
+    # (dQ = scale dS K below 2^-26 D 3.6e9 2 max|k| < 7e4 / 2: no result overflows)
+    scale = 2.0 ** -26 / (D / 32)
+    want, bnd = R.packed_grad(*x[:3], [0, n], x[3], causal, scale, "float16")
+    t = [tensor(y, "float16")[0] for y in x]
+    out, stats = O.packedAttention(*t[:3], ints([0, n]), causal=causal, scale=scale, withLse=True)
+    got = O.packedAttentionGrad(*t[:3], ints([0, n]), out, stats, t[3], causal=causal, scale=scale)
+    for i in (0, 1):
+        g = E.toHostF32(got[i]).astype(np.float64)
+        fits = np.abs(want[i]) < 6e4
+        assert np.isfinite(g[fits]).all() and fits.mean() > 0.9
+        assert (np.abs(g - want[i])[fits] <= bnd[i][fits] + TINY).all()
