@@ -641,6 +641,87 @@ struct PageWriteArgs {
 };
 void launch_page_write(const PageWriteArgs& a, hipStream_t stream);
 
+// ---- embedding rows (k_embed.hip) ---------------------------------------------------
+// out[t, :] = scale * w[ids[t], :] (zeros for an id outside [0, V)), the product
+// in float32 and rounded once.  w [V, E], out [T, E] of one float dtype.
+struct EmbedArgs {
+  const void* w;
+  const int32_t* ids;
+  void* out;
+  int64_t T, V, E;
+  int dt;
+  float scale;
+};
+void launch_embed(const EmbedArgs& a, hipStream_t stream);
+// out[v, :] = scale * sum of grad[t, :] over the tokens with ids[t] = v, in
+// float32 in a fixed order, rounded once.  work: embed_grad_ws_bytes.
+struct EmbedGradArgs {
+  const int32_t* ids;
+  const void* grad;
+  void *out, *work;
+  int64_t T, V, E;
+  int dt;
+  float scale;
+};
+size_t embed_grad_ws_bytes(int64_t T, int64_t V, int64_t E);
+int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream);  // (number of launches)
+
+// ---- layer norm (k_norm.hip) --------------------------------------------------------
+// Per row: m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), y = (x - m) r gamma +
+// beta, in float32, y rounded once.  mean and rstd [rows] may be null.  x and y
+// of x_dt; gamma and beta of p_dt (x_dt or float32).
+struct NormArgs {
+  const void *x, *gamma, *beta;
+  void* y;
+  float *mean, *rstd;
+  int64_t rows, n;
+  int x_dt, p_dt;
+  float eps;
+};
+void launch_norm(const NormArgs& a, hipStream_t stream);
+// With xh = (x - mean) rstd and w = dy gamma:  dx = rstd (w - mean w - xh mean (w xh)),
+// dgamma = sum over the rows of dy xh, dbeta = that of dy.  Sums in float32 in a
+// fixed order; dgamma and dbeta of p_dt.  work: norm_grad_ws_bytes.
+struct NormGradArgs {
+  const void *x, *gamma, *dy;
+  const float *mean, *rstd;
+  void *dx, *dgamma, *dbeta;
+  float* work;
+  int64_t rows, n;
+  int x_dt, p_dt;
+};
+size_t norm_grad_ws_bytes(int64_t rows, int64_t n);
+int launch_norm_grad(const NormGradArgs& a, hipStream_t stream);
+
+// ---- cross entropy of a linear head (k_xent.hip) ------------------------------------
+// z = x w (float32), lse[t] = log sum_v exp z[t, v], loss[t] = lse[t] - z[t, target[t]],
+// 0 where the target lies outside [0, V).  x [T, H]; w [H, V], tied: [V, H]; bfloat16
+// or float16.  lse may be null.  work: xent_ws_bytes.
+struct XentArgs {
+  const void *x, *w;
+  const int32_t* target;
+  float *loss, *lse;
+  void* work;
+  int64_t T, H, V;
+  int tied, f16;
+};
+size_t xent_ws_bytes(const XentArgs& a);
+int launch_xent(const XentArgs& a, hipStream_t stream);
+// dz[t, v] = grad[t] (exp(z[t, v] - lse[t]) - [v = target[t]]), rows without a
+// target 0; dx = dz w^T, dw = x^T dz (of w's shape).  The logits are formed anew, a
+// piece of the vocabulary at a time; dz is rounded once to x's dtype for the two
+// products, divided by the largest |grad| before.  work: xent_grad_ws_bytes.
+struct XentGradArgs {
+  const void *x, *w;
+  const int32_t* target;
+  const float *lse, *grad;
+  void *dx, *dw, *work;
+  int64_t T, H, V;
+  int tied, f16;
+};
+size_t xent_grad_ws_bytes(const XentGradArgs& a);
+int launch_xent_grad(const XentGradArgs& a, hipStream_t stream);
+
 // ---- row composites (k_rows.hip) ----------------------------------------------
 // rmsNorm over rows of n contiguous elements (x row stride x_rs elements):
 // y[r, j] = gamma[j] * (x[r, j] / sqrt(sum_j x^2 / divisor + eps)).

@@ -389,6 +389,9 @@ struct Lower {
   void emit_cholesky(Node* n);
   void emit_packed_attn(Node* n);
   void emit_packed_grad(Node* n);
+  void emit_embed(Node* n);
+  void emit_norm(Node* n);
+  void emit_xent(Node* n);
   void emit_page_tables(Node* n);
   void emit_trisolve(Node* n);
   void emit_complex(Node* n);
@@ -1115,6 +1118,9 @@ void Lower::emit_anchor(Node* n) {
     case K_PACKED_ATTN: emit_packed_attn(n); break;
     case K_PACKED_GRAD: emit_packed_grad(n); break;
     case K_PAGE_TABLES: emit_page_tables(n); break;
+    case K_EMBED: emit_embed(n); break;
+    case K_NORM: emit_norm(n); break;
+    case K_XENT: emit_xent(n); break;
     case K_TRISOLVE: emit_trisolve(n); break;
     case K_COMPLEX: emit_complex(n); break;
     case K_FFT1: emit_fft1(n); break;
@@ -3562,6 +3568,135 @@ void Lower::emit_page_tables(Node* n) {
   a.log_page = (int)n->i0;
   Launch L{a};
   if (c->profiling) L.name = "page_tables{" + std::to_string(a.n) + "}";
+  run_launch(c, std::move(L));
+}
+
+static std::string sizes_label(std::initializer_list<int64_t> sizes) {
+  std::string s;
+  for (int64_t x : sizes) s += (s.empty() ? "{" : "x") + std::to_string(x);
+  return s + "}";
+}
+
+// embedding: weight, ids; embeddingGrad (sub 1): ids, gradOut.
+void Lower::emit_embed(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  const Tensor* table = n->sub ? n->out[0] : n->in[0];
+  const Tensor* ids = n->in[n->sub ? 0 : 1];
+  auto fill = [&](auto& a) {
+    a.ids = (const int32_t*)ids->data();
+    a.out = n->out[0]->data();
+    a.T = ids->numel();
+    a.V = table->shape.d[0];
+    a.E = table->shape.d[1];
+    a.dt = table->dt;
+    std::memcpy(&a.scale, &n->i1, sizeof a.scale);
+  };
+  Launch L;
+  if (n->sub) {
+    EmbedGradArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.grad = n->in[1]->data();
+    a.work = tensor_tail(n->out[0]);
+    L.args = a;
+  } else {
+    EmbedArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.w = n->in[0]->data();
+    L.args = a;
+  }
+  if (c->profiling)
+    L.name = (n->sub ? "embed_grad" : "embed") +
+             sizes_label({ids->numel(), table->shape.d[0], table->shape.d[1]});
+  run_launch(c, std::move(L));
+}
+
+// layerNorm: x, gamma, beta; layerNormGrad (sub 1): x, gamma, mean, rstd, gradOut.
+void Lower::emit_norm(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  const Tensor *x = n->in[0], *gamma = n->in[1];
+  auto fill = [&](auto& a) {
+    a.x = x->data();
+    a.gamma = gamma->data();
+    a.n = gamma->numel();
+    a.rows = x->numel() / a.n;
+    a.x_dt = x->dt;
+    a.p_dt = gamma->dt;
+  };
+  Launch L;
+  if (n->sub) {
+    NormGradArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.mean = (const float*)n->in[2]->data();
+    a.rstd = (const float*)n->in[3]->data();
+    a.dy = n->in[4]->data();
+    a.dx = n->out[0]->data();
+    a.dgamma = n->out[1]->data();
+    a.dbeta = n->out[2]->data();
+    a.work = (float*)tensor_tail(n->out[0]);
+    L.args = a;
+  } else {
+    NormArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.beta = n->in[2]->data();
+    a.y = n->out[0]->data();
+    if (n->out.size() > 1) {
+      a.mean = (float*)n->out[1]->data();
+      a.rstd = (float*)n->out[2]->data();
+    }
+    std::memcpy(&a.eps, &n->i1, sizeof a.eps);
+    L.args = a;
+  }
+  if (c->profiling)
+    L.name = (n->sub ? "layer_norm_grad" : "layer_norm") +
+             sizes_label({x->numel() / gamma->numel(), gamma->numel()});
+  run_launch(c, std::move(L));
+}
+
+// linearCrossEntropy: x, weight, targets; linearCrossEntropyGrad (sub 1): x,
+// weight, targets, lse, gradLoss.
+void Lower::emit_xent(Node* n) {
+  for (Tensor* t : n->in) ensure_mat(t);
+  for (Tensor* t : n->out) tensor_alloc(t);
+  const Tensor *x = n->in[0], *w = n->in[1];
+  const int tied = (int)n->i0;
+  auto fill = [&](auto& a) {
+    a.x = x->data();
+    a.w = w->data();
+    a.target = (const int32_t*)n->in[2]->data();
+    a.T = x->shape.d[0];
+    a.H = x->shape.d[1];
+    a.V = w->shape.d[tied ? 0 : 1];
+    a.tied = tied;
+    a.f16 = x->dt == kF16;
+    a.work = tensor_tail(n->out[0]);
+  };
+  Launch L;
+  if (n->sub) {
+    XentGradArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.lse = (const float*)n->in[3]->data();
+    a.grad = (const float*)n->in[4]->data();
+    a.dx = n->out[0]->data();
+    a.dw = n->out[1]->data();
+    L.args = a;
+  } else {
+    XentArgs a;
+    std::memset(&a, 0, sizeof a);
+    fill(a);
+    a.loss = (float*)n->out[0]->data();
+    if (n->out.size() > 1) a.lse = (float*)n->out[1]->data();
+    L.args = a;
+  }
+  if (c->profiling)
+    L.name = (n->sub ? "cross_entropy_grad" : "cross_entropy") +
+             sizes_label({x->shape.d[0], x->shape.d[1], w->shape.d[tied ? 0 : 1]});
   run_launch(c, std::move(L));
 }
 

@@ -119,6 +119,10 @@ static const std::unordered_map<std::string, OpSpec>& op_table() {
       // reference; pagedCacheWrite, which updates its pages, is not recorded)
       {"packedAttention", {K_PACKED_ATTN, 0}}, {"pagedAttention", {K_PACKED_ATTN, 1}},
       {"packedAttentionGrad", {K_PACKED_GRAD, 0}}, {"pagedBlockTables", {K_PAGE_TABLES, 0}},
+      // the ends of a training step (no eager counterpart in the reference)
+      {"embedding", {K_EMBED, 0}}, {"embeddingGrad", {K_EMBED, 1}},
+      {"layerNorm", {K_NORM, 0}}, {"layerNormGrad", {K_NORM, 1}},
+      {"linearCrossEntropy", {K_XENT, 0}}, {"linearCrossEntropyGrad", {K_XENT, 1}},
   };
   return t;
 }
@@ -454,6 +458,150 @@ static void prepare_page_tables(const std::string& op, const std::vector<Tensor*
   outs.push_back({kI32, vec(1)});
 }
 
+// ---- the ends of a training step -----------------------------------------------------
+
+// A finite float32 attr (positive: above zero), as the bits of Node::i1.
+static void float_attr(const Attrs& attrs, const char* key, bool positive, const std::string& op,
+                       Node* n) {
+  const std::string v = strip(find_attr(attrs, key, op));
+  char* end = nullptr;
+  const float x = std::strtof(v.c_str(), &end);
+  if (v.empty() || *end || !std::isfinite(x) || (positive && !(x > 0.0f)))
+    invalid("eager '" + op + "': " + key + " must be a " + (positive ? "positive" : "finite") +
+            " float32, got '" + v + "'");
+  n->i1 = 0;
+  std::memcpy(&n->i1, &x, sizeof x);
+}
+
+static void check_row_dtype(int dt, const std::string& op) {
+  if (dt != kF32 && dt != kBF16 && dt != kF16)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': only float32 / bfloat16 / float16, got " +
+                                         dt_enum_name(dt));
+}
+
+// embedding(weight, ids): attr scale; rows.  embeddingGrad(ids, gradOut): attrs
+// vocab, scale; gradWeight.
+static void prepare_embed(const std::string& op, const std::vector<Tensor*>& ins,
+                          const Attrs& attrs, Node* n, OutSpecs& outs) {
+  const Tensor* ids = ins[n->sub ? 0 : 1];
+  const Tensor* rows = ins[n->sub ? 1 : 0];
+  if (ids->dt != kI32)
+    invalid("eager '" + op + "': ids must be an int32 tensor, got " + dt_enum_name(ids->dt));
+  if (ids->shape.rank >= kMaxRank) invalid("eager '" + op + "': ids of rank " +
+                                           std::to_string(ids->shape.rank));
+  check_row_dtype(rows->dt, op);
+  float_attr(attrs, "scale", false, op, n);
+  std::vector<int64_t> shape = ids->shape.vec();
+  if (!n->sub) {
+    if (rows->shape.rank != 2)
+      invalid("eager '" + op + "': weight must be [vocab, embed], got " + rows->shape.str());
+    shape.push_back(rows->shape.d[1]);
+    outs.push_back({rows->dt, Shape(shape)});
+  } else {
+    const int r = rows->shape.rank;
+    if (r < 1) invalid("eager '" + op + "': gradOut must be [ids.., embed], got " + rows->shape.str());
+    shape.push_back(rows->shape.d[r - 1]);
+    if (rows->shape != Shape(shape))
+      invalid("eager '" + op + "': gradOut must be [ids.., embed], got " + rows->shape.str() +
+              " for ids " + ids->shape.str());
+    n->i0 = parse_int(find_attr(attrs, "vocab", op), op);
+    if (n->i0 < 1 || n->i0 >= kMaxElems) invalid("eager '" + op + "': vocab must be positive");
+    outs.push_back({rows->dt, Shape(std::vector<int64_t>{n->i0, shape.back()})});
+    n->tail = embed_grad_ws_bytes(ids->numel(), n->i0, shape.back());
+  }
+  if (shape.back() < 1 || shape.back() > (1 << 20))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': rows must have 1 to 2^20 values");
+}
+
+// layerNorm(x, gamma, beta): attrs eps, stats; y and, with stats, mean and rstd.
+// layerNormGrad(x, gamma, mean, rstd, gradOut): the gradients of x, gamma, beta.
+static void prepare_norm(const std::string& op, const std::vector<Tensor*>& ins,
+                         const Attrs& attrs, Node* n, OutSpecs& outs) {
+  const Tensor *x = ins[0], *gamma = ins[1];
+  check_row_dtype(x->dt, op);
+  if (gamma->dt != x->dt && gamma->dt != kF32)
+    invalid("eager '" + op + "': gamma must have x's dtype or float32, got " +
+            dt_enum_name(gamma->dt));
+  const int lead = x->shape.rank - gamma->shape.rank;
+  bool fits = gamma->shape.rank >= 1 && lead >= 0;
+  for (int i = 0; fits && i < gamma->shape.rank; ++i)
+    fits = gamma->shape.d[i] == x->shape.d[lead + i];
+  if (!fits)
+    invalid("eager '" + op + "': gamma " + gamma->shape.str() + " must be the last dims of x " +
+            x->shape.str());
+  if (gamma->numel() < 1) invalid("eager '" + op + "': rows must have at least one value");
+  const Shape rows(std::vector<int64_t>(x->shape.d, x->shape.d + lead));
+  if (!n->sub) {
+    if (ins[2]->dt != gamma->dt || ins[2]->shape != gamma->shape)
+      invalid("eager '" + op + "': beta must have gamma's dtype and shape");
+    float_attr(attrs, "eps", true, op, n);
+    outs.push_back({x->dt, x->shape});
+    if (flag_attr(attrs, "stats", op)) {
+      outs.push_back({kF32, rows});
+      outs.push_back({kF32, rows});
+    }
+    return;
+  }
+  for (int i : {2, 3})
+    if (ins[i]->dt != kF32 || ins[i]->shape != rows)
+      invalid("eager '" + op + "': mean and rstd must be float32 " + rows.str());
+  if (ins[4]->dt != x->dt || ins[4]->shape != x->shape)
+    invalid("eager '" + op + "': gradOut must have x's dtype and shape");
+  n->tail = norm_grad_ws_bytes(x->numel() / gamma->numel(), gamma->numel());
+  outs.push_back({x->dt, x->shape});
+  outs.push_back({gamma->dt, gamma->shape});
+  outs.push_back({gamma->dt, gamma->shape});
+}
+
+// linearCrossEntropy(x, weight, targets): attrs tied, stats; loss and, with
+// stats, lse.  linearCrossEntropyGrad(x, weight, targets, lse, gradLoss): attr
+// tied; the gradients of x and weight.
+static void prepare_xent(const std::string& op, const std::vector<Tensor*>& ins,
+                         const Attrs& attrs, Node* n, OutSpecs& outs) {
+  const Tensor *x = ins[0], *w = ins[1];
+  if (x->shape.rank != 2 || w->shape.rank != 2)
+    invalid("eager '" + op + "': x must be [tokens, embed] and weight of rank 2, got " +
+            x->shape.str() + " and " + w->shape.str());
+  if (w->dt != x->dt)
+    invalid("eager '" + op + "': dtype mismatch (" + dt_enum_name(x->dt) + " vs " +
+            dt_enum_name(w->dt) + ")");
+  if (x->dt != kBF16 && x->dt != kF16)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': only bfloat16 / float16, got " +
+                                         dt_enum_name(x->dt));
+  const int tied = flag_attr(attrs, "tied", op);
+  n->i0 = tied;
+  const int64_t T = x->shape.d[0], H = x->shape.d[1], V = w->shape.d[tied ? 0 : 1];
+  if (w->shape.d[tied ? 1 : 0] != H)
+    invalid("eager '" + op + "': x " + x->shape.str() + " and weight " + w->shape.str() +
+            (tied ? " ([vocab, embed])" : " ([embed, vocab])") + " differ in embed");
+  if (H < 1 || V < 1) invalid("eager '" + op + "': embed and vocab must be positive");
+  if (H > (1 << 21) || V > (1 << 21))
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': embed and vocab up to 2^21");
+  check_i32(ins[2], 1, "targets", op);
+  const Shape rows(std::vector<int64_t>{T});
+  if (ins[2]->shape != rows)
+    invalid("eager '" + op + "': targets must be [" + std::to_string(T) + "], got " +
+            ins[2]->shape.str());
+  if (!n->sub) {
+    XentArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.T = T, a.H = H, a.V = V, a.tied = tied;
+    n->tail = xent_ws_bytes(a);
+    outs.push_back({kF32, rows});
+    if (flag_attr(attrs, "stats", op)) outs.push_back({kF32, rows});
+    return;
+  }
+  if (ins[3]->dt != kF32 || ins[3]->shape != rows)
+    invalid("eager '" + op + "': lse must be float32 [" + std::to_string(T) + "]");
+  if (ins[4]->dt != kF32 || ins[4]->shape != rows)
+    invalid("eager '" + op + "': gradLoss must be float32 [" + std::to_string(T) + "]");
+  XentGradArgs a;
+  std::memset(&a, 0, sizeof a);
+  a.T = T, a.H = H, a.V = V, a.tied = tied;
+  n->tail = xent_grad_ws_bytes(a);
+  outs.push_back({x->dt, x->shape});
+  outs.push_back({w->dt, w->shape});
+}
 
 // ---- record ------------------------------------------------------------------------
 
@@ -1127,6 +1275,18 @@ Node* prepare_node(Ctx* c, const std::string& op, const std::vector<Tensor*>& in
       case K_PAGE_TABLES:
         nin(4);
         prepare_page_tables(op, ins, attrs, n, outs);
+        break;
+      case K_EMBED:
+        nin(2);
+        prepare_embed(op, ins, attrs, n, outs);
+        break;
+      case K_NORM:
+        nin(spec.sub ? 5 : 3);
+        prepare_norm(op, ins, attrs, n, outs);
+        break;
+      case K_XENT:
+        nin(spec.sub ? 5 : 3);
+        prepare_xent(op, ins, attrs, n, outs);
         break;
       case K_CHOLESKY: {
         // stablehlo.cholesky (src/rew/ops/linalg.nim:177-202)

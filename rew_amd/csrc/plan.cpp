@@ -179,6 +179,46 @@ struct PtrVisit {
     for (int32_t** p : {&a.out_table, &a.slots, &a.positions, &a.starts, &a.lens, &a.taken})
       field(f, *p);
   }
+  void operator()(EmbedArgs& a) {
+    field(f, a.w);
+    field(f, a.ids);
+    field(f, a.out);
+  }
+  void operator()(EmbedGradArgs& a) {
+    field(f, a.ids);
+    field(f, a.grad);
+    field(f, a.out);
+    field(f, a.work);
+  }
+  void operator()(NormArgs& a) {
+    for (const void** p : {&a.x, &a.gamma, &a.beta}) field(f, *p);
+    field(f, a.y);
+    field(f, a.mean);
+    field(f, a.rstd);
+  }
+  void operator()(NormGradArgs& a) {
+    for (const void** p : {&a.x, &a.gamma, &a.dy}) field(f, *p);
+    field(f, a.mean);
+    field(f, a.rstd);
+    for (void** p : {&a.dx, &a.dgamma, &a.dbeta}) field(f, *p);
+    field(f, a.work);
+  }
+  void operator()(XentArgs& a) {
+    field(f, a.x);
+    field(f, a.w);
+    field(f, a.target);
+    field(f, a.loss);
+    field(f, a.lse);
+    field(f, a.work);
+  }
+  void operator()(XentGradArgs& a) {
+    field(f, a.x);
+    field(f, a.w);
+    field(f, a.target);
+    field(f, a.lse);
+    field(f, a.grad);
+    for (void** p : {&a.dx, &a.dw, &a.work}) field(f, *p);
+  }
   void operator()(RouterArgs& a) {
     field(f, a.x);
     field(f, a.w);
@@ -243,6 +283,18 @@ struct Exec {
     c->stats.kernels_launched += launch_packed_grad(a, c->stream) - 1;
   }
   void operator()(PageTablesArgs& a) { launch_page_tables(a, c->stream); }
+  void operator()(EmbedArgs& a) { launch_embed(a, c->stream); }
+  void operator()(EmbedGradArgs& a) {
+    c->stats.kernels_launched += launch_embed_grad(a, c->stream) - 1;
+  }
+  void operator()(NormArgs& a) { launch_norm(a, c->stream); }
+  void operator()(NormGradArgs& a) {
+    c->stats.kernels_launched += launch_norm_grad(a, c->stream) - 1;
+  }
+  void operator()(XentArgs& a) { c->stats.kernels_launched += launch_xent(a, c->stream) - 1; }
+  void operator()(XentGradArgs& a) {
+    c->stats.kernels_launched += launch_xent_grad(a, c->stream) - 1;
+  }
   void operator()(FillL& l) {
     if (l.bytes == 0) return;
     if (l.src)
@@ -417,10 +469,12 @@ std::string flush_signature(Ctx* c, const std::vector<Node*>& nodes,
     i32((int64_t)n->in.size());
     i32((int64_t)n->out.size());
     // Lowering may put the value of a scalar known on the host into a launch; the
-    // lengths and tables of the sequence ops are read on the device alone, and
-    // those of a few requests, another each step, must not make another plan.
-    const bool reads_host =
-        n->kind != K_PACKED_ATTN && n->kind != K_PACKED_GRAD && n->kind != K_PAGE_TABLES;
+    // lengths and tables of the sequence ops, ids and targets are read on the device
+    // alone, and those of a few requests, another each step, must not make another
+    // plan.
+    const bool reads_host = n->kind != K_PACKED_ATTN && n->kind != K_PACKED_GRAD &&
+                            n->kind != K_PAGE_TABLES && n->kind != K_EMBED &&
+                            n->kind != K_NORM && n->kind != K_XENT;
     auto host_value = [&](const Tensor* t) {
       const bool known = reads_host && t->has_host && t->numel() == 1;
       i32(known ? 1 : 0);

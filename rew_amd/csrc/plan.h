@@ -60,7 +60,8 @@ using LaunchArgs = std::variant<EwL, ReduceL, GemmL, FlashArgs, RowNormArgs, Sof
                                 RopeArgs, GatherArgs, ArgmaxArgs, TopkArgs, SortArgs,
                                 IndexMapL, MoeL, FillL, WindowArgs, CholeskyArgs, TriSolveArgs, ComplexArgs, Fft1Args,
                                 BatchNormArgs, HeadArgs, RouterArgs, PackedArgs,
-                                PackedGradArgs, PageTablesArgs>;
+                                PackedGradArgs, PageTablesArgs, EmbedArgs, EmbedGradArgs,
+                                NormArgs, NormGradArgs, XentArgs, XentGradArgs>;
 
 struct Launch {
   LaunchArgs args;

@@ -73,6 +73,9 @@ enum Kind : int {
   K_PACKED_ATTN,  // packedAttention, pagedAttention (sub 1)
   K_PACKED_GRAD,  // packedAttentionGrad
   K_PAGE_TABLES,  // pagedBlockTables
+  K_EMBED,        // embedding, embeddingGrad (sub 1)
+  K_NORM,         // layerNorm, layerNormGrad (sub 1)
+  K_XENT,         // linearCrossEntropy, linearCrossEntropyGrad (sub 1)
   K_BATCHNORM, // batchNormInference / Training / Grad (sub: kBn*)
   // composite kernels created by the planner (never recorded directly)
   K_COUNT

@@ -979,3 +979,168 @@ def pagedAttention(q: Tensor, kPages: Tensor, vPages: Tensor, blockTable: Tensor
         raise TensorError(f"{op}: maxNew must be non-negative, got {maxNew}")
     attrs = _attn_attrs(op, causal, scale) + [("max_new", str(maxNew))]
     return _packed_call(op, [q, kPages, vPages, blockTable, starts, lens], attrs, 1)[0]
+
+
+# ---- the ends of a training step ------------------------------------------------------
+# Backend extensions without a counterpart in the reference, eager only: embedding
+# rows, layer norm and the loss over the vocabulary, each with its gradients.  Sums are
+# float32 in a fixed order (the same call gives the same bits) and every result is
+# rounded once.  Ids and targets are device tensors that no call reads back.
+
+_ROW_DTYPES = (DType.FLOAT32, DType.BFLOAT16, DType.FLOAT16)
+
+
+def _float_attr(op: str, name: str, value: float, positive: bool = False) -> tuple:
+    with np.errstate(over="ignore", under="ignore"):
+        v = float(np.float32(value))
+    if not abs(v) < float("inf") or positive and not v > 0.0:
+        raise TensorError(f"{op}: {name} must be a {'positive' if positive else 'finite'} "
+                          f"float32, got {value}")
+    return name, repr(v)
+
+
+def _check_rows(op: str, t: Tensor) -> None:
+    if t.dtype not in _ROW_DTYPES:
+        raise TensorError(f"{op}: only float32, bfloat16 or float16, got {t.dtype.rew_name}")
+
+
+def _check_ids(op: str, ids: Tensor, width: int) -> None:
+    if ids.dtype != DType.INT32:
+        raise TensorError(f"{op}: ids must be an int32 tensor, got {ids.dtype.rew_name}")
+    if not 1 <= width <= 2 ** 20:
+        raise TensorError(f"{op}: rows must have 1 to 2^20 values, got {width}")
+
+
+def embedding(weight: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
+    """scale * weight[ids]: rows of ``weight`` [vocab, embed] (float32, bfloat16 or float16)
+    for int32 ``ids`` of any shape; [*ids.shape, embed].  The product is float32, rounded once.
+    An id outside [0, vocab) (padding: -1) gives zeros, unlike ``torchIndexSelect``, which
+    clamps it."""
+    op = "embedding"
+    if len(weight.shape) != 2:
+        raise TensorError(f"{op}: weight must be [vocab, embed], got {list(weight.shape)}")
+    _check_rows(op, weight)
+    _check_ids(op, ids, weight.shape[1])
+    return _packed_call(op, [weight, ids], [_float_attr(op, "scale", scale)], 1)[0]
+
+
+def embeddingGrad(ids: Tensor, gradOut: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
+    """The gradient [vocab, embed] of ``embedding``'s weight for the gradient ``gradOut``
+    [*ids.shape, embed] of its result: row v is scale times the sum of gradOut over the places
+    of ids that hold v, in their order (rows of many places: in parts), zeros where none does.
+    Places with an id outside [0, vocab) take no part, whatever their gradOut."""
+    op = "embeddingGrad"
+    if len(gradOut.shape) < 1 or tuple(gradOut.shape[:-1]) != tuple(ids.shape):
+        raise TensorError(f"{op}: gradOut must be [*ids.shape, embed], got "
+                          f"{list(gradOut.shape)} for ids {list(ids.shape)}")
+    _check_rows(op, gradOut)
+    _check_ids(op, ids, gradOut.shape[-1])
+    if vocab < 1:
+        raise TensorError(f"{op}: vocab must be positive, got {vocab}")
+    return _packed_call(op, [ids, gradOut], [("vocab", str(int(vocab))),
+                                             _float_attr(op, "scale", scale)], 1)[0]
+
+
+class NormStats(NamedTuple):
+    """What ``layerNorm`` leaves for its gradient, beside its result (float32, the shape of
+    x without the normalised dims)."""
+    mean: Tensor
+    rstd: Tensor  # 1 / sqrt(variance + eps)
+
+
+def _check_norm(op: str, x: Tensor, gamma: Tensor) -> tuple:
+    _check_rows(op, x)
+    if gamma.dtype not in (x.dtype, DType.FLOAT32):
+        raise TensorError(f"{op}: gamma must have x's dtype or float32, got "
+                          f"{gamma.dtype.rew_name}")
+    lead = len(x.shape) - len(gamma.shape)
+    if len(gamma.shape) < 1 or lead < 0 or x.shape[lead:] != gamma.shape:
+        raise TensorError(f"{op}: gamma {list(gamma.shape)} must be the last dims of x "
+                          f"{list(x.shape)}")
+    if gamma.numElements < 1:
+        raise TensorError(f"{op}: rows must have at least one value")
+    return x.shape[:lead]
+
+
+def layerNorm(x: Tensor, gamma: Tensor, beta: Tensor, eps: float = 1e-5,
+              withStats: bool = False):
+    """gamma * (x - mean) / sqrt(variance + eps) + beta over the last dims of ``x`` (float32,
+    bfloat16 or float16), those of ``gamma`` and ``beta`` (of x's dtype or float32).  The
+    arithmetic is float32 and the result, of x's dtype, rounded once.
+
+    ``withStats``: (y, stats), the ``NormStats`` that ``layerNormGrad`` takes."""
+    op = "layerNorm"
+    _check_norm(op, x, gamma)
+    if beta.dtype != gamma.dtype or beta.shape != gamma.shape:
+        raise TensorError(f"{op}: beta must have gamma's dtype and shape")
+    attrs = [_float_attr(op, "eps", eps, positive=True),
+             ("stats", "true" if withStats else "false")]
+    res = _packed_call(op, [x, gamma, beta], attrs, 3 if withStats else 1)
+    return (res[0], NormStats(res[1], res[2])) if withStats else res[0]
+
+
+def layerNormGrad(x: Tensor, gamma: Tensor, stats: NormStats, gradOut: Tensor):
+    """(gradX, gradGamma, gradBeta) of ``layerNorm(x, gamma, beta, eps)`` for the gradient
+    ``gradOut`` of its result, given its ``stats``: gradX of x's dtype, the others of
+    gamma's, summed over all rows."""
+    op = "layerNormGrad"
+    rows = _check_norm(op, x, gamma)
+    mean, rstd = stats
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != DType.FLOAT32 or t.shape != rows:
+            raise TensorError(f"{op}: {name} must be float32 {list(rows)}")
+    if gradOut.dtype != x.dtype or gradOut.shape != x.shape:
+        raise TensorError(f"{op}: gradOut must have x's dtype and shape")
+    return tuple(_packed_call(op, [x, gamma, mean, rstd, gradOut], [], 3))
+
+
+def _check_head(op: str, x: Tensor, weight: Tensor, targets: Tensor, tied: bool) -> None:
+    if len(x.shape) != 2 or len(weight.shape) != 2:
+        raise TensorError(f"{op}: x must be [tokens, embed] and weight of rank 2, got "
+                          f"{list(x.shape)} and {list(weight.shape)}")
+    if x.dtype != weight.dtype:
+        raise TensorError(f"{op}: dtype mismatch ({x.dtype.enum_name} vs "
+                          f"{weight.dtype.enum_name})")
+    if x.dtype not in (DType.BFLOAT16, DType.FLOAT16):
+        raise TensorError(f"{op}: only bfloat16 or float16, got {x.dtype.rew_name}")
+    if weight.shape[1 if tied else 0] != x.shape[1]:
+        raise TensorError(f"{op}: x {list(x.shape)} and weight {list(weight.shape)} "
+                          f"({'[vocab, embed]' if tied else '[embed, vocab]'}) differ in embed")
+    if not all(1 <= d <= 2 ** 21 for d in weight.shape):
+        raise TensorError(f"{op}: embed and vocab must be 1 to 2^21, got {list(weight.shape)}")
+    _check_i32(op, targets, "targets", (x.shape[0],))
+
+
+def linearCrossEntropy(x: Tensor, weight: Tensor, targets: Tensor, tied: bool = False,
+                       withLse: bool = False):
+    """The cross entropy of softmax(x weight) and ``targets`` [tokens], float32 [tokens], not
+    reduced: log sum_v exp z[t, v] - z[t, targets[t]], z the logits.  ``x`` [tokens, embed];
+    ``weight`` [embed, vocab] as ``nn.Linear``'s or, ``tied``, [vocab, embed] as
+    ``nn.Embedding``'s; both bfloat16 or float16.  A target outside [0, vocab) (padding: -1)
+    gives 0.  The logits are float32, never rounded and never stored.
+
+    ``withLse``: (loss, lse), the float32 [tokens] that ``linearCrossEntropyGrad`` takes."""
+    op = "linearCrossEntropy"
+    _check_head(op, x, weight, targets, tied)
+    res = _packed_call(op, [x, weight, targets],
+                       [("tied", "true" if tied else "false"),
+                        ("stats", "true" if withLse else "false")], 2 if withLse else 1)
+    return tuple(res) if withLse else res[0]
+
+
+def linearCrossEntropyGrad(x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor,
+                           gradLoss: Tensor, tied: bool = False):
+    """(gradX, gradWeight) of ``linearCrossEntropy(x, weight, targets, tied)`` for the gradient
+    ``gradLoss`` (float32 [tokens]: 1 / tokens for the mean) of its result, given its ``lse``,
+    of the dtypes of x and weight.  The logits are formed anew, a piece of the vocabulary at a
+    time.  Their gradient is rounded once to x's dtype for the two products, relative to the
+    largest |gradLoss|, whose scale is applied to the float32 sums (float16 loses what is below
+    2^-39 of it).  Tokens without a target in [0, vocab) take no part, whatever their x and
+    gradLoss: their gradX is 0."""
+    op = "linearCrossEntropyGrad"
+    _check_head(op, x, weight, targets, tied)
+    for t, name in ((lse, "lse"), (gradLoss, "gradLoss")):
+        if t.dtype != DType.FLOAT32 or t.shape != (x.shape[0],):
+            raise TensorError(f"{op}: {name} must be float32 [{x.shape[0]}]")
+    return tuple(_packed_call(op, [x, weight, targets, lse, gradLoss],
+                              [("tied", "true" if tied else "false")], 2))

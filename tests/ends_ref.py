@@ -1,0 +1,169 @@
+"""Plain float64 forms of embeddings, layer norm and the cross entropy of a linear head, with
+their gradients, and error bounds for the kernels.
+
+Every bound counts roundings: U = 2^-24 is half a step of float32, HALF[t] that of t relative to
+the value, TINY[t] half of t's smallest step (float16 2^-24, the others far below anything here).
+A sum of n float32 terms whose longest chain of additions has d of them is off by at most
+d U (sum of absolute values).
+"""
+import numpy as np
+
+from rew_amd import eager as E
+from rew_amd.eager import DType
+
+U = 2.0 ** -24
+HALF = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11, "float32": U}
+TINY = {"bfloat16": 1e-38, "float16": 2.0 ** -25, "float32": 1e-38}
+DT = {"bfloat16": DType.BFLOAT16, "float16": DType.FLOAT16, "float32": DType.FLOAT32}
+
+
+def tensor(a, dtype):
+    """(device tensor, its values in float64) of the array rounded to dtype."""
+    t = E.fromHost(np.asarray(a, np.float32), DT[dtype])
+    if dtype == "bfloat16":
+        h = E.bf16_bits_to_f32(E.f32_to_bf16_bits(np.asarray(a, np.float32)))
+    else:
+        h = np.asarray(a, np.float32).astype(np.float16 if dtype == "float16" else np.float32)
+    return t, h.reshape(np.shape(a)).astype(np.float64)
+
+
+def ints(a):
+    return E.fromHost(np.asarray(a, np.int32), DType.INT32)
+
+
+def host(t):
+    return E.toHostF32(t).astype(np.float64)
+
+
+def check(got, want, bound):
+    """Every value of the device tensor within its bound of `want` (NaN where `want` is)."""
+    got = host(got)
+    assert got.shape == want.shape, (got.shape, want.shape)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        off = ~same & ~(np.abs(got - want) <= bound)
+    assert not off.any(), (f"{off.sum()} of {off.size} off, first at {np.argwhere(off)[0]}: "
+                           f"{got[off][0]} for {want[off][0]}, bound "
+                           f"{np.broadcast_to(bound, got.shape)[off][0]}")
+
+
+# ---- embedding ------------------------------------------------------------------------------
+
+def embedding(w, ids, scale, dtype):
+    ids = np.asarray(ids)
+    there = (ids >= 0) & (ids < len(w))
+    want = np.where(there[..., None], w[np.clip(ids, 0, len(w) - 1)], 0.0) * np.float32(scale)
+    return want, (HALF[dtype] + 2 * U) * np.abs(want) + TINY[dtype]
+
+
+def embedding_grad(ids, g, vocab, scale, dtype):
+    ids, g = np.asarray(ids).reshape(-1), g.reshape(-1, g.shape[-1])
+    want, mag = np.zeros((vocab, g.shape[1])), np.zeros((vocab, g.shape[1]))
+    count = np.zeros(vocab)
+    for t, v in enumerate(ids):
+        if 0 <= v < vocab:
+            want[v] += g[t]
+            mag[v] += np.abs(g[t])
+            count[v] += 1
+    s = float(np.float32(scale))
+    bound = (count[:, None] + 2) * U * mag * abs(s) + HALF[dtype] * np.abs(want * s) + TINY[dtype]
+    return want * s, bound
+
+
+# ---- layer norm -----------------------------------------------------------------------------
+# A row's sums: at most 16 values a thread in a chain, 6 steps in a wave, 16 waves, or n / 1024
+# values a thread in long rows.
+
+def _row(x, eps):
+    n = x.shape[1]
+    d = n / 1024 + 40
+    mean = x.mean(1, keepdims=True)
+    rstd = 1.0 / np.sqrt(((x - mean) ** 2).mean(1, keepdims=True) + eps)
+    xh = (x - mean) * rstd
+    # the mean's error, and that of rstd (half of the variance's; the mean's enters it squared)
+    e_mean = (d + 2) * U * np.abs(x).mean(1, keepdims=True)
+    e_xh = rstd * (e_mean + 2 * U * np.abs(x)) + np.abs(xh) * (d / 2 + 8) * U
+    return d, mean, rstd, xh, e_mean, e_xh
+
+
+def layer_norm(x, gamma, beta, eps, dtype):
+    """y, mean, rstd [rows] and the bounds of each."""
+    d, mean, rstd, xh, e_mean, e_xh = _row(x, eps)
+    y = xh * gamma + beta
+    e_y = np.abs(gamma) * (e_xh + 2 * U * np.abs(xh)) + 2 * U * np.abs(y) + \
+        HALF[dtype] * np.abs(y) + TINY[dtype]
+    return (y, e_y), (mean[:, 0], e_mean[:, 0]), (rstd[:, 0], (d / 2 + 8) * U * rstd[:, 0])
+
+
+def layer_norm_grad(x, gamma, eps, dy, dtype, ptype):
+    """dx, dgamma, dbeta and their bounds."""
+    d, _, rstd, xh, _, e_xh = _row(x, eps)
+    w = dy * gamma
+    aw, ax = np.abs(w), np.abs(xh)
+    q = (w * xh).mean(1, keepdims=True)
+    dx = rstd * (w - w.mean(1, keepdims=True) - xh * q)
+    e_in = 4 * U * aw + (d + 4) * U * aw.mean(1, keepdims=True) + e_xh * np.abs(q) + ax * (
+        (d + 8) * U * (aw * ax).mean(1, keepdims=True) + (aw * e_xh).mean(1, keepdims=True)) + \
+        4 * U * ax * np.abs(q)
+    e_dx = rstd * e_in + ((d / 2 + 12) * U + HALF[dtype]) * np.abs(dx) + TINY[dtype]
+    # over the rows: one in 256 in a chain, then the parts
+    rows = len(x) / 256 + 60
+    dg, db = (dy * xh).sum(0), dy.sum(0)
+    e_dg = (rows + 4) * U * np.abs(dy * xh).sum(0) + (np.abs(dy) * e_xh).sum(0)
+    e_db = rows * U * np.abs(dy).sum(0)
+    return ((dx, e_dx), (dg, e_dg + HALF[ptype] * np.abs(dg) + TINY[ptype]),
+            (db, e_db + HALF[ptype] * np.abs(db) + TINY[ptype]))
+
+
+# ---- cross entropy --------------------------------------------------------------------------
+# The products of a logit are exact in float32 and each addition of the H of them loses at most
+# one step (2 U); lse moves no more than its logits.  exp2: its argument's rounding, (z - m)
+# log2 e, and one step of the result.
+
+def _softmax(x, w):
+    with np.errstate(invalid="ignore"):
+        z = x @ w
+    e_z = 2 * (x.shape[1] + 4) * U * (np.abs(x) @ np.abs(w))
+    m = z.max(1, keepdims=True)
+    e = np.exp(z - m)
+    lse = m + np.log(e.sum(1, keepdims=True))
+    spread = (m - z.min(1, keepdims=True))
+    # of the sum of exponentials, relative: the exponentials' own and a lane's chain
+    e_sum = (4 * np.minimum(spread, 100.0) + 8) * U + (w.shape[1] / 8 + 80) * U
+    e_lse = e_z.max(1, keepdims=True) + e_sum + 4 * U * (np.abs(lse) + np.abs(m))
+    return z, e_z, lse, e_lse
+
+
+def cross_entropy(x, w, targets):
+    """loss, lse [tokens] and their bounds; w [embed, vocab]."""
+    z, e_z, lse, e_lse = _softmax(x, w)
+    t = np.asarray(targets)
+    live = (t >= 0) & (t < w.shape[1])
+    at = (np.arange(len(t)), np.where(live, t, 0))
+    loss = np.where(live, lse[:, 0] - z[at], 0.0)
+    return (loss, np.where(live, e_lse[:, 0] + e_z[at] + 2 * U * np.abs(loss), 0.0)), \
+        (lse[:, 0], e_lse[:, 0])
+
+
+def cross_entropy_grad(x, w, targets, grad, dtype):
+    """dx, dw [embed, vocab] and their bounds."""
+    h = HALF[dtype]
+    z, e_z, lse, e_lse = _softmax(x, w)
+    t = np.asarray(targets)
+    live = (t >= 0) & (t < w.shape[1])
+    g = np.where(live, grad, 0.0)[:, None]
+    p = np.exp(z - lse)
+    hit = np.zeros_like(p)
+    hit[np.arange(len(t))[live], t[live]] = 1.0
+    dz = g * (p - hit)
+    # p's relative error, the subtraction, two roundings of the scale, one to dtype
+    e_p = p * (np.expm1(e_z + e_lse) + (4 * np.abs(z - lse) + 8) * U)
+    e_dz = np.abs(g) * (e_p + U) + (h + 6 * U) * np.abs(dz)
+    if dtype == "float16":  # dz lies in units of the largest |grad| / 2^14
+        e_dz = e_dz + np.abs(g).max(initial=0.0) * 2.0 ** -39 * live[:, None]
+    xx = np.where(live[:, None], x, 0.0)
+    dx, dw = dz @ w.T, xx.T @ dz
+    e_dx = e_dz @ np.abs(w).T + 2 * (w.shape[1] + 8) * U * (np.abs(dz) @ np.abs(w).T)
+    e_dw = np.abs(xx).T @ e_dz + 2 * (len(t) + 8) * U * (np.abs(xx).T @ np.abs(dz))
+    return ((dx, e_dx + (h + 4 * U) * np.abs(dx) + TINY[dtype]),
+            (dw, e_dw + (h + 4 * U) * np.abs(dw) + TINY[dtype]))

@@ -1,0 +1,120 @@
+"""GPU checks of ``ops.embedding`` and its gradient against float64."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import ends_ref as R
+from ends_ref import ints, tensor
+from rew_amd import ops as O
+
+DTYPES = ["float32", "bfloat16", "float16"]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 12, 64, 250, 1000, 4096])
+@pytest.mark.parametrize("tokens,vocab", [(1, 1), (37, 100), (300, 5)])
+def test_rows(gpu, dtype, width, tokens, vocab):
+    r = np.random.default_rng(width)
+    w, wh = tensor(r.standard_normal((vocab, width)), dtype)
+    ids = r.integers(-2, vocab + 2, tokens)
+    for scale in (1.0, width ** 0.5, -0.3):
+        R.check(O.embedding(w, ints(ids), scale), *R.embedding(wh, ids, scale, dtype))
+
+
+def test_ids_of_any_shape(gpu):
+    r = np.random.default_rng(0)
+    w, wh = tensor(r.standard_normal((50, 16)), "bfloat16")
+    g, gh = tensor(r.standard_normal((2, 3, 4, 16)), "bfloat16")
+    ids = r.integers(0, 50, (2, 3, 4))
+    R.check(O.embedding(w, ints(ids)), *R.embedding(wh, ids, 1.0, "bfloat16"))
+    R.check(O.embeddingGrad(ints(ids), g, 50), *R.embedding_grad(ids, gh, 50, 1.0, "bfloat16"))
+    R.check(O.embedding(w, ints(7)), *R.embedding(wh, 7, 1.0, "bfloat16"))
+    R.check(O.embeddingGrad(ints(7), tensor(gh[0, 0, 0], "bfloat16")[0], 50),
+            *R.embedding_grad(7, gh[0, 0, 0], 50, 1.0, "bfloat16"))
+
+
+def test_nothing(gpu):
+    w, _ = tensor(np.ones((5, 8)), "float32")
+    none = ints(np.zeros(0))
+    assert O.embedding(w, none).shape == (0, 8)
+    got = O.embeddingGrad(none, tensor(np.zeros((0, 8)), "float32")[0], 700)
+    R.check(got, np.zeros((700, 8)), 0.0)
+
+
+def test_bits_are_kept_without_a_scale(gpu):
+    """Infinities, NaN, subnormals and zeros of either sign pass through scale 1."""
+    v = np.array([[np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-40, 2.0 ** -24, 65504.0]], np.float32)
+    for dtype in DTYPES:
+        w, wh = tensor(np.repeat(v, 3, 0), dtype)
+        got = R.host(O.embedding(w, ints([2, 0])))
+        np.testing.assert_array_equal(got, wh[:2])
+        np.testing.assert_array_equal(np.signbit(got), np.signbit(wh[:2]))
+
+
+def text(r, n, vocab):
+    """Ids of which a few are frequent and most never occur; some outside the table."""
+    v = np.floor(np.exp(r.uniform(0, np.log(vocab + 1), n)) - 1).astype(np.int64)
+    return np.where(r.random(n) < 0.05, r.choice([-1, -2 ** 31, vocab, 2 ** 31 - 1], n), v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,vocab,width", [
+    (1, 1, 1), (1, 513, 8), (63, 2, 3), (64, 512, 250), (65, 1, 64), (200, 511, 5),
+    (1000, 3, 40), (1025, 1025, 16), (5000, 2000, 24), (70000, 40, 8), (70000, 700, 1)])
+def test_gradient(gpu, dtype, tokens, vocab, width):
+    r = np.random.default_rng(tokens + vocab)
+    ids = text(r, tokens, vocab)
+    g, gh = tensor(r.standard_normal((tokens, width)), dtype)
+    want, bound = R.embedding_grad(ids, gh, vocab, 1.5, dtype)
+    got = O.embeddingGrad(ints(ids), g, vocab, 1.5)
+    R.check(got, want, bound)
+    # the same call, the same bits
+    np.testing.assert_array_equal(R.host(got), R.host(O.embeddingGrad(ints(ids), g, vocab, 1.5)))
+
+
+@pytest.mark.parametrize("ids", [[3] * 65, [3] * 64, [3] * 63 + [2], [3] * 128 + [4] * 129,
+                                 [5] + [3] * 127 + [4] * 64 + [0] * 300, [1, 2] * 500])
+def test_rows_of_many_tokens(gpu, ids):
+    """Rows that end on, before and behind the end of a part."""
+    r = np.random.default_rng(len(ids))
+    for order in (ids, ids[::-1], r.permutation(ids)):
+        g, gh = tensor(r.standard_normal((len(ids), 12)), "float32")
+        R.check(O.embeddingGrad(ints(order), g, 7), *R.embedding_grad(order, gh, 7, 1.0, "float32"))
+
+
+def test_padding_may_hold_anything(gpu):
+    r = np.random.default_rng(3)
+    ids = np.array([4, -1, 2, 4, 9, 2 ** 30])
+    gh = r.standard_normal((6, 16))
+    gh[[1, 4, 5]] = [[np.nan], [np.inf], [-np.inf]]
+    g, gh = tensor(gh, "bfloat16")
+    R.check(O.embeddingGrad(ints(ids), g, 9), *R.embedding_grad(ids, gh, 9, 1.0, "bfloat16"))
+
+
+def test_gradient_against_differences(gpu):
+    """<gradOut, embedding(w + h d) - embedding(w - h d)> / 2 h = <embeddingGrad, d>: both
+    sides of values that are small whole numbers, exact in float32."""
+    r = np.random.default_rng(5)
+    ids = r.integers(0, 30, 200)
+    w, d = r.integers(-8, 9, (30, 12)), r.integers(-8, 9, (30, 12))
+    g, gh = tensor(r.integers(-8, 9, (200, 12)), "float32")
+    up, down = (R.host(O.embedding(tensor(w + s * d, "float32")[0], ints(ids), 2.0))
+                for s in (1, -1))
+    grad = R.host(O.embeddingGrad(ints(ids), g, 30, 2.0))
+    assert (gh * (up - down)).sum() / 2 == (grad * d).sum()
+
+
+def test_offsets_past_32_bits(gpu):
+    """A table of more than 2^32 bytes: its last rows."""
+    from rew_amd import eager as E
+    V, W = 530000, 4000  # 4.24e9 bytes
+    ids = np.array([V - 1, 0, V - 1, V - 2])
+    g, gh = tensor(np.random.default_rng(1).standard_normal((4, W)), "bfloat16")
+    grad = O.embeddingGrad(ints(ids), g, V)
+    rows = O.embedding(grad, ints([V - 1, V - 2, 5, 0]))
+    small = np.array([2, 0, 2, 1])
+    want, bound = R.embedding_grad(small, gh, 3, 1.0, "bfloat16")
+    R.check(rows, np.stack([want[2], want[1], 0 * want[0], want[0]]),
+            np.stack([bound[2], bound[1], 0 * bound[0], bound[0]]))
+    E.sync()

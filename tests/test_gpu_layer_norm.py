@@ -1,0 +1,135 @@
+"""GPU checks of ``ops.layerNorm`` and its gradients against float64."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import ends_ref as R
+from ends_ref import tensor
+from rew_amd import ops as O
+
+TYPES = [("float32", "float32"), ("bfloat16", "float32"), ("bfloat16", "bfloat16"),
+         ("float16", "float32"), ("float16", "float16")]
+WIDTHS = [1, 2, 3, 8, 63, 64, 250, 512, 520, 1001, 1024, 2048, 4096, 4104, 5001, 8192, 16384,
+          16385, 20000, 40008]
+
+
+def case(r, rows, n, dtype, ptype, shift=0.3):
+    x, xh = tensor(r.standard_normal((rows, n)) * 1.5 + shift, dtype)
+    g, gh = tensor(1.0 + 0.3 * r.standard_normal(n), ptype)
+    b, bh = tensor(0.3 * r.standard_normal(n), ptype)
+    dy, dyh = tensor(r.standard_normal((rows, n)), dtype)
+    return (x, g, b, dy), (xh, gh, bh, dyh)
+
+
+def run(t, h, dtype, ptype, eps=1e-5):
+    (x, g, b, dy), (xh, gh, bh, dyh) = t, h
+    e = float(np.float32(eps))
+    y, stats = O.layerNorm(x, g, b, eps, withStats=True)
+    for got, (want, bound) in zip((y, *stats), R.layer_norm(xh, gh, bh, e, dtype)):
+        R.check(got, want, bound)
+    np.testing.assert_array_equal(R.host(y), R.host(O.layerNorm(x, g, b, eps)))
+    grads = O.layerNormGrad(x, g, stats, dy)
+    for got, (want, bound) in zip(grads, R.layer_norm_grad(xh, gh, e, dyh, dtype, ptype)):
+        R.check(got, want, bound)
+    for a, c in zip(grads, O.layerNormGrad(x, g, stats, dy)):  # the same call, the same bits
+        np.testing.assert_array_equal(R.host(a), R.host(c))
+
+
+@pytest.mark.parametrize("dtype,ptype", TYPES)
+@pytest.mark.parametrize("n", WIDTHS)
+def test_widths(gpu, dtype, ptype, n):
+    r = np.random.default_rng(n)
+    for rows in (1, 5, 67):
+        run(*case(r, rows, n, dtype, ptype), dtype, ptype)
+
+
+@pytest.mark.parametrize("dtype,ptype", TYPES)
+@pytest.mark.parametrize("rows,n", [(1000, 64), (5000, 8), (300, 1024), (3001, 130), (700, 2049)])
+def test_rows(gpu, dtype, ptype, rows, n):
+    run(*case(np.random.default_rng(rows), rows, n, dtype, ptype), dtype, ptype)
+
+
+def test_rows_far_from_zero(gpu):
+    """The variance of values about 1000, from their deviations."""
+    run(*case(np.random.default_rng(0), 9, 777, "float32", "float32", shift=1000.0), "float32",
+        "float32")
+
+
+def test_equal_values(gpu):
+    x, _ = tensor(np.full((3, 96), 2.5), "float32")
+    g, gh = tensor(np.linspace(0.5, 1.5, 96), "float32")
+    b, bh = tensor(np.linspace(-1, 1, 96), "float32")
+    y, stats = O.layerNorm(x, g, b, withStats=True)
+    np.testing.assert_array_equal(R.host(y), np.tile(bh, (3, 1)))
+    dy, dyh = tensor(np.random.default_rng(1).standard_normal((3, 96)), "float32")
+    for got, (want, bound) in zip(O.layerNormGrad(x, g, stats, dy), R.layer_norm_grad(
+            np.full((3, 96), 2.5), gh, float(np.float32(1e-5)), dyh, "float32", "float32")):
+        R.check(got, want, bound)
+
+
+def test_several_dims(gpu):
+    r = np.random.default_rng(2)
+    (x, g, b, dy), h = case(r, 12, 30, "float32", "float32")
+    shaped = lambda t, s: O.reshape(t, s)  # noqa: E731
+    y, st = O.layerNorm(x, g, b, withStats=True)
+    y2, st2 = O.layerNorm(shaped(x, [3, 4, 5, 6]), shaped(g, [5, 6]), shaped(b, [5, 6]),
+                          withStats=True)
+    assert y2.shape == (3, 4, 5, 6) and st2.mean.shape == (3, 4)
+    np.testing.assert_array_equal(R.host(y2).reshape(12, 30), R.host(y))
+    got = O.layerNormGrad(shaped(x, [3, 4, 5, 6]), shaped(g, [5, 6]), st2, shaped(dy, [3, 4, 5, 6]))
+    for a, c in zip(got, O.layerNormGrad(x, g, st, dy)):
+        np.testing.assert_array_equal(R.host(a).reshape(c.shape), R.host(c))
+    # one row: all of x
+    y3, st3 = O.layerNorm(O.reshape(x, [360]), O.reshape(x, [360]), O.reshape(x, [360]),
+                          withStats=True)
+    assert y3.shape == (360,) and st3.mean.shape == ()
+
+
+def test_no_rows(gpu):
+    x, _ = tensor(np.zeros((0, 40)), "bfloat16")
+    g, _ = tensor(np.ones(40), "float32")
+    y, st = O.layerNorm(x, g, g, withStats=True)
+    assert y.shape == (0, 40) and st.rstd.shape == (0,)
+    dx, dg, db = O.layerNormGrad(x, g, st, x)
+    assert dx.shape == (0, 40)
+    R.check(dg, np.zeros(40), 0.0)
+    R.check(db, np.zeros(40), 0.0)
+
+
+def test_infinities_stay_in_their_rows(gpu):
+    r = np.random.default_rng(4)
+    (x, g, b, dy), (xh, gh, bh, dyh) = case(r, 9, 200, "bfloat16", "float32")
+    bad = xh.copy()
+    bad[2, 7], bad[5, 0], bad[6, 199] = np.inf, np.nan, -np.inf
+    y, st = O.layerNorm(tensor(bad, "bfloat16")[0], g, b, withStats=True)
+    want = R.host(O.layerNorm(x, g, b))
+    got = R.host(y)
+    keep = [0, 1, 3, 4, 7, 8]
+    np.testing.assert_array_equal(got[keep], want[keep])
+    assert np.isnan(got[[2, 5, 6]]).all()
+    dx = R.host(O.layerNormGrad(tensor(bad, "bfloat16")[0], g, st, dy)[0])
+    st = O.layerNorm(x, g, b, withStats=True)[1]
+    np.testing.assert_array_equal(dx[keep], R.host(O.layerNormGrad(x, g, st, dy)[0])[keep])
+
+
+def test_gradient_against_differences(gpu):
+    """Central differences of <dy, layerNorm> in float64 over a step of 1e-4 (their own error
+    about 1e-8), against the float32 kernel."""
+    r = np.random.default_rng(6)
+    (x, g, b, dy), (xh, gh, bh, dyh) = case(r, 4, 24, "float32", "float32")
+    st = O.layerNorm(x, g, b, withStats=True)[1]
+    dx, dg, db = (R.host(t) for t in O.layerNormGrad(x, g, st, dy))
+
+    def f(xv, gv, bv):
+        return (dyh * R.layer_norm(xv, gv, bv, 1e-5, "float32")[0][0]).sum()
+
+    for k, (v, d) in enumerate(((xh, dx), (gh, dg), (bh, db))):
+        for i in r.choice(v.size, 12, replace=False):
+            at = np.unravel_index(i, v.shape)
+            side = []
+            for s in (1e-4, -1e-4):
+                args = [xh.copy(), gh.copy(), bh.copy()]
+                args[k][at] += s
+                side.append(f(*args))
+            assert abs((side[0] - side[1]) / 2e-4 - d[at]) < 2e-5
