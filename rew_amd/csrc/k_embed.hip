@@ -13,26 +13,23 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// f(type, run length): the element type and the longest run of at most 16
-// bytes that divides a row of n values.
+// f(element type, run length) for rows of n values.
 template <class F>
 void by_run(int dt, int64_t n, F&& f) {
-  auto runs = [&](auto t, auto most) {
-    constexpr int M = decltype(most)::value;
-    if (n % M == 0) f(t, std::integral_constant<int, M>());
-    else if (M == 8 && n % 4 == 0) f(t, std::integral_constant<int, 4>());
-    else if (n % 2 == 0) f(t, std::integral_constant<int, 2>());
+  auto with = [&](auto t) {
+    constexpr int N = kRun<decltype(t)>;
+    if (n >= N) f(t, std::integral_constant<int, N>());
     else f(t, std::integral_constant<int, 1>());
   };
-  if (dt == kF32) runs(RowF32(), std::integral_constant<int, 4>());
-  else if (dt == kBF16) runs(RowBf16(), std::integral_constant<int, 8>());
-  else runs(RowF16(), std::integral_constant<int, 8>());
+  if (dt == kF32) with(RowF32());
+  else if (dt == kBF16) with(RowBf16());
+  else with(RowF16());
 }
 
-// Threads side by side on a row of `runs` runs: a power of two up to kThreads.
-int row_threads(int64_t runs) {
+// Threads side by side on a row of `runs` runs: a power of two up to `most`.
+int row_threads(int64_t runs, int most) {
   int x = 1;
-  while (x < kThreads && x < runs) x *= 2;
+  while (x < most && x < runs) x *= 2;
   return x;
 }
 
@@ -43,15 +40,17 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedArgs a) {
   const int64_t id = a.ids[t];
   const bool there = id >= 0 && id < a.V;
   const int64_t src = there ? id * a.E : 0, dst = t * a.E;
-  for (int64_t c = threadIdx.x * N; c < a.E; c += (int64_t)blockDim.x * N) {
+  for (int64_t i = threadIdx.x * N; i < a.E; i += (int64_t)blockDim.x * N) {
+    const int64_t c = run_start(i, a.E, N);
     float f[N];
-    if (there) {
-      run_load<T, N>(a.w, src + c, f);
+    run_load<T, N>(a.w, src + c, f);
 #pragma unroll
-      for (int x = 0; x < N; ++x) f[x] *= a.scale;
-    } else {
-#pragma unroll
-      for (int x = 0; x < N; ++x) f[x] = 0.0f;
+    for (int x = 0; x < N; ++x) {
+      f[x] *= a.scale;
+      // (a product by itself: with the rounding to float16 the compiler makes it
+      // v_fma_mixlo f scale + 0, which turns -0 into 0)
+      asm("" : "+v"(f[x]));
+      f[x] = there ? f[x] : 0.0f;
     }
     run_store<T, N>(a.out, dst + c, f);
   }
@@ -64,10 +63,12 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedArgs a) {
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSortRows = 512, kSortBits = 9;  // rows of the table per workgroup
 
-// Tokens per part of a row that is split; a row of more is "long".
+// A row of more than part_tokens tokens is "long": it is summed in parts of so many
+// places of the order, at most about a thousand of them.
 int64_t part_tokens(int64_t T) {
-  return std::max<int64_t>(64, ((T + 1023) / 1024 + 63) & ~(int64_t)63);
+  return std::max<int64_t>(128, ((T + 1023) / 1024 + 127) & ~(int64_t)127);
 }
+constexpr int kFew = 8;  // a row of more tokens is summed by the whole workgroup
 
 struct GradWork {
   int32_t *first, *order;  // [V + 1]: a row's first place in order; [T]: tokens by row
@@ -94,19 +95,36 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t*
                                                                   int64_t V, GradWork w) {
   __shared__ int32_t cnt[kSortWaves][kSortRows];
   __shared__ int32_t tmp[kSortWaves];
+  constexpr int kAhead = 8;       // loads under way
+  constexpr int kOneByOne = 8;    // tokens of 64
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t lo = (int64_t)blockIdx.x * kSortRows;
   const int rows = (int)min((int64_t)kSortRows, V - lo);
-  for (int i = tid; i < kSortWaves * kSortRows; i += kSortThreads) (&cnt[0][0])[i] = 0;
-  __syncthreads();
   const int64_t per = ((T + kSortWaves - 1) / kSortWaves + 63) & ~(int64_t)63;
   const int64_t t0 = min((int64_t)wave * per, T), t1 = min(t0 + per, T);
+  // f(first token of 64, the lane's id) over this wave's share, -1 past its end
+  auto walk = [&](auto&& f) {
+    for (int64_t t = t0; t < t1; t += 64 * kAhead) {
+      int32_t id[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t at = t + i * 64 + lane;
+        id[i] = ids[min(at, T - 1)];
+        if (at >= t1) id[i] = -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (t + i * 64 < t1) f(t + i * 64, id[i]);
+    }
+  };
+  for (int i = tid; i < kSortWaves * kSortRows; i += kSortThreads) (&cnt[0][0])[i] = 0;
+  __syncthreads();
   int32_t below = 0;
-  for (int64_t t = t0 + lane; t < t1; t += 64) {
-    const int64_t r = ids[t] - lo;
-    if (ids[t] >= 0 && r < 0) ++below;
+  walk([&](int64_t, int32_t id) {
+    const int64_t r = id - lo;
+    if (id >= 0 && r < 0) ++below;
     else if (r >= 0 && r < rows) atomicAdd(&cnt[wave][r], 1);
-  }
+  });
   // the tokens of the rows before: this workgroup's first place
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) below += __shfl_xor(below, d);
@@ -119,6 +137,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t*
   // row r of thread r: the waves' counts become offsets within the row
   int32_t total = 0;
   if (tid < kSortRows)
+#pragma unroll
     for (int i = 0; i < kSortWaves; ++i) {
       const int32_t n = cnt[i][tid];
       cnt[i][tid] = total;
@@ -135,55 +154,91 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t*
   int32_t at = base + sum - total;
   for (int i = 0; i < wave; ++i) at += tmp[i];
   if (tid < kSortRows) {
+#pragma unroll
     for (int i = 0; i < kSortWaves; ++i) cnt[i][tid] += at;
     if (tid < rows) w.first[lo + tid] = at;
     if (lo + tid == V - 1) w.first[V] = at + total;
   }
   __syncthreads();
-  // (a wave's lanes agree on the number of turns, for the ballots)
-  for (int64_t t = t0 + lane; t - lane < t1; t += 64) {
-    const int64_t r = t < t1 ? (int64_t)ids[t] - lo : -1;
-    const bool mine = r >= 0 && r < rows;
-    uint64_t same = __ballot(mine);
-    if (same == 0) continue;
+  walk([&](int64_t t, int32_t id) {
+    const int64_t r64 = id - lo;
+    const bool mine = id >= 0 && r64 >= 0 && r64 < rows;
+    const int r = mine ? (int)r64 : -1;
+    uint64_t todo = __ballot(mine);
+    if (todo == 0) return;
+    const uint64_t before = (1ull << lane) - 1;
+    volatile int32_t* count = cnt[wave];
+    if (__popcll(todo) <= kOneByOne) {
+      // row by row
+      while (todo) {
+        const int key = __builtin_amdgcn_readlane(r, __ffsll((unsigned long long)todo) - 1);
+        const uint64_t same = __ballot(r == key);
+        const int32_t p = count[key];
+        if (r == key) w.order[p + __popcll(same & before)] = (int32_t)(t + lane);
+        if (lane == 0) count[key] = p + __popcll(same);
+        todo &= ~same;
+      }
+    } else {
+      // all rows at once: the lanes that agree with this one in every bit
+      uint64_t same = todo;
 #pragma unroll
-    for (int b = 0; b < kSortBits; ++b) {
-      const uint64_t set = __ballot(mine && (r >> b & 1));
-      same &= r >> b & 1 ? set : ~set;
-    }
-    if (mine) {
-      const int before = __popcll(same & ((1ull << lane) - 1));
-      volatile int32_t* c = &cnt[wave][r];
-      const int32_t p = *c;
-      w.order[p + before] = (int32_t)t;
-      if (before == 0) *c = p + __popcll(same);
+      for (int b = 0; b < kSortBits; ++b) {
+        const uint64_t set = __ballot(mine && (r >> b & 1));
+        same &= r >> b & 1 ? set : ~set;
+      }
+      if (mine) {
+        const int ahead = __popcll(same & before);
+        const int32_t p = count[r];
+        w.order[p + ahead] = (int32_t)(t + lane);
+        if (ahead == 0) count[r] = p + __popcll(same);
+      }
     }
     __builtin_amdgcn_wave_barrier();
+  });
+}
+
+// The sum of gradOut's columns c .. over places [p0, p1), one after another.
+template <class T, int N>
+__device__ __forceinline__ void sum_places(const EmbedGradArgs& a, const int32_t* order, int32_t p0,
+                                           int32_t p1, int64_t c, float (&s)[N]) {
+  constexpr int kAhead = 8;  // rows under way
+#pragma unroll
+  for (int x = 0; x < N; ++x) s[x] = 0.0f;
+  int32_t p = p0;
+  for (; p + kAhead <= p1; p += kAhead) {
+    RowRun<T, N> r[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      r[i] = run_at<T, N>(a.grad, (int64_t)order[p + i] * a.E + c);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int x = 0; x < N; ++x) s[x] += T::get(r[i].v[x]);
+  }
+  for (; p < p1; ++p) {
+    const RowRun<T, N> r = run_at<T, N>(a.grad, (int64_t)order[p] * a.E + c);
+#pragma unroll
+    for (int x = 0; x < N; ++x) s[x] += T::get(r.v[x]);
   }
 }
 
-// Rows of at most `part` tokens (none: zeros), summed in the tokens' order.
+// The same by the whole workgroup, its groups of `lanes` threads a share of the
+// places each, joined in order; the first group's threads have the sum.
 template <class T, int N>
-__global__ void __launch_bounds__(kThreads) embed_rows_kernel(EmbedGradArgs a, GradWork w,
-                                                              int64_t part) {
-  const int64_t v = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (v >= a.V) return;
-  const int32_t p0 = w.first[v], p1 = w.first[v + 1];
-  if (p1 - p0 > part) return;
-  for (int64_t c = threadIdx.x * N; c < a.E; c += (int64_t)blockDim.x * N) {
-    float s[N];
+__device__ __forceinline__ void sum_together(const EmbedGradArgs& a, const int32_t* order,
+                                             int32_t p0, int32_t p1, int64_t c, int lanes,
+                                             float (*tmp)[N], float (&s)[N]) {
+  const int groups = kThreads / lanes, own = threadIdx.x / lanes;
+  const int32_t n = p1 - p0, per = (n + groups - 1) / groups;
+  sum_places<T, N>(a, order, p0 + min(own * per, n), p0 + min(own * per + per, n), c, s);
 #pragma unroll
-    for (int x = 0; x < N; ++x) s[x] = 0.0f;
-    for (int32_t p = p0; p < p1; ++p) {
-      float f[N];
-      run_load<T, N>(a.grad, (int64_t)w.order[p] * a.E + c, f);
+  for (int x = 0; x < N; ++x) tmp[threadIdx.x][x] = s[x];
+  __syncthreads();
+  if (own == 0)
+    for (int i = 1; i < groups; ++i)
 #pragma unroll
-      for (int x = 0; x < N; ++x) s[x] += f[x];
-    }
-#pragma unroll
-    for (int x = 0; x < N; ++x) s[x] *= a.scale;
-    run_store<T, N>(a.out, v * a.E + c, s);
-  }
+      for (int x = 0; x < N; ++x) s[x] += tmp[i * lanes + threadIdx.x][x];
+  __syncthreads();
 }
 
 // The long rows that places [j part, j part + part) of the order touch: at most
@@ -203,35 +258,77 @@ __device__ __forceinline__ LongRow long_row(const EmbedGradArgs& a, const GradWo
   return l;
 }
 
+// Workgroups before `part_blocks`: one slab of columns of one part's long rows,
+// float32.  The others: `rows` rows of the table each, by groups of `lanes` threads;
+// zeros for a row without tokens.  A row of more than kFew tokens is left to the
+// whole workgroup, a long one to its parts.
 template <class T, int N>
-__global__ void __launch_bounds__(kThreads) embed_part_kernel(EmbedGradArgs a, GradWork w,
-                                                              int64_t part) {
-  const int32_t n = w.first[a.V];
-  const int64_t j = blockIdx.x;
-  if (j * part >= n) return;
-  const int32_t q0 = (int32_t)(j * part), q1 = (int32_t)min(j * part + part, (int64_t)n);
-  const int64_t c = ((int64_t)blockIdx.y * kThreads + threadIdx.x) * N;
+__global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, GradWork w,
+                                                             int64_t part, uint32_t part_blocks,
+                                                             int lanes, int rows) {
+  __shared__ float tmp[kThreads][N];
+  __shared__ int32_t first[kThreads + 1];
+  const int lane = threadIdx.x % lanes, own = threadIdx.x / lanes, groups = kThreads / lanes;
+  const int slab = lanes * N;  // columns
+  if (blockIdx.x < part_blocks) {
+    const uint32_t slabs = (uint32_t)((a.E + slab - 1) / slab);
+    const int64_t j = blockIdx.x / slabs;
+    const int64_t c = run_start((int64_t)(blockIdx.x % slabs) * slab + lane * N, a.E, N);
+    const int32_t n = w.first[a.V];
+    if (j * part >= n) return;
+    const int32_t q0 = (int32_t)(j * part), q1 = (int32_t)min(j * part + part, (int64_t)n);
+    for (int side = 0; side < 2; ++side) {
+      const LongRow l = long_row(a, w, side ? q1 - 1 : q0, part);
+      if (l.row < 0 || (side && l.p0 <= q0)) continue;
+      float s[N];
+      sum_together<T, N>(a, w.order, max(l.p0, q0), min(l.p1, q1), c, lanes, tmp, s);
+      if (own == 0)
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const LongRow l = long_row(a, w, side ? q1 - 1 : q0, part);
-    if (l.row < 0 || (side && l.p0 <= q0)) continue;
-    if (c >= a.E) continue;
-    float s[N];
-#pragma unroll
-    for (int x = 0; x < N; ++x) s[x] = 0.0f;
-    for (int32_t p = max(l.p0, q0); p < min(l.p1, q1); ++p) {
-      float f[N];
-      run_load<T, N>(a.grad, (int64_t)w.order[p] * a.E + c, f);
-#pragma unroll
-      for (int x = 0; x < N; ++x) s[x] += f[x];
+        for (int x = 0; x < N; ++x)
+          w.part[(j * 2 + side) * a.E + c + x] = s[x];
     }
+    return;
+  }
+  const int64_t v0 = (int64_t)(blockIdx.x - part_blocks) * rows;
+  const int here = (int)min((int64_t)rows, a.V - v0);
+  for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
+  __syncthreads();
+  auto store = [&](int64_t v, int64_t c, float (&s)[N]) {
 #pragma unroll
-    for (int x = 0; x < N; ++x) w.part[(j * 2 + side) * a.E + c + x] = s[x];
+    for (int x = 0; x < N; ++x) s[x] *= a.scale;
+    run_store<T, N>(a.out, v * a.E + c, s);
+  };
+  for (int r = own; r < here; r += groups) {
+    const int32_t p0 = first[r], p1 = first[r + 1];
+    if (p1 - p0 > kFew) continue;
+    if (p1 == p0) {
+      for (int64_t i = lane * N; i < a.E; i += slab) {
+        float zero[N] = {};
+        run_store<T, N, true>(a.out, (v0 + r) * a.E + run_start(i, a.E, N), zero);
+      }
+      continue;
+    }
+    for (int64_t i = lane * N; i < a.E; i += slab) {
+      const int64_t c = run_start(i, a.E, N);
+      float s[N];
+      sum_places<T, N>(a, w.order, p0, p1, c, s);
+      store(v0 + r, c, s);
+    }
+  }
+  for (int r = 0; r < here; ++r) {
+    const int32_t p0 = first[r], p1 = first[r + 1];
+    if (p1 - p0 <= kFew || p1 - p0 > part) continue;
+    for (int64_t c0 = 0; c0 < a.E; c0 += slab) {
+      const int64_t c = run_start(c0 + lane * N, a.E, N);
+      float s[N];
+      sum_together<T, N>(a, w.order, p0, p1, c, lanes, tmp, s);
+      if (own == 0) store(v0 + r, c, s);
+    }
   }
 }
 
 // The long row that begins in part j, from its parts in order.
-template <class T, int N>
+template <class T>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(EmbedGradArgs a, GradWork w,
                                                               int64_t part) {
   const int32_t n = w.first[a.V];
@@ -239,17 +336,12 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(EmbedGradArgs a, G
   if (j * part >= n) return;
   const int32_t q0 = (int32_t)(j * part), q1 = (int32_t)min(j * part + part, (int64_t)n);
   const LongRow l = long_row(a, w, q1 - 1, part);
-  const int64_t c = ((int64_t)blockIdx.y * kThreads + threadIdx.x) * N;
+  const int64_t c = (int64_t)blockIdx.y * kThreads + threadIdx.x;
   if (l.row < 0 || l.p0 < q0 || c >= a.E) return;
-  float s[N];
-#pragma unroll
-  for (int x = 0; x < N; ++x) s[x] = w.part[(j * 2 + (l.p0 > q0)) * a.E + c + x];
-  for (int64_t i = j + 1; i * part < l.p1; ++i)
-#pragma unroll
-    for (int x = 0; x < N; ++x) s[x] += w.part[i * 2 * a.E + c + x];
-#pragma unroll
-  for (int x = 0; x < N; ++x) s[x] *= a.scale;
-  run_store<T, N>(a.out, l.row * a.E + c, s);
+  float s = w.part[(j * 2 + (l.p0 > q0)) * a.E + c];
+#pragma unroll 8
+  for (int64_t i = j + 1; i < (l.p1 + part - 1) / part; ++i) s += w.part[i * 2 * a.E + c];
+  ((typename T::elem*)a.out)[l.row * a.E + c] = T::put(s * a.scale);
 }
 
 }  // namespace
@@ -258,7 +350,7 @@ void launch_embed(const EmbedArgs& a, hipStream_t stream) {
   if (a.T * a.E == 0) return;
   by_run(a.dt, a.E, [&](auto t, auto n) {
     constexpr int N = decltype(n)::value;
-    const int x = row_threads(a.E / N), y = kThreads / x;
+    const int x = row_threads((a.E + N - 1) / N, kThreads), y = kThreads / x;
     hipLaunchKernelGGL((embed_kernel<decltype(t), N>), dim3((unsigned)((a.T + y - 1) / y)),
                        dim3(x, y), 0, stream, a);
   });
@@ -273,23 +365,30 @@ size_t embed_grad_ws_bytes(int64_t T, int64_t V, int64_t E) {
 int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
   if (a.V * a.E == 0) return 0;
   const GradWork w = grad_work(a);
-  const int64_t part = part_tokens(a.T);
+  const int64_t part = part_tokens(a.T), parts = a.T > part ? (a.T + part - 1) / part : 0;
   hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)((a.V + kSortRows - 1) / kSortRows)),
                      dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w);
   by_run(a.dt, a.E, [&](auto t, auto n) {
     typedef decltype(t) Ty;
     constexpr int N = decltype(n)::value;
-    const int x = row_threads(a.E / N), y = kThreads / x;
-    hipLaunchKernelGGL((embed_rows_kernel<Ty, N>), dim3((unsigned)((a.V + y - 1) / y)),
-                       dim3(x, y), 0, stream, a, w, part);
-    if (a.T <= part) return;
-    const dim3 grid((unsigned)((a.T + part - 1) / part),
-                    (unsigned)((a.E / N + kThreads - 1) / kThreads));
-    hipLaunchKernelGGL((embed_part_kernel<Ty, N>), grid, dim3(kThreads), 0, stream, a, w, part);
-    hipLaunchKernelGGL((embed_join_kernel<Ty, N>), grid, dim3(kThreads), 0, stream, a, w, part);
+    const int64_t runs = (a.E + N - 1) / N;
+    const int lanes = row_threads(runs, 64), groups = kThreads / lanes;
+    // about 64 KiB of the table per workgroup, as long as that fills the card
+    const int64_t bytes = a.E * (int64_t)sizeof(typename Ty::elem);
+    int rows = (int)std::max<int64_t>(1, std::min<int64_t>(kThreads, 65536 / bytes));
+    while (rows > groups && a.V < (int64_t)rows * 1024) rows /= 2;
+    rows = std::max(groups, rows / groups * groups);
+    const int64_t slabs = (runs + lanes - 1) / lanes;
+    const int64_t blocks = parts * slabs + (a.V + rows - 1) / rows;
+    hipLaunchKernelGGL((embed_sum_kernel<Ty, N>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                       a, w, part, (uint32_t)(parts * slabs), lanes, rows);
+    if (parts == 0) return;
+    hipLaunchKernelGGL((embed_join_kernel<Ty>),
+                       dim3((unsigned)parts, (unsigned)((a.E + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, a, w, part);
   });
   REW_HIP(hipGetLastError());
-  return a.T > part ? 4 : 2;
+  return parts ? 3 : 2;
 }
 
 }  // namespace rew

@@ -3,7 +3,7 @@
 //
 // A row lies in the registers of a group of 64 to 1024 threads, kept from the
 // first pass (mean) to the last: it is read once.  Thread i of the group holds
-// runs i, i + G, ... of at most 16 bytes.
+// the runs i, i + G, ... of 16 bytes (rows_device.h).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,19 +42,20 @@ __device__ __forceinline__ void group_sum2(float& x, float& y, float2* tmp) {
   }
 }
 
-// A row of n values in registers: C runs of N.
-template <class T, int N, int G, int C>
-__device__ __forceinline__ void row_load(const void* x, int64_t row, int64_t n, int g,
-                                         float (&f)[C][N]) {
+// The runs of thread g of a row's group: where they start, and from which value on
+// they hold what no earlier run does (N: none).
+template <int G, int C, int N>
+struct Runs {
+  int at[C], own[C];
+  __device__ __forceinline__ Runs(int64_t n, int g) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int64_t i = ((int64_t)c * G + g) * N;
-    if (i < n) run_load<T, N>(x, row * n + i, f[c]);
-    else
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[c][e] = 0.0f;
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = ((int64_t)c * G + g) * N;
+      at[c] = (int)run_start(i, n, N);
+      own[c] = (int)min(i - at[c], (int64_t)N);
+    }
   }
-}
+};
 
 // Workgroups of 256 threads, or of G where that is more: 256 / G rows each.
 template <class T, class P, int N, int G, int C>
@@ -64,28 +65,29 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
   const int g = threadIdx.x % G;
   const int64_t n = a.n;
   const float inv = 1.0f / (float)n;
+  const Runs<G, C, N> run(n, g);
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
     const int64_t row = r0 + threadIdx.x / G;
     const bool there = row < a.rows;
+    const int64_t base = (there ? row : a.rows - 1) * n;
     float f[C][N];
-    row_load<T, N, G, C>(a.x, there ? row : a.rows - 1, n, g, f);
+#pragma unroll
+    for (int c = 0; c < C; ++c) run_load<T, N>(a.x, base + run.at[c], f[c]);
     float s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += f[c][e];
+      for (int e = 0; e < N; ++e) s += e >= run.own[c] ? f[c][e] : 0.0f;
     group_sum2<G>(s, q, tmp);
     const float mean = s * inv;
     q = 0.0f;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const bool in = ((int64_t)c * G + g) * N < n;
+    for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         f[c][e] -= mean;
-        q += in ? f[c][e] * f[c][e] : 0.0f;
+        q += e >= run.own[c] ? f[c][e] * f[c][e] : 0.0f;
       }
-    }
     group_sum2<G>(q, s, tmp);
     const float rstd = 1.0f / sqrtf(q * inv + a.eps);
     if (!there) continue;
@@ -95,114 +97,134 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + g) * N;
-      if (i >= n) continue;
+      if (run.own[c] == N) continue;
       float w[N], b[N];
-      run_load<P, N>(a.gamma, i, w);
-      run_load<P, N>(a.beta, i, b);
+      run_load<P, N>(a.gamma, run.at[c], w);
+      run_load<P, N>(a.beta, run.at[c], b);
 #pragma unroll
       for (int e = 0; e < N; ++e) f[c][e] = f[c][e] * rstd * w[e] + b[e];
-      run_store<T, N>(a.y, row * n + i, f[c]);
+      run_store<T, N>(a.y, base + run.at[c], f[c]);
     }
   }
 }
 
 // Rows too long for the registers of 1024 threads: three walks over the row,
 // the second and third from the caches.
-template <class T, class P, int N>
+template <class T, class P>
 __global__ void __launch_bounds__(kMaxGroup) norm_long_kernel(NormArgs a) {
+  constexpr int N = kRun<T>;
   __shared__ float2 tmp[kMaxGroup / 64];
   const int64_t row = blockIdx.x, n = a.n;
-  constexpr int64_t kStep = (int64_t)kMaxGroup * N;
-  const int64_t i0 = threadIdx.x * N;
   const float inv = 1.0f / (float)n;
+  auto walk = [&](auto&& f) {
+    for (int64_t i = threadIdx.x * N; i < n; i += (int64_t)kMaxGroup * N) {
+      const int64_t at = run_start(i, n, N);
+      float v[N];
+      run_load<T, N>(a.x, row * n + at, v);
+      f(at, (int)(i - at), v);
+    }
+  };
   float s = 0.0f, q = 0.0f;
-  for (int64_t i = i0; i < n; i += kStep) {
-    float f[N];
-    run_load<T, N>(a.x, row * n + i, f);
+  walk([&](int64_t, int own, float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += f[e];
-  }
+    for (int e = 0; e < N; ++e) s += e >= own ? v[e] : 0.0f;
+  });
   group_sum2<kMaxGroup>(s, q, tmp);
   const float mean = s * inv;
   q = 0.0f;
-  for (int64_t i = i0; i < n; i += kStep) {
-    float f[N];
-    run_load<T, N>(a.x, row * n + i, f);
+  walk([&](int64_t, int own, float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) q += (f[e] - mean) * (f[e] - mean);
-  }
+    for (int e = 0; e < N; ++e) q += e >= own ? (v[e] - mean) * (v[e] - mean) : 0.0f;
+  });
   group_sum2<kMaxGroup>(q, s, tmp);
   const float rstd = 1.0f / sqrtf(q * inv + a.eps);
   if (a.mean && threadIdx.x == 0) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
   }
-  for (int64_t i = i0; i < n; i += kStep) {
-    float f[N], w[N], b[N];
-    run_load<T, N>(a.x, row * n + i, f);
-    run_load<P, N>(a.gamma, i, w);
-    run_load<P, N>(a.beta, i, b);
+  walk([&](int64_t at, int, float (&v)[N]) {
+    float w[N], b[N];
+    run_load<P, N>(a.gamma, at, w);
+    run_load<P, N>(a.beta, at, b);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = (f[e] - mean) * rstd * w[e] + b[e];
-    run_store<T, N>(a.y, row * n + i, f);
-  }
+    for (int e = 0; e < N; ++e) v[e] = (v[e] - mean) * rstd * w[e] + b[e];
+    run_store<T, N>(a.y, row * n + at, v);
+  });
 }
 
 // ---- gradients ----------------------------------------------------------------------
 
-// Workgroups of 1024 threads, 1024 / G rows at a time, that walk the rows
-// blockIdx.x * (1024 / G), + gridDim.x * (1024 / G), ... and keep the columns'
-// sums of dy xh and dy in registers; the row groups add theirs in LDS, in order,
-// and leave one row of partial sums per workgroup: part[b][2][n].
+// Threads of a workgroup of norm_grad_kernel.
+constexpr int grad_block(int G) { return G > 512 ? G : 512; }
+
+// Workgroups that walk the rows, grad_block / G of them at a time (the next ones'
+// values on their way while this one's sums are formed), and keep the columns' sums of
+// dy xh and dy in registers; the row groups add theirs in LDS, in order, and leave one
+// row of partial sums per workgroup: part[b][2][n].
 template <class T, class P, int N, int G, int C>
-__global__ void __launch_bounds__(kMaxGroup) norm_grad_kernel(NormGradArgs a) {
-  constexpr int kRows = kMaxGroup / G;
-  __shared__ float2 tmp[kMaxGroup / 64];
+__global__ void __launch_bounds__(grad_block(G)) norm_grad_kernel(NormGradArgs a, float* part) {
+  constexpr int kRows = grad_block(G) / G;
+  __shared__ float2 tmp[grad_block(G) / 64];
   __shared__ float sums[kRows > 1 ? G * N * C : 1];
   const int g = threadIdx.x % G, own = threadIdx.x / G;
-  const int64_t n = a.n;
+  const int64_t n = a.n, step = (int64_t)gridDim.x * kRows;
   const float inv = 1.0f / (float)n;
+  const Runs<G, C, N> run(n, g);
   float w[C][N], dg[C][N], db[C][N];
-  row_load<P, N, G, C>(a.gamma, 0, n, g, w);
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < C; ++c) {
+    run_load<P, N>(a.gamma, run.at[c], w[c]);
 #pragma unroll
     for (int e = 0; e < N; ++e) dg[c][e] = db[c][e] = 0.0f;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
-    const bool there = r0 + own < a.rows;
-    const int64_t row = there ? r0 + own : a.rows - 1;
-    float x[C][N], dy[C][N];
-    row_load<T, N, G, C>(a.x, row, n, g, x);
-    row_load<T, N, G, C>(a.dy, row, n, g, dy);
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float s = 0.0f, q = 0.0f;
+  }
+  RowRun<T, N> rx[C], ry[C];
+  float mean = 0.0f, rstd = 0.0f;
+  auto fetch = [&](int64_t r0) {
+    const int64_t row = min(r0 + own, a.rows - 1);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const bool in = ((int64_t)c * G + g) * N < n;
+    for (int c = 0; c < C; ++c) rx[c] = run_at<T, N>(a.x, row * n + run.at[c]);
+#pragma unroll
+    for (int c = 0; c < C; ++c) ry[c] = run_at<T, N>(a.dy, row * n + run.at[c]);
+    mean = a.mean[row];
+    rstd = a.rstd[row];
+  };
+  int64_t r0 = (int64_t)blockIdx.x * kRows;
+  if (r0 < a.rows) fetch(r0);
+  for (; r0 < a.rows; r0 += step) {
+    const bool there = r0 + own < a.rows;
+    float x[C][N], dy[C][N];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        x[c][e] = in ? (x[c][e] - mean) * rstd : 0.0f;
-        if (there) {
-          dg[c][e] += dy[c][e] * x[c][e];
-          db[c][e] += dy[c][e];
-        }
-        dy[c][e] *= w[c][e];
-        s += dy[c][e];
-        q += dy[c][e] * x[c][e];
+        x[c][e] = T::get(rx[c].v[e]);
+        dy[c][e] = T::get(ry[c].v[e]);
       }
-    }
+    const float m = mean, r = rstd;
+    fetch(min(r0 + step, a.rows - 1));
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        x[c][e] = (x[c][e] - m) * r;
+        dg[c][e] += there ? dy[c][e] * x[c][e] : 0.0f;
+        db[c][e] += there ? dy[c][e] : 0.0f;
+        dy[c][e] *= w[c][e];
+        const float v = e >= run.own[c] ? dy[c][e] : 0.0f;
+        s += v;
+        q += e >= run.own[c] ? v * x[c][e] : 0.0f;
+      }
     group_sum2<G>(s, q, tmp);
     s *= inv;
     q *= inv;
     if (!there) continue;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + g) * N;
-      if (i >= n) continue;
+      if (run.own[c] == N) continue;
 #pragma unroll
-      for (int e = 0; e < N; ++e) dy[c][e] = rstd * (dy[c][e] - s - x[c][e] * q);
-      run_store<T, N>(a.dx, row * n + i, dy[c]);
+      for (int e = 0; e < N; ++e) dy[c][e] = r * (dy[c][e] - s - x[c][e] * q);
+      run_store<T, N>(a.dx, (r0 + own) * n + run.at[c], dy[c]);
     }
   }
   // the row groups' sums, one after another
@@ -229,86 +251,90 @@ __global__ void __launch_bounds__(kMaxGroup) norm_grad_kernel(NormGradArgs a) {
     if (own == 0)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int64_t i = ((int64_t)c * G + g) * N;
-        if (i >= n) continue;
+        if (run.own[c] == N) continue;
+        float* p = part + ((int64_t)blockIdx.x * 2 + half) * n + run.at[c];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          a.work[((int64_t)blockIdx.x * 2 + half) * n + i + e] = half ? db[c][e] : dg[c][e];
+        for (int e = 0; e < N; ++e) p[e] = half ? db[c][e] : dg[c][e];
       }
   }
 }
 
-// Long rows: dx alone, the row walked twice.
-template <class T, class P, int N>
-__global__ void __launch_bounds__(kMaxGroup) norm_grad_long_kernel(NormGradArgs a) {
+// Long rows: the two sums of each, mean w and mean w xh ...
+template <class T, class P>
+__global__ void __launch_bounds__(kMaxGroup) norm_grad_sums_kernel(NormGradArgs a, float2* out) {
+  constexpr int N = kRun<T>;
   __shared__ float2 tmp[kMaxGroup / 64];
   const int64_t row = blockIdx.x, n = a.n;
-  constexpr int64_t kStep = (int64_t)kMaxGroup * N;
-  const int64_t i0 = threadIdx.x * N;
   const float inv = 1.0f / (float)n, mean = a.mean[row], rstd = a.rstd[row];
   float s = 0.0f, q = 0.0f;
-  for (int64_t i = i0; i < n; i += kStep) {
+  for (int64_t i = threadIdx.x * N; i < n; i += (int64_t)kMaxGroup * N) {
+    const int64_t at = run_start(i, n, N);
     float x[N], dy[N], w[N];
-    run_load<T, N>(a.x, row * n + i, x);
-    run_load<T, N>(a.dy, row * n + i, dy);
-    run_load<P, N>(a.gamma, i, w);
+    run_load<T, N>(a.x, row * n + at, x);
+    run_load<T, N>(a.dy, row * n + at, dy);
+    run_load<P, N>(a.gamma, at, w);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      s += dy[e] * w[e];
-      q += dy[e] * w[e] * ((x[e] - mean) * rstd);
+      const bool in = e >= i - at;
+      const float v = dy[e] * w[e];
+      s += in ? v : 0.0f;
+      q += in ? v * ((x[e] - mean) * rstd) : 0.0f;
     }
   }
   group_sum2<kMaxGroup>(s, q, tmp);
-  s *= inv;
-  q *= inv;
-  for (int64_t i = i0; i < n; i += kStep) {
-    float x[N], dy[N], w[N];
-    run_load<T, N>(a.x, row * n + i, x);
-    run_load<T, N>(a.dy, row * n + i, dy);
-    run_load<P, N>(a.gamma, i, w);
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      dy[e] = rstd * (dy[e] * w[e] - s - (x[e] - mean) * rstd * q);
-    run_store<T, N>(a.dx, row * n + i, dy);
-  }
+  if (threadIdx.x == 0) out[row] = make_float2(s * inv, q * inv);
 }
 
-// .. and the columns' sums over the rows b, b + parts, ...: part[b][2][n].
-template <class T, int N>
-__global__ void __launch_bounds__(256) norm_columns_kernel(NormGradArgs a, int parts) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N, n = a.n;
+// .. and then dx and the columns' sums, 256 runs of columns over `per` rows in a
+// workgroup: part[b][2][n].
+template <class T, class P>
+__global__ void __launch_bounds__(256) norm_grad_columns_kernel(NormGradArgs a, const float2* sums,
+                                                                float* part, int64_t per) {
+  constexpr int N = kRun<T>;
+  const int64_t n = a.n, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
   if (i >= n) return;
-  float dg[N], db[N];
+  const int64_t at = run_start(i, n, N);
+  float w[N], dg[N], db[N];
+  run_load<P, N>(a.gamma, at, w);
 #pragma unroll
   for (int e = 0; e < N; ++e) dg[e] = db[e] = 0.0f;
-  for (int64_t row = blockIdx.y; row < a.rows; row += parts) {
+  const int64_t end = min(a.rows, ((int64_t)blockIdx.y + 1) * per);
+#pragma unroll 4
+  for (int64_t row = blockIdx.y * per; row < end; ++row) {
     float x[N], dy[N];
-    run_load<T, N>(a.x, row * n + i, x);
-    run_load<T, N>(a.dy, row * n + i, dy);
+    run_load<T, N>(a.x, row * n + at, x);
+    run_load<T, N>(a.dy, row * n + at, dy);
     const float mean = a.mean[row], rstd = a.rstd[row];
+    const float2 m = sums[row];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      dg[e] += dy[e] * ((x[e] - mean) * rstd);
+      const float xh = (x[e] - mean) * rstd;
+      dg[e] += dy[e] * xh;
       db[e] += dy[e];
+      dy[e] = rstd * (dy[e] * w[e] - m.x - xh * m.y);
     }
+    run_store<T, N>(a.dx, row * n + at, dy);
   }
+  float* p = part + (int64_t)blockIdx.y * 2 * n + at;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    a.work[(int64_t)blockIdx.y * 2 * n + i + e] = dg[e];
-    a.work[((int64_t)blockIdx.y * 2 + 1) * n + i + e] = db[e];
+    p[e] = dg[e];
+    p[n + e] = db[e];
   }
 }
 
 // dgamma and dbeta: the sum of the `parts` rows of partial sums, 16 waves a
 // sixteenth of them each, joined in order.
 template <class P>
-__global__ void __launch_bounds__(1024) norm_join_kernel(NormGradArgs a, int parts) {
+__global__ void __launch_bounds__(1024) norm_join_kernel(NormGradArgs a, const float* part,
+                                                         int parts) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i = (int64_t)blockIdx.x * 64 + lane;  // of the 2 n columns
   float s = 0.0f;
   if (i < 2 * a.n)
-    for (int p = wave; p < parts; p += 16) s += a.work[(int64_t)p * 2 * a.n + i];
+#pragma unroll 4
+    for (int p = wave; p < parts; p += 16) s += part[(int64_t)p * 2 * a.n + i];
   sums[wave][lane] = s;
   __syncthreads();
   if (wave || i >= 2 * a.n) return;
@@ -317,51 +343,50 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(NormGradArgs a, int par
   ((typename P::elem*)out)[i < a.n ? i : i - a.n] = P::put(s);
 }
 
-// f(element type, parameter type, run length): the longest run of at most 16
-// bytes of x's values that divides a row.  (A run of parameters in float32 is
-// then up to 32 bytes: two loads.)
+// f(element type, parameter type, run length) for rows of n values.
 template <class F>
 void by_types(int dt, int p_dt, int64_t n, F&& f) {
-  auto runs = [&](auto t, auto p, auto most) {
-    constexpr int M = decltype(most)::value;
-    if (n % M == 0) f(t, p, std::integral_constant<int, M>());
+  auto with = [&](auto t, auto p) {
+    constexpr int N = kRun<decltype(t)>;
+    if (n >= N) f(t, p, std::integral_constant<int, N>());
     else f(t, p, std::integral_constant<int, 1>());
   };
-  std::integral_constant<int, 8> eight;
-  if (dt == kF32) runs(RowF32(), RowF32(), std::integral_constant<int, 4>());
-  else if (dt == kBF16 && p_dt == kF32) runs(RowBf16(), RowF32(), eight);
-  else if (dt == kBF16) runs(RowBf16(), RowBf16(), eight);
-  else if (p_dt == kF32) runs(RowF16(), RowF32(), eight);
-  else runs(RowF16(), RowF16(), eight);
+  if (dt == kF32) with(RowF32(), RowF32());
+  else if (dt == kBF16 && p_dt == kF32) with(RowBf16(), RowF32());
+  else if (dt == kBF16) with(RowBf16(), RowBf16());
+  else if (p_dt == kF32) with(RowF16(), RowF32());
+  else with(RowF16(), RowF16());
 }
 
-// f(group, runs per thread) for a row of `runs` runs of N values, false where it
-// is too long: at most 16 values a thread.
-template <int N, class F>
+// f(group, runs of a thread) for a row of `runs` runs; false where it is longer than
+// `Most` runs in each of 1024 threads (0: a row of single values).
+template <int Most, class F>
 bool by_group(int64_t runs, F&& f) {
-  constexpr int C = 16 / N;  // most runs of a thread
-  auto with = [&](auto g) {
-    constexpr int G = decltype(g)::value;
-    if constexpr (C <= 4) {
-      if (runs <= G) f(g, std::integral_constant<int, 1>());
-      else if (runs <= 2 * G) f(g, std::integral_constant<int, 2>());
-      else f(g, std::integral_constant<int, C>());
-    } else {
-      if (runs <= 4 * G) f(g, std::integral_constant<int, 4>());
-      else f(g, std::integral_constant<int, C>());
-    }
-  };
-  if (runs > (int64_t)C * kMaxGroup) return false;
-  if (runs <= 64 * C) with(std::integral_constant<int, 64>());
-  else if (runs <= 256 * C) with(std::integral_constant<int, 256>());
-  else with(std::integral_constant<int, kMaxGroup>());
-  return true;
+  if constexpr (Most == 0) {
+    f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    return true;
+  } else {
+    auto with = [&](auto g, auto c) { f(g, c); };
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, 2> two;
+    if (runs <= 64) with(std::integral_constant<int, 64>(), one);
+    else if (runs <= 128) with(std::integral_constant<int, 64>(), two);
+    else if (runs <= 256) with(std::integral_constant<int, 256>(), one);
+    else if (runs <= 512) with(std::integral_constant<int, 256>(), two);
+    else if (runs <= 1024) with(std::integral_constant<int, 512>(), two);
+    else if (Most >= 2 && runs <= 2048)
+      with(std::integral_constant<int, 1024>(), std::integral_constant<int, Most >= 2 ? 2 : 1>());
+    else if (Most >= 4 && runs <= 4096)
+      with(std::integral_constant<int, 1024>(), std::integral_constant<int, Most >= 4 ? 4 : 1>());
+    else return false;
+    return true;
+  }
 }
 
-// Workgroups of norm_grad_kernel (or shares of norm_columns_kernel's rows): one
-// per CU, since each leaves a row of partial sums that is written and read once
-// more.
-int64_t grad_parts(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(rows, 256)); }
+// Workgroups of norm_grad_kernel at most, one per CU, since each leaves a row of
+// partial sums that is written and read once more; rows of a part of long rows.
+constexpr int64_t kParts = 256;
+constexpr int64_t kPartRows = 16;
 
 }  // namespace
 
@@ -371,7 +396,7 @@ void launch_norm(const NormArgs& a, hipStream_t stream) {
     typedef decltype(t) T;
     typedef decltype(p) P;
     constexpr int N = decltype(nn)::value;
-    const bool fits = by_group<N>(a.n / N, [&](auto g, auto c) {
+    const bool fits = by_group<N == 1 ? 0 : 4>((a.n + N - 1) / N, [&](auto g, auto c) {
       constexpr int G = decltype(g)::value, C = decltype(c)::value;
       constexpr int rows = G > 256 ? 1 : 256 / G;
       const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, kMaxBlocks);
@@ -379,41 +404,51 @@ void launch_norm(const NormArgs& a, hipStream_t stream) {
                          dim3(G > 256 ? G : 256), 0, stream, a);
     });
     if (!fits)
-      hipLaunchKernelGGL((norm_long_kernel<T, P, N>), dim3((unsigned)a.rows), dim3(kMaxGroup), 0,
+      hipLaunchKernelGGL((norm_long_kernel<T, P>), dim3((unsigned)a.rows), dim3(kMaxGroup), 0,
                          stream, a);
   });
   REW_HIP(hipGetLastError());
 }
 
+// (the sums of long rows, then the parts)
 size_t norm_grad_ws_bytes(int64_t rows, int64_t n) {
-  return (size_t)grad_parts(rows) * 2 * n * sizeof(float);
+  return (size_t)rows * sizeof(float2) + (size_t)std::min(std::max<int64_t>(rows, 1), kParts) * 2 *
+                                             n * sizeof(float);
 }
 
 int launch_norm_grad(const NormGradArgs& a, hipStream_t stream) {
   if (a.n == 0) return 0;
-  int parts = (int)grad_parts(a.rows), launches = 2;
+  int launches = 2;
+  float2* sums = (float2*)a.work;
+  float* part = a.work + 2 * a.rows;
   by_types(a.x_dt, a.p_dt, a.n, [&](auto t, auto p, auto nn) {
     typedef decltype(t) T;
     typedef decltype(p) P;
     constexpr int N = decltype(nn)::value;
-    const bool fits = by_group<N>(a.n / N, [&](auto g, auto c) {
+    const int64_t runs = (a.n + N - 1) / N;
+    int parts = 1;
+    // (16-bit rows of 2 runs in each of 1024 threads would spill)
+    constexpr int most = N == 1 ? 0 : N == 4 ? 2 : 1;
+    const bool fits = by_group<most>(runs, [&](auto g, auto c) {
       constexpr int G = decltype(g)::value, C = decltype(c)::value;
-      constexpr int rows = kMaxGroup / G;
-      parts = (int)std::min<int64_t>(parts, std::max<int64_t>(1, (a.rows + rows - 1) / rows));
-      hipLaunchKernelGGL((norm_grad_kernel<T, P, N, G, C>), dim3(parts), dim3(kMaxGroup), 0,
-                         stream, a);
+      constexpr int rows = grad_block(G) / G;
+      parts = (int)std::max<int64_t>(1, std::min((a.rows + rows - 1) / rows, kParts));
+      hipLaunchKernelGGL((norm_grad_kernel<T, P, N, G, C>), dim3(parts), dim3(grad_block(G)), 0,
+                         stream, a, part);
     });
     if (!fits) {
       launches = 3;
+      const int64_t per = std::max(kPartRows, (a.rows + kParts - 1) / kParts);
+      parts = (int)std::max<int64_t>(1, (a.rows + per - 1) / per);
       if (a.rows)
-        hipLaunchKernelGGL((norm_grad_long_kernel<T, P, N>), dim3((unsigned)a.rows),
-                           dim3(kMaxGroup), 0, stream, a);
-      hipLaunchKernelGGL((norm_columns_kernel<T, N>),
-                         dim3((unsigned)((a.n / N + 255) / 256), parts), dim3(256), 0, stream, a,
-                         parts);
+        hipLaunchKernelGGL((norm_grad_sums_kernel<T, P>), dim3((unsigned)a.rows), dim3(kMaxGroup),
+                           0, stream, a, sums);
+      hipLaunchKernelGGL((norm_grad_columns_kernel<T, P>),
+                         dim3((unsigned)((runs + 255) / 256), parts), dim3(256), 0, stream, a, sums,
+                         part, per);
     }
     hipLaunchKernelGGL((norm_join_kernel<P>), dim3((unsigned)((2 * a.n + 63) / 64)), dim3(1024), 0,
-                       stream, a, parts);
+                       stream, a, part, parts);
   });
   REW_HIP(hipGetLastError());
   return launches;

@@ -493,7 +493,7 @@ static void prepare_embed(const std::string& op, const std::vector<Tensor*>& ins
   float_attr(attrs, "scale", false, op, n);
   std::vector<int64_t> shape = ids->shape.vec();
   if (!n->sub) {
-    if (rows->shape.rank != 2)
+    if (rows->shape.rank != 2 || rows->shape.d[0] < 1)
       invalid("eager '" + op + "': weight must be [vocab, embed], got " + rows->shape.str());
     shape.push_back(rows->shape.d[1]);
     outs.push_back({rows->dt, Shape(shape)});

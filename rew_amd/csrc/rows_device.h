@@ -24,26 +24,52 @@ struct RowF16 {
   static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
 };
 
-// N values side by side, loaded and stored as one access (N * the element's
-// size is 16 bytes or less, a power of two, and the address a multiple of it).
+// Rows are walked in runs of N values: 16 bytes, or single values in rows of fewer.
+// The run that would reach past a row's end, and any behind it, lies on the row's
+// last N values instead: no access is under a condition (at whose end the compiler
+// would wait for every load under way), and values that two runs hold are computed
+// and stored twice, the same.  Sums over a row leave out what an earlier run holds.
+template <class T>
+constexpr int kRun = 16 / (int)sizeof(typename T::elem);
+
+__device__ __forceinline__ int64_t run_start(int64_t i, int64_t n, int N) {
+  return i < n - N ? i : n - N;
+}
+
+// (The address need not be a multiple of 16 in rows of an odd number of values: the
+// access is one instruction all the same, since those of a wave may be unaligned.)
 template <class T, int N>
-struct alignas(sizeof(typename T::elem) * N) RowRun {
+struct __attribute__((packed, aligned(sizeof(typename T::elem)))) RowRun {
   typename T::elem v[N];
 };
 
 template <class T, int N>
+__device__ __forceinline__ RowRun<T, N> run_at(const void* base, int64_t i) {
+  return *(const RowRun<T, N>*)((const typename T::elem*)base + i);
+}
+
+template <class T, int N>
 __device__ __forceinline__ void run_load(const void* base, int64_t i, float (&f)[N]) {
-  const RowRun<T, N> r = *(const RowRun<T, N>*)((const typename T::elem*)base + i);
+  const RowRun<T, N> r = run_at<T, N>(base, i);
 #pragma unroll
   for (int x = 0; x < N; ++x) f[x] = T::get(r.v[x]);
 }
 
-template <class T, int N>
+// Past: nontemporal, for a large result that the caches need not keep.
+template <class T, int N, bool Past = false>
 __device__ __forceinline__ void run_store(void* base, int64_t i, const float (&f)[N]) {
   RowRun<T, N> r;
 #pragma unroll
   for (int x = 0; x < N; ++x) r.v[x] = T::put(f[x]);
-  *(RowRun<T, N>*)((typename T::elem*)base + i) = r;
+  RowRun<T, N>* p = (RowRun<T, N>*)((typename T::elem*)base + i);
+  if constexpr (Past && sizeof r == 16) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4 v;
+    __builtin_memcpy(&v, &r, 16);
+    __builtin_nontemporal_store(v, (u32x4*)p);
+  } else {
+    *p = r;
+  }
 }
 
 }  // namespace rew

@@ -1017,7 +1017,7 @@ def embedding(weight: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
     An id outside [0, vocab) (padding: -1) gives zeros, unlike ``torchIndexSelect``, which
     clamps it."""
     op = "embedding"
-    if len(weight.shape) != 2:
+    if len(weight.shape) != 2 or weight.shape[0] < 1:
         raise TensorError(f"{op}: weight must be [vocab, embed], got {list(weight.shape)}")
     _check_rows(op, weight)
     _check_ids(op, ids, weight.shape[1])
