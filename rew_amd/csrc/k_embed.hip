@@ -63,16 +63,14 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedArgs a) {
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSortRows = 512, kSortBits = 9;  // rows of the table per workgroup
 
-// A row of more than part_tokens tokens is "long": it is summed in parts of so many
-// places of the order, at most about a thousand of them.
-int64_t part_tokens(int64_t T) {
-  return std::max<int64_t>(128, ((T + 1023) / 1024 + 127) & ~(int64_t)127);
-}
-constexpr int kFew = 8;  // a row of more tokens is summed by the whole workgroup
+// A row of more than kFew tokens is summed by the workgroups of the windows of
+// kWindow places of the order that it touches.
+constexpr int kFew = 8, kWindow = 64;
+int64_t windows_of(int64_t T) { return T > kFew ? (T + kWindow - 1) / kWindow : 0; }
 
 struct GradWork {
   int32_t *first, *order;  // [V + 1]: a row's first place in order; [T]: tokens by row
-  float* part;             // [parts][2][E]
+  float* part;             // [windows][2][E]
 };
 __host__ __device__ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 GradWork grad_work(const EmbedGradArgs& a) {
@@ -204,144 +202,130 @@ __device__ __forceinline__ void sum_places(const EmbedGradArgs& a, const int32_t
   constexpr int kAhead = 8;  // rows under way
 #pragma unroll
   for (int x = 0; x < N; ++x) s[x] = 0.0f;
-  int32_t p = p0;
-  for (; p + kAhead <= p1; p += kAhead) {
+  for (int32_t p = p0; p < p1; p += kAhead) {
     RowRun<T, N> r[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      r[i] = run_at<T, N>(a.grad, (int64_t)order[p + i] * a.E + c);
+      r[i] = run_at<T, N>(a.grad, (int64_t)order[min(p + i, p1 - 1)] * a.E + c);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-      for (int x = 0; x < N; ++x) s[x] += T::get(r[i].v[x]);
-  }
-  for (; p < p1; ++p) {
-    const RowRun<T, N> r = run_at<T, N>(a.grad, (int64_t)order[p] * a.E + c);
-#pragma unroll
-    for (int x = 0; x < N; ++x) s[x] += T::get(r.v[x]);
+      for (int x = 0; x < N; ++x) s[x] += p + i < p1 ? T::get(r[i].v[x]) : 0.0f;
   }
 }
 
-// The same by the whole workgroup, its groups of `lanes` threads a share of the
-// places each, joined in order; the first group's threads have the sum.
-template <class T, int N>
-__device__ __forceinline__ void sum_together(const EmbedGradArgs& a, const int32_t* order,
-                                             int32_t p0, int32_t p1, int64_t c, int lanes,
-                                             float (*tmp)[N], float (&s)[N]) {
-  const int groups = kThreads / lanes, own = threadIdx.x / lanes;
-  const int32_t n = p1 - p0, per = (n + groups - 1) / groups;
-  sum_places<T, N>(a, order, p0 + min(own * per, n), p0 + min(own * per + per, n), c, s);
-#pragma unroll
-  for (int x = 0; x < N; ++x) tmp[threadIdx.x][x] = s[x];
-  __syncthreads();
-  if (own == 0)
-    for (int i = 1; i < groups; ++i)
-#pragma unroll
-      for (int x = 0; x < N; ++x) s[x] += tmp[i * lanes + threadIdx.x][x];
-  __syncthreads();
-}
-
-// The long rows that places [j part, j part + part) of the order touch: at most
-// the row of the first place (side 0) and that of the last (side 1, where it is
-// another one), since a row between them has fewer than `part` tokens.
-struct LongRow {
-  int64_t row = -1;
-  int32_t p0, p1;  // its places
-};
-__device__ __forceinline__ LongRow long_row(const EmbedGradArgs& a, const GradWork& w, int32_t p,
-                                            int64_t part) {
-  LongRow l;
-  const int64_t v = a.ids[w.order[p]];
-  l.p0 = w.first[v];
-  l.p1 = w.first[v + 1];
-  if (l.p1 - l.p0 > part) l.row = v;
-  return l;
-}
-
-// Workgroups before `part_blocks`: one slab of columns of one part's long rows,
-// float32.  The others: `rows` rows of the table each, by groups of `lanes` threads;
-// zeros for a row without tokens.  A row of more than kFew tokens is left to the
-// whole workgroup, a long one to its parts.
-template <class T, int N>
+// Workgroups before `window_blocks`: one slab of columns of the rows of more than
+// kFew tokens in a window of the order; a row that lies in the window alone is
+// finished, of another the sum goes to part[window][side], side 1 if it begins here.
+// The others: `rows` rows of the table each, by groups of `lanes` threads; zeros for a
+// row without tokens.  Both in one launch: the long sums hide behind the table's zeros.
+template <class T, int N, int S>
 __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, GradWork w,
-                                                             int64_t part, uint32_t part_blocks,
-                                                             int lanes, int rows) {
-  __shared__ float tmp[kThreads][N];
+                                                             uint32_t window_blocks, int lanes,
+                                                             int rows) {
   __shared__ int32_t first[kThreads + 1];
   const int lane = threadIdx.x % lanes, own = threadIdx.x / lanes, groups = kThreads / lanes;
-  const int slab = lanes * N;  // columns
-  if (blockIdx.x < part_blocks) {
-    const uint32_t slabs = (uint32_t)((a.E + slab - 1) / slab);
-    const int64_t j = blockIdx.x / slabs;
-    const int64_t c = run_start((int64_t)(blockIdx.x % slabs) * slab + lane * N, a.E, N);
-    const int32_t n = w.first[a.V];
-    if (j * part >= n) return;
-    const int32_t q0 = (int32_t)(j * part), q1 = (int32_t)min(j * part + part, (int64_t)n);
-    for (int side = 0; side < 2; ++side) {
-      const LongRow l = long_row(a, w, side ? q1 - 1 : q0, part);
-      if (l.row < 0 || (side && l.p0 <= q0)) continue;
-      float s[N];
-      sum_together<T, N>(a, w.order, max(l.p0, q0), min(l.p1, q1), c, lanes, tmp, s);
-      if (own == 0)
-#pragma unroll
-        for (int x = 0; x < N; ++x)
-          w.part[(j * 2 + side) * a.E + c + x] = s[x];
-    }
-    return;
-  }
-  const int64_t v0 = (int64_t)(blockIdx.x - part_blocks) * rows;
-  const int here = (int)min((int64_t)rows, a.V - v0);
-  for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
-  __syncthreads();
+  const int64_t slab = (int64_t)lanes * N;  // columns
   auto store = [&](int64_t v, int64_t c, float (&s)[N]) {
 #pragma unroll
     for (int x = 0; x < N; ++x) s[x] *= a.scale;
     run_store<T, N>(a.out, v * a.E + c, s);
   };
+  if (blockIdx.x < window_blocks) {
+    __shared__ float tmp[kThreads][N];
+    __shared__ int32_t row_of[kWindow];
+    __shared__ int n_rows;
+    const uint32_t slabs = (uint32_t)((a.E + slab - 1) / slab);
+    const int64_t j = blockIdx.x / slabs;
+    const int64_t c = run_start((int64_t)(blockIdx.x % slabs) * slab + lane * N, a.E, N);
+    const int32_t n = w.first[a.V];
+    const int64_t q = j * kWindow;
+    if (q >= n) return;
+    const int32_t q0 = (int32_t)q, q1 = (int32_t)min(q + kWindow, (int64_t)n);
+    if (threadIdx.x < 64) {
+      const int32_t p = min(q0 + (int32_t)threadIdx.x, q1 - 1);
+      const int32_t v = a.ids[w.order[p]];
+      const int32_t p0 = w.first[v], p1 = w.first[v + 1];
+      const bool mine = q0 + (int32_t)threadIdx.x < q1 && p1 - p0 > kFew && p == max(p0, q0);
+      const uint64_t all = __ballot(mine);
+      if (mine) row_of[__popcll(all & ((1ull << threadIdx.x) - 1))] = v;
+      if (threadIdx.x == 0) n_rows = __popcll(all);
+    }
+    __syncthreads();
+    for (int i = 0; i < n_rows; ++i) {
+      const int32_t v = row_of[i], p0 = w.first[v], p1 = w.first[v + 1];
+      const int32_t b = max(p0, q0), e = min(p1, q1), per = (e - b + groups - 1) / groups;
+      // the groups a share of the places each, joined in order
+      float s[N];
+      sum_places<T, N>(a, w.order, min(b + own * per, e), min(b + own * per + per, e), c, s);
+#pragma unroll
+      for (int x = 0; x < N; ++x) tmp[threadIdx.x][x] = s[x];
+      __syncthreads();
+      if (own == 0) {
+        for (int g = 1; g < groups; ++g)
+#pragma unroll
+          for (int x = 0; x < N; ++x) s[x] += tmp[g * lanes + threadIdx.x][x];
+        if (p0 >= q0 && p1 <= q1) {
+          store(v, c, s);
+        } else {
+          float* out = w.part + (j * 2 + (p0 >= q0)) * a.E + c;
+#pragma unroll
+          for (int x = 0; x < N; ++x) out[x] = s[x];
+        }
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  const int64_t v0 = (int64_t)(blockIdx.x - window_blocks) * rows;
+  const int here = (int)min((int64_t)rows, a.V - v0);
+  for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
+  __syncthreads();
   for (int r = own; r < here; r += groups) {
     const int32_t p0 = first[r], p1 = first[r + 1];
     if (p1 - p0 > kFew) continue;
-    if (p1 == p0) {
-      for (int64_t i = lane * N; i < a.E; i += slab) {
-        float zero[N] = {};
-        run_store<T, N, true>(a.out, (v0 + r) * a.E + run_start(i, a.E, N), zero);
+    // S slabs at a time: a row of one token is S loads under way
+    for (int64_t i = lane * N; i < a.E; i += S * slab) {
+      int64_t c[S];
+      float s[S][N];
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        c[k] = run_start(i + k * slab, a.E, N);
+#pragma unroll
+        for (int x = 0; x < N; ++x) s[k][x] = 0.0f;
       }
-      continue;
-    }
-    for (int64_t i = lane * N; i < a.E; i += slab) {
-      const int64_t c = run_start(i, a.E, N);
-      float s[N];
-      sum_places<T, N>(a, w.order, p0, p1, c, s);
-      store(v0 + r, c, s);
-    }
-  }
-  for (int r = 0; r < here; ++r) {
-    const int32_t p0 = first[r], p1 = first[r + 1];
-    if (p1 - p0 <= kFew || p1 - p0 > part) continue;
-    for (int64_t c0 = 0; c0 < a.E; c0 += slab) {
-      const int64_t c = run_start(c0 + lane * N, a.E, N);
-      float s[N];
-      sum_together<T, N>(a, w.order, p0, p1, c, lanes, tmp, s);
-      if (own == 0) store(v0 + r, c, s);
+      for (int32_t p = p0; p < p1; ++p) {
+        const int64_t row = (int64_t)w.order[p] * a.E;
+        RowRun<T, N> v[S];
+#pragma unroll
+        for (int k = 0; k < S; ++k) v[k] = run_at<T, N>(a.grad, row + c[k]);
+#pragma unroll
+        for (int k = 0; k < S; ++k)
+#pragma unroll
+          for (int x = 0; x < N; ++x) s[k][x] += T::get(v[k].v[x]);
+      }
+#pragma unroll
+      for (int k = 0; k < S; ++k)
+        if (i + k * slab < a.E) store(v0 + r, c[k], s[k]);
     }
   }
 }
 
-// The long row that begins in part j, from its parts in order.
+// The row that begins in window j and goes on behind it (its last place's, if any),
+// from its parts in order.
 template <class T>
-__global__ void __launch_bounds__(kThreads) embed_join_kernel(EmbedGradArgs a, GradWork w,
-                                                              int64_t part) {
+__global__ void __launch_bounds__(kThreads) embed_join_kernel(EmbedGradArgs a, GradWork w) {
   const int32_t n = w.first[a.V];
-  const int64_t j = blockIdx.x;
-  if (j * part >= n) return;
-  const int32_t q0 = (int32_t)(j * part), q1 = (int32_t)min(j * part + part, (int64_t)n);
-  const LongRow l = long_row(a, w, q1 - 1, part);
+  const int64_t j = blockIdx.x, q0 = j * kWindow, q1 = q0 + kWindow;
+  if (q1 >= n) return;
+  const int64_t v = a.ids[w.order[q1 - 1]];
+  const int32_t p0 = w.first[v], p1 = w.first[v + 1];
   const int64_t c = (int64_t)blockIdx.y * kThreads + threadIdx.x;
-  if (l.row < 0 || l.p0 < q0 || c >= a.E) return;
-  float s = w.part[(j * 2 + (l.p0 > q0)) * a.E + c];
+  if (p1 - p0 <= kFew || p0 < q0 || p1 <= q1 || c >= a.E) return;
+  float s = w.part[(j * 2 + 1) * a.E + c];
 #pragma unroll 8
-  for (int64_t i = j + 1; i < (l.p1 + part - 1) / part; ++i) s += w.part[i * 2 * a.E + c];
-  ((typename T::elem*)a.out)[l.row * a.E + c] = T::put(s * a.scale);
+  for (int64_t i = j + 1; i * kWindow < p1; ++i) s += w.part[i * 2 * a.E + c];
+  ((typename T::elem*)a.out)[v * a.E + c] = T::put(s * a.scale);
 }
 
 }  // namespace
@@ -358,14 +342,15 @@ void launch_embed(const EmbedArgs& a, hipStream_t stream) {
 }
 
 size_t embed_grad_ws_bytes(int64_t T, int64_t V, int64_t E) {
-  const int64_t part = part_tokens(T), parts = T > part ? (T + part - 1) / part : 0;
-  return up256((size_t)(V + 1) * 4) + up256((size_t)T * 4) + (size_t)parts * 2 * E * 4;
+  const int64_t windows = windows_of(T);
+  return up256((size_t)(V + 1) * 4) + up256((size_t)T * 4) +
+         (windows > 1 ? (size_t)windows * 2 * E * 4 : 0);
 }
 
 int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
   if (a.V * a.E == 0) return 0;
   const GradWork w = grad_work(a);
-  const int64_t part = part_tokens(a.T), parts = a.T > part ? (a.T + part - 1) / part : 0;
+  const int64_t windows = windows_of(a.T);
   hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)((a.V + kSortRows - 1) / kSortRows)),
                      dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w);
   by_run(a.dt, a.E, [&](auto t, auto n) {
@@ -379,16 +364,22 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
     while (rows > groups && a.V < (int64_t)rows * 1024) rows /= 2;
     rows = std::max(groups, rows / groups * groups);
     const int64_t slabs = (runs + lanes - 1) / lanes;
-    const int64_t blocks = parts * slabs + (a.V + rows - 1) / rows;
-    hipLaunchKernelGGL((embed_sum_kernel<Ty, N>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
-                       a, w, part, (uint32_t)(parts * slabs), lanes, rows);
-    if (parts == 0) return;
+    const int64_t blocks = windows * slabs + (a.V + rows - 1) / rows;
+    auto sum = [&](auto together) {
+      hipLaunchKernelGGL((embed_sum_kernel<Ty, N, decltype(together)::value>),
+                         dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, w,
+                         (uint32_t)(windows * slabs), lanes, rows);
+    };
+    if (slabs >= 4) sum(std::integral_constant<int, 4>());
+    else if (slabs >= 2) sum(std::integral_constant<int, 2>());
+    else sum(std::integral_constant<int, 1>());
+    if (windows <= 1) return;
     hipLaunchKernelGGL((embed_join_kernel<Ty>),
-                       dim3((unsigned)parts, (unsigned)((a.E + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, a, w, part);
+                       dim3((unsigned)windows, (unsigned)((a.E + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, a, w);
   });
   REW_HIP(hipGetLastError());
-  return parts ? 3 : 2;
+  return windows > 1 ? 3 : 2;
 }
 
 }  // namespace rew

@@ -55,21 +55,12 @@ __device__ __forceinline__ void run_load(const void* base, int64_t i, float (&f)
   for (int x = 0; x < N; ++x) f[x] = T::get(r.v[x]);
 }
 
-// Past: nontemporal, for a large result that the caches need not keep.
-template <class T, int N, bool Past = false>
+template <class T, int N>
 __device__ __forceinline__ void run_store(void* base, int64_t i, const float (&f)[N]) {
   RowRun<T, N> r;
 #pragma unroll
   for (int x = 0; x < N; ++x) r.v[x] = T::put(f[x]);
-  RowRun<T, N>* p = (RowRun<T, N>*)((typename T::elem*)base + i);
-  if constexpr (Past && sizeof r == 16) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
-    u32x4 v;
-    __builtin_memcpy(&v, &r, 16);
-    __builtin_nontemporal_store(v, (u32x4*)p);
-  } else {
-    *p = r;
-  }
+  *(RowRun<T, N>*)((typename T::elem*)base + i) = r;
 }
 
 }  // namespace rew

@@ -11,7 +11,9 @@ format, so the native backend sees exactly what rew would send it:
 """
 from __future__ import annotations
 
+from ctypes import c_float
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import NamedTuple, Sequence
 
 import numpy as np
@@ -990,9 +992,9 @@ def pagedAttention(q: Tensor, kPages: Tensor, vPages: Tensor, blockTable: Tensor
 _ROW_DTYPES = (DType.FLOAT32, DType.BFLOAT16, DType.FLOAT16)
 
 
+@lru_cache(maxsize=256)
 def _float_attr(op: str, name: str, value: float, positive: bool = False) -> tuple:
-    with np.errstate(over="ignore", under="ignore"):
-        v = float(np.float32(value))
+    v = c_float(value).value  # (rounded to float32, to infinity past its range)
     if not abs(v) < float("inf") or positive and not v > 0.0:
         raise TensorError(f"{op}: {name} must be a {'positive' if positive else 'finite'} "
                           f"float32, got {value}")
@@ -1057,7 +1059,7 @@ def _check_norm(op: str, x: Tensor, gamma: Tensor) -> tuple:
     if len(gamma.shape) < 1 or lead < 0 or x.shape[lead:] != gamma.shape:
         raise TensorError(f"{op}: gamma {list(gamma.shape)} must be the last dims of x "
                           f"{list(x.shape)}")
-    if gamma.numElements < 1:
+    if 0 in gamma.shape:
         raise TensorError(f"{op}: rows must have at least one value")
     return x.shape[:lead]
 
