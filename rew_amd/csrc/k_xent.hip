@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_device.h"
 #include "kernels.h"
@@ -559,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
 // reads LDS of its own; the waves' sums are joined in LDS.  For products of few
 // 256 x 256 tiles, whose k-steps would follow one another on a few CUs.
 template <class Ty, bool AKC, bool BKC, int MODE>
-__global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
-  __shared__ __attribute__((aligned(1024))) uint8_t L[8][2 * kSmallHalf];
+__device__ __forceinline__ void small_product(const Product& g, uint32_t bid, float scale,
+                                              uint8_t (*L)[2 * kSmallHalf]) {
   typedef typename Ty::frag frag;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -568,16 +569,16 @@ __global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
 
   int tm, tn, split = 0, nk = (int)(g.K / BK), k_first = 0;
   if constexpr (MODE == kStats) {
-    tile_at(blockIdx.x, g.tiles_m, g.splits, &tm, &split);
+    tile_at(bid, g.tiles_m, g.splits, &tm, &split);
     tn = split * g.per;
   } else if constexpr (MODE == kSum) {
     const uint32_t tiles = g.tiles_m * g.tiles_n;
-    split = blockIdx.x / tiles;
-    tile_at(blockIdx.x - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
+    split = bid / tiles;
+    tile_at(bid - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
     k_first = split * g.per;
     nk = min(g.per, nk - k_first);
   } else {
-    tile_at(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
+    tile_at(bid, g.tiles_m, g.tiles_n, &tm, &tn);
   }
   const int64_t m0 = (int64_t)tm * SM;
   const int tn_end = MODE == kStats ? min(tn + g.per, g.tiles_n) : tn + 1;
@@ -598,11 +599,11 @@ __global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
   }
   if constexpr (MODE == kDz) {
     d.load(g, row);
-    f = d.factor(g.scale[0]);
+    f = d.factor(scale);
   }
   bool alive = true;
   if constexpr (MODE == kOut) {
-    gain = g.scale[0] / kDzScale;
+    gain = scale / kDzScale;
     if (g.target) alive = row < g.M && g.target[row] >= 0 && g.target[row] < g.V;
   }
 
@@ -720,6 +721,93 @@ __global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
   }
 }
 
+// The largest finite |grad| of a token with a target, 1 if none is above 0; in every
+// thread.
+template <int Threads>
+__device__ __forceinline__ float largest_grad(const int32_t* target, const float* grad, int64_t T,
+                                              int64_t V, float* tmp) {
+  float m = 0.0f;
+  for (int64_t t = threadIdx.x; t < T; t += Threads) {
+    const float f = fabsf(grad[t]);
+    if (target[t] >= 0 && target[t] < V && f < INFINITY) m = fmaxf(m, f);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Threads / 64; ++i) m = fmaxf(m, tmp[i]);
+  __syncthreads();
+  return m > 0.0f ? m : 1.0f;
+}
+
+// x with zeros in rows without a target (`all`: every row as it is), in rows behind T
+// and columns behind H: 16 bytes from every `step`-th thread.
+struct Copy {
+  const uint16_t* x;
+  const int32_t* target;
+  uint16_t* out;
+  int64_t T, H, V, Tp, Hp, ld;
+  int all;
+};
+__device__ __forceinline__ void copy_x(const Copy& c, int64_t first, int64_t step) {
+  const int64_t per = c.Hp / 8, total = c.Tp * per;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t r = total >> 32 ? i / per : (int64_t)((uint32_t)i / (uint32_t)per);
+    const int64_t k = (i - r * per) * 8;
+    const bool live = r < c.T && (c.all || (c.target[r] >= 0 && c.target[r] < c.V));
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (live) {
+      const uint16_t* p = c.x + r * c.H + k;
+      if (k + 8 <= c.H) {
+        const Loose16 h = *(const Loose16*)p;
+        v = make_uint4(h.v[0], h.v[1], h.v[2], h.v[3]);
+      } else {
+        uint16_t* h = (uint16_t*)&v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k + e < c.H) h[e] = p[e];
+      }
+    }
+    *(uint4*)(c.out + r * c.ld + k) = v;
+  }
+}
+
+template <class Ty, bool AKC, bool BKC, int MODE>
+__global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
+  __shared__ __attribute__((aligned(1024))) uint8_t L[8][2 * kSmallHalf];
+  small_product<Ty, AKC, BKC, MODE>(g, blockIdx.x, MODE == kDz || MODE == kOut ? g.scale[0] : 1.0f,
+                                    L);
+}
+
+// The small form's first launch of a gradient where x needs no copy for dz: dz from x
+// as it is (its rows without a target are zeros whatever x holds), the largest gradient
+// by each workgroup itself, and the copy that dw reads by the workgroups behind
+// `tiles`.  A launch less.
+template <class Ty, bool BKC>
+__global__ void __launch_bounds__(kThreads, 1) xent_first_kernel(Product g, Copy c, uint32_t tiles,
+                                                                 float* scale) {
+  __shared__ __attribute__((aligned(1024))) uint8_t L[8][2 * kSmallHalf];
+  if (blockIdx.x >= tiles) {
+    copy_x(c, (int64_t)(blockIdx.x - tiles) * kThreads + threadIdx.x,
+           (int64_t)(gridDim.x - tiles) * kThreads);
+    return;
+  }
+  const float m = largest_grad<kThreads>(g.target, g.grad, g.M, g.V, (float*)L);
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = m;
+  small_product<Ty, true, BKC, kDz>(g, blockIdx.x, m, L);
+}
+
+// dw and dx in one launch: `tiles` workgroups for dw, the others for dx.
+template <class Ty, bool TIED, int MW, int MX>
+__global__ void __launch_bounds__(kThreads, 1) xent_pair_kernel(Product w, Product x,
+                                                                uint32_t tiles) {
+  __shared__ __attribute__((aligned(1024))) uint8_t L[8][2 * kSmallHalf];
+  const float scale = w.scale[0];
+  if (blockIdx.x < tiles) small_product<Ty, false, false, MW>(w, blockIdx.x, scale, L);
+  else small_product<Ty, true, !TIED, MX>(x, blockIdx.x - tiles, scale, L);
+}
+
 // lse and loss of every row from its `slots` partial results: 256 / rows threads
 // a row, joined in order.
 __global__ void __launch_bounds__(256) xent_join_kernel(XentArgs a, const float2* part,
@@ -748,52 +836,18 @@ __global__ void __launch_bounds__(256) xent_join_kernel(XentArgs a, const float2
   if (a.lse) a.lse[row] = lse;
 }
 
-// Block 0: the largest finite |grad| of a row with a target (1 if there is none
-// above 0).  The others: x with zeros in rows without a target, in rows behind T
-// and columns behind H.
-__global__ void __launch_bounds__(1024) xent_prepare_kernel(const uint16_t* x,
-                                                            const int32_t* target,
-                                                            const float* grad, int64_t T,
-                                                            int64_t H, int64_t V, int64_t Tp,
-                                                            int64_t Hp, int64_t ld, uint16_t* out,
+// Block 0 (scale set): the largest gradient.  The others: the copy of x.
+__global__ void __launch_bounds__(1024) xent_prepare_kernel(Copy c, const float* grad,
                                                             float* scale) {
-  if (grad && blockIdx.x == 0) {
-    __shared__ float tmp[16];
-    float m = 0.0f;
-    for (int64_t t = threadIdx.x; t < T; t += 1024) {
-      const float f = fabsf(grad[t]);
-      if (target[t] >= 0 && target[t] < V && f < INFINITY) m = fmaxf(m, f);
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 16; ++i) m = fmaxf(m, tmp[i]);
-      scale[0] = m > 0.0f ? m : 1.0f;
-    }
+  __shared__ float tmp[16];
+  const int first = scale ? 1 : 0;
+  if (scale && blockIdx.x == 0) {
+    const float m = largest_grad<1024>(c.target, grad, c.T, c.V, tmp);
+    if (threadIdx.x == 0) scale[0] = m;
     return;
   }
-  const int64_t first = grad ? 1 : 0;
-  const int64_t per = Hp / 8, total = Tp * per;
-  for (int64_t i = (blockIdx.x - first) * 1024 + threadIdx.x; i < total;
-       i += (gridDim.x - first) * 1024) {
-    const int64_t r = i / per, c = (i - r * per) * 8;
-    // (without gradients every row is taken as it is)
-    const bool live = r < T && (!grad || (target[r] >= 0 && target[r] < V));
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (live) {
-      if (H % 8 == 0) {
-        if (c < H) v = *(const uint4*)(x + r * H + c);
-      } else {
-        uint16_t h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = c + e < H ? x[r * H + c + e] : (uint16_t)0;
-        __builtin_memcpy(&v, h, 16);
-      }
-    }
-    *(uint4*)(out + r * ld + c) = v;
-  }
+  copy_x(c, (int64_t)(blockIdx.x - first) * 1024 + threadIdx.x,
+         (int64_t)(gridDim.x - first) * 1024);
 }
 
 // A [rows, cols] window of w (row pitch ld) as [rows, pitch] with zeros behind cols.
@@ -863,6 +917,7 @@ __global__ void __launch_bounds__(256) xent_round_kernel(const float* sums, int6
 // ---- plans (sizes alone) --------------------------------------------------------------
 
 constexpr int64_t kCus = 256;
+constexpr int64_t kFirstTokens = 2048;  // whose gradients each workgroup looks through itself
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 int64_t cdiv(int64_t n, int64_t m) { return (n + m - 1) / m; }
 
@@ -993,6 +1048,35 @@ void launch_product(Product g, const Cut& c, hipStream_t stream) {
   REW_HIP(hipGetLastError());
 }
 
+// dw and dx of small cuts.
+template <class Ty>
+void launch_pair(Product w, Product x, const XentPlan& p, int tied, hipStream_t stream) {
+  for (Product* g : {&w, &x}) {
+    g->tiles_m = (int)cdiv(g->M, SM);
+    g->tiles_n = (int)cdiv(g->N, SM);
+  }
+  w.per = (int)p.dw.per;
+  x.per = (int)p.dx.per;
+  const int64_t nw = (int64_t)w.tiles_m * w.tiles_n * (p.dw.splits > 1 ? w.splits : 1);
+  const int64_t nx = (int64_t)x.tiles_m * x.tiles_n * (p.dx_sums ? x.splits : 1);
+  auto launch = [&](auto t, auto mw, auto mx) {
+    hipLaunchKernelGGL(
+        (xent_pair_kernel<Ty, decltype(t)::value, decltype(mw)::value, decltype(mx)::value>),
+        dim3((unsigned)(nw + nx)), dim3(kThreads), 0, stream, w, x, (uint32_t)nw);
+  };
+  auto by_x = [&](auto t, auto mw) {
+    if (p.dx_sums) launch(t, mw, std::integral_constant<int, kSum>());
+    else launch(t, mw, std::integral_constant<int, kOut>());
+  };
+  auto by_w = [&](auto t) {
+    if (p.dw.splits > 1) by_x(t, std::integral_constant<int, kSum>());
+    else by_x(t, std::integral_constant<int, kOut>());
+  };
+  if (tied) by_w(std::true_type());
+  else by_w(std::false_type());
+  REW_HIP(hipGetLastError());
+}
+
 template <class Ty>
 void launch_round(const float* sums, int64_t rows, int64_t cols, int64_t splits,
                   const float* scale, const int32_t* target, int64_t V, void* out, int64_t ldo,
@@ -1034,10 +1118,10 @@ int run_xent(const XentArgs& a, hipStream_t stream) {
   g.a = {(const uint16_t*)a.x, a.H, a.T * a.H, a.H};
   if (p.copy_x) {
     uint16_t* x = (uint16_t*)(work + p.x);
+    const Copy c = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 1};
     const int64_t blocks = std::min<int64_t>(cdiv(p.Tp * p.Hp / 8, 1024), kCus * 4);
-    hipLaunchKernelGGL(xent_prepare_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream,
-                       (const uint16_t*)a.x, a.target, (const float*)nullptr, a.T, a.H, a.V, p.Tp,
-                       p.Hp, p.ldx, x, (float*)nullptr);
+    hipLaunchKernelGGL(xent_prepare_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream, c,
+                       (const float*)nullptr, (float*)nullptr);
     REW_HIP(hipGetLastError());
     ++launches;
     g.a = {x, p.ldx, p.Tp * p.ldx, p.Hp};
@@ -1076,12 +1160,16 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
   uint16_t* x = (uint16_t*)(work + p.x);
   uint16_t* dz = (uint16_t*)(work + p.dz);
   float* scale = (float*)(work + p.scale);
-  const int64_t blocks = 1 + std::min<int64_t>(cdiv(p.Tp * p.Hp / 8, 1024), kCus * 4);
-  hipLaunchKernelGGL(xent_prepare_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream,
-                     (const uint16_t*)a.x, a.target, a.grad, a.T, a.H, a.V, p.Tp, p.Hp,
-                     p.ldx, x, scale);
-  REW_HIP(hipGetLastError());
-  ++launches;
+  const Copy copy = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 0};
+  const bool first = a.T && p.z.small && p.pieces == 1 && !p.pack_w && a.H % BK == 0 &&
+                     a.T <= kFirstTokens;
+  if (!first) {
+    const int64_t blocks = 1 + std::min<int64_t>(cdiv(p.Tp * p.Hp / 8, 1024), kCus * 4);
+    hipLaunchKernelGGL(xent_prepare_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream, copy,
+                       a.grad, scale);
+    REW_HIP(hipGetLastError());
+    ++launches;
+  }
   const Opnd xk = {x, p.ldx, p.Tp * p.ldx, p.Hp};   // k = embed
   const Opnd xt = {x, p.ldx, p.Tp * p.ldx, p.Tp};   // k = tokens
   for (int64_t i = 0; i < p.pieces; ++i) {
@@ -1106,12 +1194,30 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
       d.out = dz;
       d.ldo = p.ldz;
       d.rows_out = p.Tp;
-      if (a.tied) launch_product<Ty, true, true, kDz>(d, p.z, stream);
-      else launch_product<Ty, true, false, kDz>(d, p.z, stream);
+      if (first) {
+        d.a = {(const uint16_t*)a.x, a.H, a.T * a.H, a.H};
+        d.tiles_m = (int)p.z.tiles_m;
+        d.tiles_n = (int)p.z.tiles_n;
+        const uint32_t tiles = (uint32_t)(d.tiles_m * d.tiles_n);
+        const uint32_t blocks =
+            tiles + (uint32_t)std::min<int64_t>(cdiv(p.Tp * p.Hp / 8, kThreads), kCus);
+        if (a.tied)
+          hipLaunchKernelGGL((xent_first_kernel<Ty, true>), dim3(blocks), dim3(kThreads), 0, stream,
+                             d, copy, tiles, scale);
+        else
+          hipLaunchKernelGGL((xent_first_kernel<Ty, false>), dim3(blocks), dim3(kThreads), 0,
+                             stream, d, copy, tiles, scale);
+        REW_HIP(hipGetLastError());
+      } else if (a.tied) {
+        launch_product<Ty, true, true, kDz>(d, p.z, stream);
+      } else {
+        launch_product<Ty, true, false, kDz>(d, p.z, stream);
+      }
       ++launches;
     }
+    Product dw = g;
     {
-      Product d = g;
+      Product& d = dw;
       const Opnd dzt = {dz, p.ldz, p.Tp * p.ldz, p.Tp};
       d.a = a.tied ? dzt : xt;
       d.b = a.tied ? xt : dzt;
@@ -1121,40 +1227,45 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
       d.out = (uint16_t*)a.dw + (a.tied ? v0 * a.H : v0);
       d.ldo = a.tied ? a.H : a.V;
       d.splits = (int)p.dw.splits;
-      if (d.splits > 1) {
-        float* sums = (float*)(work + p.dw_sums);
-        void* out = d.out;
-        d.out = sums;
-        launch_product<Ty, false, false, kSum>(d, p.dw, stream);
-        launch_round<Ty>(sums, d.M, d.N, d.splits, scale, nullptr, 1, out, d.ldo, stream);
+    }
+    const bool dw_sums = dw.splits > 1;
+    void* dw_out = dw.out;
+    if (dw_sums) dw.out = work + p.dw_sums;
+    Product dx = g;
+    if (a.T) {
+      Product& d = dx;
+      d.K = up(n, BK);
+      d.a = {dz, p.ldz, p.Tp * p.ldz, d.K};
+      // (a packed piece has zeros behind n; else the rows' or columns' end is w's own)
+      d.b = {w.p, w.ld, w.len, a.tied ? n : p.pack_w ? d.K : n};
+      d.M = d.rows_out = a.T;
+      d.N = a.H;
+      d.splits = (int)cdiv(d.K / BK, p.dx.per);  // (the first piece has the most)
+      d.add = i > 0;
+      d.out = p.dx_sums ? (void*)(work + p.sums) : a.dx;
+      d.ldo = a.H;
+      d.target = p.dx_sums ? nullptr : a.target;
+    }
+    if (a.T && p.dw.small && p.dx.small) {
+      launch_pair<Ty>(dw, dx, p, a.tied, stream);
+      ++launches;
+    } else {
+      if (dw_sums) launch_product<Ty, false, false, kSum>(dw, p.dw, stream);
+      else launch_product<Ty, false, false, kOut>(dw, p.dw, stream);
+      ++launches;
+      if (a.T) {
+        if (p.dx_sums && a.tied) launch_product<Ty, true, false, kSum>(dx, p.dx, stream);
+        else if (p.dx_sums) launch_product<Ty, true, true, kSum>(dx, p.dx, stream);
+        else if (a.tied) launch_product<Ty, true, false, kOut>(dx, p.dx, stream);
+        else launch_product<Ty, true, true, kOut>(dx, p.dx, stream);
         ++launches;
-      } else {
-        launch_product<Ty, false, false, kOut>(d, p.dw, stream);
       }
+    }
+    if (dw_sums) {
+      launch_round<Ty>((const float*)dw.out, dw.M, dw.N, dw.splits, scale, nullptr, 1, dw_out,
+                       dw.ldo, stream);
       ++launches;
     }
-    if (!a.T) continue;
-    Product d = g;
-    d.K = up(n, BK);
-    d.a = {dz, p.ldz, p.Tp * p.ldz, d.K};
-    // (a packed piece has zeros behind n; else the rows' or columns' end is w's own)
-    d.b = {w.p, w.ld, w.len, a.tied ? n : p.pack_w ? d.K : n};
-    d.M = d.rows_out = a.T;
-    d.N = a.H;
-    d.splits = (int)cdiv(d.K / BK, p.dx.per);  // (the first piece has the most)
-    d.add = i > 0;
-    if (p.dx_sums) {
-      d.out = work + p.sums;
-      if (a.tied) launch_product<Ty, true, false, kSum>(d, p.dx, stream);
-      else launch_product<Ty, true, true, kSum>(d, p.dx, stream);
-    } else {
-      d.out = a.dx;
-      d.ldo = a.H;
-      d.target = a.target;
-      if (a.tied) launch_product<Ty, true, false, kOut>(d, p.dx, stream);
-      else launch_product<Ty, true, true, kOut>(d, p.dx, stream);
-    }
-    ++launches;
   }
   if (a.T && p.dx_sums) {
     launch_round<Ty>((const float*)(work + p.sums), a.T, a.H, p.dx.splits, scale, a.target, a.V,
