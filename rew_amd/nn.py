@@ -107,6 +107,15 @@ class LayerNorm:
         betaB = O.broadcastTo(self.beta, x.shape, red)
         return O.add(O.mul(gammaB, normalized), betaB)
 
+    def forwardTrain(self, x: Tensor):
+        """(y, stats) as one op, x float32, bfloat16 or float16 (``ops.layerNorm``): the
+        arithmetic of ``forward`` in float32, rounded once.  A backend extension."""
+        return O.layerNorm(x, self.gamma, self.beta, self.eps, withStats=True)
+
+    def grad(self, x: Tensor, stats: O.NormStats, gradOut: Tensor):
+        """(gradX, gradGamma, gradBeta) of ``forwardTrain`` (``ops.layerNormGrad``)."""
+        return O.layerNormGrad(x, self.gamma, stats, gradOut)
+
 
 @dataclass
 class RMSNorm:
@@ -446,6 +455,41 @@ class Embedding:
     def lookup(self, ids: Tensor) -> Tensor:
         """Row gather; equal to ``forward(one_hot(ids))`` (one nonzero product per sum)."""
         return O.torchIndexSelect(self.weight, ids, 0, 0)
+
+    # ---- training (backend extensions) ----
+
+    def rows(self, ids: Tensor, scale: float = 1.0) -> Tensor:
+        """scale times the rows of int32 ids, zeros for ids outside the table
+        (``ops.embedding``)."""
+        return O.embedding(self.weight, ids, scale)
+
+    def rowsGrad(self, ids: Tensor, gradOut: Tensor, scale: float = 1.0) -> Tensor:
+        """The weight's gradient of ``rows`` (``ops.embeddingGrad``)."""
+        return O.embeddingGrad(ids, gradOut, self.weight.shape[0], scale)
+
+    def loss(self, x: Tensor, targets: Tensor):
+        """(loss, lse) per token of the table as the output projection: the cross entropy
+        of x [tokens, embed] times its transpose (``ops.linearCrossEntropy``)."""
+        return O.linearCrossEntropy(x, self.weight, targets, tied=True, withLse=True)
+
+    def lossGrad(self, x: Tensor, targets: Tensor, lse: Tensor, gradLoss: Tensor):
+        """(gradX, gradWeight) of ``loss`` (``ops.linearCrossEntropyGrad``)."""
+        return O.linearCrossEntropyGrad(x, self.weight, targets, lse, gradLoss, tied=True)
+
+
+@dataclass
+class LossHead:
+    """An output projection without a bias under softmax cross entropy, its logits never
+    stored.  A backend extension."""
+    weight: Tensor  # [embed, vocab], as Linear's
+
+    def loss(self, x: Tensor, targets: Tensor):
+        """(loss, lse) per token (``ops.linearCrossEntropy``)."""
+        return O.linearCrossEntropy(x, self.weight, targets, withLse=True)
+
+    def lossGrad(self, x: Tensor, targets: Tensor, lse: Tensor, gradLoss: Tensor):
+        """(gradX, gradWeight) of ``loss`` (``ops.linearCrossEntropyGrad``)."""
+        return O.linearCrossEntropyGrad(x, self.weight, targets, lse, gradLoss)
 
 
 @dataclass
