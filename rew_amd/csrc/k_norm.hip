@@ -66,13 +66,36 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
   const int64_t n = a.n;
   const float inv = 1.0f / (float)n;
   const Runs<G, C, N> run(n, g);
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
+  // Wide rows: one or two workgroups fit a CU, so each has its next row on the way, and
+  // (up to 512 threads: the registers) keeps gamma and beta: read anew for every row
+  // they are twice the bytes of x and y in 16 bits (3000 x 10000: 40 us).
+  constexpr bool kAhead = G >= 256, kHold = G == 256 || G == 512;
+  float w[C][N], b[C][N];
+  if constexpr (kHold)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      run_load<P, N>(a.gamma, run.at[c], w[c]);
+      run_load<P, N>(a.beta, run.at[c], b[c]);
+    }
+  RowRun<T, N> next[C];
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  auto fetch = [&](int64_t r0) {
+    const int64_t base = min(r0 + threadIdx.x / G, a.rows - 1) * n;
+#pragma unroll
+    for (int c = 0; c < C; ++c) next[c] = run_at<T, N>(a.x, base + run.at[c]);
+  };
+  if (kAhead) fetch((int64_t)blockIdx.x * kRows);
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += step) {
     const int64_t row = r0 + threadIdx.x / G;
     const bool there = row < a.rows;
     const int64_t base = (there ? row : a.rows - 1) * n;
+    if (!kAhead) fetch(r0);
     float f[C][N];
 #pragma unroll
-    for (int c = 0; c < C; ++c) run_load<T, N>(a.x, base + run.at[c], f[c]);
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[c][e] = T::get(next[c].v[e]);
+    if (kAhead) fetch(r0 + step);
     float s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -98,11 +121,12 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (run.own[c] == N) continue;
-      float w[N], b[N];
-      run_load<P, N>(a.gamma, run.at[c], w);
-      run_load<P, N>(a.beta, run.at[c], b);
+      if constexpr (!kHold) {
+        run_load<P, N>(a.gamma, run.at[c], w[c]);
+        run_load<P, N>(a.beta, run.at[c], b[c]);
+      }
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[c][e] = f[c][e] * rstd * w[e] + b[e];
+      for (int e = 0; e < N; ++e) f[c][e] = f[c][e] * rstd * w[c][e] + b[c][e];
       run_store<T, N>(a.y, base + run.at[c], f[c]);
     }
   }
@@ -358,11 +382,12 @@ void by_types(int dt, int p_dt, int64_t n, F&& f) {
   else with(RowF16(), RowF16());
 }
 
-// f(group, runs of a thread) for a row of `runs` runs; false where it is longer than
-// `Most` runs in each of 1024 threads (0: a row of single values).
-template <int Most, class F>
+// f(group, runs of a thread) for a row of `runs` runs; false where it is too long: 4
+// runs in each of 1024 threads, or (gradients, which hold six values for each of x) in
+// each of 512.  Single: a row of fewer values than a run.
+template <bool Grad, bool Single, class F>
 bool by_group(int64_t runs, F&& f) {
-  if constexpr (Most == 0) {
+  if constexpr (Single) {
     f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     return true;
   } else {
@@ -373,12 +398,16 @@ bool by_group(int64_t runs, F&& f) {
     else if (runs <= 128) with(std::integral_constant<int, 64>(), two);
     else if (runs <= 256) with(std::integral_constant<int, 256>(), one);
     else if (runs <= 512) with(std::integral_constant<int, 256>(), two);
+    else if (runs <= 768)
+      with(std::integral_constant<int, 256>(), std::integral_constant<int, 3>());
     else if (runs <= 1024) with(std::integral_constant<int, 512>(), two);
-    else if (Most >= 2 && runs <= 2048)
-      with(std::integral_constant<int, 1024>(), std::integral_constant<int, Most >= 2 ? 2 : 1>());
-    else if (Most >= 4 && runs <= 4096)
-      with(std::integral_constant<int, 1024>(), std::integral_constant<int, Most >= 4 ? 4 : 1>());
-    else return false;
+    else if (runs <= 1536)
+      with(std::integral_constant<int, 512>(), std::integral_constant<int, 3>());
+    else if (runs <= 2048)
+      with(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+    else if (Grad || runs > 4096) return false;
+    else if constexpr (!Grad)
+      with(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
     return true;
   }
 }
@@ -396,10 +425,11 @@ void launch_norm(const NormArgs& a, hipStream_t stream) {
     typedef decltype(t) T;
     typedef decltype(p) P;
     constexpr int N = decltype(nn)::value;
-    const bool fits = by_group<N == 1 ? 0 : 4>((a.n + N - 1) / N, [&](auto g, auto c) {
+    const bool fits = by_group<false, N == 1>((a.n + N - 1) / N, [&](auto g, auto c) {
       constexpr int G = decltype(g)::value, C = decltype(c)::value;
       constexpr int rows = G > 256 ? 1 : 256 / G;
-      const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, kMaxBlocks);
+      const int64_t most = G == 1024 ? 256 : G == 512 ? 512 : G == 256 ? 1024 : kMaxBlocks;
+      const int64_t blocks = std::min((a.rows + rows - 1) / rows, most);
       hipLaunchKernelGGL((norm_kernel<T, P, N, G, C>), dim3((unsigned)blocks),
                          dim3(G > 256 ? G : 256), 0, stream, a);
     });
@@ -427,9 +457,7 @@ int launch_norm_grad(const NormGradArgs& a, hipStream_t stream) {
     constexpr int N = decltype(nn)::value;
     const int64_t runs = (a.n + N - 1) / N;
     int parts = 1;
-    // (16-bit rows of 2 runs in each of 1024 threads would spill)
-    constexpr int most = N == 1 ? 0 : N == 4 ? 2 : 1;
-    const bool fits = by_group<most>(runs, [&](auto g, auto c) {
+    const bool fits = by_group<true, N == 1>(runs, [&](auto g, auto c) {
       constexpr int G = decltype(g)::value, C = decltype(c)::value;
       constexpr int rows = grad_block(G) / G;
       parts = (int)std::max<int64_t>(1, std::min((a.rows + rows - 1) / rows, kParts));

@@ -994,8 +994,13 @@ XentPlan make_plan(int64_t T, int64_t H, int64_t V, int tied, bool grad) {
   p.Hp = up(H, BK);
   p.Tp = up(T, BK);
   p.piece = V;
-  if (grad) p.piece = std::max(kPiece, (int64_t)(1 << 25) / std::max<int64_t>(T, 1));
-  else if (p.pack_w) p.piece = kPiece;
+  if (grad) {
+    // dz of a piece: 2^25 values at least, 2^31 at most beyond 2^17 tokens
+    const int64_t t = std::max<int64_t>(T, 1);
+    p.piece = std::max(std::min(kPiece, ((int64_t)1 << 31) / t), ((int64_t)1 << 25) / t);
+    p.piece = std::max<int64_t>(p.piece, BN);
+  }
+  if (!grad && p.pack_w) p.piece = kPiece;
   p.piece = std::min(up(p.piece, BN), up(V, BN));
   p.pieces = cdiv(V, p.piece);
   // (rows a power of two apart would meet in the same channels of the L2)
