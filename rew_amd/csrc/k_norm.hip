@@ -406,8 +406,12 @@ bool by_group(int64_t runs, F&& f) {
     else if (runs <= 2048)
       with(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
     else if (Grad || runs > 4096) return false;
-    else if constexpr (!Grad)
-      with(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    else if constexpr (!Grad) {
+      if (runs <= 3072)
+        with(std::integral_constant<int, 1024>(), std::integral_constant<int, 3>());
+      else
+        with(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    }
     return true;
   }
 }

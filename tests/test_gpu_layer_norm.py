@@ -11,7 +11,7 @@ from rew_amd import ops as O
 TYPES = [("float32", "float32"), ("bfloat16", "float32"), ("bfloat16", "bfloat16"),
          ("float16", "float32"), ("float16", "float16")]
 WIDTHS = [1, 2, 3, 8, 63, 64, 250, 512, 520, 1001, 1024, 2048, 4096, 4104, 5001, 8192, 16384,
-          16385, 20000, 40008]
+          16385, 20000, 30001, 40008]
 
 
 def case(r, rows, n, dtype, ptype, shift=0.3):
