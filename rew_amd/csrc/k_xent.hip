@@ -82,12 +82,13 @@ __device__ __forceinline__ void tile_at(uint32_t bid, uint32_t tiles_m, uint32_t
 // KC: rows of 128 bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  Else rows
 // of one k and R r's, for the transposing fragment reads: chunk c of row k at
 // c ^ (4 (k & 3)) (R = 256) or c ^ (2 ((k >> 1) & 3)) (R = 64), so that the four
-// rows that a read touches lie in different banks.  Past `len` zeros arrive; a KC
-// chunk past k is another of its row's (the other operand is zero there).
+// rows that a read touches lie in different banks.  Past `len`, and past k in a KC
+// row, zeros arrive.
 template <bool KC, int R, int Q>
 struct Fetch {
   static constexpr int kRowChunks = KC ? BK / 8 : R / 8;
   static constexpr int kBlockRows = 64 / kRowChunks;
+  static constexpr uint32_t kPast = 0x80000000u;  // (behind any descriptor's end)
   const uint16_t* base;
   int64_t left;  // elements from base that may be read
   int64_t step;  // elements per k-step
@@ -119,7 +120,7 @@ struct Fetch {
     const uint32_t lim = (uint32_t)(min(left_k, (int64_t)BK) * 2 - 16);
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-      dma16_lds(r, KC ? off[q] + min(cols[KC ? q : 0], lim) : off[q], 0,
+      dma16_lds(r, !KC ? off[q] : cols[KC ? q : 0] <= lim ? off[q] + cols[KC ? q : 0] : kPast, 0,
                 (lds_void*)(lds + q * 1024));
   }
   __device__ __forceinline__ void next(int n = 1) {

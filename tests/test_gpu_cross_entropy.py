@@ -131,6 +131,30 @@ def test_infinite_logits(gpu):
     assert lse[0] == -np.inf
 
 
+@pytest.mark.parametrize("tied", [True, False])
+@pytest.mark.parametrize("H", [8, 72, 100, 320])
+@pytest.mark.parametrize("T,V", [(3, 56), (700, 6000)])
+def test_infinite_weights(gpu, tied, H, T, V):
+    """A word whose logit is -infinity takes no part, whatever the width of the rows; one of
+    +infinity makes lse infinite.  The logits of the others are zero: log(V - 1), to a few
+    roundings of a float32 sum of ones (exact) and its logarithm."""
+    w = np.zeros((V, H))
+    w[5] = -np.inf
+    x = tensor(np.ones((T, H)), "bfloat16")[0]
+    t = ints(np.arange(T) % 4)
+    wt = tensor(w if tied else w.T, "bfloat16")[0]
+    loss, lse = O.linearCrossEntropy(x, wt, t, tied=tied, withLse=True)
+    np.testing.assert_allclose(R.host(loss), np.log(V - 1), rtol=4 * 2.0 ** -24)
+    dw = R.host(O.linearCrossEntropyGrad(x, wt, t, lse, f32(np.ones(T)), tied=tied)[1])
+    dw = dw if tied else dw.T
+    assert np.isfinite(dw).all() and not dw[5].any()
+    w[5, 0] = np.inf
+    w[5, 1:] = 0.0
+    lse = O.linearCrossEntropy(x, tensor(w if tied else w.T, "bfloat16")[0], t, tied=tied,
+                               withLse=True)[1]
+    assert (R.host(lse) == np.inf).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [1e-30, 1e-4, 1.0, 1e20])
 def test_size_of_the_gradient(gpu, dtype, size):
