@@ -64,9 +64,21 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSortRows = 512, kSortBits = 9;  // rows of the table per workgroup
 
 // A row of more than kFew tokens is summed by the workgroups of the windows of
-// kWindow places of the order that it touches.
+// kWindow places of the order that it touches.  (16384 tokens of text, 128256 x 4096:
+// 64 instead of 8 takes 100 us more, 2 saves 5; 300 tokens, 1001 x 250 float32: 2 takes
+// 17 us for 11, 4 takes 14.)
 constexpr int kFew = 8, kWindow = 64;
 int64_t windows_of(int64_t T) { return T > kFew ? (T + kWindow - 1) / kWindow : 0; }
+
+// A large table of which most rows have no token is cleared as a whole beside the sort,
+// in the order of its addresses (6.3 TB/s; zeros stored row by row between the sums
+// come to 5.3), and the places of the order then write the rows that have tokens.
+// 16384 tokens, 4096 wide: 128256 rows 264 -> 235 us, 65537 rows 173 -> 157; tables of
+// 64 MB are the same either way, smaller ones 1 us slower.
+bool clear_first(int64_t T, int64_t V, int64_t bytes) {
+  return T <= V / 4 && bytes >= (int64_t)1 << 26;
+}
+constexpr int kPlaces = 8;  // of a workgroup (16: 5 us more)
 
 struct GradWork {
   int32_t *first, *order;  // [V + 1]: a row's first place in order; [T]: tokens by row
@@ -89,13 +101,23 @@ GradWork grad_work(const EmbedGradArgs& a) {
 // not show), and, once all counts are summed, walks it again and puts each
 // token behind those of the same row before it.  Reading all ids in each of
 // V / 512 workgroups costs less than the several launches of a sort by digits.
+// The workgroups behind them clear `bytes` of `out`, 16 by each thread.
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t* ids, int64_t T,
-                                                                  int64_t V, GradWork w) {
+                                                                  int64_t V, GradWork w,
+                                                                  uint8_t* out, int64_t bytes) {
   __shared__ int32_t cnt[kSortWaves][kSortRows];
   __shared__ int32_t tmp[kSortWaves];
   constexpr int kAhead = 8;       // loads under way
-  constexpr int kOneByOne = 8;    // tokens of 64
+  constexpr int kOneByOne = 8;    // tokens of 64 (0, all rows at once always: 22 us for 15)
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t sorts = (uint32_t)((V + kSortRows - 1) / kSortRows);
+  if (blockIdx.x >= sorts) {
+    const int64_t at = ((int64_t)(blockIdx.x - sorts) * kSortThreads + tid) * 16;
+    if (at + 16 <= bytes) *(uint4*)(out + at) = make_uint4(0, 0, 0, 0);
+    else
+      for (int64_t i = at; i < bytes; i += 2) *(uint16_t*)(out + i) = 0;
+    return;
+  }
   const int64_t lo = (int64_t)blockIdx.x * kSortRows;
   const int rows = (int)min((int64_t)kSortRows, V - lo);
   const int64_t per = ((T + kSortWaves - 1) / kSortWaves + 63) & ~(int64_t)63;
@@ -219,6 +241,7 @@ __device__ __forceinline__ void sum_places(const EmbedGradArgs& a, const int32_t
 // finished, of another the sum goes to part[window][side], side 1 if it begins here.
 // The others: `rows` rows of the table each, by groups of `lanes` threads; zeros for a
 // row without tokens.  Both in one launch: the long sums hide behind the table's zeros.
+// Or, rows 0 (a cleared table), the rows that begin in kPlaces places of the order each.
 template <class T, int N, int S>
 __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, GradWork w,
                                                              uint32_t window_blocks, int lanes,
@@ -277,13 +300,7 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
     }
     return;
   }
-  const int64_t v0 = (int64_t)(blockIdx.x - window_blocks) * rows;
-  const int here = (int)min((int64_t)rows, a.V - v0);
-  for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
-  __syncthreads();
-  for (int r = own; r < here; r += groups) {
-    const int32_t p0 = first[r], p1 = first[r + 1];
-    if (p1 - p0 > kFew) continue;
+  auto sum_row = [&](int64_t v, int32_t p0, int32_t p1) {
     // S slabs at a time: a row of one token is S loads under way
     for (int64_t i = lane * N; i < a.E; i += S * slab) {
       int64_t c[S];
@@ -296,19 +313,44 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
       }
       for (int32_t p = p0; p < p1; ++p) {
         const int64_t row = (int64_t)w.order[p] * a.E;
-        RowRun<T, N> v[S];
+        RowRun<T, N> g[S];
 #pragma unroll
-        for (int k = 0; k < S; ++k) v[k] = run_at<T, N>(a.grad, row + c[k]);
+        for (int k = 0; k < S; ++k) g[k] = run_at<T, N>(a.grad, row + c[k]);
 #pragma unroll
         for (int k = 0; k < S; ++k)
 #pragma unroll
-          for (int x = 0; x < N; ++x) s[k][x] += T::get(v[k].v[x]);
+          for (int x = 0; x < N; ++x) s[k][x] += T::get(g[k].v[x]);
       }
 #pragma unroll
       for (int k = 0; k < S; ++k)
-        if (i + k * slab < a.E) store(v0 + r, c[k], s[k]);
+        if (i + k * slab < a.E) store(v, c[k], s[k]);
     }
+  };
+  if (rows == 0) {
+    __shared__ int32_t row_of[kPlaces], end[kPlaces];
+    const int32_t n = w.first[a.V];
+    const int64_t q = (int64_t)(blockIdx.x - window_blocks) * kPlaces;
+    if (q >= n) return;
+    if (threadIdx.x < kPlaces) {
+      const int32_t p = (int32_t)min(q + threadIdx.x, (int64_t)n - 1);
+      const int32_t v = a.ids[w.order[p]];
+      const bool mine = q + threadIdx.x < n && w.first[v] == p;
+      row_of[threadIdx.x] = mine ? v : -1;
+      end[threadIdx.x] = w.first[v + 1];
+    }
+    __syncthreads();
+    for (int i = own; i < kPlaces; i += groups) {
+      const int32_t p0 = (int32_t)q + i;
+      if (row_of[i] >= 0 && end[i] - p0 <= kFew) sum_row(row_of[i], p0, end[i]);
+    }
+    return;
   }
+  const int64_t v0 = (int64_t)(blockIdx.x - window_blocks) * rows;
+  const int here = (int)min((int64_t)rows, a.V - v0);
+  for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
+  __syncthreads();
+  for (int r = own; r < here; r += groups)
+    if (first[r + 1] - first[r] <= kFew) sum_row(v0 + r, first[r], first[r + 1]);
 }
 
 // The row that begins in window j and goes on behind it (its last place's, if any),
@@ -351,8 +393,17 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
   if (a.V * a.E == 0) return 0;
   const GradWork w = grad_work(a);
   const int64_t windows = windows_of(a.T);
-  hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)((a.V + kSortRows - 1) / kSortRows)),
-                     dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w);
+  const int64_t table = a.V * a.E * (a.dt == kF32 ? 4 : 2);
+  const bool clear = clear_first(a.T, a.V, table);
+  const int64_t bytes = clear ? table : 0;
+  const int64_t sorts = (a.V + kSortRows - 1) / kSortRows;
+  hipLaunchKernelGGL(embed_sort_kernel,
+                     dim3((unsigned)(sorts + (bytes + 16 * kSortThreads - 1) / (16 * kSortThreads))),
+                     dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w, (uint8_t*)a.out, bytes);
+  if (a.T == 0 && clear) {
+    REW_HIP(hipGetLastError());
+    return 1;
+  }
   by_run(a.dt, a.E, [&](auto t, auto n) {
     typedef decltype(t) Ty;
     constexpr int N = decltype(n)::value;
@@ -364,7 +415,9 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
     while (rows > groups && a.V < (int64_t)rows * 1024) rows /= 2;
     rows = std::max(groups, rows / groups * groups);
     const int64_t slabs = (runs + lanes - 1) / lanes;
-    const int64_t blocks = windows * slabs + (a.V + rows - 1) / rows;
+    if (clear) rows = 0;
+    const int64_t blocks =
+        windows * slabs + (clear ? (a.T + kPlaces - 1) / kPlaces : (a.V + rows - 1) / rows);
     auto sum = [&](auto together) {
       hipLaunchKernelGGL((embed_sum_kernel<Ty, N, decltype(together)::value>),
                          dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, w,

@@ -73,6 +73,28 @@ def test_gradient(gpu, dtype, tokens, vocab, width):
     np.testing.assert_array_equal(R.host(got), R.host(O.embeddingGrad(ints(ids), g, vocab, 1.5)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,vocab,width", [
+    (1, 4, 1), (63, 253, 3), (300, 1203, 5), (5000, 19999, 24), (2000, 9000, 1032),
+    (1, 33000, 1024), (3000, 34001, 1003), (8500, 34001, 1003), (5000, 20001, 2048)])
+def test_gradient_of_large_tables(gpu, dtype, tokens, vocab, width):
+    """Tables of up to and from four times the tokens and 64 MiB on; nothing is left of what the
+    memory held before."""
+    r = np.random.default_rng(tokens + width)
+    ids = text(r, tokens, vocab)
+    g, gh = tensor(r.standard_normal((tokens, width)), dtype)
+    want, bound = R.embedding_grad(ids, gh, vocab, -0.75, dtype)
+    got = O.embeddingGrad(ints(ids), g, vocab, -0.75)
+    R.check(got, want, bound)
+    bits = R.host(got)
+    del got
+    full = O.embeddingGrad(ints(r.permutation(vocab)), tensor(np.ones((vocab, width)), dtype)[0],
+                           vocab)
+    assert (R.host(full) == 1).all()
+    del full
+    np.testing.assert_array_equal(R.host(O.embeddingGrad(ints(ids), g, vocab, -0.75)), bits)
+
+
 @pytest.mark.parametrize("ids", [[3] * 65, [3] * 64, [3] * 63 + [2], [3] * 128 + [4] * 129,
                                  [5] + [3] * 127 + [4] * 64 + [0] * 300, [1, 2] * 500])
 def test_rows_of_many_tokens(gpu, ids):
