@@ -1,5 +1,9 @@
 // Embedding rows and the gradient of their table (EmbedArgs and EmbedGradArgs
 // in kernels.h).
+//
+// Bound: HBM.  16384 ids of text, 128256 x 4096 bfloat16: rows in 42.5 us (54 MB of the
+// table and 134 MB written, 4.4 TB/s); gradient 155 us (sort and zeros, 1.05 GB at 6.8
+// TB/s) + 75 (sums) + 6 (join).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -71,7 +75,7 @@ constexpr int kFew = 8, kWindow = 64;
 int64_t windows_of(int64_t T) { return T > kFew ? (T + kWindow - 1) / kWindow : 0; }
 
 // A large table of which most rows have no token is cleared as a whole beside the sort,
-// in the order of its addresses (6.3 TB/s; zeros stored row by row between the sums
+// in the order of its addresses (6.8 TB/s; zeros stored row by row between the sums
 // come to 5.3), and the places of the order then write the rows that have tokens.
 // 16384 tokens, 4096 wide: 128256 rows 264 -> 235 us, 65537 rows 173 -> 157; tables of
 // 64 MB are the same either way, smaller ones 1 us slower.
