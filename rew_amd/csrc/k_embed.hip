@@ -401,8 +401,9 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
   const bool clear = clear_first(a.T, a.V, table);
   const int64_t bytes = clear ? table : 0;
   const int64_t sorts = (a.V + kSortRows - 1) / kSortRows;
+  constexpr int64_t kCleared = 16 * kSortThreads;  // bytes of a workgroup
   hipLaunchKernelGGL(embed_sort_kernel,
-                     dim3((unsigned)(sorts + (bytes + 16 * kSortThreads - 1) / (16 * kSortThreads))),
+                     dim3((unsigned)(sorts + (bytes + kCleared - 1) / kCleared)),
                      dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w, (uint8_t*)a.out, bytes);
   if (a.T == 0 && clear) {
     REW_HIP(hipGetLastError());

@@ -413,9 +413,9 @@ bool by_group(int64_t runs, F&& f) {
       with(std::integral_constant<int, 512>(), std::integral_constant<int, 3>());
     else if (runs <= 2048)
       with(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
-    else if (Grad || runs > 4096) return false;
+    else if (Grad || runs > 4 * kMaxGroup) return false;
     else if constexpr (!Grad) {
-      if (runs <= 3072)
+      if (runs <= 3 * kMaxGroup)
         with(std::integral_constant<int, 1024>(), std::integral_constant<int, 3>());
       else
         with(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());

@@ -956,7 +956,8 @@ Cut choose_cut(int64_t M, int64_t N, int64_t nk, int64_t most) {
     const int64_t size = small ? SM : BM;
     const int64_t tm = cdiv(M, size), tn = cdiv(N, size);
     for (int rounds = 0; rounds <= 4; ++rounds) {  // of workgroups on all CUs
-      const int64_t s = std::max<int64_t>(1, std::min({rounds * kCus / std::max<int64_t>(tm * tn, 1), nk, most}));
+      const int64_t cus = rounds * kCus / std::max<int64_t>(tm * tn, 1);
+      const int64_t s = std::max<int64_t>(1, std::min({cus, nk, most}));
       const int64_t per = cdiv(nk, s);
       double us = (double)cdiv(tm * tn * s, kCus) * tile_us(small, per);
       if (s > 1) us += 4.0 + (double)(M * N * s) * 8.0 / 4.0e6;
@@ -977,7 +978,8 @@ Cut choose_runs(int64_t M, int64_t N, int64_t nk) {
     const int64_t size = small ? SM : BM;
     const int64_t tm = cdiv(M, size), tn = cdiv(N, size);
     for (int rounds = 1; rounds <= 8; ++rounds) {
-      const int64_t s = std::max<int64_t>(1, std::min(rounds * kCus / std::max<int64_t>(tm, 1), tn));
+      const int64_t cus = rounds * kCus / std::max<int64_t>(tm, 1);
+      const int64_t s = std::max<int64_t>(1, std::min(cus, tn));
       const int64_t per = cdiv(tn, s);
       const double us = (double)cdiv(tm * s, kCus) * (3.0 + (double)per * tile_us(small, nk));
       if (us < least * 0.99) {
