@@ -169,6 +169,27 @@ def test_captured_losses(gpu, form, tied):
             np.testing.assert_array_equal(E.toHost(b), k)
 
 
+@pytest.mark.parametrize("tokens,vocab,width", [(300, 700, 40), (3000, 34001, 1003)])
+def test_captured_table_gradient(gpu, tokens, vocab, width):
+    """Rows of many tokens, of few and of none, in a small table and in one that is cleared as
+    a whole."""
+    r = np.random.default_rng(11)
+    ids = ints(np.floor(np.exp(r.uniform(0, np.log(vocab), tokens))).astype(np.int64) - 1)
+    g = tensor(r.standard_normal((tokens, width)), "bfloat16")[0]
+
+    def call():
+        return [O.embeddingGrad(ids, g, vocab, 2.0)]
+
+    want = E.toHost(call()[0])
+    replay, _, out = _capture(call)
+    for _ in range(3):
+        replay()
+        between = call()
+        E.sync()
+        np.testing.assert_array_equal(E.toHost(out[0]), want)
+        np.testing.assert_array_equal(E.toHost(between[0]), want)
+
+
 def test_operands_that_are_views(gpu):
     """Slices, transposes and sums that no launch has made yet."""
     r = np.random.default_rng(10)
