@@ -43,6 +43,14 @@ constexpr float kMost = 3.402823466e38f;
 // dz is stored as 2^14 g / max|g| (p - 1): below 2^14, so float16 keeps eleven
 // bits of probabilities down to 2^-28 and the float32 sums have room.
 constexpr float kDzScale = 16384.0f;
+// The gradients of few tokens are sums of few terms that matter, which do not average
+// dz's rounding (2 tokens, 64 x 2 bfloat16: dx 0.0036 off relative to its norm, of which
+// its own rounding is 0.0017).  Up to 32 tokens fill half of the products' least tile
+// and k-step, and the other half carries what dz's rounding left.  Forward and
+// gradients as called, without / with: 1 x 64 x 1000 35 / 38 us (the join of dx), 30 x
+// 1000 x 20000 79 / 86, 32 x 4096 x 128256 915 / 929; 2 x 64 x 2 is off by its own
+// rounding alone.
+constexpr int64_t kRestRows = 32;
 // Columns of the vocabulary at a time, at least (8192 x 4096 x 128256, all kernels: 26.7
 // ms; 8192 columns 26.9; 32768 columns 26.5, with twice the working memory).
 constexpr int64_t kPiece = 16384;
@@ -68,11 +76,13 @@ struct Product {
   float* zt;            // kStats: the target's logit
   void* out;            // kDz, kOut: row pitch ldo; kSum: float32 [split][M][N]
   int64_t ldo, rows_out;
+  int64_t rest;         // kDz, kDzRest: rows from dz to its remainders, 0: none
 };
 
 // What becomes of the products: running softmax statistics; dz; a result in 16 bits;
-// a float32 share of one.
-enum { kStats, kDz, kOut, kSum };
+// a float32 share of one.  kDzRest: dz and its remainders, by 256 x 256 tiles.
+enum { kStats, kDz, kOut, kSum, kDzRest };
+constexpr bool is_dz(int mode) { return mode == kDz || mode == kDzRest; }
 
 // Workgroups whose indices agree mod 8 share an XCD and its L2: each XCD gets a
 // contiguous range, walked in groups of 4 row tiles.
@@ -211,6 +221,15 @@ __device__ __forceinline__ float stat_exp(float z, float m) {
   return fa_exp2(__builtin_fmaf(z, kLog2e, -m));
 }
 
+// What rounding two values to 16 bits leaves of them; none of an infinity.
+template <class Ty>
+__device__ __forceinline__ void rest_of(float& a, float& b) {
+  const uint32_t h = Ty::pack(a, b);
+  const float lo = Ty::lo(h), hi = Ty::hi(h);
+  a = fabsf(lo) <= kMost ? a - lo : 0.0f;
+  b = fabsf(hi) <= kMost ? b - hi : 0.0f;
+}
+
 // What a row's dz needs, loaded early; dz of a row without a target is zero.
 struct DzRow {
   int32_t target;
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
     }
   }
   float scale = 1.0f;
-  if constexpr (MODE == kDz || MODE == kOut) scale = g.scale[0];
+  if constexpr (is_dz(MODE) || MODE == kOut) scale = g.scale[0];
 
   fa.start(g.a, (int64_t)cur.tm * BM, (int64_t)cur.k0 * BK);
   fb.start(g.b, (int64_t)cur.tn * BN, (int64_t)cur.k0 * BK);
@@ -319,8 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
       if (more) nxt = tile_of(t);
     }
     const int64_t m0 = (int64_t)cur.tm * BM;
-    DzRow dz[MODE == kDz ? NI : 1];
-    if constexpr (MODE == kDz)
+    DzRow dz[is_dz(MODE) ? NI : 1];
+    if constexpr (is_dz(MODE))
 #pragma unroll
       for (int i = 0; i < NI; ++i) dz[i].load(g, m0 + wm * 128 + i * 32 + (lane & 31));
 
@@ -452,9 +471,9 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int64_t row0 = m0 + wm * 128 + i * 32;
-        if constexpr (MODE == kDz || MODE == kOut) {
+        if constexpr (is_dz(MODE) || MODE == kOut) {
           uint64_t alive = ~0ull;
-          if constexpr (MODE == kDz) {
+          if constexpr (is_dz(MODE)) {
             alive = __ballot(dz[i].live(g));
             const float f = dz[i].factor(scale), lse2 = dz[i].lse2();
 #pragma unroll
@@ -474,36 +493,46 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
             const int32_t v = g.target[row < g.M ? row : g.M - 1];
             alive = __ballot(v >= 0 && v < g.V);
           }
+          auto emit = [&](auto part) {
+            constexpr bool rest = decltype(part)::value;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v[4];
+              for (int q = 0; q < 4; ++q) {
+                float v[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                v[e] = MODE == kOut ? acc[i][j][q * 4 + e] * gain : acc[i][j][q * 4 + e];
-              *(uint2*)(put_at(j * 4 + q) + (lane >> 5) * 8) =
-                  make_uint2(Ty::pack(v[0], v[1]), Ty::pack(v[2], v[3]));
-            }
-          const int64_t cols = g.N - (n_base + ch * 8);  // (dz: zeros behind)
-          uint16_t* out = (uint16_t*)g.out + (row0 + r8) * g.ldo + n_base + ch * 8;
+                for (int e = 0; e < 4; ++e)
+                  v[e] = MODE == kOut ? acc[i][j][q * 4 + e] * gain : acc[i][j][q * 4 + e];
+                if constexpr (rest) {
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            uint4 v = *(const uint4*)get_at(p);
-            if (!(alive >> (p * 8 + r8) & 1)) v = make_uint4(0, 0, 0, 0);
-            if (row0 + p * 8 + r8 >= g.rows_out) continue;
-            if constexpr (MODE == kDz) {
-              if (cols < 8) {
-                uint16_t* h = (uint16_t*)&v;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (e >= cols) h[e] = 0;
+                  for (int e = 0; e < 4; e += 2) rest_of<Ty>(v[e], v[e + 1]);
+                }
+                *(uint2*)(put_at(j * 4 + q) + (lane >> 5) * 8) =
+                    make_uint2(Ty::pack(v[0], v[1]), Ty::pack(v[2], v[3]));
               }
-              *(uint4*)(out + p * 8 * g.ldo) = v;
-            } else {
-              store8(out + p * 8 * g.ldo, v, cols);
+            const int64_t cols = g.N - (n_base + ch * 8);  // (dz: zeros behind)
+            uint16_t* out =
+                (uint16_t*)g.out + (row0 + r8 + (rest ? g.rest : 0)) * g.ldo + n_base + ch * 8;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              uint4 v = *(const uint4*)get_at(p);
+              if (!(alive >> (p * 8 + r8) & 1)) v = make_uint4(0, 0, 0, 0);
+              if (row0 + p * 8 + r8 >= g.rows_out) continue;
+              if constexpr (is_dz(MODE)) {
+                if (cols < 8) {
+                  uint16_t* h = (uint16_t*)&v;
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (e >= cols) h[e] = 0;
+                }
+                *(uint4*)(out + p * 8 * g.ldo) = v;
+              } else {
+                store8(out + p * 8 * g.ldo, v, cols);
+              }
             }
-          }
+          };
+          emit(std::false_type());
+          if constexpr (MODE == kDzRest) emit(std::true_type());
         } else {
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
@@ -606,7 +635,7 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
     const int32_t t = row < g.M ? g.target[row] : -1;
     if (t >= 0 && t < g.V) tgt = t - g.n0;
   }
-  if constexpr (MODE == kDz) {
+  if constexpr (is_dz(MODE)) {
     d.load(g, row);
     f = d.factor(scale);
   }
@@ -692,10 +721,10 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
 #pragma unroll
       for (int e = 0; e < 8; ++e) run_s += stat_exp(v[e], m);
       run_m = m;
-    } else if constexpr (MODE == kDz || MODE == kOut) {
+    } else if constexpr (is_dz(MODE) || MODE == kOut) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if constexpr (MODE == kDz) {
+        if constexpr (is_dz(MODE)) {
           v[e] = f * fa_exp2(__builtin_fmaf(v[e], kLog2e, -d.lse2()));
           if (n + e == d.target - g.n0) v[e] -= f;
           if (e >= cols || !d.live(g)) v[e] = 0.0f;
@@ -707,8 +736,18 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
                                  Ty::pack(v[4], v[5]), Ty::pack(v[6], v[7]));
       if (row < g.rows_out) {
         uint16_t* out = (uint16_t*)g.out + row * g.ldo + n;
-        if constexpr (MODE == kDz) *(uint4*)out = h;
-        else store8(out, h, cols);
+        if constexpr (is_dz(MODE)) {
+          *(uint4*)out = h;
+          if (g.rest) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) rest_of<Ty>(v[e], v[e + 1]);
+            *(uint4*)(out + g.rest * g.ldo) =
+                make_uint4(Ty::pack(v[0], v[1]), Ty::pack(v[2], v[3]), Ty::pack(v[4], v[5]),
+                           Ty::pack(v[6], v[7]));
+          }
+        } else {
+          store8(out, h, cols);
+        }
       }
     } else if (row < g.M) {
       float* o = (float*)g.out + ((int64_t)split * g.M + row) * g.N + n;
@@ -751,19 +790,21 @@ __device__ __forceinline__ float largest_grad(const int32_t* target, const float
 }
 
 // x with zeros in rows without a target (`all`: every row as it is), in rows behind T
-// and columns behind H: 16 bytes from every `step`-th thread.
+// and columns behind H: 16 bytes from every `step`-th thread.  twice (the rows that dz's
+// remainders multiply): row r once more in row r + kRestRows.
 struct Copy {
   const uint16_t* x;
   const int32_t* target;
   uint16_t* out;
   int64_t T, H, V, Tp, Hp, ld;
-  int all;
+  int all, twice;
 };
 __device__ __forceinline__ void copy_x(const Copy& c, int64_t first, int64_t step) {
   const int64_t per = c.Hp / 8, total = c.Tp * per;
   for (int64_t i = first; i < total; i += step) {
-    const int64_t r = total >> 32 ? i / per : (int64_t)((uint32_t)i / (uint32_t)per);
-    const int64_t k = (i - r * per) * 8;
+    const int64_t to = total >> 32 ? i / per : (int64_t)((uint32_t)i / (uint32_t)per);
+    const int64_t k = (i - to * per) * 8;
+    const int64_t r = c.twice && to >= kRestRows ? to - kRestRows : to;
     const bool live = r < c.T && (c.all || (c.target[r] >= 0 && c.target[r] < c.V));
     uint4 v = make_uint4(0, 0, 0, 0);
     if (live) {
@@ -778,14 +819,14 @@ __device__ __forceinline__ void copy_x(const Copy& c, int64_t first, int64_t ste
           if (k + e < c.H) h[e] = p[e];
       }
     }
-    *(uint4*)(c.out + r * c.ld + k) = v;
+    *(uint4*)(c.out + to * c.ld + k) = v;
   }
 }
 
 template <class Ty, bool AKC, bool BKC, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) xent_small_kernel(Product g) {
   __shared__ __attribute__((aligned(1024))) uint8_t L[8][2 * kSmallHalf];
-  small_product<Ty, AKC, BKC, MODE>(g, blockIdx.x, MODE == kDz || MODE == kOut ? g.scale[0] : 1.0f,
+  small_product<Ty, AKC, BKC, MODE>(g, blockIdx.x, is_dz(MODE) || MODE == kOut ? g.scale[0] : 1.0f,
                                     L);
 }
 
@@ -885,9 +926,10 @@ __global__ void __launch_bounds__(256) xent_pack_kernel(const uint16_t* w, int64
 
 // A matrix [rows, cols] in 16 bits (row pitch ldo) from its splits' float32 sums.
 // target set (dx): rows without a target are zeros.
+// rest: the sums of row r lie in rows r and r + rest.
 template <class Ty>
 __global__ void __launch_bounds__(256) xent_round_kernel(const float* sums, int64_t rows,
-                                                         int64_t cols, int splits,
+                                                         int64_t cols, int splits, int64_t rest,
                                                          const float* scale,
                                                          const int32_t* target, int64_t V,
                                                          uint16_t* out, int64_t ldo) {
@@ -902,8 +944,9 @@ __global__ void __launch_bounds__(256) xent_round_kernel(const float* sums, int6
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     const int32_t t = target ? target[r] : 0;
     if (t >= 0 && t < V) {
-      for (int p = 0; p < splits; ++p) {
-        const float* s = sums + (p * rows + r) * cols + c;
+      for (int p = 0; p < (rest ? 2 * splits : splits); ++p) {
+        // (a split has 2 rest rows)
+        const float* s = sums + (rest ? p * rest + r : p * rows + r) * cols + c;
         if (cols % 4 == 0 && n == 8) {
           const float4 lo = *(const float4*)s, hi = *(const float4*)(s + 4);
           v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
@@ -998,6 +1041,8 @@ struct XentPlan {
   int64_t piece, pieces;   // columns of the vocabulary at a time
   Cut z, dw, dx;           // of a whole piece
   bool dx_sums;            // dx is added up in float32
+  bool rest;               // dz and x lie in rows 0 .. 31, dz's remainders and x in 32 .. 63
+  int64_t dz_rows;         // of the product for dx
   // offsets of the working memory
   size_t part, zt, x, w, dz, sums, dw_sums, scale, bytes;
 };
@@ -1033,10 +1078,12 @@ XentPlan make_plan(int64_t T, int64_t H, int64_t V, int tied, bool grad) {
   if (grad) {
     p.z = choose_cut(T, n, p.Hp / BK, 1);
     p.dw = choose_cut(tied ? n : H, tied ? H : n, p.Tp / BK, 16);
-    p.dx = choose_cut(T, H, up(n, BK) / BK, 64);
-    p.dx_sums = p.pieces > 1 || p.dx.splits > 1;
+    p.rest = T > 0 && T <= kRestRows;
+    p.dz_rows = p.rest ? 2 * kRestRows : T;
+    p.dx = choose_cut(p.dz_rows, H, up(n, BK) / BK, 64);
+    p.dx_sums = p.rest || p.pieces > 1 || p.dx.splits > 1;
     p.dz = take((size_t)p.Tp * p.ldz * 2);
-    if (p.dx_sums) p.sums = take((size_t)p.dx.splits * T * H * 4);
+    if (p.dx_sums) p.sums = take((size_t)p.dx.splits * p.dz_rows * H * 4);
     if (p.dw.splits > 1) p.dw_sums = take((size_t)p.dw.splits * n * H * 4);
     p.scale = take(4);
   } else {
@@ -1100,12 +1147,12 @@ void launch_pair(Product w, Product x, const XentPlan& p, int tied, hipStream_t 
 }
 
 template <class Ty>
-void launch_round(const float* sums, int64_t rows, int64_t cols, int64_t splits,
+void launch_round(const float* sums, int64_t rows, int64_t cols, int64_t splits, int64_t rest,
                   const float* scale, const int32_t* target, int64_t V, void* out, int64_t ldo,
                   hipStream_t stream) {
   const int64_t blocks = std::min<int64_t>(cdiv(rows * cdiv(cols, 8), 256), kCus * 16);
   hipLaunchKernelGGL((xent_round_kernel<Ty>), dim3((unsigned)blocks), dim3(256), 0, stream, sums,
-                     rows, cols, (int)splits, scale, target, V, (uint16_t*)out, ldo);
+                     rows, cols, (int)splits, rest, scale, target, V, (uint16_t*)out, ldo);
   REW_HIP(hipGetLastError());
 }
 
@@ -1140,7 +1187,7 @@ int run_xent(const XentArgs& a, hipStream_t stream) {
   g.a = {(const uint16_t*)a.x, a.H, a.T * a.H, a.H};
   if (p.copy_x) {
     uint16_t* x = (uint16_t*)(work + p.x);
-    const Copy c = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 1};
+    const Copy c = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 1, 0};
     const int64_t blocks = std::min<int64_t>(cdiv(p.Tp * p.Hp / 8, 1024), kCus * 4);
     hipLaunchKernelGGL(xent_prepare_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream, c,
                        (const float*)nullptr, (float*)nullptr);
@@ -1182,7 +1229,7 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
   uint16_t* x = (uint16_t*)(work + p.x);
   uint16_t* dz = (uint16_t*)(work + p.dz);
   float* scale = (float*)(work + p.scale);
-  const Copy copy = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 0};
+  const Copy copy = {(const uint16_t*)a.x, a.target, x, a.T, a.H, a.V, p.Tp, p.Hp, p.ldx, 0, p.rest};
   const bool first = a.T && p.z.small && p.pieces == 1 && !p.pack_w && a.H % BK == 0 &&
                      a.T <= kFirstTokens;
   if (!first) {
@@ -1215,7 +1262,8 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
       d.target = a.target;
       d.out = dz;
       d.ldo = p.ldz;
-      d.rows_out = p.Tp;
+      d.rows_out = p.rest ? kRestRows : p.Tp;
+      d.rest = p.rest ? kRestRows : 0;
       if (first) {
         d.a = {(const uint16_t*)a.x, a.H, a.T * a.H, a.H};
         d.tiles_m = (int)p.z.tiles_m;
@@ -1230,6 +1278,9 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
           hipLaunchKernelGGL((xent_first_kernel<Ty, false>), dim3(blocks), dim3(kThreads), 0,
                              stream, d, copy, tiles, scale);
         REW_HIP(hipGetLastError());
+      } else if (p.rest && !p.z.small) {
+        if (a.tied) launch_product<Ty, true, true, kDzRest>(d, p.z, stream);
+        else launch_product<Ty, true, false, kDzRest>(d, p.z, stream);
       } else if (a.tied) {
         launch_product<Ty, true, true, kDz>(d, p.z, stream);
       } else {
@@ -1260,7 +1311,7 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
       d.a = {dz, p.ldz, p.Tp * p.ldz, d.K};
       // (a packed piece has zeros behind n; else the rows' or columns' end is w's own)
       d.b = {w.p, w.ld, w.len, a.tied ? n : p.pack_w ? d.K : n};
-      d.M = d.rows_out = a.T;
+      d.M = d.rows_out = p.dz_rows;
       d.N = a.H;
       d.splits = (int)cdiv(d.K / BK, p.dx.per);  // (the first piece has the most)
       d.add = i > 0;
@@ -1284,14 +1335,14 @@ int run_xent_grad(const XentGradArgs& a, hipStream_t stream) {
       }
     }
     if (dw_sums) {
-      launch_round<Ty>((const float*)dw.out, dw.M, dw.N, dw.splits, scale, nullptr, 1, dw_out,
-                       dw.ldo, stream);
+      launch_round<Ty>((const float*)dw.out, dw.M, dw.N, dw.splits, 0, scale, nullptr, 1,
+                       dw_out, dw.ldo, stream);
       ++launches;
     }
   }
   if (a.T && p.dx_sums) {
-    launch_round<Ty>((const float*)(work + p.sums), a.T, a.H, p.dx.splits, scale, a.target, a.V,
-                     a.dx, a.H, stream);
+    launch_round<Ty>((const float*)(work + p.sums), a.T, a.H, p.dx.splits, p.rest ? kRestRows : 0,
+                     scale, a.target, a.V, a.dx, a.H, stream);
     ++launches;
   }
   return launches;

@@ -145,8 +145,9 @@ def cross_entropy(x, w, targets):
         (lse[:, 0], e_lse[:, 0])
 
 
-def cross_entropy_grad(x, w, targets, grad, dtype):
-    """dx, dw [embed, vocab] and their bounds."""
+def cross_entropy_grad(x, w, targets, grad, dtype, rest=False):
+    """dx, dw [embed, vocab] and their bounds; rest: the bounds where dz keeps the remainder
+    of its rounding in 16 bits too, so that h of h is lost."""
     h = HALF[dtype]
     z, e_z, lse, e_lse = _softmax(x, w)
     t = np.asarray(targets)
@@ -158,7 +159,7 @@ def cross_entropy_grad(x, w, targets, grad, dtype):
     dz = g * (p - hit)
     # p's relative error, the subtraction, two roundings of the scale, one to dtype
     e_p = p * (np.expm1(e_z + e_lse) + (4 * np.abs(z - lse) + 8) * U)
-    e_dz = np.abs(g) * (e_p + U) + (h + 6 * U) * np.abs(dz)
+    e_dz = np.abs(g) * (e_p + U) + ((h * h if rest else h) + 6 * U) * np.abs(dz)
     if dtype == "float16":  # dz lies in units of the largest |grad| / 2^14
         e_dz = e_dz + np.abs(g).max(initial=0.0) * 2.0 ** -39 * live[:, None]
     xx = np.where(live[:, None], x, 0.0)

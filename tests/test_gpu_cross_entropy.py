@@ -51,6 +51,22 @@ def test_sizes(gpu, tied, dtype, T, H, V):
 
 
 @pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,V", [
+    (1, 1, 2), (1, 64, 2), (2, 64, 2), (5, 3, 1000), (31, 64, 300), (32, 1, 300), (32, 72, 40),
+    (7, 1000, 5000), (16, 200, 60001), (32, 128, 40000)])
+def test_few_tokens(gpu, tied, dtype, T, H, V):
+    """Gradients that are sums of few terms: rounded once, as dz keeps its remainder."""
+    (x, w, targets, grad), (xh, wh, th, gh) = case(np.random.default_rng(T * V), T, H, V, dtype,
+                                                   tied)
+    lse = O.linearCrossEntropy(x, w, targets, tied, withLse=True)[1]
+    got = O.linearCrossEntropyGrad(x, w, targets, lse, grad, tied)
+    (dx, e_dx), (dw, e_dw) = R.cross_entropy_grad(xh, wh, th, gh, dtype, rest=True)
+    R.check(got[0], dx, e_dx)
+    R.check(got[1], dw.T if tied else dw, e_dw.T if tied else e_dw)
+
+
+@pytest.mark.parametrize("tied", [False, True])
 @pytest.mark.parametrize("V", [33000, 33001])
 def test_pieces_of_the_vocabulary(gpu, tied, V):
     """More columns than are held at a time, aligned and not."""
