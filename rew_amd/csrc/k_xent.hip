@@ -904,10 +904,11 @@ __global__ void __launch_bounds__(1024) xent_prepare_kernel(Copy c, const float*
 __global__ void __launch_bounds__(256) xent_pack_kernel(const uint16_t* w, int64_t ld,
                                                         int64_t rows, int64_t cols, int64_t pitch,
                                                         uint16_t* out) {
-  const uint32_t per = (uint32_t)(pitch / 8);  // (rows * per < 2^31)
-  const uint32_t total = (uint32_t)rows * per;
-  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
-    const uint32_t r = i / per;
+  const uint32_t per = (uint32_t)(pitch / 8);
+  const uint64_t total = (uint64_t)rows * per;  // (a piece of 2^21 x 16384: 2^32)
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (uint64_t)gridDim.x * 256) {
+    const int64_t r = total >> 32 ? (int64_t)(i / per) : (int64_t)((uint32_t)i / per);
     const int64_t c = (int64_t)(i - r * per) * 8;
     const uint16_t* p = w + r * ld + c;
     uint4 v = make_uint4(0, 0, 0, 0);
