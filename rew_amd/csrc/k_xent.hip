@@ -880,9 +880,14 @@ __global__ void __launch_bounds__(256) xent_join_kernel(XentArgs a, const float2
     __syncthreads();
   }
   if (share || row >= a.T) return;
-  const float lse = (m + log2f(s)) * kLn2;
+  const float ls = log2f(s), lse = (m + ls) * kLn2;
   const int32_t t = a.target[row];
-  a.loss[row] = t >= 0 && t < a.V ? lse - zt[row] : 0.0f;
+  // Not lse - z: lse has been rounded at its own size, which leaves nothing of the loss of a
+  // confident token (logits near 300: 6e-5 off).  m is the rounded z log2 e of the largest
+  // logit and s has what that rounding took, so that they cancel to a few roundings of 1.
+  float loss = 0.0f;
+  if (t >= 0 && t < a.V) loss = (__builtin_fmaf(-zt[row], kLog2e, m) + ls) * kLn2;
+  a.loss[row] = loss < 0.0f ? 0.0f : loss;  // (those roundings)
   if (a.lse) a.lse[row] = lse;
 }
 
