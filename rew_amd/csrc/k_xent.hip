@@ -39,6 +39,8 @@ constexpr int kHalf = BM * BK * 2;          // bytes of an operand's k-step: 32 
 constexpr int SM = 64, kSmallHalf = SM * BK * 2;  // the small form's tile
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
+// 1 / (kLog2e as it is rounded) less kLn2 as it is rounded.
+constexpr float kLn2Rest = (float)(1.0 / (double)kLog2e - (double)kLn2);
 constexpr float kMost = 3.402823466e38f;
 // dz is stored as 2^14 g / max|g| (p - 1): below 2^14, so float16 keeps eleven
 // bits of probabilities down to 2^-28 and the float32 sums have room.
@@ -246,6 +248,11 @@ struct DzRow {
   }
   __device__ __forceinline__ float factor(float scale) const { return grad / scale * kDzScale; }
   __device__ __forceinline__ float lse2() const { return lse * kLog2e; }
+  // .. of probabilities 2^(z log2 e - lse2): with what lse2's rounding took.
+  __device__ __forceinline__ float factor_p(float f) const {
+    const float d = __builtin_fmaf(lse, kLog2e, -lse2());
+    return fabsf(d) < 1.0f ? __builtin_fmaf(-d * kLn2, f, f) : f;  // (not of an infinite lse)
+  }
 };
 
 // 256 x 256 outputs at a time, from two stages of a k-step each.  Workgroups walk
@@ -475,12 +482,12 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(Product g) {
           uint64_t alive = ~0ull;
           if constexpr (is_dz(MODE)) {
             alive = __ballot(dz[i].live(g));
-            const float f = dz[i].factor(scale), lse2 = dz[i].lse2();
+            const float f = dz[i].factor(scale), lse2 = dz[i].lse2(), fp = dz[i].factor_p(f);
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                acc[i][j][e] = f * fa_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -lse2));
+                acc[i][j][e] = fp * fa_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -lse2));
             const int c = dz[i].target - g.n0;
             if (__any(dz[i].target >= g.n0 && c >= n_base && c < n_base + 64))
 #pragma unroll
@@ -630,7 +637,7 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
   float run_m = -kMost, run_s = 0.0f, gain = 0.0f;
   int tgt = -1;
   DzRow d;
-  float f = 0.0f;
+  float f = 0.0f, fp = 0.0f;
   if constexpr (MODE == kStats) {
     const int32_t t = row < g.M ? g.target[row] : -1;
     if (t >= 0 && t < g.V) tgt = t - g.n0;
@@ -638,6 +645,7 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
   if constexpr (is_dz(MODE)) {
     d.load(g, row);
     f = d.factor(scale);
+    fp = d.factor_p(f);
   }
   bool alive = true;
   if constexpr (MODE == kOut) {
@@ -725,7 +733,7 @@ __device__ __forceinline__ void small_product(const Product& g, uint32_t bid, fl
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (is_dz(MODE)) {
-          v[e] = f * fa_exp2(__builtin_fmaf(v[e], kLog2e, -d.lse2()));
+          v[e] = fp * fa_exp2(__builtin_fmaf(v[e], kLog2e, -d.lse2()));
           if (n + e == d.target - g.n0) v[e] -= f;
           if (e >= cols || !d.live(g)) v[e] = 0.0f;
         } else {
@@ -880,7 +888,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(XentArgs a, const float2
     __syncthreads();
   }
   if (share || row >= a.T) return;
-  const float ls = log2f(s), lse = (m + ls) * kLn2;
+  const float ls = log2f(s);
   const int32_t t = a.target[row];
   // Not lse - z: lse has been rounded at its own size, which leaves nothing of the loss of a
   // confident token (logits near 300: 6e-5 off).  m is the rounded z log2 e of the largest
@@ -888,7 +896,13 @@ __global__ void __launch_bounds__(256) xent_join_kernel(XentArgs a, const float2
   float loss = 0.0f;
   if (t >= 0 && t < a.V) loss = (__builtin_fmaf(-zt[row], kLog2e, m) + ls) * kLn2;
   a.loss[row] = loss < 0.0f ? 0.0f : loss;  // (those roundings)
-  if (a.lse) a.lse[row] = lse;
+  if (!a.lse) return;
+  // (m + ls) ln 2, rounded once: the gradient's probabilities are off by a step of it.
+  // lo: what the sum's rounding took.
+  const float sum = m + ls, of_ls = sum - m, lo = (m - (sum - of_ls)) + (ls - of_ls);
+  a.lse[row] = fabsf(sum) <= kMost
+                   ? __builtin_fmaf(sum, kLn2, __builtin_fmaf(sum, kLn2Rest, lo * kLn2))
+                   : sum;
 }
 
 // Block 0 (scale set): the largest gradient.  The others: the copy of x.

@@ -64,3 +64,35 @@ def test_one_word(gpu):
         w, _ = tensor(r.standard_normal((H, 1)) * 20, "bfloat16")
         got = R.host(O.linearCrossEntropy(x, w, ints(np.zeros(50))))
         assert (got >= 0).all() and got.max() <= 13 * U, got.max()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("T,V", [(24, 16), (32, 300)])
+def test_gradients_lose_one_rounding_of_lse(gpu, dtype, T, V):
+    """lse is its value rounded once, and the probabilities are off by what that rounding is of
+    them: gradX's first component, the sum of dz over the words, is next to 0."""
+    r = np.random.default_rng(V)
+    g = np.ones(T)
+    h = R.HALF[dtype]
+    for size in (8.0, 60.0, 300.0, 2000.0):
+        for gap in (1.0, 8.0, 16.0):
+            x, w, xh, wh = case(r, T, V, 0.0, gap, dtype)
+            x, xh = tensor(np.stack([size * r.uniform(0.5, 1.0, T), np.ones(T)], 1), dtype)
+            t = np.full(T, V // 2)
+            lse, grad = O.linearCrossEntropy(x, w, ints(t), withLse=True)[1], tensor(g, "float32")[0]
+            z = xh @ wh
+            loss, e_loss = loss_and_bound(xh, wh, t)
+            want = loss + z[np.arange(T), t]
+            e_lse = U * np.abs(want) + e_loss
+            R.check(lse, want, e_lse)
+            dx, dw = O.linearCrossEntropyGrad(x, w, ints(t), lse, grad)
+            d = z - want[:, None]
+            dz = np.exp(d)
+            e_dz = dz * (e_lse[:, None] + (4 * np.abs(d) + 8) * U) + U
+            dz[np.arange(T), t] = np.expm1(-loss)
+            e_dz += (h * h + 6 * U) * np.abs(dz) + (2.0 ** -39 if dtype == "float16" else 0.0)
+            for got, a, b in ((dx, dz, wh.T), (dw, xh.T, dz)):
+                want = a @ b
+                off = np.abs(a) @ e_dz if b is dz else e_dz @ np.abs(b)
+                off += 2 * (max(T, V) + 8) * U * (np.abs(a) @ np.abs(b))
+                R.check(got, want, off + (h + 4 * U) * np.abs(want) + R.TINY[dtype])
