@@ -47,6 +47,14 @@ __device__ __forceinline__ void group_sum2(float& x, float& y, float2* tmp) {
   }
 }
 
+// The first pass leaves the mean as its roundings have it: (n / 1024 + some) steps off, which
+// rstd multiplies (a row of 1001 values of 1000.1: results 0.04 off).  The second sums the
+// deviations from it beside their squares: `rest`, their mean, is what it lacks.
+__device__ __forceinline__ float rstd_of(float square, float rest, float eps) {
+  const float var = square - rest * rest;
+  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+}
+
 // The runs of thread g of a row's group: where they start, and from which value on
 // they hold what no earlier run does (N: none).
 template <int G, int C, int N>
@@ -108,19 +116,20 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
       for (int e = 0; e < N; ++e) s += e >= run.own[c] ? f[c][e] : 0.0f;
     group_sum2<G>(s, q, tmp);
     const float mean = s * inv;
-    q = 0.0f;
+    s = q = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         f[c][e] -= mean;
+        s += e >= run.own[c] ? f[c][e] : 0.0f;
         q += e >= run.own[c] ? f[c][e] * f[c][e] : 0.0f;
       }
     group_sum2<G>(q, s, tmp);
-    const float rstd = 1.0f / sqrtf(q * inv + a.eps);
+    const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps);
     if (!there) continue;
     if (a.mean && g == 0) {
-      a.mean[row] = mean;
+      a.mean[row] = mean + rest;
       a.rstd[row] = rstd;
     }
 #pragma unroll
@@ -131,7 +140,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
         run_load<P, N>(a.beta, run.at[c], b[c]);
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[c][e] = f[c][e] * rstd * w[c][e] + b[c][e];
+      for (int e = 0; e < N; ++e) f[c][e] = (f[c][e] - rest) * rstd * w[c][e] + b[c][e];
       run_store<T, N>(a.y, base + run.at[c], f[c]);
     }
   }
@@ -160,15 +169,19 @@ __global__ void __launch_bounds__(kMaxGroup) norm_long_kernel(NormArgs a) {
   });
   group_sum2<kMaxGroup>(s, q, tmp);
   const float mean = s * inv;
-  q = 0.0f;
+  s = q = 0.0f;
   walk([&](int64_t, int own, float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) q += e >= own ? (v[e] - mean) * (v[e] - mean) : 0.0f;
+    for (int e = 0; e < N; ++e) {
+      const float d = v[e] - mean;
+      s += e >= own ? d : 0.0f;
+      q += e >= own ? d * d : 0.0f;
+    }
   });
   group_sum2<kMaxGroup>(q, s, tmp);
-  const float rstd = 1.0f / sqrtf(q * inv + a.eps);
+  const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps);
   if (a.mean && threadIdx.x == 0) {
-    a.mean[row] = mean;
+    a.mean[row] = mean + rest;
     a.rstd[row] = rstd;
   }
   walk([&](int64_t at, int, float (&v)[N]) {
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(kMaxGroup) norm_long_kernel(NormArgs a) {
     run_load<P, N>(a.gamma, at, w);
     run_load<P, N>(a.beta, at, b);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = (v[e] - mean) * rstd * w[e] + b[e];
+    for (int e = 0; e < N; ++e) v[e] = (v[e] - mean - rest) * rstd * w[e] + b[e];
     run_store<T, N>(a.y, row * n + at, v);
   });
 }
