@@ -14,6 +14,7 @@ from __future__ import annotations
 from ctypes import c_float
 from dataclasses import dataclass
 from functools import lru_cache
+from math import copysign
 from typing import NamedTuple, Sequence
 
 import numpy as np
@@ -993,12 +994,16 @@ _ROW_DTYPES = (DType.FLOAT32, DType.BFLOAT16, DType.FLOAT16)
 
 
 @lru_cache(maxsize=256)
-def _float_attr(op: str, name: str, value: float, positive: bool = False) -> tuple:
+def _float_text(op: str, name: str, value: float, sign: float, positive: bool) -> tuple:
     v = c_float(value).value  # (rounded to float32, to infinity past its range)
     if not abs(v) < float("inf") or positive and not v > 0.0:
         raise TensorError(f"{op}: {name} must be a {'positive' if positive else 'finite'} "
                           f"float32, got {value}")
     return name, repr(v)
+
+
+def _float_attr(op: str, name: str, value: float, positive: bool = False) -> tuple:
+    return _float_text(op, name, value, copysign(1.0, value), positive)  # (0.0 == -0.0)
 
 
 def _check_rows(op: str, t: Tensor) -> None:
