@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(NormGradArgs a, const f
                                                          int parts) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = (int64_t)blockIdx.x * 64 + lane;  // of the 2 n columns
+  const int64_t i = block_of() * 64 + lane;  // of the 2 n columns
   float s = 0.0f;
   if (i < 2 * a.n)
 #pragma unroll 4
@@ -502,8 +502,8 @@ int launch_norm_grad(const NormGradArgs& a, hipStream_t stream) {
                          dim3((unsigned)((runs + 255) / 256), parts), dim3(256), 0, stream, a, sums,
                          part, per);
     }
-    hipLaunchKernelGGL((norm_join_kernel<P>), dim3((unsigned)((2 * a.n + 63) / 64)), dim3(1024), 0,
-                       stream, a, part, parts);
+    hipLaunchKernelGGL((norm_join_kernel<P>), grid_of((2 * a.n + 63) / 64), dim3(1024), 0, stream,
+                       a, part, parts);
   });
   REW_HIP(hipGetLastError());
   return launches;

@@ -63,4 +63,14 @@ __device__ __forceinline__ void run_store(void* base, int64_t i, const float (&f
   *(RowRun<T, N>*)((typename T::elem*)base + i) = r;
 }
 
+// Workgroups 0 .. n - 1 (and up to 2^16 - 1 more) in rows of 2^16: the x of a launch takes
+// fewer than 2^32 threads.
+inline dim3 grid_of(int64_t n) {
+  const int64_t x = n < 1 << 16 ? (n > 0 ? n : 1) : 1 << 16;
+  return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_of() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 }  // namespace rew
