@@ -115,14 +115,15 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t*
   constexpr int kOneByOne = 8;    // tokens of 64 (0, all rows at once always: 22 us for 15)
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t sorts = (uint32_t)((V + kSortRows - 1) / kSortRows);
-  if (blockIdx.x >= sorts) {
-    const int64_t at = ((int64_t)(blockIdx.x - sorts) * kSortThreads + tid) * 16;
+  const int64_t block = block_of();
+  if (block >= sorts) {
+    const int64_t at = ((block - sorts) * kSortThreads + tid) * 16;
     if (at + 16 <= bytes) *(uint4*)(out + at) = make_uint4(0, 0, 0, 0);
     else
       for (int64_t i = at; i < bytes; i += 2) *(uint16_t*)(out + i) = 0;
     return;
   }
-  const int64_t lo = (int64_t)blockIdx.x * kSortRows;
+  const int64_t lo = block * kSortRows;
   const int rows = (int)min((int64_t)kSortRows, V - lo);
   const int64_t per = ((T + kSortWaves - 1) / kSortWaves + 63) & ~(int64_t)63;
   const int64_t t0 = min((int64_t)wave * per, T), t1 = min(t0 + per, T);
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
                                                              uint32_t window_blocks, int lanes,
                                                              int rows) {
   __shared__ int32_t first[kThreads + 1];
+  const int64_t block = block_of();
   const int lane = threadIdx.x % lanes, own = threadIdx.x / lanes, groups = kThreads / lanes;
   const int64_t slab = (int64_t)lanes * N;  // columns
   auto store = [&](int64_t v, int64_t c, float (&s)[N]) {
@@ -258,15 +260,15 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
     for (int x = 0; x < N; ++x) s[x] *= a.scale;
     run_store<T, N>(a.out, v * a.E + c, s);
   };
-  if (blockIdx.x < window_blocks) {
+  if (block < window_blocks) {
     __shared__ float tmp[kThreads][N];
     __shared__ int32_t row_of[kWindow];
     __shared__ int n_rows;
     const uint32_t slabs = (uint32_t)((a.E + slab - 1) / slab);
-    const int64_t j = blockIdx.x / slabs;
-    const int64_t c = run_start((int64_t)(blockIdx.x % slabs) * slab + lane * N, a.E, N);
+    const uint32_t j = (uint32_t)block / slabs, s0 = (uint32_t)block % slabs;
+    const int64_t c = run_start(s0 * slab + lane * N, a.E, N);
     const int32_t n = w.first[a.V];
-    const int64_t q = j * kWindow;
+    const int64_t q = (int64_t)j * kWindow;
     if (q >= n) return;
     const int32_t q0 = (int32_t)q, q1 = (int32_t)min(q + kWindow, (int64_t)n);
     if (threadIdx.x < 64) {
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
         if (p0 >= q0 && p1 <= q1) {
           store(v, c, s);
         } else {
-          float* out = w.part + (j * 2 + (p0 >= q0)) * a.E + c;
+          float* out = w.part + ((int64_t)j * 2 + (p0 >= q0)) * a.E + c;
 #pragma unroll
           for (int x = 0; x < N; ++x) out[x] = s[x];
         }
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
   if (rows == 0) {
     __shared__ int32_t row_of[kPlaces], end[kPlaces];
     const int32_t n = w.first[a.V];
-    const int64_t q = (int64_t)(blockIdx.x - window_blocks) * kPlaces;
+    const int64_t q = (block - window_blocks) * kPlaces;
     if (q >= n) return;
     if (threadIdx.x < kPlaces) {
       const int32_t p = (int32_t)min(q + threadIdx.x, (int64_t)n - 1);
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(EmbedGradArgs a, Gr
     }
     return;
   }
-  const int64_t v0 = (int64_t)(blockIdx.x - window_blocks) * rows;
+  const int64_t v0 = (block - window_blocks) * rows;
   const int here = (int)min((int64_t)rows, a.V - v0);
   for (int i = threadIdx.x; i <= here; i += kThreads) first[i] = w.first[v0 + i];
   __syncthreads();
@@ -402,8 +404,7 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
   const int64_t bytes = clear ? table : 0;
   const int64_t sorts = (a.V + kSortRows - 1) / kSortRows;
   constexpr int64_t kCleared = 16 * kSortThreads;  // bytes of a workgroup
-  hipLaunchKernelGGL(embed_sort_kernel,
-                     dim3((unsigned)(sorts + (bytes + kCleared - 1) / kCleared)),
+  hipLaunchKernelGGL(embed_sort_kernel, grid_of(sorts + (bytes + kCleared - 1) / kCleared),
                      dim3(kSortThreads), 0, stream, a.ids, a.T, a.V, w, (uint8_t*)a.out, bytes);
   if (a.T == 0 && clear) {
     REW_HIP(hipGetLastError());
@@ -425,7 +426,7 @@ int launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
         windows * slabs + (clear ? (a.T + kPlaces - 1) / kPlaces : (a.V + rows - 1) / rows);
     auto sum = [&](auto together) {
       hipLaunchKernelGGL((embed_sum_kernel<Ty, N, decltype(together)::value>),
-                         dim3((unsigned)blocks), dim3(kThreads), 0, stream, a, w,
+                         grid_of(blocks), dim3(kThreads), 0, stream, a, w,
                          (uint32_t)(windows * slabs), lanes, rows);
     };
     if (slabs >= 4) sum(std::integral_constant<int, 4>());

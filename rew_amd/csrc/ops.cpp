@@ -506,6 +506,8 @@ static void prepare_embed(const std::string& op, const std::vector<Tensor*>& ins
               " for ids " + ids->shape.str());
     n->i0 = parse_int(find_attr(attrs, "vocab", op), op);
     if (n->i0 < 1 || n->i0 >= kMaxElems) invalid("eager '" + op + "': vocab must be positive");
+    if (ids->numel() >= (int64_t)1 << 30)  // (a launch takes 4 threads for each)
+      fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': fewer than 2^30 ids");
     outs.push_back({rows->dt, Shape(std::vector<int64_t>{n->i0, shape.back()})});
     n->tail = embed_grad_ws_bytes(ids->numel(), n->i0, shape.back());
   }

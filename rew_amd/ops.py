@@ -14,7 +14,7 @@ from __future__ import annotations
 from ctypes import c_float
 from dataclasses import dataclass
 from functools import lru_cache
-from math import copysign
+from math import copysign, prod
 from typing import NamedTuple, Sequence
 
 import numpy as np
@@ -1035,7 +1035,8 @@ def embeddingGrad(ids: Tensor, gradOut: Tensor, vocab: int, scale: float = 1.0) 
     """The gradient [vocab, embed] of ``embedding``'s weight for the gradient ``gradOut``
     [*ids.shape, embed] of its result: row v is scale times the sum of gradOut over the places
     of ids that hold v, in their order (rows of many places: in parts), zeros where none does.
-    Places with an id outside [0, vocab) take no part, whatever their gradOut."""
+    Places with an id outside [0, vocab) take no part, whatever their gradOut.  Fewer than
+    2^30 places."""
     op = "embeddingGrad"
     if len(gradOut.shape) < 1 or tuple(gradOut.shape[:-1]) != tuple(ids.shape):
         raise TensorError(f"{op}: gradOut must be [*ids.shape, embed], got "
@@ -1044,6 +1045,8 @@ def embeddingGrad(ids: Tensor, gradOut: Tensor, vocab: int, scale: float = 1.0) 
     _check_ids(op, ids, gradOut.shape[-1])
     if vocab < 1:
         raise TensorError(f"{op}: vocab must be positive, got {vocab}")
+    if prod(ids.shape) >= 2 ** 30:
+        raise TensorError(f"{op}: fewer than 2^30 ids, got {list(ids.shape)}")
     return _packed_call(op, [ids, gradOut], [("vocab", str(int(vocab))),
                                              _float_attr(op, "scale", scale)], 1)[0]
 
