@@ -579,6 +579,8 @@ static void prepare_xent(const std::string& op, const std::vector<Tensor*>& ins,
   if (H < 1 || V < 1) invalid("eager '" + op + "': embed and vocab must be positive");
   if (H > (1 << 21) || V > (1 << 21))
     fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': embed and vocab up to 2^21");
+  if (T >= (int64_t)1 << 30)  // (a launch takes 4 threads for each)
+    fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': fewer than 2^30 tokens");
   check_i32(ins[2], 1, "targets", op);
   const Shape rows(std::vector<int64_t>{T});
   if (ins[2]->shape != rows)

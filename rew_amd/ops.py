@@ -1118,6 +1118,8 @@ def _check_head(op: str, x: Tensor, weight: Tensor, targets: Tensor, tied: bool)
                           f"({'[vocab, embed]' if tied else '[embed, vocab]'}) differ in embed")
     if not all(1 <= d <= 2 ** 21 for d in weight.shape):
         raise TensorError(f"{op}: embed and vocab must be 1 to 2^21, got {list(weight.shape)}")
+    if x.shape[0] >= 2 ** 30:
+        raise TensorError(f"{op}: fewer than 2^30 tokens, got {x.shape[0]}")
     _check_i32(op, targets, "targets", (x.shape[0],))
 
 
