@@ -3503,7 +3503,7 @@ void Lower::emit_packed_attn(Node* n) {
     a.starts = (const int32_t*)n->in[4]->data();
     a.lens = (const int32_t*)n->in[5]->data();
     a.pages = k->shape.d[0];
-    a.work = (float*)tensor_tail(n->out[0]);
+    a.work = (float*)tensor_work(n->out[0]);
     a.max_new = n->i2;
     a.n_seq = (int)table->shape.d[0];
     a.width = (int)table->shape.d[1];
@@ -3519,6 +3519,7 @@ void Lower::emit_packed_attn(Node* n) {
   Launch L{a};
   if (c->profiling) L.name = packed_attn_variant(a) + heads_label(a.T, a.H, a.Hkv, a.D);
   run_launch(c, std::move(L));
+  tensor_drop_work(n->out[0]);
 }
 
 void Lower::emit_packed_grad(Node* n) {
@@ -3539,7 +3540,7 @@ void Lower::emit_packed_grad(Node* n) {
   a.dq = n->out[0]->data();
   a.dk = n->out[1]->data();
   a.dv = n->out[2]->data();
-  a.work = tensor_tail(n->out[0]);
+  a.work = tensor_work(n->out[0]);
   a.T = q->shape.d[0];
   a.H = (int)q->shape.d[1];
   a.Hkv = (int)k->shape.d[1];
@@ -3550,6 +3551,7 @@ void Lower::emit_packed_grad(Node* n) {
   Launch L{a};
   if (c->profiling) L.name = "packed_attn_grad" + heads_label(a.T, a.H, a.Hkv, a.D);
   run_launch(c, std::move(L));
+  tensor_drop_work(n->out[0]);
 }
 
 void Lower::emit_page_tables(Node* n) {
@@ -3598,7 +3600,7 @@ void Lower::emit_embed(Node* n) {
     std::memset(&a, 0, sizeof a);
     fill(a);
     a.grad = n->in[1]->data();
-    a.work = tensor_tail(n->out[0]);
+    a.work = tensor_work(n->out[0]);
     L.args = a;
   } else {
     EmbedArgs a;
@@ -3611,6 +3613,7 @@ void Lower::emit_embed(Node* n) {
     L.name = (n->sub ? "embed_grad" : "embed") +
              sizes_label({ids->numel(), table->shape.d[0], table->shape.d[1]});
   run_launch(c, std::move(L));
+  tensor_drop_work(n->out[0]);
 }
 
 // layerNorm: x, gamma, beta; layerNormGrad (sub 1): x, gamma, mean, rstd, gradOut.
@@ -3637,7 +3640,7 @@ void Lower::emit_norm(Node* n) {
     a.dx = n->out[0]->data();
     a.dgamma = n->out[1]->data();
     a.dbeta = n->out[2]->data();
-    a.work = (float*)tensor_tail(n->out[0]);
+    a.work = (float*)tensor_work(n->out[0]);
     L.args = a;
   } else {
     NormArgs a;
@@ -3656,6 +3659,7 @@ void Lower::emit_norm(Node* n) {
     L.name = (n->sub ? "layer_norm_grad" : "layer_norm") +
              sizes_label({x->numel() / gamma->numel(), gamma->numel()});
   run_launch(c, std::move(L));
+  tensor_drop_work(n->out[0]);
 }
 
 // linearCrossEntropy: x, weight, targets; linearCrossEntropyGrad (sub 1): x,
@@ -3674,7 +3678,7 @@ void Lower::emit_xent(Node* n) {
     a.V = w->shape.d[tied ? 0 : 1];
     a.tied = tied;
     a.f16 = x->dt == kF16;
-    a.work = tensor_tail(n->out[0]);
+    a.work = tensor_work(n->out[0]);
   };
   Launch L;
   if (n->sub) {
@@ -3698,6 +3702,7 @@ void Lower::emit_xent(Node* n) {
     L.name = (n->sub ? "cross_entropy_grad" : "cross_entropy") +
              sizes_label({x->shape.d[0], x->shape.d[1], w->shape.d[tied ? 0 : 1]});
   run_launch(c, std::move(L));
+  tensor_drop_work(n->out[0]);
 }
 
 void Lower::emit_trisolve(Node* n) {

@@ -389,7 +389,7 @@ static void prepare_packed_attn(const std::string& op, const std::vector<Tensor*
     invalid("eager '" + op + "': lse must be float32 [tokens, heads]");
   if (rest->dt != kI8 || rest->shape != q->shape)
     invalid("eager '" + op + "': rest must be int8 of q's shape");
-  n->tail = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1], (int)k->shape.d[1],
+  n->work = packed_grad_ws_bytes(q->shape.d[0], (int)q->shape.d[1], (int)k->shape.d[1],
                                  q->dt == kF16);
   outs.push_back({q->dt, q->shape});
   outs.push_back({k->dt, k->shape});
@@ -428,7 +428,7 @@ static void prepare_paged_attn(const std::string& op, const std::vector<Tensor*>
   a.width = (int)table->shape.d[1];
   a.log_page = page_log2(kp->shape.d[2], op);
   a.max_new = n->i2;
-  n->tail = paged_ws_bytes(a);
+  n->work = paged_ws_bytes(a);
   outs.push_back({q->dt, q->shape});
 }
 
@@ -509,7 +509,7 @@ static void prepare_embed(const std::string& op, const std::vector<Tensor*>& ins
     if (ids->numel() >= (int64_t)1 << 30)  // (a launch takes 4 threads for each)
       fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': fewer than 2^30 ids");
     outs.push_back({rows->dt, Shape(std::vector<int64_t>{n->i0, shape.back()})});
-    n->tail = embed_grad_ws_bytes(ids->numel(), n->i0, shape.back());
+    n->work = embed_grad_ws_bytes(ids->numel(), n->i0, shape.back());
   }
   if (shape.back() < 1 || shape.back() > (1 << 20))
     fail(REW_MI355X_ERR_UNSUPPORTED, "eager '" + op + "': rows must have 1 to 2^20 values");
@@ -549,7 +549,7 @@ static void prepare_norm(const std::string& op, const std::vector<Tensor*>& ins,
       invalid("eager '" + op + "': mean and rstd must be float32 " + rows.str());
   if (ins[4]->dt != x->dt || ins[4]->shape != x->shape)
     invalid("eager '" + op + "': gradOut must have x's dtype and shape");
-  n->tail = norm_grad_ws_bytes(x->numel() / gamma->numel(), gamma->numel());
+  n->work = norm_grad_ws_bytes(x->numel() / gamma->numel(), gamma->numel());
   outs.push_back({x->dt, x->shape});
   outs.push_back({gamma->dt, gamma->shape});
   outs.push_back({gamma->dt, gamma->shape});
@@ -590,7 +590,7 @@ static void prepare_xent(const std::string& op, const std::vector<Tensor*>& ins,
     XentArgs a;
     std::memset(&a, 0, sizeof a);
     a.T = T, a.H = H, a.V = V, a.tied = tied;
-    n->tail = xent_ws_bytes(a);
+    n->work = xent_ws_bytes(a);
     outs.push_back({kF32, rows});
     if (flag_attr(attrs, "stats", op)) outs.push_back({kF32, rows});
     return;
@@ -602,7 +602,7 @@ static void prepare_xent(const std::string& op, const std::vector<Tensor*>& ins,
   XentGradArgs a;
   std::memset(&a, 0, sizeof a);
   a.T = T, a.H = H, a.V = V, a.tied = tied;
-  n->tail = xent_grad_ws_bytes(a);
+  n->work = xent_grad_ws_bytes(a);
   outs.push_back({x->dt, x->shape});
   outs.push_back({w->dt, w->shape});
 }
@@ -1518,7 +1518,7 @@ std::vector<Tensor*> commit_node(Ctx* c, Node* n, const std::vector<Tensor*>& in
     t->prod = n;
     t->prod_out = (int)i;
     t->ext = 1;
-    if (i == 0) t->tail = n->tail;
+    if (i == 0) t->work = n->work;
     n->out.push_back(t);
     result.push_back(t);
   }

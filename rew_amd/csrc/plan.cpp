@@ -357,6 +357,8 @@ void plan_note_alloc(Tensor* t) {
   e.id = r->plan->n_slots++;
   const uintptr_t p = (uintptr_t)t->st->ptr;
   r->live[p] = {p + t->st->bytes, e.id};
+  if (const uintptr_t w = (uintptr_t)t->st->work)
+    r->live[w] = {w + t->st->work_bytes, r->plan->n_slots++};
   r->plan->events.push_back(e);
 }
 
@@ -373,17 +375,19 @@ void plan_note_alias(Tensor* t, Tensor* src) {
   r->plan->events.push_back(e);
 }
 
-void plan_note_drop(Tensor* t) {
+static void note_drop(Tensor* t, PlanEvent e) {
   PlanRecorder* r = t->ctx->rec;
   if (!r) return;
-  PlanEvent e;
-  e.type = PlanEvent::DROP;
   if (!r->find(t, &e.a)) {
     r->ok = false;
     return;
   }
   r->plan->events.push_back(e);
 }
+
+void plan_note_drop(Tensor* t) { note_drop(t, PlanEvent{PlanEvent::DROP}); }
+
+void plan_note_drop_work(Tensor* t) { note_drop(t, PlanEvent{PlanEvent::DROP_WORK}); }
 
 void plan_note_destroy(Tensor* t) {
   PlanRecorder* r = t->ctx->rec;
@@ -398,10 +402,10 @@ void plan_note_destroy(Tensor* t) {
   r->plan->events.push_back(e);
 }
 
-void plan_note_free(Storage* s) {
-  PlanRecorder* r = s->ctx->rec;
+void plan_note_free(Ctx* c, const void* p) {
+  PlanRecorder* r = c->rec;
   if (!r) return;
-  r->live.erase((uintptr_t)s->ptr);
+  r->live.erase((uintptr_t)p);
 }
 
 void run_launch(Ctx* c, Launch&& L) {
@@ -632,10 +636,12 @@ void replay_events(Ctx* c, const FlushPlan& p, const std::vector<Tensor*>& leave
           if (t->st) throw Error(REW_MI355X_ERR_INVALID, "internal: flush plan out of step");
           tensor_alloc(t);
           slot[e.id] = (uintptr_t)t->data();
+          if (tensor_work(t)) slot[e.id + 1] = (uintptr_t)tensor_work(t);
           break;
         }
         case PlanEvent::ALIAS: tensor_alias(get(e.a), get(e.b)); break;
         case PlanEvent::DROP: tensor_drop_storage(get(e.a)); break;
+        case PlanEvent::DROP_WORK: tensor_drop_work(get(e.a)); break;
         case PlanEvent::DESTROY: {
           Tensor*& t = temps[e.a.idx];
           if (t) {

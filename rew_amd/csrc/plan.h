@@ -83,10 +83,11 @@ struct PlanRef {
 };
 
 struct PlanEvent {
-  enum : int8_t { NEW, ALIAS, DROP, DESTROY, LAUNCH } type;
-  PlanRef a{};     // NEW / DROP / DESTROY: the tensor; ALIAS: the new alias
+  enum : int8_t { NEW, ALIAS, DROP, DROP_WORK, DESTROY, LAUNCH } type;
+  PlanRef a{};     // NEW / DROP / DROP_WORK / DESTROY: the tensor; ALIAS: the new alias
   PlanRef b{};     // ALIAS: the tensor aliased
-  int32_t id = 0;  // NEW: storage slot created; LAUNCH: index into launches
+  int32_t id = 0;  // NEW: storage slot created (and the next one for working memory);
+                   // LAUNCH: index into launches
 };
 
 // A device pointer of a recorded launch: byte `delta` into storage `slot`

@@ -113,16 +113,37 @@ void tensor_alloc(Tensor* t) {
   if (t->st) return;
   Storage* s = new Storage();
   s->ctx = t->ctx;
-  size_t bytes = (size_t)t->nbytes();
-  if (t->tail) bytes = tensor_tail_offset(t) + t->tail;
-  s->ptr = t->ctx->alloc.get(bytes, &s->bytes);
+  try {
+    s->ptr = t->ctx->alloc.get((size_t)t->nbytes(), &s->bytes);
+    if (t->work) s->work = t->ctx->alloc.get(t->work, &s->work_bytes);
+  } catch (...) {
+    if (s->ptr) t->ctx->alloc.put(s->ptr, s->bytes);
+    delete s;
+    throw;
+  }
   s->refs = 1;
   t->st = s;
   if (t->ctx->rec) plan_note_alloc(t);
 }
 
-void* tensor_tail(const Tensor* t) {
-  return t->tail ? (char*)t->data() + tensor_tail_offset(t) : nullptr;
+static void storage_free_work(Storage* s) {
+  if (!s->work) return;
+  if (s->ctx->rec) plan_note_free(s->ctx, s->work);
+  s->ctx->alloc.put(s->work, s->work_bytes);
+  s->work = nullptr;
+}
+
+static void storage_free(Storage* s) {
+  storage_free_work(s);
+  if (s->ctx->rec) plan_note_free(s->ctx, s->ptr);
+  s->ctx->alloc.put(s->ptr, s->bytes);
+  delete s;
+}
+
+void tensor_drop_work(Tensor* t) {
+  if (!tensor_work(t)) return;
+  if (t->ctx->rec) plan_note_drop_work(t);
+  if (!being_captured(t->ctx->stream)) storage_free_work(t->st);
 }
 
 void tensor_alias(Tensor* t, Tensor* src) {
@@ -133,11 +154,7 @@ void tensor_alias(Tensor* t, Tensor* src) {
 }
 
 void storage_release(Storage* s) {
-  if (s && --s->refs == 0) {
-    if (s->ctx->rec) plan_note_free(s);
-    s->ctx->alloc.put(s->ptr, s->bytes);
-    delete s;
-  }
+  if (s && --s->refs == 0) storage_free(s);
 }
 
 void const_cache_clear(Ctx* c) {
@@ -150,11 +167,7 @@ void tensor_drop_storage(Tensor* t) {
   if (!s) return;
   if (t->ctx->rec) plan_note_drop(t);
   t->st = nullptr;
-  if (--s->refs == 0) {
-    if (s->ctx->rec) plan_note_free(s);
-    s->ctx->alloc.put(s->ptr, s->bytes);
-    delete s;
-  }
+  if (--s->refs == 0) storage_free(s);
 }
 
 void maybe_destroy(Tensor* t) {

@@ -28,6 +28,11 @@ struct Storage {
   Ctx* ctx = nullptr;
   void* ptr = nullptr;
   size_t bytes = 0;   // rounded block size
+  // working memory of the launch that writes the data: a block of its own, returned right
+  // behind the launch.  One that is captured into a graph keeps it, as long as the storage
+  // lives, so graphs never share it with each other or with calls made later.
+  void* work = nullptr;
+  size_t work_bytes = 0;
   int refs = 0;
 };
 
@@ -41,9 +46,7 @@ struct Tensor {
   Storage* st = nullptr;    // dense row-major data once materialized
   Node* prod = nullptr;     // pending producer, nullptr once materialized
   int prod_out = 0;         // which output of `prod`
-  size_t tail = 0;          // bytes of working memory behind the data, for the launch that
-                            // writes it: they live as long as the tensor, so launches captured
-                            // into different graphs never share them
+  size_t work = 0;          // bytes of Storage::work that its launch needs
   bool writable = false;    // made by rew_mi355x_alloc: an op may update it in place
   bool has_host = false;    // small constant whose bytes are known on host
   uint8_t host[16] = {0};
@@ -92,7 +95,7 @@ struct Node {
   int64_t i0 = 0, i1 = 0, i2 = 0;
   int dt_attr = -1;
   int cmp = 0;
-  size_t tail = 0;          // output 0's Tensor::tail
+  size_t work = 0;          // output 0's Tensor::work
   int n_in_keep = -1;       // >= 0: only the first n_in_keep operands are read
                             // (the rest only fix static shapes)
   // planner scratch
@@ -179,12 +182,10 @@ struct Ctx {
 // ---- runtime services (runtime.cpp) -----------------------------------------
 Tensor* new_tensor(Ctx* c, int dt, const Shape& s);
 void tensor_alloc(Tensor* t);                 // give t fresh storage
-// where t's working memory starts in its storage (256-byte aligned)
-inline size_t tensor_tail_offset(const Tensor* t) {
-  return ((size_t)t->nbytes() + 255) & ~(size_t)255;
-}
-// .. as an address; null without any (a plan keeps no address outside its blocks)
-void* tensor_tail(const Tensor* t);
+// t's working memory; null without any (a plan keeps no address outside its blocks)
+inline void* tensor_work(const Tensor* t) { return t->st ? t->st->work : nullptr; }
+// Returns it to the allocator; to be called behind the launch that uses it.
+void tensor_drop_work(Tensor* t);
 void storage_release(Storage* s);             // drop one reference
 void const_cache_clear(Ctx* c);               // release every cached constant
 void tensor_alias(Tensor* t, Tensor* src);    // share src's storage
@@ -197,8 +198,9 @@ bool tensor_is_live_handle(const Tensor* t);
 void plan_note_alloc(Tensor* t);               // t just received fresh storage
 void plan_note_alias(Tensor* t, Tensor* src);  // t now shares src's storage
 void plan_note_drop(Tensor* t);                // t is about to drop its storage
+void plan_note_drop_work(Tensor* t);           // t's working memory is no longer needed
 void plan_note_destroy(Tensor* t);             // t is about to be deleted
-void plan_note_free(Storage* s);               // s is about to return to the allocator
+void plan_note_free(Ctx* c, const void* p);    // a block is about to return to the allocator
 
 // Stream-ordered copy of a small host table into device memory (through
 // the pinned staging ring; `src` may be reused as soon as this returns).
