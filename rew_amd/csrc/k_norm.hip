@@ -5,9 +5,9 @@
 // first pass (mean) to the last: it is read once.  Thread i of the group holds
 // the runs i, i + G, ... of 16 bytes (rows_device.h).
 //
-// Bound: HBM.  8192 x 4096 bfloat16 with float32 gamma: forward 30 us (4.4 TB/s),
+// Bound: HBM.  8192 x 4096 bfloat16 with float32 gamma: forward 31 us (4.3 TB/s),
 // gradients 42 (4.8, their inputs partly in the caches) and 4 for the join.
-// 300 x 20000 float16: 12.8, and 7.2 + 12.9 + 3.9, where a launch of a few rows on
+// 300 x 20000 float16: 13.3, and 7.4 + 13.5 + 3.9, where a launch of a few rows on
 // each CU is a chain of a row's load, two joined sums and its store.
 #include <hip/hip_runtime.h>
 
@@ -122,11 +122,12 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         f[c][e] -= mean;
-        s += e >= run.own[c] ? f[c][e] : 0.0f;
-        q += e >= run.own[c] ? f[c][e] * f[c][e] : 0.0f;
+        const float d = e >= run.own[c] ? f[c][e] : 0.0f;
+        s += d;
+        q = __builtin_fmaf(d, d, q);
       }
     group_sum2<G>(q, s, tmp);
-    const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps);
+    const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps), shift = -rest * rstd;
     if (!there) continue;
     if (a.mean && g == 0) {
       a.mean[row] = mean + rest;
@@ -140,7 +141,8 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_kernel(NormArgs a) {
         run_load<P, N>(a.beta, run.at[c], b[c]);
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[c][e] = (f[c][e] - rest) * rstd * w[c][e] + b[c][e];
+      for (int e = 0; e < N; ++e)
+        f[c][e] = __builtin_fmaf(__builtin_fmaf(f[c][e], rstd, shift), w[c][e], b[c][e]);
       run_store<T, N>(a.y, base + run.at[c], f[c]);
     }
   }
@@ -173,13 +175,13 @@ __global__ void __launch_bounds__(kMaxGroup) norm_long_kernel(NormArgs a) {
   walk([&](int64_t, int own, float (&v)[N]) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float d = v[e] - mean;
-      s += e >= own ? d : 0.0f;
-      q += e >= own ? d * d : 0.0f;
+      const float d = e >= own ? v[e] - mean : 0.0f;
+      s += d;
+      q = __builtin_fmaf(d, d, q);
     }
   });
   group_sum2<kMaxGroup>(q, s, tmp);
-  const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps);
+  const float rest = s * inv, rstd = rstd_of(q * inv, rest, a.eps), shift = -rest * rstd;
   if (a.mean && threadIdx.x == 0) {
     a.mean[row] = mean + rest;
     a.rstd[row] = rstd;
@@ -189,7 +191,8 @@ __global__ void __launch_bounds__(kMaxGroup) norm_long_kernel(NormArgs a) {
     run_load<P, N>(a.gamma, at, w);
     run_load<P, N>(a.beta, at, b);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = (v[e] - mean - rest) * rstd * w[e] + b[e];
+    for (int e = 0; e < N; ++e)
+      v[e] = __builtin_fmaf(__builtin_fmaf(v[e] - mean, rstd, shift), w[e], b[e]);
     run_store<T, N>(a.y, row * n + at, v);
   });
 }
