@@ -50,9 +50,13 @@ __device__ __forceinline__ void group_sum2(float& x, float& y, float2* tmp) {
 // The first pass leaves the mean as its roundings have it: (n / 1024 + some) steps off, which
 // rstd multiplies (a row of 1001 values of 1000.1: results 0.04 off).  The second sums the
 // deviations from it beside their squares: `rest`, their mean, is what it lacks.
+// (A row of equal values, and eps far below what is left of its variance: not less than
+// 2^-20 of the square taken away, some steps of it, so that rstd does not blow up `rest`'s
+// own rounding.)
 __device__ __forceinline__ float rstd_of(float square, float rest, float eps) {
-  const float var = square - rest * rest;
-  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+  const float away = fminf(rest * rest, 3.402823466e38f);  // (an infinite square stays so)
+  const float var = square - away, least = away * 0x1p-20f;
+  return 1.0f / sqrtf((var < least ? least : var) + eps);
 }
 
 // The runs of thread g of a row's group: where they start, and from which value on

@@ -70,3 +70,18 @@ def test_rows_far_from_zero(gpu, n, shift, std):
     e_h = rstd * (e_rest + U * (2 * np.abs(d) + first)) + np.abs(h) * (e_rstd + U)
     want = h * gh + bh
     R.check(y, want, np.abs(gh) * (e_h + U * np.abs(h)) + U * (np.abs(h * gh) + 2 * np.abs(want)))
+
+
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("eps", [1e-12, 1e-30])
+def test_equal_values_and_a_small_eps(gpu, n, eps):
+    """beta, to c U of the deviations over at least 2^-10 of them; also where their squares are
+    infinite."""
+    values = np.array([1000.1, -333.3, 0.1, 7.7e4, 3.3e-3, 0.0, 1.1e12, 1.1e30, -2.2e33])
+    x, xh = tensor(np.repeat(values[:, None], n, 1), "float32")
+    g, gh = tensor(np.linspace(0.5, 1.5, n), "float32")
+    b, bh = tensor(np.linspace(-1, 1, n), "float32")
+    got = R.host(O.layerNorm(x, g, b, eps))
+    c = chain(n)
+    assert (np.abs(got - bh) <= 1.1 * (c + 4) * U * 2.0 ** 10 * gh + 4 * U).all(), \
+        np.abs(got - bh).max()
