@@ -103,8 +103,11 @@ GradWork grad_work(const EmbedGradArgs& a) {
 // Workgroup b places the tokens of rows [512 b, 512 b + 512): every wave walks
 // its own sixteenth of the ids, counts (LDS atomics on counts, whose order does
 // not show), and, once all counts are summed, walks it again and puts each
-// token behind those of the same row before it.  Reading all ids in each of
-// V / 512 workgroups costs less than the several launches of a sort by digits.
+// token behind those of the same row before it.  All ids are read by each of V / 512
+// workgroups: one launch, whose time grows with T, and with V from 256 workgroups on.
+// (us, rows 500 / 32000 / 128256 / 2^20: 300 ids 5 / 6 / 6 / 22, 16384 ids 22 / 18 / 15 /
+// 54, 131072 ids 148 / 113 / 88 / 326, 2^20 ids 1175 / 771 / 628 / 2317.  With 2^20 ids the
+// gradient of 128256 x 4096 bfloat16 moves 9.6 GB, 2 ms; a sort by digits was not built.)
 // The workgroups behind them clear `bytes` of `out`, 16 by each thread.
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const int32_t* ids, int64_t T,
                                                                   int64_t V, GradWork w,

@@ -5,7 +5,7 @@
 // first pass (mean) to the last: it is read once.  Thread i of the group holds
 // the runs i, i + G, ... of 16 bytes (rows_device.h).
 //
-// Bound: HBM.  8192 x 4096 bfloat16 with float32 gamma: forward 31 us (4.3 TB/s),
+// Bound: HBM.  8192 x 4096 bfloat16 with float32 gamma: forward 30 us (4.4 TB/s),
 // gradients 42 (4.8, their inputs partly in the caches) and 4 for the join.
 // 300 x 20000 float16: 13.3, and 7.4 + 13.5 + 3.9, where a launch of a few rows on
 // each CU is a chain of a row's load, two joined sums and its store.

@@ -12,7 +12,7 @@
 // it: dw's columns of the piece, x^T dz, are finished there; dx = dz w^T is
 // added up over the pieces in float32.
 //
-// Bound: the matrix cores.  8192 x 4096 x 128256 bfloat16: the logits in 6.27 ms
+// Bound: the matrix cores.  8192 x 4096 x 128256 bfloat16: the logits in 6.23 ms
 // (1.37 PFLOP/s, as a large library product), matrix cores busy 78 % of the cycles
 // at 1.66 GHz; per piece of 16384 words dz 0.86 ms, dw 0.81, dx 0.87 (1.28, 1.36 and
 // 1.26 PFLOP/s; 67-75 %: dz's 270 MB of stores, dx's read and written sums).
@@ -43,7 +43,10 @@ constexpr float kLn2 = 0.693147180559945309417f;
 constexpr float kLn2Rest = (float)(1.0 / (double)kLog2e - (double)kLn2);
 constexpr float kMost = 3.402823466e38f;
 // dz is stored as 2^14 g / max|g| (p - 1): below 2^14, so float16 keeps eleven
-// bits of probabilities down to 2^-28 and the float32 sums have room.
+// bits of probabilities down to 2^-28 and the float32 sums have room.  (Its rounding makes
+// the gradients' error 0.0022 for the 0.0017 of their own in bfloat16, 0.00028 for 0.00021
+// in float16, relative to their norm; keeping the remainders of every token would double
+// the k-steps of two of the three products.)
 constexpr float kDzScale = 16384.0f;
 // The gradients of few tokens are sums of few terms that matter, which do not average
 // dz's rounding (2 tokens, 64 x 2 bfloat16: dx 0.0036 off relative to its norm, of which

@@ -1147,8 +1147,9 @@ def linearCrossEntropyGrad(x: Tensor, weight: Tensor, targets: Tensor, lse: Tens
     of the dtypes of x and weight.  The logits are formed anew, a piece of the vocabulary at a
     time.  Their gradient is rounded once to x's dtype for the two products, relative to the
     largest |gradLoss|, whose scale is applied to the float32 sums (float16 loses what is below
-    2^-39 of it); with up to 32 tokens what that rounding leaves is kept too.  Tokens without a target in [0, vocab) take no part, whatever their x and
-    gradLoss: their gradX is 0."""
+    2^-39 of it); with up to 32 tokens what that rounding leaves is kept too.  lse's own
+    rounding, a step of its size, is a relative error of every probability.  Tokens without a
+    target in [0, vocab) take no part, whatever their x and gradLoss: their gradX is 0."""
     op = "linearCrossEntropyGrad"
     _check_head(op, x, weight, targets, tied)
     for t, name in ((lse, "lse"), (gradLoss, "gradLoss")):
