@@ -1,5 +1,10 @@
 """GPU checks of what the sequence and training ops hold in device memory: their working memory is
 returned behind the launch, whatever becomes of the result; a captured call keeps its own."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -122,3 +127,60 @@ def test_captured_calls_keep_theirs(made, name, recorded):
         del between, o, b
     del out
     assert in_use() - before <= 8192
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_op_by_op(made, name):
+    call, _ = made[name]
+    want = [E.toHost(t) for t in call()]
+    before = in_use()
+    E.setMode(E.MODE_OP_BY_OP)
+    try:
+        for _ in range(2):
+            got = call()
+            for g, w in zip(got, want):
+                np.testing.assert_array_equal(E.toHost(g), w)
+    finally:
+        E.setMode(E.MODE_DEFERRED)
+    del g
+    assert in_use() - before <= 1.25 * held(got) + 8192
+
+
+CHILD = r"""
+import sys
+import numpy as np
+sys.path.insert(0, sys.argv[1])
+from rew_amd import eager as E, ops as O
+from rew_amd.eager import DType
+E.installEagerBackend(E.mi355x(0))
+r = np.random.default_rng(0)
+x = E.fromHost(r.standard_normal((64, 2000)).astype(np.float32), DType.BFLOAT16)
+w = E.fromHost(r.standard_normal((2000, 20001)).astype(np.float32), DType.BFLOAT16)  # 80 MB
+t = E.fromHost(np.zeros(64, np.int32), DType.INT32)
+E.sync()
+base = E.stats()["bytes_in_use"]
+for _ in range(3):                                # its working memory: 65 MB
+    loss = O.linearCrossEntropy(x, w, t)
+    try:
+        E.toHost(loss)
+        sys.exit("no error")
+    except E.EagerError as e:
+        assert "REW_MI355X_MAX_DEVICE_BYTES" in str(e), e
+    del loss
+    E.sync()
+    assert E.stats()["bytes_in_use"] == base, (E.stats()["bytes_in_use"], base)
+v = O.slice_(w, [0, 0], [2000, 1000])
+E.sync()
+a = E.toHost(O.linearCrossEntropy(x, v, t))
+b = E.toHost(O.linearCrossEntropy(x, v, t))
+assert np.isfinite(a).all() and (a == b).all()
+print("ok")
+"""
+
+
+def test_no_room_for_it(gpu):
+    """An error where the limit leaves no room, which leaves nothing behind."""
+    env = dict(os.environ, REW_MI355X_MAX_DEVICE_BYTES=str(128 * MIB))
+    p = subprocess.run([sys.executable, "-c", CHILD, str(Path(__file__).resolve().parents[1])],
+                       env=env, capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and p.stdout.strip().endswith("ok"), p.stderr[-3000:]
